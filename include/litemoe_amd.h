@@ -112,6 +112,46 @@ int lm_rope_kv_write(void *q, int64_t qs0, int64_t qs1, void *k, int64_t ks0,
                      int64_t head_dim, int64_t capacity, int64_t cache_batch,
                      int write_k, void *stream);
 
+/* ---------------------------------------------------- quantised kv cache -- */
+
+/* The quantised cache of one layer: every vector of 64 channels as two blocks
+ * of 32, a block as one scale byte and 32 elements of `bits` bits.
+ *   bits 4: sign, 2 exponent bits, 1 mantissa bit (0 .5 1 1.5 2 3 4 6), T = 7
+ *   bits 8: sign, 4 exponent bits, 3 mantissa bits (to 448),           T = 464
+ * Block x: e = the smallest integer with max|x_i| <= T 2^e, held to [-126, 125]
+ * (4 bits) or [-126, 119] (8); the scale byte is e + 127; element i is x_i 2^-e
+ * rounded to the type's nearest value, ties to even, held to its largest, and
+ * stands for that value times 2^e. A block with an infinity or a NaN gets byte
+ * 255 and codes 0 and reads back as NaN. Byte 0 with codes 0, as in a cleared
+ * cache, reads as zeros (of a block of zeros only the codes are given).
+ * Layout, contiguous, head_dim 64, codes 16-byte and scales 4-byte aligned:
+ *   k_codes, v_codes  uint8 [cache_batch, heads, capacity, 8*bits]; with 4 bits
+ *                     the even channel of a byte is its low half
+ *   scales            uint8 [cache_batch, heads, capacity, 4]: k channels 0-31,
+ *                     k 32-63, v 0-31, v 32-63
+ * The reference keeps its cache in the model's dtype (litemoe/cache.py:7-20).
+ *
+ * lm_kv_quant_write: lm_kv_write (litemoe/kv_write.py:23-29) with the store
+ * quantised, bf16 k and v. The same mask and skipped rows; active may be NULL
+ * (every row is written); one writer per (slot, position), as there: two rows
+ * of one call with the same target leave either's codes beside either's scale. */
+int lm_kv_quant_write(const void *k, int64_t ks0, int64_t ks1, int64_t ks3,
+                      const void *v, int64_t vs0, int64_t vs1, int64_t vs3,
+                      void *k_codes, void *v_codes, void *scales,
+                      const int64_t *positions, const uint8_t *active,
+                      const int64_t *slots, int64_t rows, int64_t heads,
+                      int64_t head_dim, int64_t capacity, int64_t cache_batch,
+                      int64_t bits, void *stream);
+
+/* What the quantised cache stands for at (slots[r], h, positions[r]), as bf16
+ * (exact): k and v [rows, heads, 64] contiguous, 16-byte aligned. Rows whose
+ * position or slot is out of range get zeros; slots may be NULL (slot = row). */
+int lm_kv_quant_read(const void *k_codes, const void *v_codes,
+                     const void *scales, const int64_t *positions,
+                     const int64_t *slots, int64_t rows, int64_t heads,
+                     int64_t head_dim, int64_t capacity, int64_t cache_batch,
+                     int64_t bits, void *k, void *v, void *stream);
+
 /* ------------------------------------------------------------ attention -- */
 
 /* Workspace for lm_flash_decode with the given split count. */
@@ -184,6 +224,44 @@ int lm_flash_decode_qkv_frag(const float *qkv_partials, int64_t qkv_splits,
                              int64_t max_len, int64_t num_splits, void *out_frag,
                              void *workspace, int64_t workspace_bytes,
                              void *stream);
+
+/* lm_flash_decode over a quantised cache (see lm_kv_quant_write): K and V are
+ * what their codes and scale bytes stand for, products and softmax in fp32, the
+ * probabilities times V's scales rounded to bf16 for the matrix cores. A
+ * position that stands for NaN makes NaN of the rows that attend it and of no
+ * others; positions from used[b] on are never looked at. q_heads / kv_heads at
+ * most 16; q 16-byte aligned, its strides multiples of 8; the cache's buffers
+ * aligned as lm_kv_quant_write says. The other arguments and the workspace
+ * (lm_flash_decode_workspace_size, 16-byte aligned) as lm_flash_decode; bits 4
+ * or 8. Two calls in flight at once need workspaces of their own. Replaces
+ * litemoe/flash_decode.py:16-34 over a cache the reference does not have. */
+int lm_flash_decode_quant(const void *q, int64_t qs0, int64_t qs1,
+                          const void *k_codes, const void *v_codes,
+                          const void *scales, const int32_t *used,
+                          int64_t batch, int64_t q_heads, int64_t kv_heads,
+                          int64_t capacity, int64_t head_dim, int64_t bits,
+                          float scale, int64_t max_len, int64_t num_splits,
+                          void *out, void *workspace, int64_t workspace_bytes,
+                          void *stream);
+
+/* lm_flash_decode_qkv over a quantised cache: the partials' sum, RoPE, the
+ * quantising store of the new token's key and value and attention over the
+ * updated cache in one launch (two with splits). The new token is attended as
+ * the cache holds it, quantised: results and cache are bitwise those of
+ * lm_rope_kv_write without caches, lm_kv_quant_write and lm_flash_decode_quant.
+ * frag_out nonzero writes out in lm_flash_decode_qkv_frag's order (batch <=
+ * 128). qkv_partials 16-byte aligned; everything else as in
+ * lm_flash_decode_qkv and lm_flash_decode_quant. */
+int lm_flash_decode_quant_qkv(const float *qkv_partials, int64_t qkv_splits,
+                              const void *cos_sin, int64_t table_len,
+                              const int64_t *positions, const uint8_t *active,
+                              void *k_codes, void *v_codes, void *scales,
+                              const int32_t *used, const int32_t *row_order,
+                              int64_t batch, int64_t q_heads, int64_t kv_heads,
+                              int64_t capacity, int64_t head_dim, int64_t bits,
+                              float scale, int64_t max_len, int64_t num_splits,
+                              int frag_out, void *out, void *workspace,
+                              int64_t workspace_bytes, void *stream);
 
 /* Variable-length attention over a packed batch (one row per token):
  * sequence s owns tokens [cu[s], cu[s+1]); token i of it attends keys

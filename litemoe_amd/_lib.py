@@ -28,6 +28,13 @@ _SIGNATURES = {
                     _i64, _i64, _i64, _i64, _i64, _i64, _v],
     "lm_rope_kv_write": [_v, _i64, _i64, _v, _i64, _i64, _v, _i64, _i64, _v, _i64, _v, _v, _v,
                          _v, _v, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _v],
+    "lm_kv_quant_write": [_v, _i64, _i64, _i64, _v, _i64, _i64, _i64, _v, _v, _v, _v, _v, _v, _i64, _i64,
+                          _i64, _i64, _i64, _i64, _v],
+    "lm_kv_quant_read": [_v, _v, _v, _v, _v, _i64, _i64, _i64, _i64, _i64, _i64, _v, _v, _v],
+    "lm_flash_decode_quant": [_v, _i64, _i64, _v, _v, _v, _v, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _i64, _i64,
+                              _v, _v, _i64, _v],
+    "lm_flash_decode_quant_qkv": [_v, _i64, _v, _i64, _v, _v, _v, _v, _v, _v, _v, _i64, _i64, _i64, _i64, _i64, _i64,
+                                  _f32, _i64, _i64, _i32, _v, _v, _i64, _v],
     "lm_flash_decode_workspace_size": [_i64, _i64, _i64, _i64, C.POINTER(C.c_int64)],
     "lm_flash_decode": [_v, _i64, _i64, _v, _v, _v, _i64, _i64, _i64, _i64, _i64, _f32, _i64,
                         _i64, _v, _v, _i64, _v],

@@ -1,0 +1,632 @@
+// Split-K decode attention over the quantised KV cache (format: kv_quant.h):
+//   out[b, h] = softmax_j(scale q_h . K_j) V,  j < used[b],
+// K and V what their codes and scales stand for, on the matrix cores.
+//
+// A cache position of one KV head takes 68 bytes (4 bits) or 132 (8) instead of
+// bf16's 256, so the KV stream that bounds the bf16 kernel is 3.8 or 1.9 times
+// shorter, and with the products on vector units (about 35 SIMD cycles per
+// position there, against 33 that the 4-bit stream leaves) they would bound it.
+//
+// Workgroup (split, kv head, row), four waves; a wave takes 64 consecutive
+// positions (a stage) at a time, every fourth stage of the workgroup's range.
+// Stages pass through LDS: codes and scale words are copied there directly
+// (global_load_lds), kSlots stages deep, each wave its own, no barriers.
+//
+// Scores: K^T . q with v_mfma_f32_16x16x32_bf16, A the codes of 16 positions as
+// bf16 without their scales (exact), one product per block of 32 channels,
+//   s_j = sl2 * (2^e0 (c_j0 . q_0) + 2^e1 (c_j1 . q_1)).
+// The G query heads of a KV head fill P = 4, 8 or 16 of the 16 columns; the
+// other columns take other positions: column c holds query head c % P of tile
+// c / P, which the product of that tile alone adds to (its B operand is zero in
+// the other columns), so one accumulator holds 16/P tiles and each lane four
+// scores, and no exponential is spent on an empty column (G = P).
+// Codes stay apart from scales so that a block that stands for NaN, stored with
+// codes 0, cannot reach another position's row or column through a product.
+//
+// P.V: V^T . p, A the transposed codes as bf16 (ds_read_b64_tr_b4 / _tr_b8
+// straight from the stage), B the probabilities times 2^e of V's block, rounded
+// to bf16 as the bf16 kernel rounds them. A lane's scores are four consecutive
+// positions of its column's tile, which is the order that B takes them in: no
+// lane moves. Each column keeps its own running maximum, shared by its four
+// lanes; they and the waves merge once, at the end.
+//
+// Reference semantics: litemoe/flash_decode.py:16-22; masking litemoe/cache.py:42-47.
+#include "internal.h"
+#include "kv_quant.h"
+
+#include <type_traits>
+
+namespace lm {
+namespace {
+
+constexpr int kD = 64;
+constexpr int kWaves = 4;
+constexpr int kThreads = kWaves * kWave;
+constexpr int kStageKeys = 64;
+constexpr int kMaxQkvSplits = 8;
+
+// Running maximum before any position: finite, so exp2(kEmpty - m) and
+// exp2(-inf - kEmpty) are 0 and the loop needs no special case.
+constexpr float kEmpty = -1e30f;
+// A column keeps its maximum until a score exceeds it by more than this (log2
+// units): probabilities stay below 2^8 and the accumulators are seldom rescaled.
+constexpr float kLazy = 8.f;
+
+template <int kBits>
+struct Stage {
+  static constexpr int kCode = code_bytes<kBits>();
+  static constexpr int kSide = kStageKeys * kCode;        // K codes, then V codes
+  static constexpr int kBytes = 2 * kSide + 4 * kStageKeys;  // then the scale words
+  static constexpr int kSideCopies = kSide / 1024;
+  static constexpr int kCopies = 2 * kSideCopies + 1;     // vector memory operations of a wave
+  static constexpr int kSlots = kBits == 4 ? 3 : 2;
+};
+
+// Four bytes per lane to LDS (see lds_copy16).
+__device__ __forceinline__ void lds_copy4(const void *base, uint32_t voff, uint32_t lds) {
+  asm volatile("global_load_lds_dword %0, %1" ::"v"(voff), "s"(base), "{m0}"(lds) : "memory");
+}
+// vm_wait that LDS reads are not moved across.
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+// Every LDS access of this wave is done: its bytes may be copied over.
+__device__ __forceinline__ void lds_reads_done() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+__device__ __forceinline__ float merge_factor(float m, float mnew) {
+  return m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mnew);
+}
+
+// The lane N places further in its row of 16 (row_ror).
+template <int N>
+__device__ __forceinline__ float row_rotate(float v) {
+  return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x120 + N, 0xF, 0xF, false));
+}
+
+// Reductions over the tiles of a query head: columns c % P equal, one row of 16 lanes.
+template <int P>
+__device__ __forceinline__ float tiles_max(float v) {
+  if constexpr (P <= 8) v = fmaxf(v, row_rotate<8>(v));
+  if constexpr (P <= 4) v = fmaxf(v, row_rotate<4>(v));
+  return v;
+}
+template <int P>
+__device__ __forceinline__ float tiles_sum(float v) {
+  if constexpr (P <= 8) v += row_rotate<8>(v);
+  if constexpr (P <= 4) v += row_rotate<4>(v);
+  return v;
+}
+
+// Neox rotation of one (x1, x2) pair with the reference's three roundings.
+__device__ __forceinline__ void rotate_pair(float x1, float x2, float c, float s, float &o1, float &o2) {
+  o1 = round_bf16(round_bf16(x1 * c) - round_bf16(x2 * s));
+  o2 = round_bf16(round_bf16(x2 * c) + round_bf16(x1 * s));
+}
+
+struct Cache {
+  uint8_t *k, *v;     // [batch, kv_heads, capacity, code_bytes]
+  uint32_t *scales;   // [batch, kv_heads, capacity]
+};
+
+struct Partial {
+  float *o;  // [batch, q_heads, splits, 64]
+  float *m;  // [batch, q_heads, splits]
+  float *l;  // [batch, q_heads, splits]
+};
+
+// The fused form's input: see lm_flash_decode_qkv.
+struct QkvIn {
+  const float *part;      // [splits][batch][(q_heads + 2*kv_heads) * 64], NULL: unfused
+  int splits;
+  const bf16 *cos_sin;    // [table_len, 64]: cos | sin halves
+  int64_t table_len;
+  const int64_t *pos;     // [batch] position of the new token
+  const uint8_t *active;  // [batch] or NULL (all rows write)
+  const int32_t *order;   // [batch] row of workgroup z (longest first), or NULL: row z
+};
+
+template <int kBits, int P, bool kFused>
+__global__ void __launch_bounds__(kThreads, 2)
+decode_quant_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, Cache cache,
+                    const int32_t *__restrict__ used, int q_heads, int kv_heads, int64_t capacity,
+                    float scale, int max_len, int chunk, int splits, Partial part, QkvIn in,
+                    bf16 *__restrict__ out, int out_mb) {
+  typedef Stage<kBits> St;
+  constexpr int kTiles = 16 / P;   // tiles of 16 positions in one accumulator
+  constexpr int kPasses = 4 / kTiles;
+  constexpr int kMergeBytes = kWaves * P * (kD + 2) * 4;
+  constexpr int kStageBytes = kWaves * St::kSlots * St::kBytes;
+  __shared__ __align__(16) uint8_t smem[kStageBytes > kMergeBytes ? kStageBytes : kMergeBytes];
+  // The fused form's row: q heads, new key, new value; then both quantised.
+  __shared__ __align__(16) float sm_qkv[kFused ? P + 2 : 1][kD];
+  __shared__ __align__(16) uint16_t sm_rot[kFused ? P + 1 : 1][kD];
+  __shared__ __align__(16) uint8_t sm_new[kFused ? 2 * St::kCode : 16];
+  __shared__ __align__(4) uint8_t sm_scale[4];
+  const int split = blockIdx.x, h = blockIdx.y;
+  const int64_t b = kFused && in.order ? in.order[blockIdx.z] : blockIdx.z;
+  const int G = q_heads / kv_heads;
+  const int lane = threadIdx.x % kWave;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int col = lane % 16, grp = lane / 16;
+  const int tile = col / P, head = col % P;   // this column's tile of a pass, its query head
+
+  int n = min(used[b], max_len);
+  n = (int)min((int64_t)n, capacity);
+  const int k0 = split * chunk;
+  const int k1 = min(n, k0 + chunk);
+  bool writer = false, own = false;
+  int64_t pnew = 0;
+  if constexpr (kFused) {
+    // The new token is stored by the split whose range holds its position
+    // (split 0 when none does); where it is attended too, its codes replace
+    // those that the stage was loaded with.
+    pnew = in.pos[b];
+    const bool writes = (!in.active || in.active[b]) && pnew >= 0 && pnew < capacity;
+    const int64_t wsplit = pnew >= 0 && pnew < (int64_t)gridDim.x * chunk ? pnew / chunk : 0;
+    writer = writes && split == wsplit;
+    own = writer && pnew >= k0 && pnew < k1;
+  }
+  if (splits > 1 && k0 >= n && !writer) return;  // the combine kernel skips empty splits
+
+  const int64_t first_pos = ((int64_t)b * kv_heads + h) * capacity;
+  // This wave's stages: stage it starts at position k0 + (it * kWaves + wave) * 64.
+  const int left = k1 - k0 - wave * kStageKeys;
+  const int niter = left > 0 ? (left + kWaves * kStageKeys - 1) / (kWaves * kStageKeys) : 0;
+  uint8_t *const my_stages = smem + wave * St::kSlots * St::kBytes;
+  const uint32_t my_lds = __builtin_amdgcn_readfirstlane(lds_address(my_stages));
+
+  // Requests stage `it` into its slot. Positions past the range repeat its last
+  // one (they are masked); offsets within a stage are below 4 KB, the stage's own
+  // start is a 64-bit scalar.
+  auto issue = [&](int it, int slot) {
+    const int start = k0 + (it * kWaves + wave) * kStageKeys;
+    const int last = k1 - 1 - start;
+    const int64_t at = first_pos + start;
+    const uint32_t lds = my_lds + slot * St::kBytes;
+#pragma unroll
+    for (int c = 0; c < St::kSideCopies; ++c) {
+      constexpr int kChunks = St::kCode / 16;  // 16-byte chunks of one position
+      const int chunk16 = c * kWave + lane;
+      const uint32_t off = (uint32_t)min(chunk16 / kChunks, last) * St::kCode + (chunk16 % kChunks) * 16;
+      lds_copy16(cache.k + at * St::kCode, off, lds + c * 1024);
+      lds_copy16(cache.v + at * St::kCode, off, lds + St::kSide + c * 1024);
+    }
+    lds_copy4(cache.scales + at, (uint32_t)min(lane, last) * 4, lds + 2 * St::kSide);
+  };
+
+  if constexpr (kFused) {
+    // The row's q|k|v slices of the packed projection, summed over the K slices
+    // in ascending order and rounded to bf16 (F.linear's output).
+    const int64_t ncols = (int64_t)(q_heads + 2 * kv_heads) * kD;
+    for (int t = threadIdx.x; t < (G + 2) * (kD / 4); t += kThreads) {
+      const int hs = t / (kD / 4), c4 = (t % (kD / 4)) * 4;
+      const int src_head = hs < G ? h * G + hs : (hs == G ? q_heads + h : q_heads + kv_heads + h);
+      const float *src = in.part + b * ncols + (int64_t)src_head * kD + c4;
+      f32x4 pv[kMaxQkvSplits];
+#pragma unroll
+      for (int s = 0; s < kMaxQkvSplits; ++s)
+        if (s < in.splits) pv[s] = *reinterpret_cast<const f32x4 *>(src + (int64_t)s * gridDim.z * ncols);
+      f32x4 acc = pv[0];
+#pragma unroll
+      for (int s = 1; s < kMaxQkvSplits; ++s)
+        if (s < in.splits) acc += pv[s];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sm_qkv[hs][c4 + i] = round_bf16(acc[i]);
+    }
+  }
+#pragma unroll
+  for (int s = 0; s < St::kSlots - 1; ++s)
+    if (s < niter) issue(s, s);
+
+  u32x4 qv[2];
+  if constexpr (kFused) {
+    __syncthreads();
+    const bool in_table = pnew >= 0 && pnew < in.table_len;
+    const bf16 *cs = in.cos_sin + (in_table ? pnew : 0) * kD;
+    for (int t = threadIdx.x; t < (G + 1) * (kD / 2); t += kThreads) {
+      const int hs = t / (kD / 2), pair = t % (kD / 2);
+      const float x1 = sm_qkv[hs][pair], x2 = sm_qkv[hs][kD / 2 + pair];
+      float o1 = x1, o2 = x2;
+      if (in_table) rotate_pair(x1, x2, bf16_to_f32(cs[pair]), bf16_to_f32(cs[kD / 2 + pair]), o1, o2);
+      sm_rot[hs][pair] = (uint16_t)f32_to_bf16(o1);
+      sm_rot[hs][kD / 2 + pair] = (uint16_t)f32_to_bf16(o2);
+    }
+    __syncthreads();
+    // Sixteen lanes quantise the new key (0-7) and value (8-15), eight channels each.
+    if (writer && threadIdx.x < 16) {
+      const int side = threadIdx.x / 8, u = threadIdx.x % 8;
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        x[i] = side ? sm_qkv[G + 1][8 * u + i] : bf16_to_f32(sm_rot[G][8 * u + i]);
+      uint32_t byte;
+      const Codes8<kBits> c = quantise8<kBits>(x, byte);
+      *reinterpret_cast<Codes8<kBits> *>(sm_new + side * St::kCode + u * kBits) = c;
+      const int64_t at = first_pos + pnew;
+      *reinterpret_cast<Codes8<kBits> *>((side ? cache.v : cache.k) + at * St::kCode + u * kBits) = c;
+      if (u % 4 == 0) {
+        sm_scale[2 * side + u / 4] = (uint8_t)byte;
+        reinterpret_cast<uint8_t *>(cache.scales + at)[2 * side + u / 4] = (uint8_t)byte;
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int bl = 0; bl < 2; ++bl)
+      qv[bl] = *reinterpret_cast<const u32x4 *>(&sm_rot[min(head, G)][32 * bl + 8 * grp]);
+  } else {
+    const bf16 *qp = q + b * qs0 + (int64_t)(h * G + min(head, G - 1)) * qs1 + 8 * grp;
+    qv[0] = *reinterpret_cast<const u32x4 *>(qp);
+    qv[1] = *reinterpret_cast<const u32x4 *>(qp + 32);
+  }
+  // B operands of the scores: tile t's are zero outside its columns.
+  u32x4 qt[kTiles][2];
+#pragma unroll
+  for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+    for (int bl = 0; bl < 2; ++bl)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) qt[t][bl][i] = tile == t && head < G ? qv[bl][i] : 0u;
+
+  const float sl2 = scale * 1.4426950408889634f;
+  float m = kEmpty, l = 0.f;
+  f32x4 acc[4];  // channels 16 mm + 4 grp + i of column col
+#pragma unroll
+  for (int mm = 0; mm < 4; ++mm) acc[mm] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  auto compute = [&](int it, int slot) {
+    uint8_t *st = my_stages + slot * St::kBytes;
+    const int start = k0 + (it * kWaves + wave) * kStageKeys;
+    const int count = k1 - start;  // positions of the stage that count, if fewer than 64
+    if constexpr (kFused) {
+      if (own && pnew >= start && pnew < start + kStageKeys) {
+        const int at = (int)(pnew - start);
+        if (lane < 2 * St::kCode / 4) {
+          const int side = lane / (St::kCode / 4), w = lane % (St::kCode / 4);
+          *reinterpret_cast<uint32_t *>(st + side * St::kSide + at * St::kCode + 4 * w) =
+              *reinterpret_cast<const uint32_t *>(sm_new + side * St::kCode + 4 * w);
+        }
+        if (lane == 0)
+          *reinterpret_cast<uint32_t *>(st + 2 * St::kSide + 4 * at) = *reinterpret_cast<const uint32_t *>(sm_scale);
+        lds_reads_done();
+      }
+    }
+    float s[kPasses][4];
+    u32x4 words[kPasses];  // scale words of the lane's four positions of each pass
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p) {
+      f32x4 c0 = {0.f, 0.f, 0.f, 0.f}, c1 = c0;
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t) {
+        const uint8_t *kp = st + ((p * kTiles + t) * 16 + col) * St::kCode + grp * kBits;
+        const Codes8<kBits> a0 = *reinterpret_cast<const Codes8<kBits> *>(kp);
+        const Codes8<kBits> a1 = *reinterpret_cast<const Codes8<kBits> *>(kp + St::kCode / 2);
+        c0 = mfma16x16x32(codes_to_bf16<kBits>(a0.w), qt[t][0], c0);
+        c1 = mfma16x16x32(codes_to_bf16<kBits>(a1.w), qt[t][1], c1);
+      }
+      const int first = (p * kTiles + tile) * 16 + 4 * grp;  // the lane's first position
+      words[p] = *reinterpret_cast<const u32x4 *>(st + 2 * St::kSide + 4 * first);
+      if (count < kStageKeys) {
+        // Masked positions: whatever their bytes hold, scale 0 and score -inf.
+#pragma unroll
+        for (int i = 0; i < 4; ++i) words[p][i] = first + i < count ? words[p][i] : 0u;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float x = c0[i] * quant_scale(words[p][i], 0) + c1[i] * quant_scale(words[p][i], 1);
+        s[p][i] = x * sl2;
+        if (count < kStageKeys) s[p][i] = first + i < count ? s[p][i] : -INFINITY;
+      }
+    }
+    float mx = m;
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[p][i]);
+    if (__any(mx > m + kLazy)) {
+      mx = fmaxf(mx, xor_lanes<16>(mx));
+      mx = fmaxf(mx, xor_lanes<32>(mx));
+      const bool up = mx > m + kLazy;
+      const float f = up ? merge_factor(m, mx) : 1.f;
+      m = up ? mx : m;
+      l *= f;
+#pragma unroll
+      for (int mm = 0; mm < 4; ++mm) acc[mm] *= f;
+    }
+    // Probabilities times the scale of each block of V, as bf16 pairs.
+    uint32_t pb[2][kPasses][2];
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p) {
+      float e[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        e[i] = __builtin_amdgcn_exp2f(s[p][i] - m);
+        l += e[i];
+      }
+#pragma unroll
+      for (int bl = 0; bl < 2; ++bl)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          pb[bl][p][i] = pack_bf16_finite(e[2 * i] * quant_scale(words[p][2 * i], 2 + bl),
+                                          e[2 * i + 1] * quant_scale(words[p][2 * i + 1], 2 + bl));
+    }
+    // B operands of tiles 2 pr and 2 pr + 1: eight positions per lane, zero in
+    // the columns of other tiles.
+    u32x4 bp[2][2];
+#pragma unroll
+    for (int pr = 0; pr < 2; ++pr)
+#pragma unroll
+      for (int bl = 0; bl < 2; ++bl)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int t = 2 * pr + half, p = t / kTiles;
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            bp[pr][bl][2 * half + i] = kTiles == 1 || tile == t % kTiles ? pb[bl][p][i] : 0u;
+        }
+    typedef int i32x2 __attribute__((ext_vector_type(2)));
+    typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
+    const uint8_t *vs = st + St::kSide;
+#pragma unroll
+    for (int mm = 0; mm < 4; ++mm) {
+      if constexpr (kBits == 4) {
+        // Lane col of a group reads the 16 channels of position 16 (col/4) + 4 grp + col%4
+        // and receives channel col of the group's 16 positions, tiles 0-3 in order.
+        const int pos = 16 * (col / 4) + 4 * grp + col % 4;
+        const i32x2 t = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
+            (lds_i32x2 *)(vs + pos * St::kCode + 8 * mm));
+#pragma unroll
+        for (int pr = 0; pr < 2; ++pr) {
+          const uint32_t w = (uint32_t)t[pr];
+          acc[mm] = mfma16x16x32(codes_to_bf16<kBits>(&w), bp[pr][mm / 2], acc[mm]);
+        }
+      } else {
+#pragma unroll
+        for (int pr = 0; pr < 2; ++pr) {
+          // Lanes 2r and 2r+1 read the 16 channels of position r of the group's
+          // eight (four of each tile); lane col receives channel col of all eight.
+          const int r = col / 2;
+          const int pos = 16 * (2 * pr + r / 4) + 4 * grp + r % 4;
+          const i32x2 t = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+              (lds_i32x2 *)(vs + pos * St::kCode + 16 * mm + 8 * (col % 2)));
+          const uint32_t w[2] = {(uint32_t)t[0], (uint32_t)t[1]};
+          acc[mm] = mfma16x16x32(codes_to_bf16<kBits>(w), bp[pr][mm / 2], acc[mm]);
+        }
+      }
+    }
+  };
+
+  int slot = 0;
+  for (int it = 0; it < niter; ++it) {
+    // Stage `it` has arrived once only the younger ones are in flight.
+    const int younger = min(niter - 1 - it, St::kSlots - 2);
+    if (younger >= 1)
+      copies_wait<(St::kSlots - 2) * St::kCopies>();
+    else
+      copies_wait<0>();
+    if (it + St::kSlots - 1 < niter) {
+      // The slot that stage it - 1 has left; its reads are done.
+      lds_reads_done();
+      issue(it + St::kSlots - 1, (slot + St::kSlots - 1) % St::kSlots);
+    }
+    compute(it, slot);
+    slot = slot + 1 == St::kSlots ? 0 : slot + 1;
+  }
+
+  // Merge the four lanes of a column (their l), the columns of a query head, then the waves.
+  l += xor_lanes<16>(l);
+  l += xor_lanes<32>(l);
+  const float mall = tiles_max<P>(m);
+  const float f = __builtin_amdgcn_exp2f(m - mall);
+  l = tiles_sum<P>(l * f);
+#pragma unroll
+  for (int mm = 0; mm < 4; ++mm)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[mm][i] = tiles_sum<P>(acc[mm][i] * f);
+  __syncthreads();  // every wave is done with its stages
+  float(*sm_o)[P][kD] = reinterpret_cast<float(*)[P][kD]>(smem);
+  float(*sm_m)[P] = reinterpret_cast<float(*)[P]>(smem + kWaves * P * kD * 4);
+  float(*sm_l)[P] = sm_m + kWaves;
+  if (tile == 0) {
+#pragma unroll
+    for (int mm = 0; mm < 4; ++mm) *reinterpret_cast<f32x4 *>(&sm_o[wave][head][16 * mm + 4 * grp]) = acc[mm];
+    if (grp == 0) {
+      sm_m[wave][head] = mall;
+      sm_l[wave][head] = l;
+    }
+  }
+  __syncthreads();
+  for (int t = threadIdx.x; t < G * kD; t += kThreads) {
+    const int g = t / kD, c = t % kD;
+    float mx = sm_m[0][g];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) mx = fmaxf(mx, sm_m[w][g]);
+    float lsum = 0.f, o = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float fw = __builtin_amdgcn_exp2f(sm_m[w][g] - mx);
+      lsum += sm_l[w][g] * fw;
+      o += sm_o[w][g][c] * fw;
+    }
+    const int hq = h * G + g;
+    if (splits == 1) {
+      const int64_t at = out_mb ? frag_offset_rows(b, (int64_t)hq * kD + c, out_mb) : (b * q_heads + hq) * kD + c;
+      out[at] = (bf16)f32_to_bf16(lsum == 0.f ? 0.f : o / lsum);
+    } else {
+      const int64_t at = ((int64_t)b * q_heads + hq) * splits + split;
+      part.o[at * kD + c] = o;
+      if (c == 0) {
+        part.m[at] = mx;
+        part.l[at] = lsum;
+      }
+    }
+  }
+}
+
+// grid (q_heads, batch), one thread per channel: the splits' partials by
+// log-sum-exp, those of kBatch splits requested together (clamped and masked,
+// so that none waits behind the row's length).
+template <int kBatch>
+__global__ void __launch_bounds__(kD)
+decode_quant_combine_kernel(const int32_t *__restrict__ used, int q_heads, int64_t capacity, int max_len,
+                            int chunk, int splits, Partial part, bf16 *__restrict__ out, int out_mb) {
+  const int hq = blockIdx.x;
+  const int64_t b = blockIdx.y;
+  const int c = threadIdx.x;
+  const int64_t base = ((int64_t)b * q_heads + hq) * splits;
+  float ms[kBatch], ls[kBatch], os[kBatch];
+  auto load = [&](int s0) {
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int64_t at = base + min(s0 + i, splits - 1);
+      ms[i] = part.m[at];
+      ls[i] = part.l[at];
+      os[i] = part.o[at * kD + c];
+    }
+  };
+  load(0);
+  int n = min(used[b], max_len);
+  n = (int)min((int64_t)n, capacity);
+  const int valid = n > 0 ? min(splits, (n + chunk - 1) / chunk) : 0;
+  float mx = kEmpty;
+#pragma unroll
+  for (int i = 0; i < kBatch; ++i) mx = fmaxf(mx, i < valid ? ms[i] : kEmpty);
+  for (int s = kBatch; s < valid; ++s) mx = fmaxf(mx, part.m[base + s]);
+  float lsum = 0.f, o = 0.f;
+  for (int s0 = 0; s0 < valid; s0 += kBatch) {
+    if (s0) load(s0);
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      // a split past the row's end was never written: selected away, not scaled
+      const bool live = s0 + i < valid;
+      const float f = live ? __builtin_amdgcn_exp2f(ms[i] - mx) : 0.f;
+      lsum += live ? ls[i] * f : 0.f;
+      o += live ? os[i] * f : 0.f;
+    }
+  }
+  const int64_t at = out_mb ? frag_offset_rows(b, (int64_t)hq * kD + c, out_mb) : (b * q_heads + hq) * kD + c;
+  out[at] = (bf16)f32_to_bf16(lsum == 0.f ? 0.f : o / lsum);
+}
+
+int64_t workspace_bytes(int64_t batch, int64_t q_heads, int64_t splits) {
+  if (splits <= 1) return 0;
+  const int64_t n = batch * q_heads * splits;
+  return n * kD * 4 + 2 * align_up(n * 4, 256);
+}
+
+template <int kBits, int P, bool kFused>
+int launch_sized(const bf16 *q, int64_t qs0, int64_t qs1, const Cache &cache, const int32_t *used, int64_t batch,
+                 int64_t q_heads, int64_t kv_heads, int64_t capacity, float scale, int64_t max_len, int chunk,
+                 int grid_splits, int stride_splits, const Partial &part, const QkvIn &in, bf16 *out, int out_mb,
+                 hipStream_t s) {
+  const dim3 grid((unsigned)grid_splits, (unsigned)kv_heads, (unsigned)batch);
+  decode_quant_kernel<kBits, P, kFused><<<grid, kThreads, 0, s>>>(
+      q, qs0, qs1, cache, used, (int)q_heads, (int)kv_heads, capacity, scale, (int)max_len, chunk, stride_splits,
+      part, in, out, out_mb);
+  LM_CHECK_LAUNCH();
+  return LM_OK;
+}
+
+struct Call {
+  int64_t batch, q_heads, kv_heads, capacity, head_dim, max_len, num_splits, bits;
+};
+
+// Argument checks of both entry points; *run false where nothing is to launch.
+int check_call(const Call &c, bool *run) {
+  *run = false;
+  LM_REQUIRE(c.batch >= 0 && c.q_heads > 0 && c.kv_heads > 0 && c.q_heads % c.kv_heads == 0 && c.capacity > 0 &&
+             c.max_len > 0 && c.num_splits > 0 && c.num_splits <= 1024 && c.max_len < ((int64_t)1 << 30) &&
+             c.batch <= 65535 && c.kv_heads <= 65535);
+  if (c.head_dim != kD || (c.bits != 4 && c.bits != 8) || c.q_heads / c.kv_heads > 16) return LM_EUNSUPPORTED;
+  *run = c.batch > 0;
+  return LM_OK;
+}
+
+bool aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+int launch_decode_quant(const Call &c, const void *q, int64_t qs0, int64_t qs1, const Cache &cache,
+                        const int32_t *used, float scale, const QkvIn &in, void *out, int out_mb, void *workspace,
+                        int64_t workspace_bytes_, void *stream) {
+  LM_REQUIRE(aligned16(cache.k) && aligned16(cache.v) && reinterpret_cast<uintptr_t>(cache.scales) % 4 == 0);
+  const int64_t need = workspace_bytes(c.batch, c.q_heads, c.num_splits);
+  if (need > 0 && (!workspace || workspace_bytes_ < need)) return LM_EWORKSPACE;
+  LM_REQUIRE(need == 0 || aligned16(workspace));
+  const int chunk = (int)align_up(cdiv(c.max_len, c.num_splits), kStageKeys);
+  const int splits = (int)cdiv(c.max_len, chunk);
+  Partial part{nullptr, nullptr, nullptr};
+  if (splits > 1) {
+    const int64_t n = c.batch * c.q_heads * c.num_splits;
+    char *w = static_cast<char *>(workspace);
+    part.o = reinterpret_cast<float *>(w);
+    part.m = reinterpret_cast<float *>(w + n * kD * 4);
+    part.l = reinterpret_cast<float *>(w + n * kD * 4 + align_up(n * 4, 256));
+  }
+  // Partials are indexed with the caller's split count as the stride.
+  const int stride_splits = splits > 1 ? (int)c.num_splits : 1;
+  hipStream_t s = (hipStream_t)stream;
+  const int64_t G = c.q_heads / c.kv_heads;
+  auto pick = [&](auto fused) {
+    constexpr bool kFused = decltype(fused)::value;
+    auto go = c.bits == 4 ? (G <= 4   ? launch_sized<4, 4, kFused>
+                             : G <= 8 ? launch_sized<4, 8, kFused>
+                                      : launch_sized<4, 16, kFused>)
+                          : (G <= 4   ? launch_sized<8, 4, kFused>
+                             : G <= 8 ? launch_sized<8, 8, kFused>
+                                      : launch_sized<8, 16, kFused>);
+    return go((const bf16 *)q, qs0, qs1, cache, used, c.batch, c.q_heads, c.kv_heads, c.capacity, scale, c.max_len,
+              chunk, splits, stride_splits, part, in, (bf16 *)out, out_mb, s);
+  };
+  const int status = in.part ? pick(std::true_type{}) : pick(std::false_type{});
+  if (status != LM_OK || splits == 1) return status;
+  auto combine = splits <= 4 ? decode_quant_combine_kernel<4> : decode_quant_combine_kernel<16>;
+  combine<<<dim3((unsigned)c.q_heads, (unsigned)c.batch), kD, 0, s>>>(
+      used, (int)c.q_heads, c.capacity, (int)c.max_len, chunk, stride_splits, part, (bf16 *)out, out_mb);
+  LM_CHECK_LAUNCH();
+  return LM_OK;
+}
+
+}  // namespace
+}  // namespace lm
+
+using namespace lm;
+
+extern "C" int lm_flash_decode_quant(const void *q, int64_t qs0, int64_t qs1, const void *k_codes,
+                                     const void *v_codes, const void *scales, const int32_t *used,
+                                     int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t capacity,
+                                     int64_t head_dim, int64_t bits, float scale, int64_t max_len,
+                                     int64_t num_splits, void *out, void *workspace,
+                                     int64_t workspace_bytes_, void *stream) {
+  const Call c{batch, q_heads, kv_heads, capacity, head_dim, max_len, num_splits, bits};
+  bool run;
+  const int status = check_call(c, &run);
+  if (status != LM_OK || !run) return status;
+  LM_REQUIRE(q && k_codes && v_codes && scales && used && out);
+  LM_REQUIRE(aligned16(q) && qs0 % 8 == 0 && qs1 % 8 == 0);
+  const Cache cache{(uint8_t *)const_cast<void *>(k_codes), (uint8_t *)const_cast<void *>(v_codes),
+                    (uint32_t *)const_cast<void *>(scales)};
+  const QkvIn in{nullptr, 0, nullptr, 0, nullptr, nullptr, nullptr};
+  return launch_decode_quant(c, q, qs0, qs1, cache, used, scale, in, out, 0, workspace, workspace_bytes_, stream);
+}
+
+extern "C" int lm_flash_decode_quant_qkv(const float *qkv_partials, int64_t qkv_splits, const void *cos_sin,
+                                         int64_t table_len, const int64_t *positions,
+                                         const uint8_t *active, void *k_codes, void *v_codes, void *scales,
+                                         const int32_t *used, const int32_t *row_order, int64_t batch,
+                                         int64_t q_heads, int64_t kv_heads, int64_t capacity,
+                                         int64_t head_dim, int64_t bits, float scale, int64_t max_len,
+                                         int64_t num_splits, int frag_out, void *out, void *workspace,
+                                         int64_t workspace_bytes_, void *stream) {
+  const Call c{batch, q_heads, kv_heads, capacity, head_dim, max_len, num_splits, bits};
+  bool run;
+  const int status = check_call(c, &run);
+  if (status != LM_OK) return status;
+  LM_REQUIRE(qkv_splits >= 1 && table_len > 0);
+  if (qkv_splits > kMaxQkvSplits || (frag_out && batch > 128)) return LM_EUNSUPPORTED;
+  if (!run) return LM_OK;
+  LM_REQUIRE(qkv_partials && cos_sin && positions && k_codes && v_codes && scales && used && out);
+  LM_REQUIRE(aligned16(qkv_partials));
+  const QkvIn in{qkv_partials, (int)qkv_splits, (const bf16 *)cos_sin, table_len, positions, active, row_order};
+  const Cache cache{(uint8_t *)k_codes, (uint8_t *)v_codes, (uint32_t *)scales};
+  return launch_decode_quant(c, nullptr, 0, 0, cache, used, scale, in, out, frag_out ? frag_row_blocks(batch) : 0,
+                             workspace, workspace_bytes_, stream);
+}

@@ -2,7 +2,8 @@
 
 The public surface is the reference's (litemoe/engine.py:15-221): ``Request``,
 ``Engine(model, requests, world, rank, mode, ignore_eos, poll, capacity,
-host_process)``, ``decode_step()``, ``prefill()``, ``prepare_graph()``,
+host_process, kv_bits)`` (``kv_bits`` 8 or 4 holds the KV cache quantised, which
+the reference does not have), ``decode_step()``, ``prefill()``, ``prepare_graph()``,
 ``stopped()`` and ``generate()`` with the same metrics keys, the same
 ``emit [B, 3] = (token, index, valid)`` snapshot and its ordering check.
 The engine runs one GPU (world 1). What differs is how a step runs:
@@ -29,7 +30,7 @@ from dataclasses import dataclass
 
 import torch
 
-from .cache import KVCache
+from .cache import KVCache, QuantKVCache
 from .execution import OutputRing, capture_decode
 from .step import greedy_epilogue
 
@@ -85,7 +86,9 @@ class Engine:
     ring_depth = 4
 
     def __init__(self, model, requests, world=1, rank=0, mode="eager", ignore_eos=False, poll=1,
-                 capacity=None, host_process=None):
+                 capacity=None, host_process=None, kv_bits=16):
+        if kv_bits not in (4, 8, 16):
+            raise ValueError("The KV cache holds 16 bits per element, or 8 or 4 quantised")
         if world != 1 or rank != 0:
             raise ValueError("This build runs one engine per GPU (world == 1)")
         if poll < 1 or mode not in ("eager", "graph", "graph-async"):
@@ -110,7 +113,8 @@ class Engine:
         if mode != "eager" and not model.ep.backend.graph_safe:
             raise ValueError("Full Decode Graph requires a graph-safe expert backend")
         cfg = model.cfg
-        self.cache = self.cache_type(cfg, self.batch, self.capacity, self.device, self.dtype)
+        sizes = cfg, self.batch, self.capacity, self.device, self.dtype
+        self.cache = self.cache_type(*sizes) if kv_bits == 16 else QuantKVCache(*sizes, bits=kv_bits)
         self.state = {name: torch.zeros(self.batch, dtype=dtype, device=self.device)
                       for name, dtype in STATE_FIELDS}
         self.emit = torch.zeros(self.batch, 3, dtype=torch.int64, device=self.device)

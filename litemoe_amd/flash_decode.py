@@ -15,7 +15,7 @@ import math
 
 import torch
 
-from . import _lib
+from . import _lib, kv_quant
 from .linear import FragRows
 
 
@@ -131,4 +131,107 @@ class FlashDecode:
                   k.data_ptr(), v.data_ptr(), used.data_ptr(), _lib.ptr(row_order), b,
                   q_heads, hkv, self.capacity, 64, float(scale), self.maximum, self.splits,
                   out_ptr, self.workspace.data_ptr(), self.workspace.numel(), _lib.stream(k.device))
+        return out
+
+
+class QuantFlashDecode:
+    """:class:`FlashDecode` over a :class:`~litemoe_amd.cache.QuantKVCache`
+    (``lm_flash_decode_quant``, ``lm_flash_decode_quant_qkv``): the same plan and
+    calls, the cache layer given as its three buffers ``k, v, scales``
+    (``cache.layer(i)``), up to 16 query heads per KV head. Calls that overlap
+    (on two streams, or recorded into graphs that replay at once) need an object
+    each: the splits' partials lie in its workspace."""
+
+    def __init__(self, batch, kv_heads, groups, capacity, device, maximum=None, num_splits=None, ordered=False,
+                 bits=4):
+        if maximum is not None and not 0 < maximum <= capacity:
+            raise ValueError("Decode attention requires a valid length bound")
+        if bits not in kv_quant.BITS:
+            raise ValueError("A quantised KV cache holds 4 or 8 bits per element")
+        if not 1 <= groups <= 16:
+            raise ValueError("Decode attention over a quantised cache takes 1 to 16 query heads per KV head")
+        self.batch, self.kv_heads, self.groups, self.capacity, self.bits = batch, kv_heads, groups, capacity, bits
+        self.maximum = capacity if maximum is None else maximum
+        self.splits = num_splits or default_splits(batch, kv_heads, self.maximum)
+        self.device = torch.device(device)
+        size = _lib.size_query("lm_flash_decode_workspace_size", batch, kv_heads * groups, 64,
+                               self.splits) if self.device.type == "cuda" else 0
+        self.workspace = torch.empty(max(size, 1), dtype=torch.uint8, device=self.device)
+        self.row_order = (torch.empty(batch, dtype=torch.int32, device=self.device)
+                          if ordered and self.device.type == "cuda" else None)
+
+    def _check(self, k, v, scales, q_heads, rows):
+        if kv_quant.check_layer(k, v, scales) != self.bits:
+            raise ValueError("Decode attention built for another cache type")
+        if rows > self.batch or k.shape[0] < rows or k.shape[2] != self.capacity or k.shape[1] != self.kv_heads:
+            raise ValueError("Decode attention built for another batch/capacity")
+        if q_heads != self.kv_heads * self.groups:
+            raise ValueError("Query heads do not match the cache heads")
+        if self.workspace.device != k.device:
+            raise ValueError("Decode attention built for another device")
+
+    @staticmethod
+    def _rows(t, rows, dtype, device, what):
+        t = t if t.dtype == dtype else t.to(dtype)
+        if t.shape != (rows,) or t.device != device:
+            raise ValueError(f"{what} needs one entry per row, on the cache's device")
+        return t.contiguous()
+
+    def __call__(self, q, k, v, scales, lengths, active, scale, used=None):
+        """Attention of ``q [B, Hq, 1, 64]`` over the first ``used[b]`` positions
+        of each row (``where(active, lengths + 1, 1)`` unless given); a row with
+        ``used`` 0 gives zeros."""
+        b, hq, s, d = q.shape
+        if s != 1 or d != 64:
+            raise ValueError("Decode attention takes one query position with head_dim 64")
+        self._check(k, v, scales, hq, b)
+        if q.dtype != torch.bfloat16:
+            raise ValueError("Decode attention supports BF16")
+        if q.device != k.device:
+            raise ValueError("Queries and cache must be on one device")
+        if q.stride(3) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
+            raise ValueError("Decode attention needs contiguous channels and 16-byte aligned query heads")
+        if used is None:
+            used = torch.where(active, lengths + 1, 1)
+        used = self._rows(used, b, torch.int32, k.device, "used")
+        out = torch.empty(b, hq, 1, d, device=q.device, dtype=q.dtype)
+        with torch.cuda.device(k.device):
+            _lib.call("lm_flash_decode_quant", q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), v.data_ptr(),
+                      scales.data_ptr(), used.data_ptr(), b, hq, self.kv_heads, self.capacity, d, self.bits,
+                      float(scale), self.maximum, self.splits, out.data_ptr(), self.workspace.data_ptr(),
+                      self.workspace.numel(), _lib.stream(k.device))
+        return out
+
+    def fused_qkv(self, partials, cos_sin, positions, active, k, v, scales, scale, used, q_heads, row_order=None,
+                  frag_out=False):
+        """:meth:`FlashDecode.fused_qkv`, the new token's key and value quantised
+        into the layer's buffers and attended as they stand there."""
+        splits, b, ncols = partials.shape
+        self._check(k, v, scales, q_heads, b)
+        device = k.device
+        if ncols != (q_heads + 2 * self.kv_heads) * 64:
+            raise ValueError("QKV partials do not match the cache heads")
+        if partials.dtype != torch.float32 or not partials.is_contiguous() or partials.device != device:
+            raise ValueError("QKV partials must be contiguous fp32 on the cache's device")
+        if (cos_sin.dtype != torch.bfloat16 or cos_sin.dim() != 2 or cos_sin.shape[1] != 64
+                or not cos_sin.is_contiguous() or cos_sin.device != device):
+            raise ValueError("Decode attention needs a contiguous BF16 [table_len, 64] cos/sin table")
+        positions = self._rows(positions, b, torch.int64, device, "positions")
+        used = self._rows(used, b, torch.int32, device, "used")
+        active = None if active is None else self._rows(active, b, torch.bool, device, "active")
+        if row_order is not None and (row_order.dtype != torch.int32 or row_order.shape != (b,)
+                                      or row_order.device != device or not row_order.is_contiguous()):
+            raise ValueError("row_order must be an int32 [B] permutation")
+        if frag_out:
+            out = FragRows(b, q_heads * 64, device)
+            out_ptr = out.data.data_ptr()
+        else:
+            out = torch.empty(b, q_heads, 1, 64, device=device, dtype=torch.bfloat16)
+            out_ptr = out.data_ptr()
+        with torch.cuda.device(device):
+            _lib.call("lm_flash_decode_quant_qkv", partials.data_ptr(), splits, cos_sin.data_ptr(), cos_sin.shape[0],
+                      positions.data_ptr(), _lib.ptr(active), k.data_ptr(), v.data_ptr(), scales.data_ptr(),
+                      used.data_ptr(), _lib.ptr(row_order), b, q_heads, self.kv_heads, self.capacity, 64, self.bits,
+                      float(scale), self.maximum, self.splits, int(bool(frag_out)), out_ptr,
+                      self.workspace.data_ptr(), self.workspace.numel(), _lib.stream(device))
         return out

@@ -31,14 +31,15 @@ import torch
 import torch.nn.functional as F
 
 from . import _lib
+from .cache import QuantKVCache
 from .config import validate_config
-from .flash_decode import FlashDecode
+from .flash_decode import FlashDecode, QuantFlashDecode
 from .experts import combine_supported, finish_add_rmsnorm, pack_expert_weights, scan_path
 from .linear import (linear_dense, linear_rope_kv, linear_splitk, linear_splitk_frag, linear_splitk_rmsnorm,
                      pick_splits)
 from .norm import add_rmsnorm, rmsnorm
 from .packed import PackedPrefill, build_packed, varlen_attention
-from .rope import rope_kv_write
+from .rope import rope_kv_write, rotary_embedding
 from .router import add_rmsnorm_route as route_add_rmsnorm
 from .router import add_rmsnorm_route_splitk as route_add_rmsnorm_splitk
 from .router import route
@@ -113,15 +114,23 @@ class Granite:
                 w["input_linear_packed"], w["output_linear_packed"] = pack_expert_weights(w1, w2)
 
     def _decode_attention(self, batch, cache):
+        bits = getattr(cache, "bits", 16)
         if self.decode_flash is not None:
+            if getattr(self.decode_flash, "bits", 16) != bits:
+                raise ValueError("The decode attention was built for another KV cache type")
             return self.decode_flash
-        key = (batch, cache.capacity)
+        key = (batch, cache.capacity, bits)
         if key not in self._flash:
             cfg = self.cfg
-            self._flash[key] = FlashDecode(batch, cfg.num_key_value_heads,
-                                           cfg.num_attention_heads // cfg.num_key_value_heads,
-                                           cache.capacity, cache.k.device)
+            kind, more = (FlashDecode, {}) if bits == 16 else (QuantFlashDecode, dict(bits=bits))
+            self._flash[key] = kind(batch, cfg.num_key_value_heads, cfg.num_attention_heads // cfg.num_key_value_heads,
+                                    cache.capacity, cache.k.device, **more)
         return self._flash[key]
+
+    @staticmethod
+    def _layer_cache(cache, layer):
+        """The buffers of one cache layer as the decode attention takes them."""
+        return cache.layer(layer) if isinstance(cache, QuantKVCache) else (cache.k[layer], cache.v[layer])
 
     def attention(self, z, w, cache, layer, rope_positions, active, positions, slot):
         """Packed QKV projection, RoPE + KV store, attention, output projection
@@ -132,22 +141,29 @@ class Granite:
         hq, hkv = cfg.num_attention_heads, cfg.num_key_value_heads
         packed = isinstance(slot, PackedPrefill)
         slots = slot.slots if packed else None
+        # a quantised cache is written from the rotated rows, in a pass of its own
+        quant = isinstance(cache, QuantKVCache)
         if self.qkv_epilogue:
             qkv = linear_rope_kv(z, w["self_attn.qkv_proj"], hq, hkv, rope_positions, active, self.cos_sin,
-                                 cache, layer, slots)
+                                 None if quant else cache, layer, slots)
         else:
             qkv = linear_dense(z, w["self_attn.qkv_proj"])
         q = qkv[:, :hq * d].view(rows, hq, d)
         k = qkv[:, hq * d:(hq + hkv) * d].view(rows, hkv, d)
         v = qkv[:, (hq + hkv) * d:].view(rows, hkv, d)
         if not self.qkv_epilogue:
-            rope_kv_write(q, k, v, rope_positions, active, self.cos_sin, cache, layer, slots=slots,
-                          write_k=packed)
+            if quant:
+                rotary_embedding(rope_positions, q, k, d, self.cos_sin)
+            else:
+                rope_kv_write(q, k, v, rope_positions, active, self.cos_sin, cache, layer, slots=slots,
+                              write_k=packed)
+        if quant:
+            cache.write(layer, k.unsqueeze(2), v.unsqueeze(2), rope_positions, active, slots)
         if packed:
             a = varlen_attention(q, k, v, slot.cu, slot.maximum, cfg.attention_multiplier)
         else:
             flash = self._decode_attention(rows, cache)
-            a = flash(q.unsqueeze(2), cache.k[layer], cache.v[layer], positions, active,
+            a = flash(q.unsqueeze(2), *self._layer_cache(cache, layer), positions, active,
                       cfg.attention_multiplier, self.used)
         return linear_dense(a.reshape(rows, hq * d), w["self_attn.o_proj"])
 
@@ -181,7 +197,7 @@ class Granite:
             part = linear_splitk(z, w["self_attn.qkv_proj"], splits[0])
         flash = self._decode_attention(rows, cache)
         order = self._row_order if self._row_order is not None and self._row_order.shape[0] == rows else None
-        a = flash.fused_qkv(part, self.cos_sin, rope_positions, active, cache.k[layer], cache.v[layer],
+        a = flash.fused_qkv(part, self.cos_sin, rope_positions, active, *self._layer_cache(cache, layer),
                             cfg.attention_multiplier, self.used, cfg.num_attention_heads, row_order=order,
                             frag_out=True)
         return linear_splitk_frag(a, w["self_attn.o_proj"], splits[1])
@@ -414,6 +430,9 @@ class Granite:
             raise ValueError("Prompt width exceeds the KV capacity")
         for row, n in zip(rows, counts):  # cache.py:28-29 stores k * valid: zeros past the prompt
             if n < s:
+                if isinstance(cache, QuantKVCache):
+                    cache.clear(row, n, s)
+                    continue
                 cache.k[:, row, :, n:s].zero_()
                 cache.v[:, row, :, n:s].zero_()
         x = (F.embedding(tokens, self.w["embedding"]) * cfg.embedding_multiplier).reshape(b * s, cfg.hidden_size)
