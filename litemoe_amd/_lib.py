@@ -152,7 +152,21 @@ def ptr(t: torch.Tensor | None) -> int | None:
 
 
 def stream(device: torch.device | None = None) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    """The current stream of ``device`` (the current device's by default) as the
+    handle a C call takes, without a ``torch.cuda.Stream`` object around it (1.9 us
+    of a call's host time)."""
+    index = None if device is None else device.index
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
+
+
+def call_on(index: int, name: str, *args) -> None:
+    """:func:`call` with device ``index`` current and its current stream as the
+    last argument. Kernels run on the current device, so a call on another
+    device's tensors has to make it current; the usual call has nothing to change."""
+    if index == torch.cuda.current_device():
+        return call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+    with torch.cuda.device(index):
+        return call(name, *args, torch._C._cuda_getCurrentRawStream(index))
 
 
 def require_cuda(*tensors: torch.Tensor, what: str = "tensors") -> None:

@@ -123,9 +123,11 @@ class QuantKVCache:
         self.bits, self.capacity = k.shape[4] // 8, k.shape[3]
         self.keys = torch.arange(self.capacity, device=k.device)
         self.slots = torch.arange(k.shape[1], device=k.device)
+        self._layers = [QuantLayer(*buffers) for buffers in zip(k, v, scales)]  # views, made once
 
     def layer(self, layer):
-        return QuantLayer(self.k[layer], self.v[layer], self.scales[layer])
+        """Layer ``layer``'s buffers, views of ``k``, ``v`` and ``scales``."""
+        return self._layers[layer]
 
     def reset(self):
         for t in (self.k, self.v, self.scales):

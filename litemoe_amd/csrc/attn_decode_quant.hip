@@ -12,23 +12,32 @@
 // Stages pass through LDS: codes and scale words are copied there directly
 // (global_load_lds), kSlots stages deep, each wave its own, no barriers.
 //
-// Scores: K^T . q with v_mfma_f32_16x16x32_bf16, A the codes of 16 positions as
-// bf16 without their scales (exact), one product per block of 32 channels,
+// Scores: K . q with v_mfma_f32_16x16x128_f8f6f4, A the codes of two tiles of 16
+// positions as they lie in the cache, one product per block of 32 channels,
 //   s_j = sl2 * (2^e0 (c_j0 . q_0) + 2^e1 (c_j1 . q_1)).
+// The 128 products of an output are a block of both tiles, each twice: against q's
+// 8-bit leading part and against the rest (q 2^-e = hi + lo, e4m3 both, with max|q|
+// at 2^7: hi keeps 4 of bf16's 8 significant bits and lo the other 4, exactly for
+// channels down to 2^-9 of the head's largest and to within 2^-17 of that below).
+// No code is converted for the scores: 32 conversions less per stage than bf16
+// operands take, a sixth of the stage's instructions.
 // The G query heads of a KV head fill P = 4, 8 or 16 of the 16 columns; the
 // other columns take other positions: column c holds query head c % P of tile
-// c / P, which the product of that tile alone adds to (its B operand is zero in
-// the other columns), so one accumulator holds 16/P tiles and each lane four
-// scores, and no exponential is spent on an empty column (G = P).
+// c / P of a pass, and the B operand is zero where a tile is not its column's, so
+// one accumulator holds 16/P tiles and each lane four scores, and no exponential
+// is spent on an empty column (G = P).
 // Codes stay apart from scales so that a block that stands for NaN, stored with
 // codes 0, cannot reach another position's row or column through a product.
 //
-// P.V: V^T . p, A the transposed codes as bf16 (ds_read_b64_tr_b4 / _tr_b8
-// straight from the stage), B the probabilities times 2^e of V's block, rounded
-// to bf16 as the bf16 kernel rounds them. A lane's scores are four consecutive
-// positions of its column's tile, which is the order that B takes them in: no
-// lane moves. Each column keeps its own running maximum, shared by its four
-// lanes; they and the waves merge once, at the end.
+// P.V: V^T . p with v_mfma_f32_16x16x32_bf16, A the transposed codes as bf16
+// (ds_read_b64_tr_b4 / _tr_b8 straight from the stage), B the probabilities times
+// 2^e of V's block, rounded to bf16 as the bf16 kernel rounds them (8-bit parts
+// would lose the tail of a long row: 2^-18 of the largest probability, times its
+// length). A lane's scores are four consecutive positions of its column's tile,
+// which is the order that B takes them in; tiles 1 to 3 of a pass come to the
+// columns of tile 0 by row rotation, and only those columns of the result are
+// kept. A query head's columns share their running maximum; the waves merge once,
+// at the end.
 //
 // Reference semantics: litemoe/flash_decode.py:16-22; masking litemoe/cache.py:42-47.
 #include "internal.h"
@@ -59,12 +68,19 @@ struct Stage {
   static constexpr int kBytes = 2 * kSide + 4 * kStageKeys;  // then the scale words
   static constexpr int kSideCopies = kSide / 1024;
   static constexpr int kCopies = 2 * kSideCopies + 1;     // vector memory operations of a wave
-  static constexpr int kSlots = kBits == 4 ? 3 : 2;
+  static constexpr int kSlots = 2;
 };
 
-// Four bytes per lane to LDS (see lds_copy16).
-__device__ __forceinline__ void lds_copy4(const void *base, uint32_t voff, uint32_t lds) {
-  asm volatile("global_load_lds_dword %0, %1" ::"v"(voff), "s"(base), "{m0}"(lds) : "memory");
+// Direct global -> LDS copies (see lds_copy16) of 16 and 4 bytes per lane; kOffset
+// moves both addresses. Non-temporal: every byte is read once per step by one
+// workgroup, and the whole cache streams through between two reads of it.
+template <int kOffset>
+__device__ __forceinline__ void stage_copy16(const void *base, uint32_t voff, uint32_t lds) {
+  asm volatile("global_load_lds_dwordx4 %0, %1 offset:%2 nt" ::"v"(voff), "s"(base), "n"(kOffset), "{m0}"(lds)
+               : "memory");
+}
+__device__ __forceinline__ void stage_copy4(const void *base, uint32_t voff, uint32_t lds) {
+  asm volatile("global_load_lds_dword %0, %1 nt" ::"v"(voff), "s"(base), "{m0}"(lds) : "memory");
 }
 // vm_wait that LDS reads are not moved across.
 template <int N>
@@ -74,27 +90,56 @@ __device__ __forceinline__ void copies_wait() {
 // Every LDS access of this wave is done: its bytes may be copied over.
 __device__ __forceinline__ void lds_reads_done() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
-__device__ __forceinline__ float merge_factor(float m, float mnew) {
-  return m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mnew);
+// The value of the lane N places further in its row of 16, round the end (row_ror by 16 - N).
+template <int N>
+__device__ __forceinline__ uint32_t row_from(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x120 + 16 - N, 0xF, 0xF, false);
+}
+template <int N>
+__device__ __forceinline__ float row_from(float v) {
+  return __uint_as_float(row_from<N>(__float_as_uint(v)));
 }
 
-// The lane N places further in its row of 16 (row_ror).
-template <int N>
-__device__ __forceinline__ float row_rotate(float v) {
-  return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x120 + N, 0xF, 0xF, false));
+// Scale byte kByte of a position's word as a float (quant_scale), in one instruction.
+template <int kByte>
+__device__ __forceinline__ float scale_of(uint32_t word) {
+  float r;
+  const uint32_t by = 23;
+#define LM_SCALE(sel)                                                                             \
+  asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:" sel \
+      : "=v"(r)                                                                                   \
+      : "v"(by), "v"(word))
+  if constexpr (kByte == 0) LM_SCALE("BYTE_0");
+  if constexpr (kByte == 1) LM_SCALE("BYTE_1");
+  if constexpr (kByte == 2) LM_SCALE("BYTE_2");
+  if constexpr (kByte == 3) LM_SCALE("BYTE_3");
+#undef LM_SCALE
+  return r;
+}
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+// MFMA 16x16x128, A codes of kBits and B e4m3, no scales. k runs over four groups
+// of 32. A of 4 bits: lane l holds row l%16, group l/16, in its first four words.
+// 8-bit operands: lane l holds, of row or column l%16, the 16 bytes k = 16 (l/16) and
+// on in words 0-3 and the 16 bytes k = 64 + 16 (l/16) and on in words 4-7 (checked on
+// the device). C as mfma16x16x32.
+template <int kBits>
+__device__ __forceinline__ f32x4 mfma_codes(const i32x8 &a, const i32x8 &b, f32x4 c) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, kBits == 4 ? 4 : 0, 0, 0, 0, 0, 0);
 }
 
 // Reductions over the tiles of a query head: columns c % P equal, one row of 16 lanes.
 template <int P>
 __device__ __forceinline__ float tiles_max(float v) {
-  if constexpr (P <= 8) v = fmaxf(v, row_rotate<8>(v));
-  if constexpr (P <= 4) v = fmaxf(v, row_rotate<4>(v));
+  if constexpr (P <= 8) v = fmaxf(v, row_from<8>(v));
+  if constexpr (P <= 4) v = fmaxf(v, row_from<4>(v));
   return v;
 }
 template <int P>
 __device__ __forceinline__ float tiles_sum(float v) {
-  if constexpr (P <= 8) v += row_rotate<8>(v);
-  if constexpr (P <= 4) v += row_rotate<4>(v);
+  if constexpr (P <= 8) v += row_from<8>(v);
+  if constexpr (P <= 4) v += row_from<4>(v);
   return v;
 }
 
@@ -176,24 +221,43 @@ decode_quant_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, Cache 
   uint8_t *const my_stages = smem + wave * St::kSlots * St::kBytes;
   const uint32_t my_lds = __builtin_amdgcn_readfirstlane(lds_address(my_stages));
 
-  // Requests stage `it` into its slot. Positions past the range repeat its last
-  // one (they are masked); offsets within a stage are below 4 KB, the stage's own
-  // start is a 64-bit scalar.
+  // Requests stage `it` into its slot, its start a 64-bit scalar. Positions past the
+  // range repeat its last one (they are masked).
   auto issue = [&](int it, int slot) {
     const int start = k0 + (it * kWaves + wave) * kStageKeys;
     const int last = k1 - 1 - start;
     const int64_t at = first_pos + start;
     const uint32_t lds = my_lds + slot * St::kBytes;
+    const uint8_t *kg = cache.k + at * St::kCode, *vg = cache.v + at * St::kCode;
+    if (last >= kStageKeys - 1) {
+      stage_copy16<0>(kg, lane * 16, lds);
+      stage_copy16<1024>(kg, lane * 16, lds);
+      if constexpr (kBits == 8) {
+        stage_copy16<2048>(kg, lane * 16, lds);
+        stage_copy16<3072>(kg, lane * 16, lds);
+      }
+      stage_copy16<0>(vg, lane * 16, lds + St::kSide);
+      stage_copy16<1024>(vg, lane * 16, lds + St::kSide);
+      if constexpr (kBits == 8) {
+        stage_copy16<2048>(vg, lane * 16, lds + St::kSide);
+        stage_copy16<3072>(vg, lane * 16, lds + St::kSide);
+      }
+      stage_copy4(cache.scales + at, lane * 4, lds + 2 * St::kSide);
+      return;
+    }
 #pragma unroll
     for (int c = 0; c < St::kSideCopies; ++c) {
       constexpr int kChunks = St::kCode / 16;  // 16-byte chunks of one position
       const int chunk16 = c * kWave + lane;
       const uint32_t off = (uint32_t)min(chunk16 / kChunks, last) * St::kCode + (chunk16 % kChunks) * 16;
-      lds_copy16(cache.k + at * St::kCode, off, lds + c * 1024);
-      lds_copy16(cache.v + at * St::kCode, off, lds + St::kSide + c * 1024);
+      stage_copy16<0>(kg, off, lds + c * 1024);
+      stage_copy16<0>(vg, off, lds + St::kSide + c * 1024);
     }
-    lds_copy4(cache.scales + at, (uint32_t)min(lane, last) * 4, lds + 2 * St::kSide);
+    stage_copy4(cache.scales + at, (uint32_t)min(lane, last) * 4, lds + 2 * St::kSide);
   };
+#pragma unroll
+  for (int s = 0; s < St::kSlots - 1; ++s)
+    if (s < niter) issue(s, s);
 
   if constexpr (kFused) {
     // The row's q|k|v slices of the packed projection, summed over the K slices
@@ -215,11 +279,9 @@ decode_quant_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, Cache 
       for (int i = 0; i < 4; ++i) sm_qkv[hs][c4 + i] = round_bf16(acc[i]);
     }
   }
-#pragma unroll
-  for (int s = 0; s < St::kSlots - 1; ++s)
-    if (s < niter) issue(s, s);
 
-  u32x4 qv[2];
+  // Channels 32 bl + 16 (grp % 2) and on, sixteen of each block, of the column's head.
+  u32x4 qw[2][2];
   if constexpr (kFused) {
     __syncthreads();
     const bool in_table = pnew >= 0 && pnew < in.table_len;
@@ -253,24 +315,67 @@ decode_quant_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, Cache 
     __syncthreads();
 #pragma unroll
     for (int bl = 0; bl < 2; ++bl)
-      qv[bl] = *reinterpret_cast<const u32x4 *>(&sm_rot[min(head, G)][32 * bl + 8 * grp]);
-  } else {
-    const bf16 *qp = q + b * qs0 + (int64_t)(h * G + min(head, G - 1)) * qs1 + 8 * grp;
-    qv[0] = *reinterpret_cast<const u32x4 *>(qp);
-    qv[1] = *reinterpret_cast<const u32x4 *>(qp + 32);
-  }
-  // B operands of the scores: tile t's are zero outside its columns.
-  u32x4 qt[kTiles][2];
 #pragma unroll
-  for (int t = 0; t < kTiles; ++t)
+      for (int i = 0; i < 2; ++i)
+        qw[bl][i] = *reinterpret_cast<const u32x4 *>(&sm_rot[min(head, G)][32 * bl + 16 * (grp % 2) + 8 * i]);
+  } else {
+    const bf16 *qp = q + b * qs0 + (int64_t)(h * G + min(head, G - 1)) * qs1 + 16 * (grp % 2);
 #pragma unroll
     for (int bl = 0; bl < 2; ++bl)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) qt[t][bl][i] = tile == t && head < G ? qv[bl][i] : 0u;
+      for (int i = 0; i < 2; ++i) qw[bl][i] = *reinterpret_cast<const u32x4 *>(qp + 32 * bl + 8 * i);
+  }
+  // q's two e4m3 parts, lanes of groups 0 and 1 the leading one: 2^(134 - E) q, E the
+  // exponent field of the head's largest (at least 8, so that both powers are normal).
+  float qx[2][16];
+  uint32_t qmax = 0;
+#pragma unroll
+  for (int bl = 0; bl < 2; ++bl)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) unpack8(qw[bl][i], &qx[bl][8 * i]);
+#pragma unroll
+  for (int bl = 0; bl < 2; ++bl)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) qmax = max(qmax, __float_as_uint(qx[bl][i]) & 0x7fffffffu);
+  qmax = max(qmax, __float_as_uint(xor_lanes<16>(__uint_as_float(qmax))));
+  const uint32_t qe = max(qmax >> 23, 8u);
+  const float q_up = __uint_as_float((261u - qe) << 23);
+  uint32_t qpart[2][4];
+#pragma unroll
+  for (int bl = 0; bl < 2; ++bl)
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      uint32_t r[2] = {0u, 0u};
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        typedef short s16x2 __attribute__((ext_vector_type(2)));
+        const float x0 = qx[bl][4 * w + 2 * half] * q_up, x1 = qx[bl][4 * w + 2 * half + 1] * q_up;
+        s16x2 hi = (s16x2){0, 0}, lo = hi;
+        hi = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(hi, x0, x1, 1.f, false);
+        const f32x2 back =
+            __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(__builtin_bit_cast(uint32_t, hi), 1.f, false);
+        lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lo, x0 - back[0], x1 - back[1], 1.f, false);
+        r[half] = __builtin_bit_cast(uint32_t, grp < 2 ? hi : lo) & 0xffffu;
+      }
+      qpart[bl][w] = head < G ? r[0] | r[1] << 16 : 0u;
+    }
+  // B operands of the scores. Words 0-3 meet the first tile of a pair, words 4-7 the
+  // second; variant 0 is pair 0's (P = 4), any pair's (P = 8) or the first tile's (P = 16).
+  constexpr int kVariants = P == 8 ? 1 : 2;
+  i32x8 qb[kVariants][2];
+#pragma unroll
+  for (int v = 0; v < kVariants; ++v)
+#pragma unroll
+    for (int bl = 0; bl < 2; ++bl)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const bool mine = P == 16 ? v == i / 4 : tile == 2 * v + i / 4;
+        qb[v][bl][i] = mine ? (int)qpart[bl][i % 4] : 0;
+      }
 
-  const float sl2 = scale * 1.4426950408889634f;
+  const float sl2 = scale * 1.4426950408889634f * __uint_as_float((qe - 7u) << 23);
   float m = kEmpty, l = 0.f;
-  f32x4 acc[4];  // channels 16 mm + 4 grp + i of column col
+  f32x4 acc[4];  // channels 16 mm + 4 grp + i of column col, of use where tile is 0
 #pragma unroll
   for (int mm = 0; mm < 4; ++mm) acc[mm] = f32x4{0.f, 0.f, 0.f, 0.f};
 
@@ -291,32 +396,53 @@ decode_quant_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, Cache 
         lds_reads_done();
       }
     }
+    f32x4 c[kPasses][2];
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p) c[p][0] = c[p][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int pr = 0; pr < 2; ++pr)
+#pragma unroll
+      for (int bl = 0; bl < 2; ++bl) {
+        i32x8 a;
+        if constexpr (kBits == 4) {
+          // lane (col, grp): the block of position col of tile 2 pr + grp / 2
+          const u32x4 w = *reinterpret_cast<const u32x4 *>(st + (32 * pr + 16 * (grp / 2) + col) * St::kCode + 16 * bl);
+          a = i32x8{(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
+        } else {
+          // lane (col, grp): sixteen channels of position col of tiles 2 pr and 2 pr + 1
+          const uint8_t *kp = st + (32 * pr + col) * St::kCode + 32 * bl + 16 * (grp % 2);
+          const u32x4 w0 = *reinterpret_cast<const u32x4 *>(kp);
+          const u32x4 w1 = *reinterpret_cast<const u32x4 *>(kp + 16 * St::kCode);
+          a = i32x8{(int)w0[0], (int)w0[1], (int)w0[2], (int)w0[3], (int)w1[0], (int)w1[1], (int)w1[2], (int)w1[3]};
+        }
+        if constexpr (P == 4) {
+          c[0][bl] = mfma_codes<kBits>(a, qb[pr][bl], c[0][bl]);
+        } else if constexpr (P == 8) {
+          c[pr][bl] = mfma_codes<kBits>(a, qb[0][bl], c[pr][bl]);
+        } else {
+          c[2 * pr][bl] = mfma_codes<kBits>(a, qb[0][bl], c[2 * pr][bl]);
+          c[2 * pr + 1][bl] = mfma_codes<kBits>(a, qb[kVariants - 1][bl], c[2 * pr + 1][bl]);
+        }
+      }
     float s[kPasses][4];
     u32x4 words[kPasses];  // scale words of the lane's four positions of each pass
 #pragma unroll
     for (int p = 0; p < kPasses; ++p) {
-      f32x4 c0 = {0.f, 0.f, 0.f, 0.f}, c1 = c0;
+      words[p] = *reinterpret_cast<const u32x4 *>(st + 2 * St::kSide + 4 * ((p * kTiles + tile) * 16 + 4 * grp));
 #pragma unroll
-      for (int t = 0; t < kTiles; ++t) {
-        const uint8_t *kp = st + ((p * kTiles + t) * 16 + col) * St::kCode + grp * kBits;
-        const Codes8<kBits> a0 = *reinterpret_cast<const Codes8<kBits> *>(kp);
-        const Codes8<kBits> a1 = *reinterpret_cast<const Codes8<kBits> *>(kp + St::kCode / 2);
-        c0 = mfma16x16x32(codes_to_bf16<kBits>(a0.w), qt[t][0], c0);
-        c1 = mfma16x16x32(codes_to_bf16<kBits>(a1.w), qt[t][1], c1);
-      }
-      const int first = (p * kTiles + tile) * 16 + 4 * grp;  // the lane's first position
-      words[p] = *reinterpret_cast<const u32x4 *>(st + 2 * St::kSide + 4 * first);
-      if (count < kStageKeys) {
-        // Masked positions: whatever their bytes hold, scale 0 and score -inf.
+      for (int i = 0; i < 4; ++i)
+        s[p][i] = (c[p][0][i] * scale_of<0>(words[p][i]) + c[p][1][i] * scale_of<1>(words[p][i])) * sl2;
+    }
+    if (count < kStageKeys) {
+      // Masked positions: whatever their bytes hold, score -inf and V's scales 0.
 #pragma unroll
-        for (int i = 0; i < 4; ++i) words[p][i] = first + i < count ? words[p][i] : 0u;
-      }
+      for (int p = 0; p < kPasses; ++p)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float x = c0[i] * quant_scale(words[p][i], 0) + c1[i] * quant_scale(words[p][i], 1);
-        s[p][i] = x * sl2;
-        if (count < kStageKeys) s[p][i] = first + i < count ? s[p][i] : -INFINITY;
-      }
+        for (int i = 0; i < 4; ++i) {
+          const bool ok = (p * kTiles + tile) * 16 + 4 * grp + i < count;
+          words[p][i] = ok ? words[p][i] : 0u;
+          s[p][i] = ok ? s[p][i] : -INFINITY;
+        }
     }
     float mx = m;
 #pragma unroll
@@ -325,9 +451,9 @@ decode_quant_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, Cache 
       for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[p][i]);
     if (__any(mx > m + kLazy)) {
       mx = fmaxf(mx, xor_lanes<16>(mx));
-      mx = fmaxf(mx, xor_lanes<32>(mx));
+      mx = tiles_max<P>(fmaxf(mx, xor_lanes<32>(mx)));
       const bool up = mx > m + kLazy;
-      const float f = up ? merge_factor(m, mx) : 1.f;
+      const float f = up ? __builtin_amdgcn_exp2f(m - mx) : 1.f;
       m = up ? mx : m;
       l *= f;
 #pragma unroll
@@ -344,26 +470,35 @@ decode_quant_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, Cache 
         l += e[i];
       }
 #pragma unroll
-      for (int bl = 0; bl < 2; ++bl)
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          pb[bl][p][i] = pack_bf16_finite(e[2 * i] * quant_scale(words[p][2 * i], 2 + bl),
-                                          e[2 * i + 1] * quant_scale(words[p][2 * i + 1], 2 + bl));
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t w0 = words[p][2 * i], w1 = words[p][2 * i + 1];
+        pb[0][p][i] = pack_bf16_finite(e[2 * i] * scale_of<2>(w0), e[2 * i + 1] * scale_of<2>(w1));
+        pb[1][p][i] = pack_bf16_finite(e[2 * i] * scale_of<3>(w0), e[2 * i + 1] * scale_of<3>(w1));
+      }
     }
-    // B operands of tiles 2 pr and 2 pr + 1: eight positions per lane, zero in
-    // the columns of other tiles.
+    // B operands of tiles 2 pr and 2 pr + 1: a pass's first tile from the column's own
+    // lanes, the others from the columns that hold them.
     u32x4 bp[2][2];
 #pragma unroll
-    for (int pr = 0; pr < 2; ++pr)
+    for (int bl = 0; bl < 2; ++bl)
 #pragma unroll
-      for (int bl = 0; bl < 2; ++bl)
+      for (int i = 0; i < 2; ++i) {
+        if constexpr (P == 4) {
+          bp[0][bl][i] = pb[bl][0][i];
+          bp[0][bl][2 + i] = row_from<4>(pb[bl][0][i]);
+          bp[1][bl][i] = row_from<8>(pb[bl][0][i]);
+          bp[1][bl][2 + i] = row_from<12>(pb[bl][0][i]);
+        } else if constexpr (P == 8) {
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int t = 2 * pr + half, p = t / kTiles;
+          for (int pr = 0; pr < 2; ++pr) {
+            bp[pr][bl][i] = pb[bl][pr][i];
+            bp[pr][bl][2 + i] = row_from<8>(pb[bl][pr][i]);
+          }
+        } else {
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
-            bp[pr][bl][2 * half + i] = kTiles == 1 || tile == t % kTiles ? pb[bl][p][i] : 0u;
+          for (int t = 0; t < 4; ++t) bp[t / 2][bl][2 * (t % 2) + i] = pb[bl][t][i];
         }
+      }
     typedef int i32x2 __attribute__((ext_vector_type(2)));
     typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
     const uint8_t *vs = st + St::kSide;
@@ -413,16 +548,11 @@ decode_quant_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, Cache 
     slot = slot + 1 == St::kSlots ? 0 : slot + 1;
   }
 
-  // Merge the four lanes of a column (their l), the columns of a query head, then the waves.
+  // A query head's sum of probabilities: over the four lanes of its columns and the
+  // columns of its tiles. The maximum and the accumulators are whole already.
   l += xor_lanes<16>(l);
   l += xor_lanes<32>(l);
-  const float mall = tiles_max<P>(m);
-  const float f = __builtin_amdgcn_exp2f(m - mall);
-  l = tiles_sum<P>(l * f);
-#pragma unroll
-  for (int mm = 0; mm < 4; ++mm)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) acc[mm][i] = tiles_sum<P>(acc[mm][i] * f);
+  l = tiles_sum<P>(l);
   __syncthreads();  // every wave is done with its stages
   float(*sm_o)[P][kD] = reinterpret_cast<float(*)[P][kD]>(smem);
   float(*sm_m)[P] = reinterpret_cast<float(*)[P]>(smem + kWaves * P * kD * 4);
@@ -431,7 +561,7 @@ decode_quant_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, Cache 
 #pragma unroll
     for (int mm = 0; mm < 4; ++mm) *reinterpret_cast<f32x4 *>(&sm_o[wave][head][16 * mm + 4 * grp]) = acc[mm];
     if (grp == 0) {
-      sm_m[wave][head] = mall;
+      sm_m[wave][head] = m;
       sm_l[wave][head] = l;
     }
   }

@@ -161,21 +161,18 @@ class QuantFlashDecode:
                           if ordered and self.device.type == "cuda" else None)
 
     def _check(self, k, v, scales, q_heads, rows):
-        if kv_quant.check_layer(k, v, scales) != self.bits:
+        """The layer's device index, once it is what this object was built for."""
+        bits, index = kv_quant.check_layer(k, v, scales)
+        batch, heads, capacity, _ = k.shape
+        if bits != self.bits:
             raise ValueError("Decode attention built for another cache type")
-        if rows > self.batch or k.shape[0] < rows or k.shape[2] != self.capacity or k.shape[1] != self.kv_heads:
+        if rows > self.batch or batch < rows or capacity != self.capacity or heads != self.kv_heads:
             raise ValueError("Decode attention built for another batch/capacity")
-        if q_heads != self.kv_heads * self.groups:
+        if q_heads != heads * self.groups:
             raise ValueError("Query heads do not match the cache heads")
-        if self.workspace.device != k.device:
+        if self.workspace.get_device() != index:
             raise ValueError("Decode attention built for another device")
-
-    @staticmethod
-    def _rows(t, rows, dtype, device, what):
-        t = t if t.dtype == dtype else t.to(dtype)
-        if t.shape != (rows,) or t.device != device:
-            raise ValueError(f"{what} needs one entry per row, on the cache's device")
-        return t.contiguous()
+        return index
 
     def __call__(self, q, k, v, scales, lengths, active, scale, used=None):
         """Attention of ``q [B, Hq, 1, 64]`` over the first ``used[b]`` positions
@@ -184,22 +181,21 @@ class QuantFlashDecode:
         b, hq, s, d = q.shape
         if s != 1 or d != 64:
             raise ValueError("Decode attention takes one query position with head_dim 64")
-        self._check(k, v, scales, hq, b)
+        index = self._check(k, v, scales, hq, b)
         if q.dtype != torch.bfloat16:
             raise ValueError("Decode attention supports BF16")
-        if q.device != k.device:
+        if q.get_device() != index:
             raise ValueError("Queries and cache must be on one device")
-        if q.stride(3) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
+        rows, heads, _, channels = q.stride()
+        if channels != 1 or rows % 8 or heads % 8 or q.data_ptr() % 16:
             raise ValueError("Decode attention needs contiguous channels and 16-byte aligned query heads")
         if used is None:
             used = torch.where(active, lengths + 1, 1)
-        used = self._rows(used, b, torch.int32, k.device, "used")
-        out = torch.empty(b, hq, 1, d, device=q.device, dtype=q.dtype)
-        with torch.cuda.device(k.device):
-            _lib.call("lm_flash_decode_quant", q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), v.data_ptr(),
-                      scales.data_ptr(), used.data_ptr(), b, hq, self.kv_heads, self.capacity, d, self.bits,
-                      float(scale), self.maximum, self.splits, out.data_ptr(), self.workspace.data_ptr(),
-                      self.workspace.numel(), _lib.stream(k.device))
+        used = kv_quant.per_row(used, b, torch.int32, index, "used")
+        out = torch.empty((b, hq, 1, 64), device=q.device, dtype=torch.bfloat16)
+        _lib.call_on(index, "lm_flash_decode_quant", q.data_ptr(), rows, heads, k.data_ptr(), v.data_ptr(),
+                     scales.data_ptr(), used.data_ptr(), b, hq, self.kv_heads, self.capacity, 64, self.bits, scale,
+                     self.maximum, self.splits, out.data_ptr(), self.workspace.data_ptr(), self.workspace.numel())
         return out
 
     def fused_qkv(self, partials, cos_sin, positions, active, k, v, scales, scale, used, q_heads, row_order=None,
@@ -207,31 +203,30 @@ class QuantFlashDecode:
         """:meth:`FlashDecode.fused_qkv`, the new token's key and value quantised
         into the layer's buffers and attended as they stand there."""
         splits, b, ncols = partials.shape
-        self._check(k, v, scales, q_heads, b)
-        device = k.device
+        index = self._check(k, v, scales, q_heads, b)
         if ncols != (q_heads + 2 * self.kv_heads) * 64:
             raise ValueError("QKV partials do not match the cache heads")
-        if partials.dtype != torch.float32 or not partials.is_contiguous() or partials.device != device:
+        if partials.dtype != torch.float32 or not partials.is_contiguous() or partials.get_device() != index:
             raise ValueError("QKV partials must be contiguous fp32 on the cache's device")
-        if (cos_sin.dtype != torch.bfloat16 or cos_sin.dim() != 2 or cos_sin.shape[1] != 64
-                or not cos_sin.is_contiguous() or cos_sin.device != device):
+        table = cos_sin.shape
+        if (cos_sin.dtype != torch.bfloat16 or len(table) != 2 or table[1] != 64 or not cos_sin.is_contiguous()
+                or cos_sin.get_device() != index):
             raise ValueError("Decode attention needs a contiguous BF16 [table_len, 64] cos/sin table")
-        positions = self._rows(positions, b, torch.int64, device, "positions")
-        used = self._rows(used, b, torch.int32, device, "used")
-        active = None if active is None else self._rows(active, b, torch.bool, device, "active")
+        positions = kv_quant.per_row(positions, b, torch.int64, index, "positions")
+        used = kv_quant.per_row(used, b, torch.int32, index, "used")
+        active = None if active is None else kv_quant.per_row(active, b, torch.bool, index, "active")
         if row_order is not None and (row_order.dtype != torch.int32 or row_order.shape != (b,)
-                                      or row_order.device != device or not row_order.is_contiguous()):
+                                      or row_order.get_device() != index or not row_order.is_contiguous()):
             raise ValueError("row_order must be an int32 [B] permutation")
         if frag_out:
-            out = FragRows(b, q_heads * 64, device)
+            out = FragRows(b, q_heads * 64, k.device)
             out_ptr = out.data.data_ptr()
         else:
-            out = torch.empty(b, q_heads, 1, 64, device=device, dtype=torch.bfloat16)
+            out = torch.empty((b, q_heads, 1, 64), device=k.device, dtype=torch.bfloat16)
             out_ptr = out.data_ptr()
-        with torch.cuda.device(device):
-            _lib.call("lm_flash_decode_quant_qkv", partials.data_ptr(), splits, cos_sin.data_ptr(), cos_sin.shape[0],
-                      positions.data_ptr(), _lib.ptr(active), k.data_ptr(), v.data_ptr(), scales.data_ptr(),
-                      used.data_ptr(), _lib.ptr(row_order), b, q_heads, self.kv_heads, self.capacity, 64, self.bits,
-                      float(scale), self.maximum, self.splits, int(bool(frag_out)), out_ptr,
-                      self.workspace.data_ptr(), self.workspace.numel(), _lib.stream(device))
+        _lib.call_on(index, "lm_flash_decode_quant_qkv", partials.data_ptr(), splits, cos_sin.data_ptr(), table[0],
+                     positions.data_ptr(), _lib.ptr(active), k.data_ptr(), v.data_ptr(), scales.data_ptr(),
+                     used.data_ptr(), _lib.ptr(row_order), b, q_heads, self.kv_heads, self.capacity, 64, self.bits,
+                     scale, self.maximum, self.splits, int(frag_out), out_ptr, self.workspace.data_ptr(),
+                     self.workspace.numel())
         return out

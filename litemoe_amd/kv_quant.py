@@ -16,23 +16,27 @@ BITS = (4, 8)
 
 
 def check_layer(k, v, scales):
-    """Bits of one layer's buffers ``k, v [B, H, C, 8*bits]``, ``scales [B, H, C, 4]``."""
-    _lib.require_cuda(k, v, scales, what="quantised KV cache")
-    bits = k.shape[-1] // 8
-    if k.dim() != 4 or bits not in BITS or k.shape[-1] % 8 or v.shape != k.shape or scales.shape != (*k.shape[:3], 4):
-        raise ValueError("Quantised KV cache layers are k, v [B, H, C, 8*bits] and scales [B, H, C, 4], bits 4 or 8")
-    if any(t.dtype != torch.uint8 or not t.is_contiguous() for t in (k, v, scales)):
-        raise ValueError("Quantised KV cache layers must be contiguous uint8")
-    if v.device != k.device or scales.device != k.device:
+    """``(bits, device index)`` of one layer's buffers ``k, v [B, H, C, 8*bits]``,
+    ``scales [B, H, C, 4]``."""
+    index, shape = k.get_device(), k.shape
+    if index < 0 or v.get_device() != index or scales.get_device() != index:
+        _lib.require_cuda(k, v, scales, what="quantised KV cache")
         raise ValueError("Quantised KV cache layers must share one device")
-    return bits
+    if len(shape) != 4 or shape[3] not in (32, 64) or v.shape != shape or scales.shape != (*shape[:3], 4):
+        raise ValueError("Quantised KV cache layers are k, v [B, H, C, 8*bits] and scales [B, H, C, 4], bits 4 or 8")
+    for t in (k, v, scales):
+        if t.dtype != torch.uint8 or not t.is_contiguous():
+            raise ValueError("Quantised KV cache layers must be contiguous uint8")
+    return shape[3] // 8, index
 
 
-def _index(t, rows, dtype, device, what):
-    t = t if t.dtype == dtype else t.to(dtype)
-    if t.numel() != rows or t.device != device:
+def per_row(t, rows, dtype, index, what):
+    """``t [rows]`` on device ``index`` as a contiguous tensor of ``dtype``."""
+    if t.get_device() != index or t.shape != (rows,):
         raise ValueError(f"{what} needs one entry per row, on the cache's device")
-    return t.contiguous()
+    if t.dtype != dtype:
+        t = t.to(dtype)
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def write(cache, layer, k, v, positions, active, slots):
@@ -41,23 +45,23 @@ def write(cache, layer, k, v, positions, active, slots):
     stores them. ``k, v [rows, H, 1, 64]`` bf16 with any strides; ``active`` may
     be None (every row). Rows out of range are skipped. One row per target."""
     kc, vc, scales = cache.layer(layer)
-    bits = check_layer(kc, vc, scales)
-    if k.dim() != 4 or k.shape != v.shape or k.shape[1] != kc.shape[1] or k.shape[2] != 1 or k.shape[3] != 64:
+    bits, index = check_layer(kc, vc, scales)
+    batch, heads, capacity, _ = kc.shape
+    shape = k.shape
+    if len(shape) != 4 or shape[1:] != (heads, 1, 64) or v.shape != shape:
         raise ValueError("KV write takes k, v [rows, H, 1, 64] of the cache's heads")
-    _lib.require_cuda(k, v, what="KV write tensors")
     if k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
         raise ValueError("The quantised KV write supports BF16")
-    device, rows = kc.device, k.shape[0]
-    if k.device != device or v.device != device:
+    if k.get_device() != index or v.get_device() != index:
         raise ValueError("KV write tensors must be on the cache's device")
-    positions = _index(positions, rows, torch.int64, device, "positions")
-    slots = _index(slots, rows, torch.int64, device, "slots")
-    active = None if active is None else _index(active, rows, torch.bool, device, "active")
-    with torch.cuda.device(device):
-        _lib.call("lm_kv_quant_write", k.data_ptr(), k.stride(0), k.stride(1), k.stride(3), v.data_ptr(),
-                  v.stride(0), v.stride(1), v.stride(3), kc.data_ptr(), vc.data_ptr(), scales.data_ptr(),
-                  positions.data_ptr(), _lib.ptr(active), slots.data_ptr(), rows, kc.shape[1], 64, kc.shape[2],
-                  kc.shape[0], bits, _lib.stream(device))
+    rows = shape[0]
+    positions = per_row(positions, rows, torch.int64, index, "positions")
+    slots = per_row(slots, rows, torch.int64, index, "slots")
+    active = None if active is None else per_row(active, rows, torch.bool, index, "active")
+    ks, vs = k.stride(), v.stride()
+    _lib.call_on(index, "lm_kv_quant_write", k.data_ptr(), ks[0], ks[1], ks[3], v.data_ptr(), vs[0], vs[1], vs[3],
+                 kc.data_ptr(), vc.data_ptr(), scales.data_ptr(), positions.data_ptr(), _lib.ptr(active),
+                 slots.data_ptr(), rows, heads, 64, capacity, batch, bits)
 
 
 def read(cache, layer, positions, slots):
@@ -65,13 +69,13 @@ def read(cache, layer, positions, slots):
     ``k, v [rows, H, 1, 64]`` bf16, the layout :func:`write` takes. Rows out of
     range give zeros."""
     kc, vc, scales = cache.layer(layer)
-    bits = check_layer(kc, vc, scales)
-    device, rows = kc.device, positions.numel()
-    positions = _index(positions, rows, torch.int64, device, "positions")
-    slots = _index(slots, rows, torch.int64, device, "slots")
-    k, v = torch.empty(2, rows, kc.shape[1], 1, 64, dtype=torch.bfloat16, device=device)
-    with torch.cuda.device(device):
-        _lib.call("lm_kv_quant_read", kc.data_ptr(), vc.data_ptr(), scales.data_ptr(), positions.data_ptr(),
-                  slots.data_ptr(), rows, kc.shape[1], 64, kc.shape[2], kc.shape[0], bits, k.data_ptr(),
-                  v.data_ptr(), _lib.stream(device))
+    bits, index = check_layer(kc, vc, scales)
+    batch, heads, capacity, _ = kc.shape
+    rows = positions.numel()
+    positions = per_row(positions, rows, torch.int64, index, "positions")
+    slots = per_row(slots, rows, torch.int64, index, "slots")
+    k = torch.empty((rows, heads, 1, 64), dtype=torch.bfloat16, device=kc.device)
+    v = torch.empty_like(k)
+    _lib.call_on(index, "lm_kv_quant_read", kc.data_ptr(), vc.data_ptr(), scales.data_ptr(), positions.data_ptr(),
+                 slots.data_ptr(), rows, heads, 64, capacity, batch, bits, k.data_ptr(), v.data_ptr())
     return k, v
