@@ -10,7 +10,7 @@
 // Workgroup (split, kv head, row), four waves; a wave takes 64 consecutive
 // positions (a stage) at a time, every fourth stage of the workgroup's range.
 // Stages pass through LDS: codes and scale words are copied there directly
-// (global_load_lds), kSlots stages deep, each wave its own, no barriers.
+// (global_load_lds), the next stage while one is computed, each wave its own, no barriers.
 //
 // Scores: K . q with v_mfma_f32_16x16x128_f8f6f4, A the codes of two tiles of 16
 // positions as they lie in the cache, one product per block of 32 channels,
@@ -67,9 +67,11 @@ struct Stage {
   static constexpr int kSide = kStageKeys * kCode;        // K codes, then V codes
   static constexpr int kBytes = 2 * kSide + 4 * kStageKeys;  // then the scale words
   static constexpr int kSideCopies = kSide / 1024;
-  static constexpr int kCopies = 2 * kSideCopies + 1;     // vector memory operations of a wave
-  static constexpr int kSlots = 2;
 };
+// Stages of a wave in LDS: one computed, one on its way. Three (4 bits) keep a wave's
+// loads in flight better, but four workgroups of two fit a CU: 128 ragged rows to
+// 4095 positions 36.2 us with three, 34.0 with two; 64 rows to 1279 the same.
+constexpr int kSlots = 2;
 
 // Direct global -> LDS copies (see lds_copy16) of 16 and 4 bytes per lane; kOffset
 // moves both addresses. Non-temporal: every byte is read once per step by one
@@ -82,11 +84,8 @@ __device__ __forceinline__ void stage_copy16(const void *base, uint32_t voff, ui
 __device__ __forceinline__ void stage_copy4(const void *base, uint32_t voff, uint32_t lds) {
   asm volatile("global_load_lds_dword %0, %1 nt" ::"v"(voff), "s"(base), "{m0}"(lds) : "memory");
 }
-// vm_wait that LDS reads are not moved across.
-template <int N>
-__device__ __forceinline__ void copies_wait() {
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
-}
+// Every copy of this wave has arrived; LDS reads are not moved across.
+__device__ __forceinline__ void copies_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 // Every LDS access of this wave is done: its bytes may be copied over.
 __device__ __forceinline__ void lds_reads_done() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
@@ -181,13 +180,10 @@ decode_quant_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, Cache 
   constexpr int kTiles = 16 / P;   // tiles of 16 positions in one accumulator
   constexpr int kPasses = 4 / kTiles;
   constexpr int kMergeBytes = kWaves * P * (kD + 2) * 4;
-  constexpr int kStageBytes = kWaves * St::kSlots * St::kBytes;
+  constexpr int kStageBytes = kWaves * kSlots * St::kBytes;
   __shared__ __align__(16) uint8_t smem[kStageBytes > kMergeBytes ? kStageBytes : kMergeBytes];
-  // The fused form's row: q heads, new key, new value; then both quantised.
-  __shared__ __align__(16) float sm_qkv[kFused ? P + 2 : 1][kD];
-  __shared__ __align__(16) uint16_t sm_rot[kFused ? P + 1 : 1][kD];
-  __shared__ __align__(16) uint8_t sm_new[kFused ? 2 * St::kCode : 16];
-  __shared__ __align__(4) uint8_t sm_scale[4];
+  // The fused form's row as bf16: rotated q heads, rotated new key, new value.
+  __shared__ __align__(16) uint16_t sm_row[kFused ? P + 2 : 1][kD];
   const int split = blockIdx.x, h = blockIdx.y;
   const int64_t b = kFused && in.order ? in.order[blockIdx.z] : blockIdx.z;
   const int G = q_heads / kv_heads;
@@ -196,9 +192,31 @@ decode_quant_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, Cache 
   const int col = lane % 16, grp = lane / 16;
   const int tile = col / P, head = col % P;   // this column's tile of a pass, its query head
 
+  const int k0 = split * chunk;
+  const int64_t first_pos = ((int64_t)b * kv_heads + h) * capacity;
+  uint8_t *const my_stages = smem + wave * kSlots * St::kBytes;
+  const uint32_t my_lds = __builtin_amdgcn_readfirstlane(lds_address(my_stages));
+
+  // The fused form's loads: eight lanes per head of the row take channels 4j .. 4j+3 and
+  // 32 + 4j .. of it, the rotation's pairs.
+  const int hs = threadIdx.x / 8, j4 = (threadIdx.x % 8) * 4;
+  const bool row_thread = hs < G + 2;
+  f32x4 pa[kMaxQkvSplits], pb[kMaxQkvSplits];
+  if constexpr (kFused) {
+    if (row_thread) {
+      const int64_t ncols = (int64_t)(q_heads + 2 * kv_heads) * kD;
+      const int src_head = hs < G ? h * G + hs : (hs == G ? q_heads + h : q_heads + kv_heads + h);
+      const float *src = in.part + b * ncols + (int64_t)src_head * kD + j4;
+#pragma unroll
+      for (int s = 0; s < kMaxQkvSplits; ++s)
+        if (s < in.splits) {
+          pa[s] = *reinterpret_cast<const f32x4 *>(src + (int64_t)s * gridDim.z * ncols);
+          pb[s] = *reinterpret_cast<const f32x4 *>(src + (int64_t)s * gridDim.z * ncols + kD / 2);
+        }
+    }
+  }
   int n = min(used[b], max_len);
   n = (int)min((int64_t)n, capacity);
-  const int k0 = split * chunk;
   const int k1 = min(n, k0 + chunk);
   bool writer = false, own = false;
   int64_t pnew = 0;
@@ -213,16 +231,12 @@ decode_quant_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, Cache 
     own = writer && pnew >= k0 && pnew < k1;
   }
   if (splits > 1 && k0 >= n && !writer) return;  // the combine kernel skips empty splits
-
-  const int64_t first_pos = ((int64_t)b * kv_heads + h) * capacity;
   // This wave's stages: stage it starts at position k0 + (it * kWaves + wave) * 64.
   const int left = k1 - k0 - wave * kStageKeys;
   const int niter = left > 0 ? (left + kWaves * kStageKeys - 1) / (kWaves * kStageKeys) : 0;
-  uint8_t *const my_stages = smem + wave * St::kSlots * St::kBytes;
-  const uint32_t my_lds = __builtin_amdgcn_readfirstlane(lds_address(my_stages));
-
   // Requests stage `it` into its slot, its start a 64-bit scalar. Positions past the
-  // range repeat its last one (they are masked).
+  // range repeat its last one: masked, and never bytes that the row does not hold (an
+  // 8-bit code may be a NaN there).
   auto issue = [&](int it, int slot) {
     const int start = k0 + (it * kWaves + wave) * kStageKeys;
     const int last = k1 - 1 - start;
@@ -255,69 +269,59 @@ decode_quant_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, Cache 
     }
     stage_copy4(cache.scales + at, (uint32_t)min(lane, last) * 4, lds + 2 * St::kSide);
   };
-#pragma unroll
-  for (int s = 0; s < St::kSlots - 1; ++s)
-    if (s < niter) issue(s, s);
+  if (niter > 0) issue(0, 0);
 
   if constexpr (kFused) {
-    // The row's q|k|v slices of the packed projection, summed over the K slices
-    // in ascending order and rounded to bf16 (F.linear's output).
-    const int64_t ncols = (int64_t)(q_heads + 2 * kv_heads) * kD;
-    for (int t = threadIdx.x; t < (G + 2) * (kD / 4); t += kThreads) {
-      const int hs = t / (kD / 4), c4 = (t % (kD / 4)) * 4;
-      const int src_head = hs < G ? h * G + hs : (hs == G ? q_heads + h : q_heads + kv_heads + h);
-      const float *src = in.part + b * ncols + (int64_t)src_head * kD + c4;
-      f32x4 pv[kMaxQkvSplits];
-#pragma unroll
-      for (int s = 0; s < kMaxQkvSplits; ++s)
-        if (s < in.splits) pv[s] = *reinterpret_cast<const f32x4 *>(src + (int64_t)s * gridDim.z * ncols);
-      f32x4 acc = pv[0];
+    if (row_thread) {
+      // Summed over the K slices in ascending order and rounded to bf16 (F.linear's
+      // output), then rotated, v as it is.
+      const bool rotated = hs <= G && pnew >= 0 && pnew < in.table_len;
+      const bf16 *cs = in.cos_sin + (rotated ? pnew : 0) * kD + j4;
+      const uint64_t cw = *reinterpret_cast<const uint64_t *>(cs), sw = *reinterpret_cast<const uint64_t *>(cs + kD / 2);
+      f32x4 x1 = pa[0], x2 = pb[0];
 #pragma unroll
       for (int s = 1; s < kMaxQkvSplits; ++s)
-        if (s < in.splits) acc += pv[s];
+        if (s < in.splits) {
+          x1 += pa[s];
+          x2 += pb[s];
+        }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sm_qkv[hs][c4 + i] = round_bf16(acc[i]);
+      for (int i = 0; i < 4; ++i) {
+        float o1 = round_bf16(x1[i]), o2 = round_bf16(x2[i]);
+        if (rotated)
+          rotate_pair(o1, o2, bf16_to_f32((uint32_t)(cw >> (16 * i)) & 0xffffu),
+                      bf16_to_f32((uint32_t)(sw >> (16 * i)) & 0xffffu), o1, o2);
+        sm_row[hs][j4 + i] = (uint16_t)f32_to_bf16(o1);
+        sm_row[hs][kD / 2 + j4 + i] = (uint16_t)f32_to_bf16(o2);
+      }
+    }
+    __syncthreads();
+  }
+  // The new key (lanes 0-7 of a wave) and value (8-15), eight channels each, quantised:
+  // by the wave that stores them and by the one whose stage holds their position.
+  auto quantise_new = [&](uint32_t &byte) {
+    float x[8];
+    unpack8(*reinterpret_cast<const u32x4 *>(&sm_row[kFused ? G + lane / 8 : 0][8 * (lane % 8)]), x);
+    return quantise8<kBits>(x, byte);
+  };
+  if constexpr (kFused) {
+    if (writer && wave == 0 && lane < 16) {
+      uint32_t byte;
+      const Codes8<kBits> c = quantise_new(byte);
+      const int64_t at = first_pos + pnew;
+      *reinterpret_cast<Codes8<kBits> *>((lane < 8 ? cache.k : cache.v) + at * St::kCode + lane % 8 * kBits) = c;
+      if (lane % 4 == 0) reinterpret_cast<uint8_t *>(cache.scales + at)[lane / 4] = (uint8_t)byte;
     }
   }
 
   // Channels 32 bl + 16 (grp % 2) and on, sixteen of each block, of the column's head.
   u32x4 qw[2][2];
   if constexpr (kFused) {
-    __syncthreads();
-    const bool in_table = pnew >= 0 && pnew < in.table_len;
-    const bf16 *cs = in.cos_sin + (in_table ? pnew : 0) * kD;
-    for (int t = threadIdx.x; t < (G + 1) * (kD / 2); t += kThreads) {
-      const int hs = t / (kD / 2), pair = t % (kD / 2);
-      const float x1 = sm_qkv[hs][pair], x2 = sm_qkv[hs][kD / 2 + pair];
-      float o1 = x1, o2 = x2;
-      if (in_table) rotate_pair(x1, x2, bf16_to_f32(cs[pair]), bf16_to_f32(cs[kD / 2 + pair]), o1, o2);
-      sm_rot[hs][pair] = (uint16_t)f32_to_bf16(o1);
-      sm_rot[hs][kD / 2 + pair] = (uint16_t)f32_to_bf16(o2);
-    }
-    __syncthreads();
-    // Sixteen lanes quantise the new key (0-7) and value (8-15), eight channels each.
-    if (writer && threadIdx.x < 16) {
-      const int side = threadIdx.x / 8, u = threadIdx.x % 8;
-      float x[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        x[i] = side ? sm_qkv[G + 1][8 * u + i] : bf16_to_f32(sm_rot[G][8 * u + i]);
-      uint32_t byte;
-      const Codes8<kBits> c = quantise8<kBits>(x, byte);
-      *reinterpret_cast<Codes8<kBits> *>(sm_new + side * St::kCode + u * kBits) = c;
-      const int64_t at = first_pos + pnew;
-      *reinterpret_cast<Codes8<kBits> *>((side ? cache.v : cache.k) + at * St::kCode + u * kBits) = c;
-      if (u % 4 == 0) {
-        sm_scale[2 * side + u / 4] = (uint8_t)byte;
-        reinterpret_cast<uint8_t *>(cache.scales + at)[2 * side + u / 4] = (uint8_t)byte;
-      }
-    }
-    __syncthreads();
 #pragma unroll
     for (int bl = 0; bl < 2; ++bl)
 #pragma unroll
       for (int i = 0; i < 2; ++i)
-        qw[bl][i] = *reinterpret_cast<const u32x4 *>(&sm_rot[min(head, G)][32 * bl + 16 * (grp % 2) + 8 * i]);
+        qw[bl][i] = *reinterpret_cast<const u32x4 *>(&sm_row[min(head, G)][32 * bl + 16 * (grp % 2) + 8 * i]);
   } else {
     const bf16 *qp = q + b * qs0 + (int64_t)(h * G + min(head, G - 1)) * qs1 + 16 * (grp % 2);
 #pragma unroll
@@ -386,14 +390,57 @@ decode_quant_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, Cache 
     if constexpr (kFused) {
       if (own && pnew >= start && pnew < start + kStageKeys) {
         const int at = (int)(pnew - start);
-        if (lane < 2 * St::kCode / 4) {
-          const int side = lane / (St::kCode / 4), w = lane % (St::kCode / 4);
-          *reinterpret_cast<uint32_t *>(st + side * St::kSide + at * St::kCode + 4 * w) =
-              *reinterpret_cast<const uint32_t *>(sm_new + side * St::kCode + 4 * w);
+        if (lane < 16) {
+          uint32_t byte;
+          const Codes8<kBits> c = quantise_new(byte);
+          *reinterpret_cast<Codes8<kBits> *>(st + lane / 8 * St::kSide + at * St::kCode + lane % 8 * kBits) = c;
+          if (lane % 4 == 0) st[2 * St::kSide + 4 * at + lane / 4] = (uint8_t)byte;
         }
-        if (lane == 0)
-          *reinterpret_cast<uint32_t *>(st + 2 * St::kSide + 4 * at) = *reinterpret_cast<const uint32_t *>(sm_scale);
         lds_reads_done();
+      }
+    }
+    // Everything that the stage's products take from LDS is requested before the
+    // first product, so that one latency serves them all.
+    typedef int i32x2 __attribute__((ext_vector_type(2)));
+    typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
+    i32x8 a[2][2];
+#pragma unroll
+    for (int pr = 0; pr < 2; ++pr)
+#pragma unroll
+      for (int bl = 0; bl < 2; ++bl) {
+        if constexpr (kBits == 4) {
+          // lane (col, grp): the block of position col of tile 2 pr + grp / 2
+          const u32x4 w = *reinterpret_cast<const u32x4 *>(st + (32 * pr + 16 * (grp / 2) + col) * St::kCode + 16 * bl);
+          a[pr][bl] = i32x8{(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
+        } else {
+          // lane (col, grp): sixteen channels of position col of tiles 2 pr and 2 pr + 1
+          const uint8_t *kp = st + (32 * pr + col) * St::kCode + 32 * bl + 16 * (grp % 2);
+          const u32x4 w0 = *reinterpret_cast<const u32x4 *>(kp);
+          const u32x4 w1 = *reinterpret_cast<const u32x4 *>(kp + 16 * St::kCode);
+          a[pr][bl] = i32x8{(int)w0[0], (int)w0[1], (int)w0[2], (int)w0[3],
+                            (int)w1[0], (int)w1[1], (int)w1[2], (int)w1[3]};
+        }
+      }
+    u32x4 words[kPasses];  // scale words of the lane's four positions of each pass
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p)
+      words[p] = *reinterpret_cast<const u32x4 *>(st + 2 * St::kSide + 4 * ((p * kTiles + tile) * 16 + 4 * grp));
+    const uint8_t *vs = st + St::kSide;
+    i32x2 vt[4][kBits / 4];  // V^T: channel 16 mm + col, eight positions of tiles 2 pr and 2 pr + 1 each
+#pragma unroll
+    for (int mm = 0; mm < 4; ++mm) {
+      if constexpr (kBits == 4) {
+        // Lane col of a group reads the 16 channels of position 16 (col/4) + 4 grp + col%4
+        // and receives channel col of the group's 16 positions, tiles 0-3 in order.
+        vt[mm][0] = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
+            (lds_i32x2 *)(vs + (16 * (col / 4) + 4 * grp + col % 4) * St::kCode + 8 * mm));
+      } else {
+        // Lanes 2r and 2r+1 read the 16 channels of position r of the group's eight
+        // (four of each tile); lane col receives channel col of all eight.
+#pragma unroll
+        for (int pr = 0; pr < 2; ++pr)
+          vt[mm][pr] = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+              (lds_i32x2 *)(vs + (16 * (2 * pr + col / 8) + 4 * grp + col / 2 % 4) * St::kCode + 16 * mm + 8 * (col % 2)));
       }
     }
     f32x4 c[kPasses][2];
@@ -403,32 +450,18 @@ decode_quant_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, Cache 
     for (int pr = 0; pr < 2; ++pr)
 #pragma unroll
       for (int bl = 0; bl < 2; ++bl) {
-        i32x8 a;
-        if constexpr (kBits == 4) {
-          // lane (col, grp): the block of position col of tile 2 pr + grp / 2
-          const u32x4 w = *reinterpret_cast<const u32x4 *>(st + (32 * pr + 16 * (grp / 2) + col) * St::kCode + 16 * bl);
-          a = i32x8{(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
-        } else {
-          // lane (col, grp): sixteen channels of position col of tiles 2 pr and 2 pr + 1
-          const uint8_t *kp = st + (32 * pr + col) * St::kCode + 32 * bl + 16 * (grp % 2);
-          const u32x4 w0 = *reinterpret_cast<const u32x4 *>(kp);
-          const u32x4 w1 = *reinterpret_cast<const u32x4 *>(kp + 16 * St::kCode);
-          a = i32x8{(int)w0[0], (int)w0[1], (int)w0[2], (int)w0[3], (int)w1[0], (int)w1[1], (int)w1[2], (int)w1[3]};
-        }
         if constexpr (P == 4) {
-          c[0][bl] = mfma_codes<kBits>(a, qb[pr][bl], c[0][bl]);
+          c[0][bl] = mfma_codes<kBits>(a[pr][bl], qb[pr][bl], c[0][bl]);
         } else if constexpr (P == 8) {
-          c[pr][bl] = mfma_codes<kBits>(a, qb[0][bl], c[pr][bl]);
+          c[pr][bl] = mfma_codes<kBits>(a[pr][bl], qb[0][bl], c[pr][bl]);
         } else {
-          c[2 * pr][bl] = mfma_codes<kBits>(a, qb[0][bl], c[2 * pr][bl]);
-          c[2 * pr + 1][bl] = mfma_codes<kBits>(a, qb[kVariants - 1][bl], c[2 * pr + 1][bl]);
+          c[2 * pr][bl] = mfma_codes<kBits>(a[pr][bl], qb[0][bl], c[2 * pr][bl]);
+          c[2 * pr + 1][bl] = mfma_codes<kBits>(a[pr][bl], qb[kVariants - 1][bl], c[2 * pr + 1][bl]);
         }
       }
     float s[kPasses][4];
-    u32x4 words[kPasses];  // scale words of the lane's four positions of each pass
 #pragma unroll
     for (int p = 0; p < kPasses; ++p) {
-      words[p] = *reinterpret_cast<const u32x4 *>(st + 2 * St::kSide + 4 * ((p * kTiles + tile) * 16 + 4 * grp));
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         s[p][i] = (c[p][0][i] * scale_of<0>(words[p][i]) + c[p][1][i] * scale_of<1>(words[p][i])) * sl2;
@@ -499,53 +532,24 @@ decode_quant_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, Cache 
           for (int t = 0; t < 4; ++t) bp[t / 2][bl][2 * (t % 2) + i] = pb[bl][t][i];
         }
       }
-    typedef int i32x2 __attribute__((ext_vector_type(2)));
-    typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
-    const uint8_t *vs = st + St::kSide;
 #pragma unroll
-    for (int mm = 0; mm < 4; ++mm) {
-      if constexpr (kBits == 4) {
-        // Lane col of a group reads the 16 channels of position 16 (col/4) + 4 grp + col%4
-        // and receives channel col of the group's 16 positions, tiles 0-3 in order.
-        const int pos = 16 * (col / 4) + 4 * grp + col % 4;
-        const i32x2 t = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
-            (lds_i32x2 *)(vs + pos * St::kCode + 8 * mm));
+    for (int mm = 0; mm < 4; ++mm)
 #pragma unroll
-        for (int pr = 0; pr < 2; ++pr) {
-          const uint32_t w = (uint32_t)t[pr];
-          acc[mm] = mfma16x16x32(codes_to_bf16<kBits>(&w), bp[pr][mm / 2], acc[mm]);
-        }
-      } else {
+      for (int pr = 0; pr < 2; ++pr) {
+        uint32_t w[kBits / 4];
 #pragma unroll
-        for (int pr = 0; pr < 2; ++pr) {
-          // Lanes 2r and 2r+1 read the 16 channels of position r of the group's
-          // eight (four of each tile); lane col receives channel col of all eight.
-          const int r = col / 2;
-          const int pos = 16 * (2 * pr + r / 4) + 4 * grp + r % 4;
-          const i32x2 t = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-              (lds_i32x2 *)(vs + pos * St::kCode + 16 * mm + 8 * (col % 2)));
-          const uint32_t w[2] = {(uint32_t)t[0], (uint32_t)t[1]};
-          acc[mm] = mfma16x16x32(codes_to_bf16<kBits>(w), bp[pr][mm / 2], acc[mm]);
-        }
+        for (int j = 0; j < kBits / 4; ++j) w[j] = (uint32_t)(kBits == 4 ? vt[mm][0][pr] : vt[mm][pr * (kBits / 8)][j]);
+        acc[mm] = mfma16x16x32(codes_to_bf16<kBits>(w), bp[pr][mm / 2], acc[mm]);
       }
-    }
   };
 
-  int slot = 0;
   for (int it = 0; it < niter; ++it) {
-    // Stage `it` has arrived once only the younger ones are in flight.
-    const int younger = min(niter - 1 - it, St::kSlots - 2);
-    if (younger >= 1)
-      copies_wait<(St::kSlots - 2) * St::kCopies>();
-    else
-      copies_wait<0>();
-    if (it + St::kSlots - 1 < niter) {
-      // The slot that stage it - 1 has left; its reads are done.
-      lds_reads_done();
-      issue(it + St::kSlots - 1, (slot + St::kSlots - 1) % St::kSlots);
+    copies_wait();  // stage `it` has arrived
+    if (it + 1 < niter) {
+      lds_reads_done();  // of stage it - 1, whose slot the next one takes
+      issue(it + 1, (it + 1) % 2);
     }
-    compute(it, slot);
-    slot = slot + 1 == St::kSlots ? 0 : slot + 1;
+    compute(it, it % 2);
   }
 
   // A query head's sum of probabilities: over the four lanes of its columns and the
