@@ -7,8 +7,8 @@
 // shorter, and with the products on vector units (about 35 SIMD cycles per
 // position there, against 33 that the 4-bit stream leaves) they would bound it.
 //
-// Workgroup (split, kv head, row), four waves; a wave takes 64 consecutive
-// positions (a stage) at a time, every fourth stage of the workgroup's range.
+// Workgroup (split, kv head, row), four or eight waves; a wave takes 64 consecutive
+// positions (a stage) at a time, the workgroup's stages in turn.
 // Stages pass through LDS: codes and scale words are copied there directly
 // (global_load_lds), the next stage while one is computed, each wave its own, no barriers.
 //
@@ -49,8 +49,6 @@ namespace lm {
 namespace {
 
 constexpr int kD = 64;
-constexpr int kWaves = 4;
-constexpr int kThreads = kWaves * kWave;
 constexpr int kStageKeys = 64;
 constexpr int kMaxQkvSplits = 8;
 
@@ -170,13 +168,14 @@ struct QkvIn {
   const int32_t *order;   // [batch] row of workgroup z (longest first), or NULL: row z
 };
 
-template <int kBits, int P, bool kFused>
-__global__ void __launch_bounds__(kThreads, 2)
+template <int kBits, int P, bool kFused, int kWaves>
+__global__ void __launch_bounds__(kWaves * kWave, 2)
 decode_quant_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, Cache cache,
                     const int32_t *__restrict__ used, int q_heads, int kv_heads, int64_t capacity,
                     float scale, int max_len, int chunk, int splits, Partial part, QkvIn in,
                     bf16 *__restrict__ out, int out_mb) {
   typedef Stage<kBits> St;
+  constexpr int kThreads = kWaves * kWave;
   constexpr int kTiles = 16 / P;   // tiles of 16 positions in one accumulator
   constexpr int kPasses = 4 / kTiles;
   constexpr int kMergeBytes = kWaves * P * (kD + 2) * 4;
@@ -648,13 +647,13 @@ int64_t workspace_bytes(int64_t batch, int64_t q_heads, int64_t splits) {
   return n * kD * 4 + 2 * align_up(n * 4, 256);
 }
 
-template <int kBits, int P, bool kFused>
+template <int kBits, int P, bool kFused, int kWaves>
 int launch_sized(const bf16 *q, int64_t qs0, int64_t qs1, const Cache &cache, const int32_t *used, int64_t batch,
                  int64_t q_heads, int64_t kv_heads, int64_t capacity, float scale, int64_t max_len, int chunk,
                  int grid_splits, int stride_splits, const Partial &part, const QkvIn &in, bf16 *out, int out_mb,
                  hipStream_t s) {
   const dim3 grid((unsigned)grid_splits, (unsigned)kv_heads, (unsigned)batch);
-  decode_quant_kernel<kBits, P, kFused><<<grid, kThreads, 0, s>>>(
+  decode_quant_kernel<kBits, P, kFused, kWaves><<<grid, kWaves * kWave, 0, s>>>(
       q, qs0, qs1, cache, used, (int)q_heads, (int)kv_heads, capacity, scale, (int)max_len, chunk, stride_splits,
       part, in, out, out_mb);
   LM_CHECK_LAUNCH();
@@ -699,18 +698,27 @@ int launch_decode_quant(const Call &c, const void *q, int64_t qs0, int64_t qs1, 
   const int stride_splits = splits > 1 ? (int)c.num_splits : 1;
   hipStream_t s = (hipStream_t)stream;
   const int64_t G = c.q_heads / c.kv_heads;
-  auto pick = [&](auto fused) {
+  auto pick = [&](auto fused, auto bits, auto waves) {
     constexpr bool kFused = decltype(fused)::value;
-    auto go = c.bits == 4 ? (G <= 4   ? launch_sized<4, 4, kFused>
-                             : G <= 8 ? launch_sized<4, 8, kFused>
-                                      : launch_sized<4, 16, kFused>)
-                          : (G <= 4   ? launch_sized<8, 4, kFused>
-                             : G <= 8 ? launch_sized<8, 8, kFused>
-                                      : launch_sized<8, 16, kFused>);
+    constexpr int kBits = decltype(bits)::value, kWaves = decltype(waves)::value;
+    auto go = G <= 4   ? launch_sized<kBits, 4, kFused, kWaves>
+              : G <= 8 ? launch_sized<kBits, 8, kFused, kWaves>
+                       : launch_sized<kBits, 16, kFused, kWaves>;
     return go((const bf16 *)q, qs0, qs1, cache, used, c.batch, c.q_heads, c.kv_heads, c.capacity, scale, c.max_len,
               chunk, splits, stride_splits, part, in, (bf16 *)out, out_mb, s);
   };
-  const int status = in.part ? pick(std::true_type{}) : pick(std::false_type{});
+  // Up to one workgroup per CU a wave has its SIMD to itself, and a 4-bit stage's chain
+  // of dependent steps (0.57 us) takes longer than its bytes: eight waves where
+  // they get two stages each. 32 rows to 4095 positions 15.7 us with four, 13.9 with
+  // eight; 24 rows to 2000 9.0 and 8.1; 10 rows to 1000 5.9 and 6.0, one row of 512 4.1
+  // and 4.6. In 8 bits the two are alike (32 rows to 4095 21.9 and 22.0).
+  const bool wide = c.bits == 4 && (int64_t)splits * c.kv_heads * c.batch <= 256 && chunk >= 16 * kStageKeys;
+  typedef std::integral_constant<int, 4> Four;
+  typedef std::integral_constant<int, 8> Eight;
+  auto run = [&](auto fused) {
+    return c.bits == 8 ? pick(fused, Eight{}, Four{}) : wide ? pick(fused, Four{}, Eight{}) : pick(fused, Four{}, Four{});
+  };
+  const int status = in.part ? run(std::true_type{}) : run(std::false_type{});
   if (status != LM_OK || splits == 1) return status;
   auto combine = splits <= 4 ? decode_quant_combine_kernel<4> : decode_quant_combine_kernel<16>;
   combine<<<dim3((unsigned)c.q_heads, (unsigned)c.batch), kD, 0, s>>>(

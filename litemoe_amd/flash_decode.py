@@ -134,6 +134,22 @@ class FlashDecode:
         return out
 
 
+def quant_splits(batch, kv_heads, maximum):
+    """Key-range splits over a quantised cache: :func:`default_splits` with other
+    lines, since a position takes a quarter or half of the bytes.
+
+    Up to 256 (row, head) pairs, one workgroup per CU, the splits fill the CUs
+    and no more; a split keeps 512 positions at least and contexts below three
+    times that are not split, since the second launch costs 1.6 to 2 us. us per
+    launch in a graph: one row x 8 heads to 1000 positions 7.3 (1 split) and 7.7
+    (4); to 4000 12.0 (1), 8.0 (4) and 7.6 (7); 5 rows to 4000 10.0 (1), 8.4 (4)
+    and 9.2 (8); 8 rows to 32768 30.3 (2), 22.0 (4) and 23.1 (8); 32 rows to 4095
+    13.9 (1) and 15.7 (2); 64 rows to 1279 10.0 (1) and 13.0 (2). More than 16
+    only for contexts past 65536: the second launch loads 16 at a time."""
+    longest = maximum // 512 if maximum >= 3 * 512 else 1
+    return max(1, min(max(16, maximum // 4096), 256 // max(1, batch * kv_heads), longest))
+
+
 class QuantFlashDecode:
     """:class:`FlashDecode` over a :class:`~litemoe_amd.cache.QuantKVCache`
     (``lm_flash_decode_quant``, ``lm_flash_decode_quant_qkv``): the same plan and
@@ -152,7 +168,7 @@ class QuantFlashDecode:
             raise ValueError("Decode attention over a quantised cache takes 1 to 16 query heads per KV head")
         self.batch, self.kv_heads, self.groups, self.capacity, self.bits = batch, kv_heads, groups, capacity, bits
         self.maximum = capacity if maximum is None else maximum
-        self.splits = num_splits or default_splits(batch, kv_heads, self.maximum)
+        self.splits = num_splits or quant_splits(batch, kv_heads, self.maximum)
         self.device = torch.device(device)
         size = _lib.size_query("lm_flash_decode_workspace_size", batch, kv_heads * groups, 64,
                                self.splits) if self.device.type == "cuda" else 0
@@ -187,6 +203,7 @@ class QuantFlashDecode:
         if q.get_device() != index:
             raise ValueError("Queries and cache must be on one device")
         rows, heads, _, channels = q.stride()
+        rows, heads = rows if b > 1 else 0, heads if hq > 1 else 0  # of a single one the stride says nothing
         if channels != 1 or rows % 8 or heads % 8 or q.data_ptr() % 16:
             raise ValueError("Decode attention needs contiguous channels and 16-byte aligned query heads")
         if used is None:
@@ -194,7 +211,7 @@ class QuantFlashDecode:
         used = kv_quant.per_row(used, b, torch.int32, index, "used")
         out = torch.empty((b, hq, 1, 64), device=q.device, dtype=torch.bfloat16)
         _lib.call_on(index, "lm_flash_decode_quant", q.data_ptr(), rows, heads, k.data_ptr(), v.data_ptr(),
-                     scales.data_ptr(), used.data_ptr(), b, hq, self.kv_heads, self.capacity, 64, self.bits, scale,
+                     scales.data_ptr(), used.data_ptr(), b, hq, self.kv_heads, self.capacity, 64, self.bits, float(scale),
                      self.maximum, self.splits, out.data_ptr(), self.workspace.data_ptr(), self.workspace.numel())
         return out
 
@@ -227,6 +244,6 @@ class QuantFlashDecode:
         _lib.call_on(index, "lm_flash_decode_quant_qkv", partials.data_ptr(), splits, cos_sin.data_ptr(), table[0],
                      positions.data_ptr(), _lib.ptr(active), k.data_ptr(), v.data_ptr(), scales.data_ptr(),
                      used.data_ptr(), _lib.ptr(row_order), b, q_heads, self.kv_heads, self.capacity, 64, self.bits,
-                     scale, self.maximum, self.splits, int(frag_out), out_ptr, self.workspace.data_ptr(),
+                     float(scale), self.maximum, self.splits, int(frag_out), out_ptr, self.workspace.data_ptr(),
                      self.workspace.numel())
         return out
