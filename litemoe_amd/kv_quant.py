@@ -39,13 +39,21 @@ def per_row(t, rows, dtype, index, what):
     return t if t.is_contiguous() else t.contiguous()
 
 
+def _device(cache):
+    """The index of the cache's GPU; a cache's own buffers are what :func:`check_layer` asks for."""
+    index = cache.k.get_device()
+    if index < 0:
+        _lib.require_cuda(cache.k, what="quantised KV cache")
+    return index
+
+
 def write(cache, layer, k, v, positions, active, slots):
     """Quantise ``k[row, h, 0, :]`` into position ``positions[row]`` of
     ``slots[row]`` for active rows (same for v), as :func:`kv_write.write`
     stores them. ``k, v [rows, H, 1, 64]`` bf16 with any strides; ``active`` may
     be None (every row). Rows out of range are skipped. One row per target."""
     kc, vc, scales = cache.layer(layer)
-    bits, index = check_layer(kc, vc, scales)
+    index = _device(cache)
     batch, heads, capacity, _ = kc.shape
     shape = k.shape
     if len(shape) != 4 or shape[1:] != (heads, 1, 64) or v.shape != shape:
@@ -61,7 +69,7 @@ def write(cache, layer, k, v, positions, active, slots):
     ks, vs = k.stride(), v.stride()
     _lib.call_on(index, "lm_kv_quant_write", k.data_ptr(), ks[0], ks[1], ks[3], v.data_ptr(), vs[0], vs[1], vs[3],
                  kc.data_ptr(), vc.data_ptr(), scales.data_ptr(), positions.data_ptr(), _lib.ptr(active),
-                 slots.data_ptr(), rows, heads, 64, capacity, batch, bits)
+                 slots.data_ptr(), rows, heads, 64, capacity, batch, cache.bits)
 
 
 def read(cache, layer, positions, slots):
@@ -69,7 +77,7 @@ def read(cache, layer, positions, slots):
     ``k, v [rows, H, 1, 64]`` bf16, the layout :func:`write` takes. Rows out of
     range give zeros."""
     kc, vc, scales = cache.layer(layer)
-    bits, index = check_layer(kc, vc, scales)
+    index = _device(cache)
     batch, heads, capacity, _ = kc.shape
     rows = positions.numel()
     positions = per_row(positions, rows, torch.int64, index, "positions")
@@ -77,5 +85,5 @@ def read(cache, layer, positions, slots):
     k = torch.empty((rows, heads, 1, 64), dtype=torch.bfloat16, device=kc.device)
     v = torch.empty_like(k)
     _lib.call_on(index, "lm_kv_quant_read", kc.data_ptr(), vc.data_ptr(), scales.data_ptr(), positions.data_ptr(),
-                 slots.data_ptr(), rows, heads, 64, capacity, batch, bits, k.data_ptr(), v.data_ptr())
+                 slots.data_ptr(), rows, heads, 64, capacity, batch, cache.bits, k.data_ptr(), v.data_ptr())
     return k, v
