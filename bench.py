@@ -81,6 +81,8 @@ def parse():
     ap.add_argument("--prefill", action="store_true", help="cfg 4 packed prefill (own JSON line)")
     ap.add_argument("--flash-decode", action="store_true", help="cfg 5 decode attention (own JSON line)")
     ap.add_argument("--long-decode", action="store_true", help="cfg 5 decode step tok/s (own JSON line)")
+    ap.add_argument("--kv-bits", type=int, default=16, choices=(4, 8, 16),
+                    help="with --long-decode: bits per KV cache element (8 and 4 hold the cache quantised)")
     return ap.parse_args()
 
 
@@ -491,7 +493,7 @@ def long_decode_bench(args):
     model = Granite(cfg, w, ep, cap)
     prompts = synth.prompts(batch, lengths, cfg.vocab_size, 1)
     requests = [Request(str(i), p, 48) for i, p in enumerate(prompts)]
-    engine = OptimizedEngine(model, requests, mode="graph", ignore_eos=True, capacity=cap)
+    engine = OptimizedEngine(model, requests, mode="graph", ignore_eos=True, capacity=cap, kv_bits=args.kv_bits)
     with torch.inference_mode():
         engine.prepare_graph()
         engine.reset()
@@ -512,7 +514,8 @@ def long_decode_bench(args):
         torch.cuda.synchronize()
         elapsed = time.perf_counter() - t0
         assert bool(engine.state["active"].all())
-    kv = sum(n + steps // 2 for n in lengths) * cfg.num_key_value_heads * 64 * 2 * 2 * cfg.num_hidden_layers
+    held = 256 if args.kv_bits == 16 else 16 * args.kv_bits + 4  # bytes of a position's key and value, per KV head
+    kv = sum(n + steps // 2 for n in lengths) * cfg.num_key_value_heads * held * cfg.num_hidden_layers
     line = {
         "metric": "decode tok/s, cfg5 (B=128, contexts U{1024..4032})", "value": round(batch * steps / elapsed, 1),
         "unit": "tok/s", "n_gpus": 1, "steps": steps, "warmup": warmup, "ms_per_step": round(elapsed * 1e3 / steps, 4),
@@ -523,6 +526,8 @@ def long_decode_bench(args):
                    "mean_context": round(sum(lengths) / batch + steps / 2, 1)},
         "kv_bytes_per_step": kv,
     }
+    if args.kv_bits != 16:
+        line["config"]["kv_bits"] = args.kv_bits
     print(json.dumps(line), flush=True)
 
 
