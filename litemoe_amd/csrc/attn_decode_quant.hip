@@ -12,15 +12,12 @@
 // Stages pass through LDS: codes and scale words are copied there directly
 // (global_load_lds), the next stage while one is computed, each wave its own, no barriers.
 //
-// Scores: K . q with v_mfma_f32_16x16x128_f8f6f4, A the codes of two tiles of 16
-// positions as they lie in the cache, one product per block of 32 channels,
+// Scores: K . q with v_mfma_f32_16x16x32_bf16, A the codes of 16 positions as bf16
+// without their scales (exact), one product per block of 32 channels,
 //   s_j = sl2 * (2^e0 (c_j0 . q_0) + 2^e1 (c_j1 . q_1)).
-// The 128 products of an output are a block of both tiles, each twice: against q's
-// 8-bit leading part and against the rest (q 2^-e = hi + lo, e4m3 both, with max|q|
-// at 2^7: hi keeps 4 of bf16's 8 significant bits and lo the other 4, exactly for
-// channels down to 2^-9 of the head's largest and to within 2^-17 of that below).
-// No code is converted for the scores: 32 conversions less per stage than bf16
-// operands take, a sixth of the stage's instructions.
+// The 8-bit matrix instructions would take the codes unconverted and q in two 8-bit
+// parts, but they sum products of unequal size with 2^-14 of the largest lost
+// (measured on random operands), where this sums in fp32.
 // The G query heads of a KV head fill P = 4, 8 or 16 of the 16 columns; the
 // other columns take other positions: column c holds query head c % P of tile
 // c / P of a pass, and the B operand is zero where a tile is not its column's, so
@@ -53,8 +50,9 @@ constexpr int kStageKeys = 64;
 constexpr int kMaxQkvSplits = 8;
 
 // Running maximum before any position: finite, so exp2(kEmpty - m) and
-// exp2(-inf - kEmpty) are 0 and the loop needs no special case.
-constexpr float kEmpty = -1e30f;
+// exp2(-inf - kEmpty) are 0 and the loop needs no special case, and below every
+// other finite score.
+constexpr float kEmpty = -3.402823466e38f;
 // A column keeps its maximum until a score exceeds it by more than this (log2
 // units): probabilities stay below 2^8 and the accumulators are seldom rescaled.
 constexpr float kLazy = 8.f;
@@ -112,18 +110,6 @@ __device__ __forceinline__ float scale_of(uint32_t word) {
   if constexpr (kByte == 3) LM_SCALE("BYTE_3");
 #undef LM_SCALE
   return r;
-}
-
-typedef int i32x8 __attribute__((ext_vector_type(8)));
-
-// MFMA 16x16x128, A codes of kBits and B e4m3, no scales. k runs over four groups
-// of 32. A of 4 bits: lane l holds row l%16, group l/16, in its first four words.
-// 8-bit operands: lane l holds, of row or column l%16, the 16 bytes k = 16 (l/16) and
-// on in words 0-3 and the 16 bytes k = 64 + 16 (l/16) and on in words 4-7 (checked on
-// the device). C as mfma16x16x32.
-template <int kBits>
-__device__ __forceinline__ f32x4 mfma_codes(const i32x8 &a, const i32x8 &b, f32x4 c) {
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, kBits == 4 ? 4 : 0, 0, 0, 0, 0, 0);
 }
 
 // Reductions over the tiles of a query head: columns c % P equal, one row of 16 lanes.
@@ -185,6 +171,7 @@ decode_quant_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, Cache 
   __shared__ __align__(16) uint16_t sm_row[kFused ? P + 2 : 1][kD];
   const int split = blockIdx.x, h = blockIdx.y;
   const int64_t b = kFused && in.order ? in.order[blockIdx.z] : blockIdx.z;
+  if (kFused && (b < 0 || b >= gridDim.z)) return;  // not a permutation: no row of this call
   const int G = q_heads / kv_heads;
   const int lane = threadIdx.x % kWave;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -309,70 +296,27 @@ decode_quant_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, Cache 
     unpack8(*reinterpret_cast<const u32x4 *>(&sm_row[kFused ? G + lane / 8 : 0][8 * (lane % 8)]), x);
     return quantise8<kBits>(x, byte);
   };
-  // Channels 32 bl + 16 (grp % 2) and on, sixteen of each block, of the column's head.
-  u32x4 qw[2][2];
+  // Channels 32 bl + 8 grp and on of the column's query head.
+  u32x4 qw[2];
   if constexpr (kFused) {
 #pragma unroll
     for (int bl = 0; bl < 2; ++bl)
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        qw[bl][i] = *reinterpret_cast<const u32x4 *>(&sm_row[min(head, G)][32 * bl + 16 * (grp % 2) + 8 * i]);
+      qw[bl] = *reinterpret_cast<const u32x4 *>(&sm_row[min(head, G)][32 * bl + 8 * grp]);
   } else {
-    const bf16 *qp = q + b * qs0 + (int64_t)(h * G + min(head, G - 1)) * qs1 + 16 * (grp % 2);
-#pragma unroll
-    for (int bl = 0; bl < 2; ++bl)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) qw[bl][i] = *reinterpret_cast<const u32x4 *>(qp + 32 * bl + 8 * i);
+    const bf16 *qp = q + b * qs0 + (int64_t)(h * G + min(head, G - 1)) * qs1 + 8 * grp;
+    qw[0] = *reinterpret_cast<const u32x4 *>(qp);
+    qw[1] = *reinterpret_cast<const u32x4 *>(qp + 32);
   }
-  // q's two e4m3 parts, lanes of groups 0 and 1 the leading one: 2^(134 - E) q, E the
-  // exponent field of the head's largest (at least 8, so that both powers are normal).
-  float qx[2][16];
-  uint32_t qmax = 0;
+  // B operands of the scores: tile t's are zero outside its columns.
+  u32x4 qt[kTiles][2];
 #pragma unroll
-  for (int bl = 0; bl < 2; ++bl)
-#pragma unroll
-    for (int i = 0; i < 2; ++i) unpack8(qw[bl][i], &qx[bl][8 * i]);
-#pragma unroll
-  for (int bl = 0; bl < 2; ++bl)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) qmax = max(qmax, __float_as_uint(qx[bl][i]) & 0x7fffffffu);
-  qmax = max(qmax, __float_as_uint(xor_lanes<16>(__uint_as_float(qmax))));
-  const uint32_t qe = max(qmax >> 23, 8u);
-  const float q_up = __uint_as_float((261u - qe) << 23);
-  uint32_t qpart[2][4];
-#pragma unroll
-  for (int bl = 0; bl < 2; ++bl)
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      uint32_t r[2] = {0u, 0u};
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        typedef short s16x2 __attribute__((ext_vector_type(2)));
-        const float x0 = qx[bl][4 * w + 2 * half] * q_up, x1 = qx[bl][4 * w + 2 * half + 1] * q_up;
-        s16x2 hi = (s16x2){0, 0}, lo = hi;
-        hi = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(hi, x0, x1, 1.f, false);
-        const f32x2 back =
-            __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(__builtin_bit_cast(uint32_t, hi), 1.f, false);
-        lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lo, x0 - back[0], x1 - back[1], 1.f, false);
-        r[half] = __builtin_bit_cast(uint32_t, grp < 2 ? hi : lo) & 0xffffu;
-      }
-      qpart[bl][w] = head < G ? r[0] | r[1] << 16 : 0u;
-    }
-  // B operands of the scores. Words 0-3 meet the first tile of a pair, words 4-7 the
-  // second; variant 0 is pair 0's (P = 4), any pair's (P = 8) or the first tile's (P = 16).
-  constexpr int kVariants = P == 8 ? 1 : 2;
-  i32x8 qb[kVariants][2];
-#pragma unroll
-  for (int v = 0; v < kVariants; ++v)
+  for (int t = 0; t < kTiles; ++t)
 #pragma unroll
     for (int bl = 0; bl < 2; ++bl)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const bool mine = P == 16 ? v == i / 4 : tile == 2 * v + i / 4;
-        qb[v][bl][i] = mine ? (int)qpart[bl][i % 4] : 0;
-      }
+      for (int i = 0; i < 4; ++i) qt[t][bl][i] = tile == t && head < G ? qw[bl][i] : 0u;
 
-  const float sl2 = scale * 1.4426950408889634f * __uint_as_float((qe - 7u) << 23);
+  const float sl2 = scale * 1.4426950408889634f;
   float m = kEmpty, l = 0.f;
   f32x4 acc[4];  // channels 16 mm + 4 grp + i of column col, of use where tile is 0
 #pragma unroll
@@ -398,24 +342,13 @@ decode_quant_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, Cache 
     // first product, so that one latency serves them all.
     typedef int i32x2 __attribute__((ext_vector_type(2)));
     typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
-    i32x8 a[2][2];
+    Codes8<kBits> a[4][2];  // tile t: channels 32 bl + 8 grp and on of position 16 t + col
 #pragma unroll
-    for (int pr = 0; pr < 2; ++pr)
+    for (int t = 0; t < 4; ++t)
 #pragma unroll
-      for (int bl = 0; bl < 2; ++bl) {
-        if constexpr (kBits == 4) {
-          // lane (col, grp): the block of position col of tile 2 pr + grp / 2
-          const u32x4 w = *reinterpret_cast<const u32x4 *>(st + (32 * pr + 16 * (grp / 2) + col) * St::kCode + 16 * bl);
-          a[pr][bl] = i32x8{(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
-        } else {
-          // lane (col, grp): sixteen channels of position col of tiles 2 pr and 2 pr + 1
-          const uint8_t *kp = st + (32 * pr + col) * St::kCode + 32 * bl + 16 * (grp % 2);
-          const u32x4 w0 = *reinterpret_cast<const u32x4 *>(kp);
-          const u32x4 w1 = *reinterpret_cast<const u32x4 *>(kp + 16 * St::kCode);
-          a[pr][bl] = i32x8{(int)w0[0], (int)w0[1], (int)w0[2], (int)w0[3],
-                            (int)w1[0], (int)w1[1], (int)w1[2], (int)w1[3]};
-        }
-      }
+      for (int bl = 0; bl < 2; ++bl)
+        a[t][bl] = *reinterpret_cast<const Codes8<kBits> *>(st + (16 * t + col) * St::kCode +
+                                                            bl * (St::kCode / 2) + grp * kBits);
     u32x4 words[kPasses];  // scale words of the lane's four positions of each pass
 #pragma unroll
     for (int p = 0; p < kPasses; ++p)
@@ -442,18 +375,10 @@ decode_quant_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, Cache 
 #pragma unroll
     for (int p = 0; p < kPasses; ++p) c[p][0] = c[p][1] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int pr = 0; pr < 2; ++pr)
+    for (int t = 0; t < 4; ++t)
 #pragma unroll
-      for (int bl = 0; bl < 2; ++bl) {
-        if constexpr (P == 4) {
-          c[0][bl] = mfma_codes<kBits>(a[pr][bl], qb[pr][bl], c[0][bl]);
-        } else if constexpr (P == 8) {
-          c[pr][bl] = mfma_codes<kBits>(a[pr][bl], qb[0][bl], c[pr][bl]);
-        } else {
-          c[2 * pr][bl] = mfma_codes<kBits>(a[pr][bl], qb[0][bl], c[2 * pr][bl]);
-          c[2 * pr + 1][bl] = mfma_codes<kBits>(a[pr][bl], qb[kVariants - 1][bl], c[2 * pr + 1][bl]);
-        }
-      }
+      for (int bl = 0; bl < 2; ++bl)
+        c[t / kTiles][bl] = mfma16x16x32(codes_to_bf16<kBits>(a[t][bl].w), qt[t % kTiles][bl], c[t / kTiles][bl]);
     float s[kPasses][4];
 #pragma unroll
     for (int p = 0; p < kPasses; ++p) {

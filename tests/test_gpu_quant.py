@@ -357,6 +357,30 @@ def test_scores_that_drift(bits, pattern, splits, hq):
     check(got, q, k, v, used, 0.125)
 
 
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("hq,splits", [(6, 1), (16, 2), (24, 1)])
+@torch.inference_mode()
+def test_scores_far_below_zero(bits, hq, splits):
+    """Every score of a row the same number near -2^110: the mean of the values.
+    One position at half of it: that one's value."""
+    b, hkv, cap = 3, 2, 300
+    cache = QuantKVCache.empty(1, b, hkv, cap, DEV, bits=bits)
+    k = torch.full((b * cap, hkv, 1, 64), 2.0 ** 50, dtype=BF16, device=DEV)
+    k.view(b, cap, hkv, 64)[1, 77] /= 2
+    v = vectors((b * cap, hkv, 1, 64), 5).to(DEV)
+    cache.write(0, k, v, torch.arange(cap, device=DEV).repeat(b), None,
+                torch.arange(b, device=DEV).repeat_interleave(cap))
+    q = torch.full((b, hq, 1, 64), -2.0 ** 57, dtype=BF16, device=DEV)
+    used = torch.tensor([300, 299, 1], dtype=torch.int32, device=DEV)
+    flash = QuantFlashDecode(b, hkv, hq // hkv, cap, DEV, num_splits=splits, bits=bits)
+    got = flash(q, *cache.layer(0), None, None, 0.125, used=used)[:, :, 0].cpu().double()
+    held = cache.read(0)[1].cpu().double()
+    want = torch.stack([held[0].mean(1), held[1, :, 77], held[2, :, 0]]).repeat_interleave(hq // hkv, 1)
+    # equal probabilities are exactly 1, so the sums' roundings and the result's remain
+    tol = 2.0 ** -8 * want.abs() + 2.0 ** -24 * 364 * held.abs().amax()
+    assert bool(((got - want).abs() <= tol).all())
+
+
 @torch.inference_mode()
 def test_attention_past_32_bit_offsets():
     """One KV head whose codes pass 4 GiB: every key zero, so the softmax is
