@@ -28,13 +28,11 @@
 //
 // P.V: V^T . p with v_mfma_f32_16x16x32_bf16, A the transposed codes as bf16
 // (ds_read_b64_tr_b4 / _tr_b8 straight from the stage), B the probabilities times
-// 2^e of V's block, the probabilities rounded to bf16 as the bf16 kernel rounds them (8-bit parts
-// would lose the tail of a long row: 2^-18 of the largest probability, times its
-// length). A lane's scores are four consecutive positions of its column's tile,
-// which is the order that B takes them in; tiles 1 to 3 of a pass come to the
-// columns of tile 0 by row rotation, and only those columns of the result are
-// kept. A query head's columns share their running maximum; the waves merge once,
-// at the end.
+// 2^e of V's block, the probabilities rounded to bf16 as the bf16 kernel rounds
+// them. A lane's scores are four consecutive positions of its column's tile, which is
+// the order that B takes them in; tiles 1 to 3 of a pass come to the columns of tile 0
+// by row rotation, and only those columns of the result are kept. A query head's
+// columns share their running maximum; the waves merge once, at the end.
 //
 // Reference semantics: litemoe/flash_decode.py:16-22; masking litemoe/cache.py:42-47.
 #include "internal.h"
@@ -75,9 +73,9 @@ __device__ __forceinline__ int chunk_order(int position) {
   return kBits == 4 ? ((position >> 3) ^ (position >> 4)) & 1 : ((position >> 2) ^ (position >> 3 & 2)) & 3;
 }
 
-// Stages of a wave in LDS: one computed, one on its way. Three (4 bits) keep a wave's
-// loads in flight better, but four workgroups of two fit a CU: 128 ragged rows to
-// 4095 positions 36.2 us with three, 34.0 with two; 64 rows to 1279 the same.
+// Stages of a wave in LDS: one computed, one on its way. Four workgroups of two 4-bit
+// stages a wave fit a CU: 128 ragged rows to 4095 positions 35.1 us, with three
+// stages 37.7, in 8 bits 59.3 and 62.0; 64 rows to 1279 9.8 and 10.2.
 constexpr int kSlots = 2;
 
 // Direct global -> LDS copies (see lds_copy16) of 16 and 4 bytes per lane; kOffset
@@ -308,11 +306,11 @@ decode_quant_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, Cache 
     }
     __syncthreads();
   }
-  // The new key (lanes 0-7 of a wave) and value (8-15), eight channels each, quantised:
-  // by the wave that stores them and by the one whose stage holds their position.
+  // The new key (lanes 0-7 of sixteen) and value (8-15), eight channels each, quantised: by
+  // the wave that stores them and by the one whose stage holds their position.
   auto quantise_new = [&](uint32_t &byte) {
     float x[8];
-    unpack8(*reinterpret_cast<const u32x4 *>(&sm_row[kFused ? G + lane / 8 : 0][8 * (lane % 8)]), x);
+    unpack8(*reinterpret_cast<const u32x4 *>(&sm_row[kFused ? G + lane % 16 / 8 : 0][8 * (lane % 8)]), x);
     return quantise8<kBits>(x, byte);
   };
   // Channels 32 bl + 8 grp and on of the column's query head.
@@ -357,7 +355,8 @@ decode_quant_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, Cache 
 #pragma unroll
   for (int c = 0; c < kBits / 2; ++c) {
     const int position = kBits == 4 ? 16 * (col / 4) + 4 * grp + col % 4 : 16 * (col / 8) + 4 * grp + col / 2 % 4;
-    v_off[c] = St::kSide + position * St::kCode + (c ^ chunk_order<kBits>(position)) * 16 + (kBits == 8 ? 8 * (col % 2) : 0);
+    v_off[c] = St::kSide + position * St::kCode + (c ^ chunk_order<kBits>(position)) * 16 +
+               (kBits == 8 ? 8 * (col % 2) : 0);
   }
 
   auto compute = [&](int it, int slot) {
@@ -366,15 +365,17 @@ decode_quant_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, Cache 
     const int count = k1 - start;  // positions of the stage that count, if fewer than 64
     if constexpr (kFused) {
       if (own && pnew >= start && pnew < start + kStageKeys) {
+        // Where it is the row's last, the masked slots behind it repeat the bytes that its
+        // position held before, which may be no numbers in 8 bits: they take its codes too.
         const int at = (int)(pnew - start);
-        if (lane < 16) {
-          uint32_t byte;
-          const Codes8<kBits> c = quantise_new(byte);
-          const int byte8 = lane % 8 * kBits;  // of the vector's codes
-          *reinterpret_cast<Codes8<kBits> *>(st + lane / 8 * St::kSide + at * St::kCode +
-                                             (byte8 / 16 ^ chunk_order<kBits>(at)) * 16 + byte8 % 16) = c;
-          if (lane % 4 == 0) st[2 * St::kSide + 4 * at + lane / 4] = (uint8_t)byte;
-        }
+        const int until = kBits == 8 && at == count - 1 ? kStageKeys : at + 1;
+        uint32_t byte;
+        const Codes8<kBits> c = quantise_new(byte);
+        const int side = lane % 16 / 8, byte8 = lane % 8 * kBits;  // of the vector's codes
+        for (int slot = at + lane / 16; slot < until; slot += 4)
+          *reinterpret_cast<Codes8<kBits> *>(st + side * St::kSide + slot * St::kCode +
+                                             (byte8 / 16 ^ chunk_order<kBits>(slot)) * 16 + byte8 % 16) = c;
+        if (lane < 16 && lane % 4 == 0) st[2 * St::kSide + 4 * at + lane / 4] = (uint8_t)byte;
         lds_reads_done();
       }
     }
@@ -676,14 +677,17 @@ int launch_decode_quant(const Call &c, const void *q, int64_t qs0, int64_t qs1, 
   };
   // Up to one workgroup per CU a wave has its SIMD to itself, and a 4-bit stage's chain
   // of dependent steps (0.57 us) takes longer than its bytes: eight waves where
-  // they get two stages each. 32 rows to 4095 positions 15.7 us with four, 13.9 with
-  // eight; 24 rows to 2000 9.0 and 8.1; 10 rows to 1000 5.9 and 6.0, one row of 512 4.1
-  // and 4.6. In 8 bits the two are alike (32 rows to 4095 21.9 and 22.0).
+  // they get two stages each. 24 rows to 2000 positions 8.6 us with four, 7.6 with eight;
+  // 32 rows to 4095 15.2 and 14.3, 8 rows to 32768 in four splits 26.9 and 21.7; 10 rows
+  // to 1000 5.4 and 5.5, one row of 509 3.6 and 3.8. In 8 bits they differ by 2 to 4% (32
+  // rows to 4095 22.5 and 21.9), which a second set of kernels is not worth.
   const bool wide = c.bits == 4 && (int64_t)splits * c.kv_heads * c.batch <= 256 && chunk >= 16 * kStageKeys;
   typedef std::integral_constant<int, 4> Four;
   typedef std::integral_constant<int, 8> Eight;
   auto run = [&](auto fused) {
-    return c.bits == 8 ? pick(fused, Eight{}, Four{}) : wide ? pick(fused, Four{}, Eight{}) : pick(fused, Four{}, Four{});
+    return c.bits == 8 ? pick(fused, Eight{}, Four{})
+           : wide      ? pick(fused, Four{}, Eight{})
+                       : pick(fused, Four{}, Four{});
   };
   const int status = in.part ? run(std::true_type{}) : run(std::false_type{});
   if (status != LM_OK || splits == 1) return status;

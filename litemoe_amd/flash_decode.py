@@ -139,14 +139,16 @@ def quant_splits(batch, kv_heads, maximum):
     lines, since a position takes a quarter or half of the bytes.
 
     Up to 256 (row, head) pairs, one workgroup per CU, the splits fill the CUs
-    and no more; a split keeps 512 positions at least and contexts below three
-    times that are not split, since the second launch costs 1.6 to 2 us. us per
-    launch in a graph: one row x 8 heads to 1000 positions 7.3 (1 split) and 7.7
-    (4); to 4000 12.0 (1), 8.0 (4) and 7.6 (7); 5 rows to 4000 10.0 (1), 8.4 (4)
-    and 9.2 (8); 8 rows to 32768 30.3 (2), 22.0 (4) and 23.1 (8); 32 rows to 4095
-    13.9 (1) and 15.7 (2); 64 rows to 1279 10.0 (1) and 13.0 (2). More than 16
-    only for contexts past 65536: the second launch loads 16 at a time."""
-    longest = maximum // 512 if maximum >= 3 * 512 else 1
+    and no more. A split takes 512 positions, two stages of each of a workgroup's
+    four waves, or more, and contexts below three times that are not split: the
+    second launch costs 1.6 to 2 us. us per launch in a graph, 4 bits: one row x 8
+    heads to 1000 positions 6.4 (1 split) and 6.8 (4); to 4000 10.1 (1), 7.5 (4),
+    7.0 (8) and 6.6 (16); 3 rows to 4001 7.8 (4), 7.9 (7), 7.4 (8) and 7.7 (16); 16
+    rows to 4095 10.3 (2) and 11.5 (8); 8 rows to 32768 32.7 (2), 21.7 (4) and 24.2
+    (8); 32 rows to 4095 14.3 (1) and 15.1 (2); 64 rows to 1279 9.9 (1) and 12.9
+    (2). More than 16 only for contexts past 65536, since the second launch loads
+    16 at a time."""
+    longest = -(-maximum // 512) if maximum >= 3 * 512 else 1
     return max(1, min(max(16, maximum // 4096), 256 // max(1, batch * kv_heads), longest))
 
 
@@ -211,8 +213,8 @@ class QuantFlashDecode:
         used = kv_quant.per_row(used, b, torch.int32, index, "used")
         out = torch.empty((b, hq, 1, 64), device=q.device, dtype=torch.bfloat16)
         _lib.call_on(index, "lm_flash_decode_quant", q.data_ptr(), rows, heads, k.data_ptr(), v.data_ptr(),
-                     scales.data_ptr(), used.data_ptr(), b, hq, self.kv_heads, self.capacity, 64, self.bits, float(scale),
-                     self.maximum, self.splits, out.data_ptr(), self.workspace.data_ptr(), self.workspace.numel())
+                     scales.data_ptr(), used.data_ptr(), b, hq, self.kv_heads, self.capacity, 64, self.bits,
+                     float(scale), self.maximum, self.splits, out.data_ptr(), self.workspace.data_ptr(), self.workspace.numel())
         return out
 
     def fused_qkv(self, partials, cos_sin, positions, active, k, v, scales, scale, used, q_heads, row_order=None,

@@ -137,7 +137,8 @@ def test_store_of_every_kind_of_block(bits):
     blocks = [torch.zeros(32), torch.full((32,), -0.0), torch.randn(32, generator=g) * 2.0 ** -130,
               torch.full((32,), 2.0 ** -133), torch.randn(32, generator=g).clamp(-1.9, 1.9) * 2.0 ** 127,
               torch.full((32,), 3.3895e38), torch.linspace(-top, top, 32), torch.linspace(0, 2, 32) * 2.0 ** 40,
-              torch.arange(32) * 0.25, torch.arange(32) * -0.125, torch.cat((torch.tensor([top]), torch.rand(31, generator=g))),
+              torch.arange(32) * 0.25, torch.arange(32) * -0.125,
+              torch.cat((torch.tensor([top]), torch.rand(31, generator=g))),
               torch.cat((torch.tensor([top * 1.01]), torch.rand(31, generator=g))), torch.full((32,), top * 2.0 ** 118),
               torch.cat((torch.tensor([1.0]), torch.full((31,), 2.0 ** -12)))]
     grid = quant.grid(bits)
@@ -256,10 +257,12 @@ def test_attention_lengths_bounds_and_strided_queries(bits):
     wide = vectors((b, hq + 4, 64), 8).to(DEV)
     q = wide[:, 2:2 + hq].unsqueeze(2)
     flash = QuantFlashDecode(7, hkv, 3, cap, DEV, maximum=150, num_splits=2, bits=bits)
-    lengths, active = torch.tensor([62, 999, 0, 149, 10], device=DEV), torch.tensor([True, False, True, True, True], device=DEV)
+    lengths = torch.tensor([62, 999, 0, 149, 10], device=DEV)
+    active = torch.tensor([True, False, True, True, True], device=DEV)
     got = flash(q, *cache.layer(0), lengths, active, 0.125)[:, :, 0]
     check(got, q[:, :, 0].cpu(), k[0], v[0], torch.tensor([63, 1, 1, 150, 11]), 0.125)
-    got = flash(q, *cache.layer(0), None, None, 0.125, used=torch.tensor([-3, 150, 151, 1 << 30, 149], device=DEV))[:, :, 0]
+    used = torch.tensor([-3, 150, 151, 1 << 30, 149], device=DEV)
+    got = flash(q, *cache.layer(0), None, None, 0.125, used=used)[:, :, 0]
     check(got, q[:, :, 0].cpu(), k[0], v[0], torch.tensor([0, 150, 150, 150, 149]), 0.125)
 
 
@@ -276,8 +279,9 @@ def test_masked_positions_are_never_seen(bits, hq, splits):
     flash = QuantFlashDecode(b, hkv, hq // hkv, cap, DEV, num_splits=splits, bits=bits)
     before = flash(q, *cache.layer(0), None, None, 0.125, used=used.to(DEV))
     past = (torch.arange(cap)[None] >= used[:, None]).to(DEV)
-    for t, fill in ((cache.k, 256), (cache.v, 256), (cache.scales, 256)):
-        t[0].copy_(torch.where(past[:, None, :, None], torch.randint(0, fill, t[0].shape, device=DEV, dtype=torch.uint8), t[0]))
+    for t in (cache.k, cache.v, cache.scales):
+        noise = torch.randint(0, 256, t[0].shape, device=DEV, dtype=torch.uint8)
+        t[0].copy_(torch.where(past[:, None, :, None], noise, t[0]))
     cache.scales[0].masked_fill_((past & (torch.arange(cap, device=DEV) % 3 == 0))[:, None, :, None], 255)
     after = flash(q, *cache.layer(0), None, None, 0.125, used=used.to(DEV))
     assert torch.equal(before, after) and torch.isfinite(after).all()
@@ -464,6 +468,30 @@ def test_fused_equals_the_separate_operators(bits, b, hq, hkv, cap, splits, slic
 
 
 @pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("hq,splits", [(6, 1), (6, 3), (16, 1), (32, 1)])
+@torch.inference_mode()
+def test_fused_over_positions_that_were_never_written(bits, hq, splits):
+    """The new token's position and all behind it hold the worst bytes there are,
+    8-bit codes that are no numbers and NaN scales: they are replaced or never
+    looked at."""
+    b, hkv, cap = 7, 2, 333
+    used = torch.tensor([1, 2, 64, 65, 100, 129, 333], dtype=torch.int32, device=DEV)
+    positions = used.long() - 1
+    caches = [random_cache(bits, b, hkv, cap, 55)[0] for _ in range(2)]
+    behind = (torch.arange(cap, device=DEV)[None] >= positions[:, None])[:, None, :, None]
+    for t, worst in zip(caches[1].layer(0), (0x7f, 0xff, 0xff)):
+        t.masked_fill_(behind, worst)
+    part, table = fused_inputs(b, hq, hkv, cap, 8)
+    flash = QuantFlashDecode(b, hkv, hq // hkv, cap, DEV, num_splits=splits, bits=bits)
+    want, got = (flash.fused_qkv(part, table, positions, None, *c.layer(0), 0.125, used, hq) for c in caches)
+    assert torch.isfinite(want).all() and torch.equal(got, want)
+    at = (torch.arange(b, device=DEV), slice(None), positions)
+    assert all(torch.equal(x[at], y[at]) for x, y in zip(caches[0].layer(0), caches[1].layer(0)))
+    again = flash(torch.zeros(b, hq, 1, 64, dtype=BF16, device=DEV), *caches[1].layer(0), None, None, 0.125, used=used)
+    assert torch.isfinite(again).all()
+
+
+@pytest.mark.parametrize("bits", [4, 8])
 @torch.inference_mode()
 def test_fused_matches_oracle(bits):
     b, hq, hkv, cap = 6, 24, 8, 150
@@ -566,7 +594,7 @@ def test_refusals_on_the_device():
     with pytest.raises(ValueError, match="another cache type"):
         flash(x, *eight.layer(0), None, None, 0.125, used=used)
     with pytest.raises(ValueError, match="batch/capacity"):
-        flash(torch.zeros(3, 2, 1, 64, dtype=BF16, device=DEV), *layer, None, None, 0.125, used=torch.ones(3, device=DEV))
+        flash(torch.zeros(3, 2, 1, 64, dtype=BF16, device=DEV), *layer, None, None, 0.125, used=used)
     with pytest.raises(ValueError, match="batch/capacity"):
         flash(x, *QuantKVCache.empty(1, 2, 2, 32, DEV, bits=4).layer(0), None, None, 0.125, used=used)
     with pytest.raises(ValueError, match="Query heads"):
@@ -607,7 +635,8 @@ def test_prefill_writes_what_the_bf16_cache_holds(bits, epilogue):
     packed, ends = build_packed(lengths, DEV)
     tokens = torch.randint(1, 512, (1, sum(lengths)), generator=gen(1)).to(DEV)
     valid = torch.ones_like(tokens, dtype=torch.bool)
-    logits = [model.forward(tokens, packed.positions[None], valid, c, slot=packed, last=ends.long() - 1) for c in caches]
+    logits = [model.forward(tokens, packed.positions[None], valid, c, slot=packed, last=ends.long() - 1)
+              for c in caches]
     assert torch.equal(*logits)
     padded = torch.randint(1, 512, (2, 20), generator=gen(2)).to(DEV)
     columns = torch.arange(20, device=DEV)[None].expand(2, -1)

@@ -10,7 +10,7 @@ from litemoe_amd import _lib, kv_quant
 from litemoe_amd.cache import KVCache, QuantKVCache
 from litemoe_amd.config import preset
 from litemoe_amd.engine import Engine
-from litemoe_amd.flash_decode import QuantFlashDecode
+from litemoe_amd.flash_decode import QuantFlashDecode, quant_splits
 from litemoe_amd.linear import linear_rope_kv
 from oracle import quant
 
@@ -163,7 +163,22 @@ def test_status_codes_before_launch(call, over, expected):
 
 def test_oracle_attention_of_an_empty_row_and_of_one_position():
     g = torch.Generator().manual_seed(5)
-    q, k, v = torch.randn(2, 4, 64, generator=g), torch.randn(2, 2, 8, 64, generator=g), torch.randn(2, 2, 8, 64, generator=g)
+    q, k, v = torch.randn(2, 4, 64, generator=g), *torch.randn(2, 2, 2, 8, 64, generator=g)
     out = quant.decode_attention(q, k, v, torch.tensor([0, 1]), 1 / math.sqrt(64))
     assert not bool(out[0].any())
     assert torch.allclose(out[1], v[1, :, 0].repeat_interleave(2, 0).double())
+
+
+@pytest.mark.parametrize("batch,kv_heads,maximum,splits", [
+    (1, 8, 1, 1), (1, 8, 1535, 1), (1, 8, 1536, 3), (1, 8, 4000, 8), (3, 8, 4001, 8), (5, 8, 4000, 6), (8, 8, 32768, 4),
+    (16, 8, 4095, 2), (17, 8, 4095, 1), (32, 8, 4095, 1), (64, 8, 1279, 1), (128, 8, 4096, 1), (1, 1, 32768, 16),
+    (1, 1, 1 << 20, 256)])
+def test_quant_splits(batch, kv_heads, maximum, splits):
+    assert quant_splits(batch, kv_heads, maximum) == splits
+
+
+def test_quant_splits_fill_the_cus_and_keep_512_positions():
+    for batch in (1, 2, 5, 16, 31, 33, 200):
+        for maximum in (1, 511, 1536, 4096, 32768, 1 << 20):
+            n = quant_splits(batch, 8, maximum)
+            assert n >= 1 and (n == 1 or (n * batch * 8 <= 256 and -(-maximum // n) > 512 - 64))
