@@ -137,8 +137,12 @@ def _check_single_runtime():
 def call(name: str, *args) -> None:
     status = getattr(lib(), name)(*args)
     if status:
-        message = lib().lm_status_string(status).decode()
-        raise NativeError(f"{name} failed with status {status} ({message})")
+        raise _error(name, status)
+
+
+def _error(name: str, status: int) -> NativeError:
+    message = lib().lm_status_string(status).decode()
+    return NativeError(f"{name} failed with status {status} ({message})")
 
 
 def size_query(name: str, *args) -> int:
@@ -163,10 +167,12 @@ def call_on(index: int, name: str, *args) -> None:
     """:func:`call` with device ``index`` current and its current stream as the
     last argument. Kernels run on the current device, so a call on another
     device's tensors has to make it current; the usual call has nothing to change."""
-    if index == torch.cuda.current_device():
-        return call(name, *args, torch._C._cuda_getCurrentRawStream(index))
-    with torch.cuda.device(index):
-        return call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+    status = getattr(lib(), name)(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        raise _error(name, status)
 
 
 def require_cuda(*tensors: torch.Tensor, what: str = "tensors") -> None:

@@ -211,7 +211,7 @@ class QuantFlashDecode:
         if used is None:
             used = torch.where(active, lengths + 1, 1)
         used = kv_quant.per_row(used, b, torch.int32, index, "used")
-        out = torch.empty((b, hq, 1, 64), device=q.device, dtype=torch.bfloat16)
+        out = torch.empty_like(q) if q.is_contiguous() else torch.empty(q.shape, device=q.device, dtype=q.dtype)
         _lib.call_on(index, "lm_flash_decode_quant", q.data_ptr(), rows, heads, k.data_ptr(), v.data_ptr(),
                      scales.data_ptr(), used.data_ptr(), b, hq, self.kv_heads, self.capacity, 64, self.bits,
                      float(scale), self.maximum, self.splits, out.data_ptr(), self.workspace.data_ptr(), self.workspace.numel())

@@ -24,9 +24,9 @@ def check_layer(k, v, scales):
         raise ValueError("Quantised KV cache layers must share one device")
     if len(shape) != 4 or shape[3] not in (32, 64) or v.shape != shape or scales.shape != (*shape[:3], 4):
         raise ValueError("Quantised KV cache layers are k, v [B, H, C, 8*bits] and scales [B, H, C, 4], bits 4 or 8")
-    for t in (k, v, scales):
-        if t.dtype != torch.uint8 or not t.is_contiguous():
-            raise ValueError("Quantised KV cache layers must be contiguous uint8")
+    if not (k.dtype == v.dtype == scales.dtype == torch.uint8 and k.is_contiguous() and v.is_contiguous()
+            and scales.is_contiguous()):
+        raise ValueError("Quantised KV cache layers must be contiguous uint8")
     return shape[3] // 8, index
 
 
