@@ -240,12 +240,14 @@ decode_quant_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, Cache 
     const int position = (c * kWave + lane) / kChunks;
     copy_off[c] = (position - c * kWave / kChunks) * St::kCode + (lane % kChunks ^ chunk_order<kBits>(position)) * 16;
   }
-  // Requests stage `it` into its slot, its start a 64-bit scalar. Positions past the
-  // range repeat its last one: masked, and never bytes that the row does not hold (an
-  // 8-bit code may be a NaN there).
+  // Requests stage `it` into its slot, its start a 64-bit scalar. Slots past the range
+  // repeat its last position: masked, and never bytes that the row does not hold (an
+  // 8-bit code may be a NaN there). So where that position is the new token's, which the
+  // cache does not hold yet, they repeat the one before it.
   auto issue = [&](int it, int slot) {
     const int start = k0 + (it * kWaves + wave) * kStageKeys;
     const int last = k1 - 1 - start;
+    const int repeat = max(kFused && own && pnew == k1 - 1 ? last - 1 : last, 0);
     const int64_t at = first_pos + start;
     const uint32_t lds = my_lds + slot * St::kBytes;
     const uint8_t *kg = cache.k + at * St::kCode, *vg = cache.v + at * St::kCode;
@@ -269,7 +271,7 @@ decode_quant_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, Cache 
 #pragma unroll
     for (int c = 0; c < St::kSideCopies; ++c) {
       const int position = (c * kWave + lane) / kChunks;
-      const uint32_t off = (uint32_t)min(position, last) * St::kCode + copy_off[c % 2] % St::kCode;
+      const uint32_t off = (uint32_t)(position <= last ? position : repeat) * St::kCode + copy_off[c % 2] % St::kCode;
       stage_copy16<0>(kg, off, lds + c * 1024);
       stage_copy16<0>(vg, off, lds + St::kSide + c * 1024);
     }
@@ -365,10 +367,10 @@ decode_quant_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, Cache 
     const int count = k1 - start;  // positions of the stage that count, if fewer than 64
     if constexpr (kFused) {
       if (own && pnew >= start && pnew < start + kStageKeys) {
-        // Where it is the row's last, the masked slots behind it repeat the bytes that its
-        // position held before, which may be no numbers in 8 bits: they take its codes too.
+        // A stage that holds nothing else repeats the bytes of its position from before,
+        // which may be no numbers in 8 bits: every slot takes the new codes.
         const int at = (int)(pnew - start);
-        const int until = kBits == 8 && at == count - 1 ? kStageKeys : at + 1;
+        const int until = kBits == 8 && count == 1 ? kStageKeys : at + 1;
         uint32_t byte;
         const Codes8<kBits> c = quantise_new(byte);
         const int side = lane % 16 / 8, byte8 = lane % 8 * kBits;  // of the vector's codes
