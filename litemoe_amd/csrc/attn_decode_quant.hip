@@ -374,9 +374,9 @@ decode_quant_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, Cache 
         uint32_t byte;
         const Codes8<kBits> c = quantise_new(byte);
         const int side = lane % 16 / 8, byte8 = lane % 8 * kBits;  // of the vector's codes
-        for (int slot = at + lane / 16; slot < until; slot += 4)
-          *reinterpret_cast<Codes8<kBits> *>(st + side * St::kSide + slot * St::kCode +
-                                             (byte8 / 16 ^ chunk_order<kBits>(slot)) * 16 + byte8 % 16) = c;
+        for (int to = at + lane / 16; to < until; to += 4)
+          *reinterpret_cast<Codes8<kBits> *>(st + side * St::kSide + to * St::kCode +
+                                             (byte8 / 16 ^ chunk_order<kBits>(to)) * 16 + byte8 % 16) = c;
         if (lane < 16 && lane % 4 == 0) st[2 * St::kSide + 4 * at + lane / 4] = (uint8_t)byte;
         lds_reads_done();
       }

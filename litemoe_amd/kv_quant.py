@@ -31,8 +31,8 @@ def check_layer(k, v, scales):
 
 
 def per_row(t, rows, dtype, index, what):
-    """``t [rows]`` on device ``index`` as a contiguous tensor of ``dtype``."""
-    if t.get_device() != index or t.shape != (rows,):
+    """``t``, one entry per row on device ``index``, as a contiguous tensor of ``dtype``."""
+    if t.get_device() != index or t.numel() != rows:
         raise ValueError(f"{what} needs one entry per row, on the cache's device")
     if t.dtype != dtype:
         t = t.to(dtype)

@@ -8,9 +8,10 @@ import pytest
 import torch
 
 from litemoe_amd import kv_quant, synth
+from litemoe_amd.batch import BatchPrefillEngine
 from litemoe_amd.cache import KVCache, QuantKVCache
 from litemoe_amd.config import preset
-from litemoe_amd.engine import Request
+from litemoe_amd.engine import Engine, Request
 from litemoe_amd.ep import ExpertParallel
 from litemoe_amd.execution import capture_decode
 from litemoe_amd.experts import HipFusedExperts
@@ -185,7 +186,7 @@ def test_store_takes_any_strides(bits):
     for k, v in zip(views, views[1:] + views[:1]):
         cache = [QuantKVCache.empty(1, rows, heads, 2, DEV, bits=bits) for _ in range(2)]
         cache[0].write(0, k, v, torch.ones_like(every), None)
-        cache[1].write(0, k.contiguous(), v.contiguous(), torch.ones_like(every), None)
+        cache[1].write(0, k.contiguous(), v.contiguous(), torch.ones_like(every)[:, None], None)
         assert bool(cache[0].scales.any())
         for a, b in zip(cache[0].layer(0), cache[1].layer(0)):
             assert torch.equal(a, b)
@@ -731,6 +732,26 @@ def test_engine_runs_on_the_quantised_cache(bits, model_name):
         assert other[0] == runs[0][0]
         assert all(torch.equal(a, c) for a, c in zip(other[1], runs[0][1]))
     assert all(runs[3][0][r][0] == o[0] for r, o in runs[0][0].items())
+
+
+@pytest.mark.parametrize("kind", [Engine, BatchPrefillEngine])
+@torch.inference_mode()
+def test_every_engine_takes_the_quantised_cache(kind):
+    """The engines without the optimized policy (masked decode, one padded
+    prefill per request or per batch): eager and captured steps agree, and the
+    first tokens are the bf16 cache's."""
+    cfg, _ = small_model()
+    prompts = synth.prompts(3, [5, 21, 9], cfg.vocab_size, 7)
+    runs = []
+    for mode, kv_bits in (("eager", 8), ("graph", 8), ("eager", 16)):
+        model = small_model()[1]
+        run = kind(model, [Request(str(i), p, 6) for i, p in enumerate(prompts)], mode=mode, ignore_eos=True,
+                   kv_bits=kv_bits, capacity=64)
+        out, _ = run.generate()
+        assert all(len(o) == 6 for o in out.values())
+        runs.append((out, run.cache.k.clone()))
+    assert runs[0][0] == runs[1][0] and torch.equal(runs[0][1], runs[1][1])
+    assert all(runs[2][0][r][0] == o[0] for r, o in runs[0][0].items())
 
 
 @torch.inference_mode()
