@@ -256,14 +256,14 @@ decode_quant_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, Cache 
       stage_copy16<0>(kg, copy_off[0], lds);
       stage_copy16<1024>(kg, copy_off[1], lds);
       if constexpr (kBits == 8) {
-        stage_copy16<2048>(kg, copy_off[0], lds);
-        stage_copy16<3072>(kg, copy_off[1], lds);
+        stage_copy16<2 * 1024>(kg, copy_off[0], lds);
+        stage_copy16<3 * 1024>(kg, copy_off[1], lds);
       }
       stage_copy16<0>(vg, copy_off[0], lds + St::kSide);
       stage_copy16<1024>(vg, copy_off[1], lds + St::kSide);
       if constexpr (kBits == 8) {
-        stage_copy16<2048>(vg, copy_off[0], lds + St::kSide);
-        stage_copy16<3072>(vg, copy_off[1], lds + St::kSide);
+        stage_copy16<2 * 1024>(vg, copy_off[0], lds + St::kSide);
+        stage_copy16<3 * 1024>(vg, copy_off[1], lds + St::kSide);
       }
       stage_copy4(cache.scales + at, lane * 4, lds + 2 * St::kSide);
       return;
