@@ -54,9 +54,13 @@ def random_cache(bits, batch, heads, capacity, seed, layers=1):
 
 
 def bound(q, k, v, used, scale, out):
-    """How far a row's outputs may be from the exact ones, per element:
-    * a probability times V's scale is rounded to bf16 (2^-8 of it), a result
-      too: 2^-8 (A + |out|), A = sum p|v| / sum p;
+    """How far a row's outputs may be from the exact ones, per element, with
+    A = sum p|v| / sum p:
+    * probabilities are rounded to bf16, p(1 + d) with |d| <= 2^-8, and summed as
+      rounded (V's scale is a power of two and adds no rounding):
+      sum p(1 + d)v / sum p(1 + d) - out = sum pd(v - out) / sum p(1 + d), at most
+      2^-8 (A + |out|) / (1 - 2^-8); the result's own rounding adds 2^-8 of it. Together
+      less than 2^-8 (1 + 2^-6) (A + 2|out|);
     * a score is a sum of 64 products in fp32 with 64 + 8 roundings of at most
       2^-24 of sum|q k|; that moves p by the same share, in numerator and
       denominator, and the sums over n positions (in any order, with the
@@ -74,8 +78,8 @@ def bound(q, k, v, used, scale, out):
         p = torch.softmax(qi @ ki.transpose(1, 2) * scale, -1)
         a = (p @ vi.abs()).reshape(hq, 64)
         size = (qi.abs() @ ki.abs().transpose(1, 2)).amax(-1).reshape(hq, 1) * scale
-        both = a + out[i].abs()
-        tol[i] = (2.0 ** -8 + 2.0 ** -24 * (2 * 72 * size + n + 64)) * both
+        o = out[i].abs()
+        tol[i] = 2.0 ** -8 * (1 + 2.0 ** -6) * (a + 2 * o) + 2.0 ** -24 * (2 * 72 * size + n + 64) * (a + o)
     return tol + 1e-30
 
 
