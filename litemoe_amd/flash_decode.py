@@ -147,9 +147,20 @@ def quant_splits(batch, kv_heads, maximum):
     rows to 4095 10.1 (2) and 10.7 (8); 8 rows to 32768 32.6 (2), 21.5 (4) and 23.7
     (8); 32 rows to 4095 13.9 (1) and 15.3 (2); 64 rows to 1279 9.9 (1) and 12.9
     (2). More than 16 only for contexts past 65536, since the second launch loads
-    16 at a time."""
+    16 at a time.
+
+    From 8192 positions on, up to 320 pairs take eight splits or more: a row's splits
+    share its length evenly, so ragged rows fill the CUs better in many short pieces.
+    20 rows of 4000 to 16000 positions 30.4 us (1) and 23.7 (8), in 8 bits 52 and 37; 12
+    rows 19.8 (2) and 15.9 (8); 40 rows of 4000 to 8192 30.8 (1) and 28.4 (8); rows of one
+    length lose less: 12 to 16000 21.4 (2) and 21.9 (8), 20 31.1 (1) and 33.3 (8), 40
+    58.9 (1) and 59.2 (8). 256 pairs fill the CUs as they are: 35.0 either way, 43.2
+    and 47.3 at one length; from 384 on there is little to gain (48 rows to 16000 55.9
+    either way) and up to 7% to lose."""
+    pairs = max(1, batch * kv_heads)
     longest = -(-maximum // 512) if maximum >= 3 * 512 else 1
-    return max(1, min(max(16, maximum // 4096), 256 // max(1, batch * kv_heads), longest))
+    filling = max(1, min(max(16, maximum // 4096), 256 // pairs, longest))
+    return max(8, filling) if maximum >= 8192 and pairs <= 320 and pairs != 256 else filling
 
 
 class QuantFlashDecode:

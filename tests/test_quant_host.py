@@ -170,8 +170,8 @@ def test_oracle_attention_of_an_empty_row_and_of_one_position():
 
 
 @pytest.mark.parametrize("batch,kv_heads,maximum,splits", [
-    (1, 8, 1, 1), (1, 8, 1535, 1), (1, 8, 1536, 3), (1, 8, 4000, 8), (3, 8, 4001, 8), (5, 8, 4000, 6), (8, 8, 32768, 4),
-    (16, 8, 4095, 2), (17, 8, 4095, 1), (32, 8, 4095, 1), (64, 8, 1279, 1), (128, 8, 4096, 1), (1, 1, 32768, 16),
+    (1, 8, 1, 1), (1, 8, 1535, 1), (1, 8, 1536, 3), (1, 8, 4000, 8), (3, 8, 4001, 8), (5, 8, 4000, 6), (8, 8, 8191, 4),
+    (8, 8, 8192, 8), (20, 8, 16000, 8), (40, 8, 8192, 8), (32, 8, 32768, 1), (41, 8, 32768, 1), (16, 8, 4095, 2), (17, 8, 4095, 1), (32, 8, 4095, 1), (64, 8, 1279, 1), (128, 8, 4096, 1), (1, 1, 32768, 16),
     (1, 1, 1 << 20, 256)])
 def test_quant_splits(batch, kv_heads, maximum, splits):
     assert quant_splits(batch, kv_heads, maximum) == splits
@@ -181,4 +181,5 @@ def test_quant_splits_fill_the_cus_and_keep_512_positions():
     for batch in (1, 2, 5, 16, 31, 33, 200):
         for maximum in (1, 511, 1536, 4096, 32768, 1 << 20):
             n = quant_splits(batch, 8, maximum)
-            assert n >= 1 and (n == 1 or (n * batch * 8 <= 256 and -(-maximum // n) > 512 - 64))
+            assert n >= 1 and (n == 1 or -(-maximum // n) > 512 - 64)
+            assert n * batch * 8 <= 256 or n == 1 or (n == 8 and maximum >= 8192)
