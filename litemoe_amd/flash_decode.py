@@ -144,7 +144,7 @@ def quant_splits(batch, kv_heads, maximum):
     second launch costs 1.5 to 2 us. us per launch in a graph, 4 bits: one row x 8
     heads to 1000 positions 6.4 (1 split) and 6.8 (4); to 4000 10.0 (1), 7.2 (4),
     6.3 (8) and 6.2 (16); 3 rows to 4001 10.2 (1), 7.5 (4), 6.7 (8) and 7.4 (16); 16
-    rows to 4095 10.1 (2) and 10.7 (8); 8 rows to 32768 32.6 (2), 21.5 (4) and 23.7
+    rows to 4095 10.1 (2) and 10.7 (8); 8 rows to 32768 32.3 (2), 21.9 (4) and 20.5
     (8); 32 rows to 4095 13.9 (1) and 15.3 (2); 64 rows to 1279 9.9 (1) and 12.9
     (2). More than 16 only for contexts past 65536, since the second launch loads
     16 at a time.
