@@ -83,7 +83,10 @@ def parse():
     ap.add_argument("--long-decode", action="store_true", help="cfg 5 decode step tok/s (own JSON line)")
     ap.add_argument("--kv-bits", type=int, default=16, choices=(4, 8, 16),
                     help="with --long-decode: bits per KV cache element (8 and 4 hold the cache quantised)")
-    return ap.parse_args()
+    args = ap.parse_args()
+    if args.kv_bits != 16 and not args.long_decode:
+        ap.error("--kv-bits goes with --long-decode")
+    return args
 
 
 def measured_traffic(name):

@@ -272,6 +272,48 @@ def test_attention_lengths_bounds_and_strided_queries(bits):
 
 
 @pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("splits,most", [(None, 8300), (7, 8300), (3, 8300), (1000, 8300), (9, 513)])
+@torch.inference_mode()
+def test_splits_share_each_rows_own_length(bits, splits, most):
+    """Rows of every kind of length in one call, at the edges of stages and of
+    splits, and the same graph over other lengths; the fused form beside it, its
+    new token in the first, a middle or the last split, or behind the row."""
+    cap, hq, hkv = 8320, 3, 1
+    lengths = torch.tensor([8300, 8192, 4097, 1025, 513, 512, 511, 449, 448, 65, 64, 1, 0], dtype=torch.int32)
+    b = lengths.numel()
+    cache, k, v = random_cache(bits, b, hkv, cap, 12)
+    q = (2 * torch.randn(b, hq, 64, generator=gen(9))).to(BF16)
+    flash = QuantFlashDecode(b, hkv, hq, cap, DEV, maximum=most, num_splits=splits, bits=bits)
+    used, qd = lengths.to(DEV), q.to(DEV)[:, :, None]
+
+    out = torch.empty_like(qd)
+
+    def step():
+        out.copy_(flash(qd, *cache.layer(0), None, None, 0.125, used=used))
+
+    graph = capture_decode(step, lambda: None)
+    for turn in range(3):
+        now = lengths.roll(turn)
+        used.copy_(now)
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        check(out[:, :, 0], q, k[0], v[0], now.clamp(max=most), 0.125)
+        assert torch.equal(out, flash(qd, *cache.layer(0), None, None, 0.125, used=used))
+
+    caches = [random_cache(bits, b, hkv, cap, 12)[0] for _ in range(2)]
+    part, table = fused_inputs(b, hq, hkv, cap, 4)
+    for back in (1, 70, 600, -40):
+        used.copy_(lengths)
+        positions = (lengths.long() - back).to(DEV)
+        want = unfused(flash, caches[0], part, table, positions, None, used, hq, hkv)
+        got = flash.fused_qkv(part, table, positions, None, *caches[1].layer(0), 0.125, used, hq)
+        assert torch.equal(got, want)
+        for x, y in zip(caches[0].layer(0), caches[1].layer(0)):
+            assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
 @pytest.mark.parametrize("hq,splits", [(6, 1), (16, 3), (2, 1)])
 @torch.inference_mode()
 def test_masked_positions_are_never_seen(bits, hq, splits):
