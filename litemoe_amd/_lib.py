@@ -155,11 +155,18 @@ def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
-def stream(device: torch.device | None = None) -> int:
+def stream(device: torch.device | str | int | None = None) -> int:
     """The current stream of ``device`` (the current device's by default) as the
     handle a C call takes, without a ``torch.cuda.Stream`` object around it (1.9 us
-    of a call's host time)."""
-    index = None if device is None else device.index
+    of a call's host time). ``device`` as ``torch.cuda.current_stream`` takes it; any
+    but a GPU is refused, so that no host tensor's address reaches a kernel."""
+    index = None
+    if device is not None:
+        if not isinstance(device, torch.device):
+            device = torch.device(device)
+        if device.type != "cuda":
+            raise ValueError(f"Kernels run on a ROCm device, not on {device}")
+        index = device.index
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 

@@ -99,3 +99,15 @@ def test_step_graph_replays_device_ring_writes():
     tokens = [[row[0] for row in snap] for snap in delivered]
     assert tokens == [[(10 + r + n) % vocab for r in range(rows)] for n in range(8)]
     assert [snap[0][1] for snap in delivered] == list(range(8))
+
+
+@torch.inference_mode()
+def test_current_stream_of_a_device_in_every_form():
+    """``_lib.stream`` names the device as torch does: none, an index, a text, a device
+    with or without its index."""
+    from litemoe_amd import _lib
+    side = torch.cuda.Stream()
+    for now in (torch.cuda.current_stream(), side):
+        with torch.cuda.stream(now):
+            for device in (None, 0, "cuda", "cuda:0", torch.device("cuda"), torch.device("cuda", 0)):
+                assert _lib.stream(device) == now.cuda_stream

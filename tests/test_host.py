@@ -223,3 +223,18 @@ def test_output_ring_dropped_during_capture_is_parked(monkeypatch):
     ring.asynchronous, ring.host, ring.events = True, host, events
     del ring  # outside a capture: freed at once
     assert execution._PARKED == []
+
+
+def test_calls_over_host_tensors_are_refused():
+    """The stream that every native call takes last comes from its tensors' device: a
+    host tensor's is refused before its address reaches a kernel, also where a
+    wrapper has no check of its own."""
+    from litemoe_amd import _lib, experts, linear
+    x = torch.zeros(4, 128, dtype=torch.bfloat16)
+    ids = torch.zeros(4, 1, dtype=torch.int32)
+    for call in (lambda: _lib.stream(torch.device("cpu")), lambda: _lib.stream("cpu"),
+                 lambda: linear.reduce(torch.zeros(2, 4, 64)),
+                 lambda: experts.gate_up(x, x.view(1, 4, 128), None, None, 1, topk_ids=ids),
+                 lambda: experts.down(x, x.view(1, 4, 128), None, None, topk_ids=ids)):
+        with pytest.raises(ValueError, match="ROCm device"):
+            call()
