@@ -51,9 +51,15 @@ constexpr int kMaxQkvSplits = 8;
 // exp2(-inf - kEmpty) are 0 and the loop needs no special case, and below every
 // other finite score.
 constexpr float kEmpty = -3.402823466e38f;
-// A column keeps its maximum until a score exceeds it by more than this (log2
-// units): probabilities stay below 2^8 and the accumulators are seldom rescaled.
-constexpr float kLazy = 8.f;
+// A column's reference lies this much (log2 units) above the score that set it, and
+// moves only for a score above it: probabilities are at most 1 and the accumulators are
+// seldom rescaled.
+constexpr float kAbove = 8.f;
+// V's codes enter P.V times 2^-32, which the result takes back. A probability of at most 1
+// times a scale of up to 2^125 is finite in bf16, and the products of 2^30 positions with
+// the largest values sum to less than 2^127: only a position that stands for NaN makes a
+// NaN. At the other end fp32 sums in these units hold 24 bits of values down to 2^-86.
+constexpr float kDown = 0x1p-32f, kBack = 0x1p32f;
 
 template <int kBits>
 struct Stage {
@@ -147,7 +153,7 @@ struct Cache {
 };
 
 struct Partial {
-  float *o;  // [batch, q_heads, splits, 64]
+  float *o;  // [batch, q_heads, splits, 64], times kDown
   float *m;  // [batch, q_heads, splits]
   float *l;  // [batch, q_heads, splits]
 };
@@ -346,7 +352,7 @@ decode_quant_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, Cache 
 
   const float sl2 = scale * 1.4426950408889634f;
   float m = kEmpty, l = 0.f;
-  f32x4 acc[4];  // channels 16 mm + 4 grp + i of column col, of use where tile is 0
+  f32x4 acc[4];  // times kDown: channels 16 mm + 4 grp + i of column col, of use where tile is 0
 #pragma unroll
   for (int mm = 0; mm < 4; ++mm) acc[mm] = f32x4{0.f, 0.f, 0.f, 0.f};
 
@@ -446,19 +452,20 @@ decode_quant_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, Cache 
     for (int p = 0; p < kPasses; ++p)
 #pragma unroll
       for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[p][i]);
-    if (__any(mx > m + kLazy)) {
+    if (__any(mx > m)) {
       mx = fmaxf(mx, xor_lanes<16>(mx));
       mx = tiles_max<P>(fmaxf(mx, xor_lanes<32>(mx)));
-      const bool up = mx > m + kLazy;
-      const float f = up ? __builtin_amdgcn_exp2f(m - mx) : 1.f;
-      m = up ? mx : m;
+      const bool up = mx > m;
+      const float to = mx + kAbove;
+      const float f = up ? __builtin_amdgcn_exp2f(m - to) : 1.f;
+      m = up ? to : m;
       l *= f;
 #pragma unroll
       for (int mm = 0; mm < 4; ++mm) acc[mm] *= f;
     }
     // Probabilities rounded to bf16, their sum from the rounded ones (so that a row
     // that one position rules keeps its value: 5 to 15% less error at no cost), times
-    // the scale of each block of V, which is exact, as bf16 pairs.
+    // the scale of each block of V, which is exact from 2^-126 up, as bf16 pairs.
     uint32_t pb[2][kPasses][2];
 #pragma unroll
     for (int p = 0; p < kPasses; ++p) {
@@ -506,7 +513,7 @@ decode_quant_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, Cache 
         uint32_t w[kBits / 4];
 #pragma unroll
         for (int j = 0; j < kBits / 4; ++j) w[j] = (uint32_t)(kBits == 4 ? vt[mm][0][pr] : vt[mm][pr * (kBits / 8)][j]);
-        acc[mm] = mfma16x16x32(codes_to_bf16<kBits>(w), bp[pr][mm / 2], acc[mm]);
+        acc[mm] = mfma16x16x32(codes_to_bf16<kBits>(w, kDown), bp[pr][mm / 2], acc[mm]);
       }
   };
 
@@ -563,7 +570,7 @@ decode_quant_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, Cache 
     const int hq = h * G + g;
     if (splits == 1) {
       const int64_t at = out_mb ? frag_offset_rows(b, (int64_t)hq * kD + c, out_mb) : (b * q_heads + hq) * kD + c;
-      out[at] = (bf16)f32_to_bf16(lsum == 0.f ? 0.f : o / lsum);
+      out[at] = (bf16)f32_to_bf16(lsum == 0.f ? 0.f : o / lsum * kBack);
     } else {
       const int64_t at = ((int64_t)b * q_heads + hq) * splits + split;
       part.o[at * kD + c] = o;
@@ -623,7 +630,7 @@ decode_quant_combine_kernel(const int32_t *__restrict__ used, int q_heads, int64
     }
   }
   const int64_t at = out_mb ? frag_offset_rows(b, (int64_t)hq * kD + c, out_mb) : (b * q_heads + hq) * kD + c;
-  out[at] = (bf16)f32_to_bf16(lsum == 0.f ? 0.f : o / lsum);
+  out[at] = (bf16)f32_to_bf16(lsum == 0.f ? 0.f : o / lsum * kBack);
 }
 
 int64_t workspace_bytes(int64_t batch, int64_t q_heads, int64_t splits) {

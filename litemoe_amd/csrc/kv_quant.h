@@ -94,20 +94,21 @@ __device__ __forceinline__ Codes8<kBits> quantise8(const float *x, uint32_t &sca
   return c;
 }
 
-// Eight codes as bf16 pairs without their scale: exact (1 or 4 significand bits).
+// Eight codes as bf16 pairs without their scale, times `unit`, a power of two: exact
+// (codes have up to 2 or 4 significand bits).
 template <int kBits>
-__device__ __forceinline__ u32x4 codes_to_bf16(const uint32_t *w) {
+__device__ __forceinline__ u32x4 codes_to_bf16(const uint32_t *w, float unit = 1.f) {
   u32x4 o;
   if constexpr (kBits == 4) {
-    o[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[0], 1.f, 0));
-    o[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[0], 1.f, 1));
-    o[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[0], 1.f, 2));
-    o[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[0], 1.f, 3));
+    o[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[0], unit, 0));
+    o[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[0], unit, 1));
+    o[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[0], unit, 2));
+    o[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[0], unit, 3));
   } else {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      o[2 * j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[j], 1.f, false));
-      o[2 * j + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[j], 1.f, true));
+      o[2 * j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[j], unit, false));
+      o[2 * j + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[j], unit, true));
     }
   }
   return o;

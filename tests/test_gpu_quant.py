@@ -432,6 +432,48 @@ def test_scores_far_below_zero(bits, hq, splits):
     assert bool(((got - want).abs() <= tol).all())
 
 
+def rising_scores(b, hq, hkv, cap, low, step, seed):
+    """Queries and keys (bf16) whose scores, scaled by 1/8, rise from ``low`` by ``step`` a
+    position for the first query head of each KV head."""
+    g = gen(seed)
+    q = torch.randn(b, hq, 64, generator=g)
+    lead = q[:, ::hq // hkv]
+    t = low + step * torch.arange(cap, dtype=torch.float32)
+    k = t[None, None, :, None] * lead[:, :, None, :] / (0.125 * lead.square().sum(-1))[:, :, None, None]
+    return q.to(BF16), k.to(BF16)
+
+
+def filled_cache(bits, k, v):
+    """A cache of ``k, v [B, Hkv, C, 64]`` (bf16, CPU) and the values it stands for (64 bits, CPU)."""
+    b, hkv, cap, _ = k.shape
+    cache = QuantKVCache.empty(1, b, hkv, cap, DEV, bits=bits)
+    slots, pos = torch.arange(b).repeat_interleave(cap).to(DEV), torch.arange(cap).repeat(b).to(DEV)
+    cache.write(0, *(x.to(DEV).transpose(1, 2).reshape(b * cap, hkv, 1, 64) for x in (k, v)), pos, None, slots)
+    return cache, *(x.cpu().double() for x in cache.read(0))
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("splits,hq,cap", [(1, 6, 300), (3, 6, 300), (1, 16, 300), (1, 32, 300), (1, 6, 1100)])
+@torch.inference_mode()
+def test_values_to_the_ends_of_the_range(bits, splits, hq, cap):
+    """Values near bf16's largest, of both signs, beside zeros in their block and at other
+    positions, under scores that rise by less than the running maximum's slack: finite
+    and within the bound. The same with values near 2^-60."""
+    hkv, b = 2, 3
+    q, k = rising_scores(b, hq, hkv, cap, -4.0, 0.02, 17)
+    used = torch.tensor([cap, cap - 1, 70], dtype=torch.int32)
+    flash = QuantFlashDecode(b, hkv, hq // hkv, cap, DEV, num_splits=splits, bits=bits)
+    for size in (1.6 * 2.0 ** 127, 2.0 ** -60):
+        v = size * (1 - 2 * torch.rand(b, hkv, cap, 64, generator=gen(18)))
+        j = torch.arange(cap)
+        one = torch.nn.functional.one_hot(j % 32, 32)[None, None] * size * (1 - 2 * (j // 5 % 2))[:, None]
+        v[..., :32] = torch.where((j % 3 == 0)[:, None], one, torch.zeros(()))
+        cache, kd, vd = filled_cache(bits, k, v.to(BF16))
+        got = flash(q.to(DEV)[:, :, None], *cache.layer(0), None, None, 0.125, used=used.to(DEV))[:, :, 0]
+        assert torch.isfinite(got).all()
+        check(got, q, kd, vd, used, 0.125)
+
+
 @torch.inference_mode()
 def test_attention_past_32_bit_offsets():
     """One KV head whose codes pass 4 GiB: every key zero, so the softmax is
