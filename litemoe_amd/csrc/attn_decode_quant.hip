@@ -60,6 +60,10 @@ constexpr float kAbove = 8.f;
 // the largest values sum to less than 2^127: only a position that stands for NaN makes a
 // NaN. At the other end fp32 sums in these units hold 24 bits of values down to 2^-86.
 constexpr float kDown = 0x1p-32f, kBack = 0x1p32f;
+// K's codes enter the scores times 2^-14, which the scale of the scores takes back: 32
+// products of codes up to 448 with q of any size stay finite, as they have to where K's
+// scale makes small scores of them.
+constexpr float kScoreDown = 0x1p-14f, kScoreBack = 0x1p14f;
 
 template <int kBits>
 struct Stage {
@@ -350,7 +354,7 @@ decode_quant_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, Cache 
 #pragma unroll
       for (int i = 0; i < 4; ++i) qt[t][bl][i] = tile == t && head < G ? qw[bl][i] : 0u;
 
-  const float sl2 = scale * 1.4426950408889634f;
+  const float sl2 = scale * (1.4426950408889634f * kScoreBack);
   float m = kEmpty, l = 0.f;
   f32x4 acc[4];  // times kDown: channels 16 mm + 4 grp + i of column col, of use where tile is 0
 #pragma unroll
@@ -428,7 +432,8 @@ decode_quant_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, Cache 
     for (int t = 0; t < 4; ++t)
 #pragma unroll
       for (int bl = 0; bl < 2; ++bl)
-        c[t / kTiles][bl] = mfma16x16x32(codes_to_bf16<kBits>(a[t][bl].w), qt[t % kTiles][bl], c[t / kTiles][bl]);
+        c[t / kTiles][bl] =
+            mfma16x16x32(codes_to_bf16<kBits>(a[t][bl].w, kScoreDown), qt[t % kTiles][bl], c[t / kTiles][bl]);
     float s[kPasses][4];
 #pragma unroll
     for (int p = 0; p < kPasses; ++p) {

@@ -474,6 +474,24 @@ def test_values_to_the_ends_of_the_range(bits, splits, hq, cap):
         check(got, q, kd, vd, used, 0.125)
 
 
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("splits,hq,cap", [(1, 6, 300), (3, 6, 300), (1, 16, 300), (1, 6, 1100)])
+@pytest.mark.parametrize("power", [123, -100])
+@torch.inference_mode()
+def test_queries_to_the_ends_of_the_range(bits, splits, hq, cap, power):
+    """Queries near bf16's largest over keys as small as they are large, and the reverse:
+    ordinary scores, so ordinary results."""
+    hkv, b = 2, 3
+    q, k = rising_scores(b, hq, hkv, cap, -4.0, 0.02, 19)
+    q, k = q * 2.0 ** power, k * 2.0 ** -power
+    used = torch.tensor([cap, cap - 1, 70], dtype=torch.int32)
+    cache, kd, vd = filled_cache(bits, k, vectors((b, hkv, cap, 64), 20))
+    flash = QuantFlashDecode(b, hkv, hq // hkv, cap, DEV, num_splits=splits, bits=bits)
+    got = flash(q.to(DEV)[:, :, None], *cache.layer(0), None, None, 0.125, used=used.to(DEV))[:, :, 0]
+    assert torch.isfinite(q).all() and torch.isfinite(got).all()
+    check(got, q, kd, vd, used, 0.125)
+
+
 @torch.inference_mode()
 def test_attention_past_32_bit_offsets():
     """One KV head whose codes pass 4 GiB: every key zero, so the softmax is
