@@ -233,7 +233,8 @@ int lm_flash_decode_qkv_frag(const float *qkv_partials, int64_t qkv_splits,
  * most 16; q 16-byte aligned, its strides multiples of 8; the cache's buffers
  * aligned as lm_kv_quant_write says. The other arguments and the workspace
  * (lm_flash_decode_workspace_size, 16-byte aligned) as lm_flash_decode; bits 4
- * or 8. Two calls in flight at once need workspaces of their own. Replaces
+ * or 8. Each row is cut by its own length, into num_splits pieces or fewer, of
+ * multiples of 64 positions. Two calls in flight at once need workspaces of their own. Replaces
  * litemoe/flash_decode.py:16-34 over a cache the reference does not have. */
 int lm_flash_decode_quant(const void *q, int64_t qs0, int64_t qs1,
                           const void *k_codes, const void *v_codes,

@@ -46,6 +46,7 @@ namespace {
 constexpr int kD = 64;
 constexpr int kStageKeys = 64;
 constexpr int kMaxQkvSplits = 8;
+constexpr int64_t kCUs = 256;
 
 // Running maximum before any position: finite, so exp2(kEmpty - m) and
 // exp2(-inf - kEmpty) are 0 and the loop needs no special case, and below every
@@ -166,9 +167,10 @@ struct Partial {
 // busy: splits * chunk >= n, splits * inv_splits just above 2^32 (a product in place of a
 // division). Cut by the longest row instead, the later splits have only the long rows:
 // 20 rows of 4000 to 16000 positions in eight splits 25.2 us against 23.7, 12 rows 17.0
-// and 15.9, 8 rows to 32768 23.4 and 20.5; rows of one length are within 2%.
-__device__ __forceinline__ int row_chunk(int n, int splits, uint32_t inv_splits) {
-  return (int)__umulhi((uint32_t)((max(n, 1) - 1) / kStageKeys + splits), inv_splits) * kStageKeys;
+// and 15.9, 8 rows to 32768 23.4 and 20.5; rows of one length are within 2%. A split takes
+// `least` positions or more (least_chunk), so a short row leaves its later splits empty.
+__device__ __forceinline__ int row_chunk(int n, int splits, uint32_t inv_splits, int least) {
+  return max((int)__umulhi((uint32_t)((max(n, 1) - 1) / kStageKeys + splits), inv_splits) * kStageKeys, least);
 }
 
 // The fused form's input: see lm_flash_decode_qkv.
@@ -186,7 +188,7 @@ template <int kBits, int P, bool kFused, int kWaves>
 __global__ void __launch_bounds__(kWaves * kWave, 2)
 decode_quant_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, Cache cache,
                     const int32_t *__restrict__ used, int q_heads, int kv_heads, int64_t capacity,
-                    float scale, int max_len, uint32_t inv_splits, int splits, Partial part, QkvIn in,
+                    float scale, int max_len, uint32_t inv_splits, int least, int splits, Partial part, QkvIn in,
                     bf16 *__restrict__ out, int out_mb) {
   typedef Stage<kBits> St;
   constexpr int kThreads = kWaves * kWave;
@@ -233,7 +235,7 @@ decode_quant_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, Cache 
   }
   int n = min(used[b], max_len);
   n = (int)min((int64_t)n, capacity);
-  const int chunk = splits > 1 ? row_chunk(n, gridDim.y, inv_splits) : max_len;
+  const int chunk = splits > 1 ? row_chunk(n, gridDim.y, inv_splits, least) : max_len;
   const int k0 = split * chunk, k1 = min(n, k0 + chunk);
   bool writer = false, own = false;
   int64_t pnew = 0;
@@ -596,7 +598,7 @@ constexpr int kCombineHeads = 2;
 template <int kBatch>
 __global__ void __launch_bounds__(kCombineHeads * kD)
 decode_quant_combine_kernel(const int32_t *__restrict__ used, int q_heads, int64_t capacity, int max_len,
-                            uint32_t inv_splits, int grid_splits, int splits, Partial part,
+                            uint32_t inv_splits, int least, int grid_splits, int splits, Partial part,
                             bf16 *__restrict__ out, int out_mb) {
   const int hq = blockIdx.x * kCombineHeads + threadIdx.x / kD;
   if (hq >= q_heads) return;
@@ -616,7 +618,7 @@ decode_quant_combine_kernel(const int32_t *__restrict__ used, int q_heads, int64
   load(0);
   int n = min(used[b], max_len);
   n = (int)min((int64_t)n, capacity);
-  const int chunk = row_chunk(n, grid_splits, inv_splits);
+  const int chunk = row_chunk(n, grid_splits, inv_splits, least);
   const int valid = n > 0 ? min(grid_splits, (n + chunk - 1) / chunk) : 0;
   float mx = kEmpty;
 #pragma unroll
@@ -647,14 +649,14 @@ int64_t workspace_bytes(int64_t batch, int64_t q_heads, int64_t splits) {
 template <int kBits, int P, bool kFused, int kWaves>
 int launch_sized(const bf16 *q, int64_t qs0, int64_t qs1, const Cache &cache, const int32_t *used, int64_t batch,
                  int64_t q_heads, int64_t kv_heads, int64_t capacity, float scale, int64_t max_len, uint32_t inv_splits,
-                 int grid_splits, int stride_splits, const Partial &part, const QkvIn &in, bf16 *out, int out_mb,
+                 int least, int grid_splits, int stride_splits, const Partial &part, const QkvIn &in, bf16 *out, int out_mb,
                  hipStream_t s) {
   // KV heads fastest: workgroups go to the XCDs in turn, and with the splits fastest one XCD
   // would have the first split of every row and another the last (8 rows of 8191 to 32768
   // positions in four splits 21.5 us against 20.7, three rows of 8 bits in eight 7.65 and 7.5).
   const dim3 grid((unsigned)kv_heads, (unsigned)grid_splits, (unsigned)batch);
   decode_quant_kernel<kBits, P, kFused, kWaves><<<grid, kWaves * kWave, 0, s>>>(
-      q, qs0, qs1, cache, used, (int)q_heads, (int)kv_heads, capacity, scale, (int)max_len, inv_splits, stride_splits,
+      q, qs0, qs1, cache, used, (int)q_heads, (int)kv_heads, capacity, scale, (int)max_len, inv_splits, least, stride_splits,
       part, in, out, out_mb);
   LM_CHECK_LAUNCH();
   return LM_OK;
@@ -675,6 +677,22 @@ int check_call(const Call &c, bool *run) {
   return LM_OK;
 }
 
+// The fewest positions of a split, `chunk` being one's share of the longest row. A CU holds
+// four workgroups in 4 bits and two in 8 (their LDS). While the grid's workgroups all run at
+// once, a row far below the plan's bound is cut to single stages, which is the shortest way
+// through it: rows of 300 to 1000 positions in eight splits of a plan to 16384, 16 rows x 8
+// heads in 4 bits 7.3 us, with 256 positions or more 8.4, 8 rows in 8 bits 7.2 and 7.6 (one
+// row of 1000 in sixteen splits 6.2, 6.5, with 512 or more 7.1). Beyond that the pieces
+// queue, and a workgroup's four waves get a stage each: 18 rows in 4 bits 8.7 and 8.4, 24
+// rows 10.2 and 9.1, fused 12.6 and 11.2; in 8 bits 10 rows 9.1 and 7.7, 20 rows 11.8 and
+// 10.5. Rows of 100 to 300 lose there (20 rows in 4 bits 7.0 and 7.9, fused 9.8 and 9.9);
+// rows whose pieces are longer anyway do not notice.
+int least_chunk(int64_t bits, int64_t workgroups, int chunk) {
+  const bool at_once = workgroups <= kCUs * (bits == 4 ? 4 : 2);
+  const int wanted = at_once ? kStageKeys : 4 * kStageKeys;
+  return chunk < wanted ? chunk : wanted;
+}
+
 bool aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 int launch_decode_quant(const Call &c, const void *q, int64_t qs0, int64_t qs1, const Cache &cache,
@@ -686,6 +704,7 @@ int launch_decode_quant(const Call &c, const void *q, int64_t qs0, int64_t qs1, 
   LM_REQUIRE(need == 0 || aligned16(workspace));
   const int chunk = (int)align_up(cdiv(c.max_len, c.num_splits), kStageKeys);
   const int splits = (int)cdiv(c.max_len, chunk);
+  const int least = least_chunk(c.bits, (int64_t)splits * c.kv_heads * c.batch, chunk);
   // Rounded up; of no use with one split.
   const uint32_t inv_splits = (uint32_t)((((uint64_t)1 << 32) + splits - 1) / splits);
   Partial part{nullptr, nullptr, nullptr};
@@ -707,7 +726,7 @@ int launch_decode_quant(const Call &c, const void *q, int64_t qs0, int64_t qs1, 
               : G <= 8 ? launch_sized<kBits, 8, kFused, kWaves>
                        : launch_sized<kBits, 16, kFused, kWaves>;
     return go((const bf16 *)q, qs0, qs1, cache, used, c.batch, c.q_heads, c.kv_heads, c.capacity, scale, c.max_len,
-              inv_splits, splits, stride_splits, part, in, (bf16 *)out, out_mb, s);
+              inv_splits, least, splits, stride_splits, part, in, (bf16 *)out, out_mb, s);
   };
   // Up to one workgroup per CU a wave has its SIMD to itself, and a 4-bit stage's chain
   // of dependent steps (0.57 us) takes longer than its bytes: eight waves where
@@ -715,7 +734,7 @@ int launch_decode_quant(const Call &c, const void *q, int64_t qs0, int64_t qs1, 
   // 32 rows to 4095 15.2 and 14.3, 8 rows to 32768 in four splits 26.9 and 21.7; 10 rows
   // to 1000 5.4 and 5.5, one row of 509 3.6 and 3.8. In 8 bits they differ by 2 to 4% (32
   // rows to 4095 22.5 and 21.9), which a second set of kernels is not worth.
-  const bool wide = c.bits == 4 && (int64_t)splits * c.kv_heads * c.batch <= 256 && chunk >= 16 * kStageKeys;
+  const bool wide = c.bits == 4 && (int64_t)splits * c.kv_heads * c.batch <= kCUs && chunk >= 16 * kStageKeys;
   typedef std::integral_constant<int, 4> Four;
   typedef std::integral_constant<int, 8> Eight;
   auto run = [&](auto fused) {
@@ -729,7 +748,7 @@ int launch_decode_quant(const Call &c, const void *q, int64_t qs0, int64_t qs1, 
                  : splits <= 8 ? decode_quant_combine_kernel<8>
                                : decode_quant_combine_kernel<16>;
   combine<<<dim3((unsigned)cdiv(c.q_heads, kCombineHeads), (unsigned)c.batch), kCombineHeads * kD, 0, s>>>(
-      used, (int)c.q_heads, c.capacity, (int)c.max_len, inv_splits, splits, stride_splits, part,
+      used, (int)c.q_heads, c.capacity, (int)c.max_len, inv_splits, least, splits, stride_splits, part,
       (bf16 *)out, out_mb);
   LM_CHECK_LAUNCH();
   return LM_OK;

@@ -139,9 +139,11 @@ def quant_splits(batch, kv_heads, maximum):
     lines, since a position takes a quarter or half of the bytes.
 
     Up to 256 (row, head) pairs, one workgroup per CU, the splits fill the CUs
-    and no more. A split takes 512 positions, two stages of each of a workgroup's
-    four waves, or more, and contexts below three times that are not split: the
-    second launch costs 1.5 to 2 us. us per launch in a graph, 4 bits: one row x 8
+    and no more. There are as many as give a row of ``maximum`` positions pieces of
+    512, two stages of each of a workgroup's four waves, or fewer, and contexts below
+    three times that are not split: the second launch costs 1.5 to 2 us. The plan sets
+    their number only; a row is cut by its own length, a short one into pieces of a
+    stage or four (see ``lm_flash_decode_quant``). us per launch in a graph, 4 bits: one row x 8
     heads to 1000 positions 6.4 (1 split) and 6.8 (4); to 4000 10.0 (1), 7.2 (4),
     6.3 (8) and 6.2 (16); 3 rows to 4001 10.2 (1), 7.5 (4), 6.7 (8) and 7.4 (16); 16
     rows to 4095 10.1 (2) and 10.7 (8); 8 rows to 32768 32.3 (2), 21.9 (4) and 20.5

@@ -314,6 +314,56 @@ def test_splits_share_each_rows_own_length(bits, splits, most):
 
 
 @pytest.mark.parametrize("bits", [4, 8])
+@torch.inference_mode()
+def test_short_rows_are_cut_by_what_runs_at_once(bits):
+    """Rows far below the plan's bound: single stages while the grid's workgroups all run at
+    once, else pieces of 256 positions or more, a stage for each wave. Which splits of a row
+    ran is read off the maxima that they left in the workspace."""
+    hkv, hq, cap, splits = 8, 16, 8192, 8
+    resident = 256 * (4 if bits == 4 else 2)
+    for b in (resident // (hkv * splits), resident // (hkv * splits) + 1):
+        lengths = torch.tensor([300, 1, 64, 65, 256, 257, 512, 513, 700, 2048, 2049, 8192, 0])[torch.arange(b) % 13]
+        lengths = lengths.tolist()
+        cache = QuantKVCache.empty(1, b, hkv, cap, DEV, bits=bits)
+        flash = QuantFlashDecode(b, hkv, 2, cap, DEV, num_splits=splits, bits=bits)
+        n = b * hq * splits
+        maxima = flash.workspace[n * 64 * 4:][:4 * n].view(torch.float32).view(b, hkv, 2, splits)
+        maxima.fill_(float("nan"))
+        flash(torch.zeros(b, hq, 1, 64, dtype=BF16, device=DEV), *cache.layer(0), None, None, 0.125,
+              used=torch.tensor(lengths, device=DEV))
+        ran = ~maxima.isnan()
+        assert torch.equal(ran, ran[:, :1, :1].expand_as(ran))
+        least = 64 if b * hkv * splits <= resident else 256
+        for row, used in zip(ran[:, 0, 0].tolist(), lengths):
+            chunk = max(least, 64 * -(-used // (64 * splits)))
+            pieces = -(-used // chunk)
+            assert row == [True] * pieces + [False] * (splits - pieces), (b, used)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@torch.inference_mode()
+def test_many_short_rows_in_splits_match_oracle(bits):
+    """More workgroups than run at once, rows of every length from none to the bound: the
+    oracle, the fused form and the cache it leaves."""
+    b, hq, hkv, cap, splits = 140, 3, 1, 2400, 8
+    cache, k, v = random_cache(bits, b, hkv, cap, 14)
+    used = torch.randint(0, 700, (b,), generator=gen(15), dtype=torch.int32)
+    used[:8] = torch.tensor([0, 1, 255, 256, 257, 512, 2399, 2400])
+    q = (2 * torch.randn(b, hq, 64, generator=gen(16))).to(BF16)
+    flash = QuantFlashDecode(b, hkv, hq, cap, DEV, num_splits=splits, bits=bits)
+    got = flash(q.to(DEV)[:, :, None], *cache.layer(0), None, None, 0.125, used=used.to(DEV))[:, :, 0]
+    check(got, q, k[0], v[0], used, 0.125)
+    part, table = fused_inputs(b, hq, hkv, cap, 4)
+    other = random_cache(bits, b, hkv, cap, 14)[0]
+    for back in (1, 100, -3):
+        positions, device_used = (used.long() - back).to(DEV), used.to(DEV)
+        want = unfused(flash, cache, part, table, positions, None, device_used, hq, hkv)
+        got = flash.fused_qkv(part, table, positions, None, *other.layer(0), 0.125, device_used, hq)
+        assert torch.equal(got, want)
+        assert all(torch.equal(x, y) for x, y in zip(cache.layer(0), other.layer(0)))
+
+
+@pytest.mark.parametrize("bits", [4, 8])
 @pytest.mark.parametrize("hq,splits", [(6, 1), (16, 3), (2, 1)])
 @torch.inference_mode()
 def test_masked_positions_are_never_seen(bits, hq, splits):
