@@ -156,13 +156,18 @@ def quant_splits(batch, kv_heads, maximum):
     20 rows of 4000 to 16000 positions 30.4 us (1) and 23.7 (8), in 8 bits 52 and 37; 12
     rows 19.8 (2) and 15.9 (8); 40 rows of 4000 to 8192 30.8 (1) and 28.4 (8); rows of one
     length lose less: 12 to 16000 21.4 (2) and 21.9 (8), 20 31.1 (1) and 33.3 (8), 40
-    58.9 (1) and 59.2 (8). 256 pairs fill the CUs as they are: 35.0 either way, 43.2
-    and 47.3 at one length; from 384 on there is little to gain (48 rows to 16000 55.9
-    either way) and up to 7% to lose."""
+    58.9 (1) and 59.2 (8); from 384 pairs on there is little to gain (48 rows to 16000
+    55.9 either way) and up to 7% to lose. Pairs that leave less than an eighth of the CUs
+    free fill them as they are. us (1) and (8), 4 bits, 4000 to 16000 positions and 15500
+    to 16000: 28 rows 32.5 and 31.3, 38.9 and 44.8; 29 rows 32.9 and 32.5, 39.9 and 45.4;
+    31 rows 34.1 and 34.5, 42.5 and 47.3; 32 rows 36.0 and 34.6, 43.8 and 48.0; one more
+    row, and the CUs have a second workgroup to run: 33 rows 44.9 and 34.6, 54.7 and 51.0. In
+    8 bits ragged rows pay for it: 28 rows 57.0 and 49.2, 69.3 and 75.5; 32 rows 60.9 and
+    55.5, 79.7 and 84.3."""
     pairs = max(1, batch * kv_heads)
     longest = -(-maximum // 512) if maximum >= 3 * 512 else 1
     filling = max(1, min(max(16, maximum // 4096), 256 // pairs, longest))
-    return max(8, filling) if maximum >= 8192 and pairs <= 320 and pairs != 256 else filling
+    return max(8, filling) if maximum >= 8192 and pairs <= 320 and not 224 < pairs <= 256 else filling
 
 
 class QuantFlashDecode:

@@ -183,3 +183,14 @@ def test_quant_splits_fill_the_cus_and_keep_512_positions():
             n = quant_splits(batch, 8, maximum)
             assert n >= 1 and (n == 1 or -(-maximum // n) > 512 - 64)
             assert n * batch * 8 <= 256 or n == 1 or (n == 8 and maximum >= 8192)
+
+
+@pytest.mark.parametrize("maximum", [8192, 16000, 32768, 1 << 20])
+def test_quant_splits_of_long_contexts_go_by_ranges(maximum):
+    """One split where the pairs leave less than an eighth of the CUs free or are too many
+    to gain, eight or more elsewhere: no number of pairs stands apart from its neighbours."""
+    for pairs in range(1, 600):
+        n = quant_splits(pairs, 1, maximum)
+        assert (n == 1) if 224 < pairs <= 256 or pairs > 320 else n >= 8
+    for batch in (29, 31, 32, 33):
+        assert quant_splits(batch, 8, maximum) == quant_splits(8 * batch, 1, maximum)
