@@ -648,6 +648,95 @@ def test_fused_over_positions_that_were_never_written(bits, hq, splits):
     assert torch.isfinite(again).all()
 
 
+# Few rows whose splits span 1024 positions or more take workgroups of eight waves in 4
+# bits. Groups of 3, 8 and 16 query heads; one split and two.
+EIGHT_WAVES = pytest.mark.parametrize("cap,splits", [(1100, 1), (2100, 1), (2100, 2)])
+GROUPS = pytest.mark.parametrize("groups", [3, 8, 16])
+
+
+def eight_wave_lengths(cap):
+    """Lengths at the edges of a workgroup's first and second round of stages."""
+    return torch.tensor([cap, 1025, 1024, 1023, 513, 512, 511, 449, 65, 64, 1, 0], dtype=torch.int32)
+
+
+@EIGHT_WAVES
+@GROUPS
+@torch.inference_mode()
+def test_eight_waves_match_oracle(cap, splits, groups):
+    hkv, used = 2, eight_wave_lengths(cap)
+    b, hq = used.numel(), groups * hkv
+    cache, k, v = random_cache(4, b, hkv, cap, 101)
+    q = (2 * torch.randn(b, hq, 64, generator=gen(102))).to(BF16)
+    flash = QuantFlashDecode(b, hkv, groups, cap, DEV, num_splits=splits, bits=4)
+    got = flash(q.to(DEV)[:, :, None], *cache.layer(0), None, None, 0.125, used=used.to(DEV))[:, :, 0]
+    check(got, q, k[0], v[0], used, 0.125)
+    assert not bool(got[-1].any())
+
+
+@EIGHT_WAVES
+@GROUPS
+@torch.inference_mode()
+def test_eight_waves_fused_equals_the_separate_operators(cap, splits, groups):
+    hkv, used = 2, eight_wave_lengths(cap)
+    b, hq = used.numel(), groups * hkv
+    caches = [random_cache(4, b, hkv, cap, 103)[0] for _ in range(3)]
+    part, table = fused_inputs(b, hq, hkv, cap, 104)
+    active = torch.ones(b, dtype=torch.bool, device=DEV)
+    active[4] = False
+    flash = QuantFlashDecode(b, hkv, groups, cap, DEV, num_splits=splits, bits=4)
+    order = torch.arange(b, device=DEV, dtype=torch.int32).flip(0).contiguous()
+    for back in (1, 500, -2):
+        positions, device_used = (used.long() - back).to(DEV), used.to(DEV)
+        want = unfused(flash, caches[0], part, table, positions, active, device_used, hq, hkv)
+        got = flash.fused_qkv(part, table, positions, active, *caches[1].layer(0), 0.125, device_used, hq)
+        frag = flash.fused_qkv(part, table, positions, active, *caches[2].layer(0), 0.125, device_used, hq,
+                               row_order=order, frag_out=True)
+        assert torch.equal(got, want) and torch.equal(frag.to_rows(), want.view(b, -1))
+        for other in caches[1:]:
+            assert all(torch.equal(x, y) for x, y in zip(caches[0].layer(0), other.layer(0)))
+
+
+@EIGHT_WAVES
+@GROUPS
+@torch.inference_mode()
+def test_eight_waves_see_only_their_rows(cap, splits, groups):
+    """Garbage and NaN scales behind the rows' ends move no bit; a key and a value that stand
+    for NaN, and a query that is none, make NaN of their own rows and heads only; the new
+    token's place may hold anything."""
+    hkv, used = 2, eight_wave_lengths(cap)
+    b, hq = used.numel(), groups * hkv
+    used = used.to(DEV)
+    cache, _, _ = random_cache(4, b, hkv, cap, 105)
+    q = vectors((b, hq, 1, 64), 106).to(DEV)
+    flash = QuantFlashDecode(b, hkv, groups, cap, DEV, num_splits=splits, bits=4)
+    clean = flash(q, *cache.layer(0), None, None, 0.125, used=used)
+    assert torch.isfinite(clean).all()
+    past = (torch.arange(cap, device=DEV)[None] >= used[:, None])[:, None, :, None]
+    for t, worst in zip(cache.layer(0), (0xff, 0x7f, 0xff)):
+        t.masked_fill_(past, worst)
+    assert torch.equal(flash(q, *cache.layer(0), None, None, 0.125, used=used), clean)
+
+    part, table = fused_inputs(b, hq, hkv, cap, 107)
+    other = QuantKVCache.over(*(t.clone() for t in (cache.k, cache.v, cache.scales)))
+    for t, worst in zip(other.layer(0), (0xff, 0xff, 0xff)):
+        t[torch.arange(b - 1), :, (used[:-1] - 1).long()] = worst
+    spare = [QuantKVCache.over(*(t.clone() for t in (cache.k, cache.v, cache.scales))), other]
+    got = [flash.fused_qkv(part, table, used.long() - 1, None, *c.layer(0), 0.125, used, hq) for c in spare]
+    assert torch.isfinite(got[0]).all() and torch.equal(*got)
+
+    nan = torch.zeros(b, hq, 1, 64, dtype=torch.bool, device=DEV)
+    for row, head, position, block in ((0, 1, 1023, 1), (1, 0, 1024, 2), (2, 1, 512, 3), (6, 0, 0, 0)):
+        cache.scales[0, row, head, position, block] = 255
+        side = cache.k if block < 2 else cache.v
+        side[0, row, head, position, 16 * (block % 2):16 * (block % 2 + 1)] = 0
+        channels = slice(None) if block < 2 else slice(32 * (block - 2), 32 * (block - 1))
+        nan[row, groups * head:groups * (head + 1), :, channels] = True
+    q[3, hq - 1, 0, 5] = float("nan")
+    nan[3, hq - 1] = True
+    got = flash(q, *cache.layer(0), None, None, 0.125, used=used)
+    assert torch.equal(got.isnan(), nan) and torch.equal(got[~nan], clean[~nan])
+
+
 @pytest.mark.parametrize("bits", [4, 8])
 @torch.inference_mode()
 def test_fused_matches_oracle(bits):
