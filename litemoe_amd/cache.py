@@ -79,6 +79,22 @@ class QuantLayer(NamedTuple):
     scales: torch.Tensor
 
 
+def _buffer(name):
+    """A buffer of a :class:`QuantKVCache`: another of the same kind may take its place, and
+    the views of the layers are then made anew."""
+    def get(self):
+        return self.__dict__[name]
+
+    def put(self, t):
+        held = self.__dict__.get(name)
+        if held is not None and (t.shape != held.shape or t.dtype != held.dtype or t.device != held.device
+                                 or not t.is_contiguous()):
+            raise ValueError("Quantised KV buffers are replaced by contiguous ones of the same shape, type and device")
+        self.__dict__[name] = t
+        self._make_layers()
+    return property(get, put)
+
+
 class QuantKVCache:
     """A :class:`KVCache` whose elements take 4 or 8 bits: codes ``k, v [L, B,
     Hkv, C, 8*bits]`` and ``scales [L, B, Hkv, C, 4]``, uint8. The store
@@ -86,6 +102,7 @@ class QuantKVCache:
     :meth:`decode` and :func:`kv_quant.read` give back what they stand for.
     Prefill attends over its own unquantised keys and values, as
     :meth:`KVCache.prefill` returns them."""
+    k, v, scales = _buffer("k"), _buffer("v"), _buffer("scales")
 
     def __init__(self, cfg, batch, capacity, device, dtype, bits=4):
         if dtype != torch.bfloat16:
@@ -123,10 +140,17 @@ class QuantKVCache:
         self.bits, self.capacity = k.shape[4] // 8, k.shape[3]
         self.keys = torch.arange(self.capacity, device=k.device)
         self.slots = torch.arange(k.shape[1], device=k.device)
-        self._layers = [QuantLayer(*buffers) for buffers in zip(k, v, scales)]  # views, made once
+
+    def _make_layers(self):
+        held = [self.__dict__.get(name) for name in QuantLayer._fields]
+        self._layers = [] if any(t is None for t in held) else [QuantLayer(*buffers) for buffers in zip(*held)]
+
+    def __setstate__(self, state):
+        self.__dict__.update(state)
+        self._make_layers()  # a copy's views are of its own buffers
 
     def layer(self, layer):
-        """Layer ``layer``'s buffers, views of ``k``, ``v`` and ``scales``."""
+        """Layer ``layer``'s buffers, views of ``k``, ``v`` and ``scales`` made once."""
         return self._layers[layer]
 
     def reset(self):

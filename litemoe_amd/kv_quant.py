@@ -39,11 +39,11 @@ def per_row(t, rows, dtype, index, what):
     return t if t.is_contiguous() else t.contiguous()
 
 
-def _device(cache):
+def _device(kc):
     """The index of the cache's GPU; a cache's own buffers are what :func:`check_layer` asks for."""
-    index = cache.k.get_device()
+    index = kc.get_device()
     if index < 0:
-        _lib.require_cuda(cache.k, what="quantised KV cache")
+        _lib.require_cuda(kc, what="quantised KV cache")
     return index
 
 
@@ -53,7 +53,7 @@ def write(cache, layer, k, v, positions, active, slots):
     stores them. ``k, v [rows, H, 1, 64]`` bf16 with any strides; ``active`` may
     be None (every row). Rows out of range are skipped. One row per target."""
     kc, vc, scales = cache.layer(layer)
-    index = _device(cache)
+    index = _device(kc)
     batch, heads, capacity, _ = kc.shape
     shape = k.shape
     if len(shape) != 4 or shape[1:] != (heads, 1, 64) or v.shape != shape:
@@ -77,7 +77,7 @@ def read(cache, layer, positions, slots):
     ``k, v [rows, H, 1, 64]`` bf16, the layout :func:`write` takes. Rows out of
     range give zeros."""
     kc, vc, scales = cache.layer(layer)
-    index = _device(cache)
+    index = _device(kc)
     batch, heads, capacity, _ = kc.shape
     rows = positions.numel()
     positions = per_row(positions, rows, torch.int64, index, "positions")

@@ -1,7 +1,9 @@
 """The quantised KV cache without a GPU: its number format, its buffers, and
 the calls that are refused before anything is launched."""
+import copy
 import ctypes as C
 import math
+import pickle
 
 import pytest
 import torch
@@ -194,3 +196,23 @@ def test_quant_splits_of_long_contexts_go_by_ranges(maximum):
         assert (n == 1) if 224 < pairs <= 256 or pairs > 320 else n >= 8
     for batch in (29, 31, 32, 33):
         assert quant_splits(batch, 8, maximum) == quant_splits(8 * batch, 1, maximum)
+
+
+def test_layers_are_views_of_the_buffers_the_cache_holds():
+    """Buffers replaced by others, a copy and a pickled cache: ``layer`` gives views of what
+    ``k``, ``v`` and ``scales`` are, as a KVCache's own indexing does."""
+    cache = QuantKVCache.empty(2, 3, 2, 16, "cpu", bits=4)
+    cache.layer(0)
+    fresh = [torch.full_like(t, 3) for t in (cache.k, cache.v, cache.scales)]
+    cache.k, cache.v, cache.scales = fresh
+    for other in (cache, copy.copy(cache), copy.deepcopy(cache), pickle.loads(pickle.dumps(cache))):
+        for layer in range(2):
+            held = other.layer(layer)
+            assert [t.data_ptr() for t in held] == [t[layer].data_ptr() for t in (other.k, other.v, other.scales)]
+            assert all(bool((t == 3).all()) for t in held)
+        assert other.bits == 4 and other.capacity == 16
+    assert copy.deepcopy(cache).k.data_ptr() != cache.k.data_ptr()
+    for bad in (fresh[0][:1], fresh[0].int(), fresh[0].transpose(1, 2)):
+        with pytest.raises(ValueError, match="same shape, type and device"):
+            cache.k = bad
+    assert cache.k is fresh[0]
