@@ -213,7 +213,9 @@ decode_quant_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, Cache 
   const uint32_t my_lds = __builtin_amdgcn_readfirstlane(lds_address(my_stages));
 
   // The fused form's row: 32 / kPairs lanes per head, each kPairs of the rotation's
-  // channel pairs (j, 32 + j); the loads go out before anything waits.
+  // channel pairs (j, 32 + j). These loads are requested first; the row's length, position
+  // and mask below are waited for one after the other before the first stage is, and the
+  // mask, a byte, with all of these.
   constexpr int kPairs = P / 4, kRowLanes = kD / 2 / kPairs;
   static_assert((P + 2) * kRowLanes <= 4 * kWave, "one pass over the row");
   typedef float pairs_t __attribute__((ext_vector_type(kPairs)));
@@ -472,7 +474,12 @@ decode_quant_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, Cache 
     }
     // Probabilities rounded to bf16, their sum from the rounded ones (so that a row
     // that one position rules keeps its value: 5 to 15% less error at no cost), times
-    // the scale of each block of V, which is exact from 2^-126 up, as bf16 pairs.
+    // the scale of each block of V, which is exact from 2^-126 up, as bf16 pairs. In two
+    // bf16 parts the result would be off by 1.65e-3 (RMS, relative), the output's own
+    // rounding, instead of 1.85e-3 to 2.15e-3, for 3 to 9% more time in 4 bits (128 ragged
+    // rows 35.0 -> 37.3 us, fused 33.4 -> 39.2, 64 rows to 1279 10.2 -> 10.9) and 1 to 2% in
+    // 8; the cache's own rounding is 1.1e-1 and 2.7e-2, so one part is taken, as over a bf16
+    // cache.
     uint32_t pb[2][kPasses][2];
 #pragma unroll
     for (int p = 0; p < kPasses; ++p) {
@@ -729,11 +736,14 @@ int launch_decode_quant(const Call &c, const void *q, int64_t qs0, int64_t qs1, 
               inv_splits, least, splits, stride_splits, part, in, (bf16 *)out, out_mb, s);
   };
   // Up to one workgroup per CU a wave has its SIMD to itself, and a 4-bit stage's chain
-  // of dependent steps (0.57 us) takes longer than its bytes: eight waves where
-  // they get two stages each. 24 rows to 2000 positions 8.6 us with four, 7.6 with eight;
-  // 32 rows to 4095 15.2 and 14.3, 8 rows to 32768 in four splits 26.9 and 21.7; 10 rows
-  // to 1000 5.4 and 5.5, one row of 509 3.6 and 3.8. In 8 bits they differ by 2 to 4% (32
-  // rows to 4095 22.5 and 21.9), which a second set of kernels is not worth.
+  // of dependent steps (0.57 us) takes longer than its bytes: eight waves where a split of
+  // the longest row gives them two stages each. 24 rows to 2000 positions 8.4 us with four,
+  // 7.6 with eight; 32 rows to 4095 14.7 and 13.6, 8 rows to 32768 in four splits 26.9 and
+  // 21.7; 10 rows to 1000 5.4 and 5.5, one row of 509 3.6 and 3.8. The host knows the bound
+  // and not the rows: under a bound of 2000 to 4095 rows of 500 to 1000 take 5.9 to 6.3 us
+  // either way, rows of 300 to 500 4.6 to 4.8 with four and 5.0 to 5.3 with eight. In 8 bits
+  // they differ by 2 to 4% (32 rows to 4095 22.5 and 21.9), which a second set of kernels is
+  // not worth.
   const bool wide = c.bits == 4 && (int64_t)splits * c.kv_heads * c.batch <= kCUs && chunk >= 16 * kStageKeys;
   typedef std::integral_constant<int, 4> Four;
   typedef std::integral_constant<int, 8> Eight;
