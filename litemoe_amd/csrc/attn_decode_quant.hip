@@ -656,15 +656,15 @@ int64_t workspace_bytes(int64_t batch, int64_t q_heads, int64_t splits) {
 template <int kBits, int P, bool kFused, int kWaves>
 int launch_sized(const bf16 *q, int64_t qs0, int64_t qs1, const Cache &cache, const int32_t *used, int64_t batch,
                  int64_t q_heads, int64_t kv_heads, int64_t capacity, float scale, int64_t max_len, uint32_t inv_splits,
-                 int least, int grid_splits, int stride_splits, const Partial &part, const QkvIn &in, bf16 *out, int out_mb,
-                 hipStream_t s) {
+                 int least, int grid_splits, int stride_splits, const Partial &part, const QkvIn &in, bf16 *out,
+                 int out_mb, hipStream_t s) {
   // KV heads fastest: workgroups go to the XCDs in turn, and with the splits fastest one XCD
   // would have the first split of every row and another the last (8 rows of 8191 to 32768
   // positions in four splits 21.5 us against 20.7, three rows of 8 bits in eight 7.65 and 7.5).
   const dim3 grid((unsigned)kv_heads, (unsigned)grid_splits, (unsigned)batch);
   decode_quant_kernel<kBits, P, kFused, kWaves><<<grid, kWaves * kWave, 0, s>>>(
-      q, qs0, qs1, cache, used, (int)q_heads, (int)kv_heads, capacity, scale, (int)max_len, inv_splits, least, stride_splits,
-      part, in, out, out_mb);
+      q, qs0, qs1, cache, used, (int)q_heads, (int)kv_heads, capacity, scale, (int)max_len, inv_splits, least,
+      stride_splits, part, in, out, out_mb);
   LM_CHECK_LAUNCH();
   return LM_OK;
 }
