@@ -250,8 +250,9 @@ def _own_flash(s):
     from litemoe_amd.flash_decode import PagedFlashDecode
     if "flash" not in s:
         case = s["case"]
-        s["flash"] = PagedFlashDecode(case["rows"], case["kv_heads"], case["groups"], s["table"].shape[1] * case["page"],
-                                      DEVICE, max(1, case["high"]), head_dim=case["dim"])
+        capacity = s["table"].shape[1] * case["page"]
+        s["flash"] = PagedFlashDecode(case["rows"], case["kv_heads"], case["groups"], capacity, DEVICE,
+                                      min(capacity, max(1, case["high"])), head_dim=case["dim"])
     return s["flash"]
 
 
