@@ -152,6 +152,84 @@ int lm_kv_quant_read(const void *k_codes, const void *v_codes,
                      int64_t head_dim, int64_t capacity, int64_t cache_batch,
                      int64_t bits, void *k, void *v, void *stream);
 
+/* -------------------------------------------------------- paged kv cache -- */
+
+/* The paged cache of one layer: k_pages, v_pages [pages, heads, page, head_dim]
+ * bf16, contiguous, 16-byte aligned, head_dim 64 or 128, page (positions of a
+ * page) a power of two from 16 to 65536. block_table [batch, width] int32
+ * names the pages of each row: position j lies in page block_table[row][j /
+ * page] at j % page. An entry outside [0, pages) names no page: its positions
+ * are not written, read as zeros and are not attended. Rows may share pages.
+ * The reference's cache holds one page of the whole capacity per row
+ * (litemoe/cache.py:7-20, block_table = arange(B), flash_decode.py:10-12).
+ *
+ * lm_paged_rotate_write: rotary positions and the store in one pass.
+ *   q_out[r,h] = rot(q[r,h]);  k_out[r,h] = rot(k[r,h])
+ *   k_pages, v_pages at (slots[r], at[r]) = rot(k[r,h]), v[r,h]
+ * where active[r] and the position has a page. rot turns the first `rotary`
+ * channels of a head (a multiple of 16, at most head_dim) by the angles of
+ * positions[r] and leaves the others: pairs (i, i + rotary/2) with neox
+ * nonzero, else (2i, 2i + 1):
+ *   o1 = x1 c - x2 s,  o2 = x2 c + x1 s
+ * cos_sin [table_len, rotary], cos of all pairs, then sin: fp32 (table_f32
+ * nonzero; products and sums in fp32, rounded once) or bf16 (each product and
+ * each sum rounded to bf16, lm_rope_kv_write's arithmetic). Positions outside
+ * the table are not turned. With cos_sin NULL and rotary 0 nothing is.
+ * at NULL: at = positions (one of the two is needed for a store); slots NULL:
+ * slot = row; active NULL: every row is written. k_pages and v_pages NULL:
+ * nothing is stored (v, block_table, at, active and slots are not looked at; any
+ * head_dim that is a multiple of 16, to 256). q_heads 0: no queries. k_out may
+ * be NULL with a store. q_out and k_out may be q and k (in place). Strides in
+ * elements, multiples of 8, pointers 16-byte aligned, channels contiguous.
+ * One row per target, as lm_kv_write. Replaces vLLM `_custom_ops.rotary_embedding`
+ * at litemoe/model.py:58,63-64 with `cache.write` (model.py:59,70). */
+int lm_paged_rotate_write(const void *q, int64_t qs0, int64_t qs1,
+                          const void *k, int64_t ks0, int64_t ks1,
+                          const void *v, int64_t vs0, int64_t vs1,
+                          const void *cos_sin, int64_t table_len,
+                          int64_t rotary, int table_f32, int neox,
+                          const int64_t *positions, const int64_t *at,
+                          const uint8_t *active, const int64_t *slots,
+                          void *q_out, int64_t qo0, int64_t qo1, void *k_out,
+                          int64_t ko0, int64_t ko1, void *k_pages,
+                          void *v_pages, const int32_t *block_table,
+                          int64_t batch, int64_t width, int64_t pages,
+                          int64_t page, int64_t rows, int64_t q_heads,
+                          int64_t kv_heads, int64_t head_dim, void *stream);
+
+/* What the paged cache holds at (slots[r], h, positions[r]): k and v [rows,
+ * heads, head_dim] contiguous, 16-byte aligned. Rows whose position or slot is
+ * out of range or in no page get zeros; slots may be NULL (slot = row). */
+int lm_paged_read(const void *k_pages, const void *v_pages,
+                  const int32_t *block_table, int64_t batch, int64_t width,
+                  int64_t pages, int64_t page, const int64_t *positions,
+                  const int64_t *slots, int64_t rows, int64_t heads,
+                  int64_t head_dim, void *k, void *v, void *stream);
+
+/* Eviction by weight, all layers at once: k_pages, v_pages [layers, pages,
+ * heads, page, head_dim], weights fp32 [layers, batch, heads, width * page].
+ * Row b holds n = used[b] positions (held to [0, width * page]). For each layer,
+ * row and head the last `recent` positions and the heaviest of the others stay,
+ * min(n, keep) in all (of equal weights the first; a NaN counts as the heaviest,
+ * -0 as 0), in their order:
+ *   kept        int32 [layers, batch, heads, keep]: their positions, then -1
+ *   weights_out like weights: theirs, then zeros; may be weights itself
+ *   used_out    int32 [batch]: min(n, keep)
+ * and their K and V are copied to positions 0 .. of the row in `target` [batch,
+ * target_width], a table over the same pages. Positions that `source` (the
+ * row's present table, [batch, width]) or `target` has no page for are not
+ * copied. No page of `target` may be one that a row of `source` reads in this
+ * call; `source`'s pages are not written, so another row may share them.
+ * 0 <= recent <= keep, 1 <= keep <= width * page, layers * batch <= 65535. The
+ * reference holds every position to the end (litemoe/cache.py:7-20). */
+int lm_kv_evict(void *k_pages, void *v_pages, const int32_t *source,
+                const int32_t *target, int64_t width, int64_t target_width,
+                int64_t pages, int64_t page, const int32_t *used,
+                const float *weights, int64_t layers, int64_t batch,
+                int64_t heads, int64_t head_dim, int64_t keep, int64_t recent,
+                float *weights_out, int32_t *kept, int32_t *used_out,
+                void *stream);
+
 /* ------------------------------------------------------------ attention -- */
 
 /* Workspace for lm_flash_decode with the given split count. */
@@ -263,6 +341,64 @@ int lm_flash_decode_quant_qkv(const float *qkv_partials, int64_t qkv_splits,
                               float scale, int64_t max_len, int64_t num_splits,
                               int frag_out, void *out, void *workspace,
                               int64_t workspace_bytes, void *stream);
+
+/* Workspace for lm_flash_decode_paged and _qkv; weighed nonzero: with weights. */
+int lm_flash_decode_paged_workspace_size(int64_t batch, int64_t q_heads,
+                                         int64_t head_dim, int64_t max_len,
+                                         int64_t num_splits, int weighed,
+                                         int64_t *bytes);
+
+/* lm_flash_decode over a paged cache (see lm_paged_rotate_write): out[b,h] =
+ * softmax(scale * q[b,h] . K_j, j < used[b]) V over the positions that have a
+ * page; a row that has none gives zeros. used[b] is held to [0, max_len] and
+ * to width * page. Scores, maxima and sums in fp32, the probabilities rounded
+ * to bf16 for the matrix cores and summed as rounded. Positions from used[b] on
+ * and positions without a page may hold anything. q_heads / kv_heads at most
+ * 16; q 16-byte aligned, its strides multiples of 8; out [batch, q_heads,
+ * head_dim] contiguous.
+ * Each row is cut by its own length into at most num_splits pieces of whole
+ * tiles of 32 positions. weights and weights_out (both or neither; fp32
+ * [batch, kv_heads, width * page], 16-byte aligned, may be one buffer): for
+ * every j below the row's length
+ *   weights_out[b,g,j] = weights[b,g,j] + sum of the probabilities of j over
+ *                        the query heads of KV head g
+ * (0 for a position without a page); other entries are not written. Two calls
+ * in flight at once need workspaces of their own (16-byte aligned). Replaces
+ * litemoe/flash_decode.py:16-22 with a block table of more than one page a row. */
+int lm_flash_decode_paged(const void *q, int64_t qs0, int64_t qs1,
+                          const void *k_pages, const void *v_pages,
+                          const int32_t *block_table, int64_t width,
+                          int64_t pages, int64_t page, const int32_t *used,
+                          int64_t batch, int64_t q_heads, int64_t kv_heads,
+                          int64_t head_dim, float scale, int64_t max_len,
+                          int64_t num_splits, const float *weights,
+                          float *weights_out, void *out, void *workspace,
+                          int64_t workspace_bytes, void *stream);
+
+/* lm_flash_decode_qkv over a paged cache, head_dim 64 or 128: the partials'
+ * sum (rounded to bf16 first where the table is bf16), the rotation of
+ * lm_paged_rotate_write by positions[b], the store of the new token's key and
+ * value at position used[b] - 1 of its row, and attention over the first used[b]
+ * positions with them. Nothing is stored, and the cache is attended as it is,
+ * where active[b] is 0, used[b] is above max_len or width * page, or the
+ * position has no page. Results are bitwise those of lm_paged_rotate_write on
+ * the same heads followed by lm_flash_decode_paged. Two rows of one call may not
+ * store to the same page. row_order and frag_out (nonzero: batch <= 128) as
+ * lm_flash_decode_quant_qkv; qkv_partials 16-byte aligned. */
+int lm_flash_decode_paged_qkv(const float *qkv_partials, int64_t qkv_splits,
+                              const void *cos_sin, int64_t table_len,
+                              int64_t rotary, int table_f32, int neox,
+                              const int64_t *positions, const uint8_t *active,
+                              void *k_pages, void *v_pages,
+                              const int32_t *block_table, int64_t width,
+                              int64_t pages, int64_t page, const int32_t *used,
+                              const int32_t *row_order, int64_t batch,
+                              int64_t q_heads, int64_t kv_heads,
+                              int64_t head_dim, float scale, int64_t max_len,
+                              int64_t num_splits, const float *weights,
+                              float *weights_out, int frag_out, void *out,
+                              void *workspace, int64_t workspace_bytes,
+                              void *stream);
 
 /* Variable-length attention over a packed batch (one row per token):
  * sequence s owns tokens [cu[s], cu[s+1]); token i of it attends keys

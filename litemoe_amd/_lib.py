@@ -35,6 +35,16 @@ _SIGNATURES = {
                               _v, _v, _i64, _v],
     "lm_flash_decode_quant_qkv": [_v, _i64, _v, _i64, _v, _v, _v, _v, _v, _v, _v, _i64, _i64, _i64, _i64, _i64, _i64,
                                   _f32, _i64, _i64, _i32, _v, _v, _i64, _v],
+    "lm_paged_rotate_write": [_v, _i64, _i64, _v, _i64, _i64, _v, _i64, _i64, _v, _i64, _i64, _i32, _i32, _v, _v, _v, _v,
+                              _v, _i64, _i64, _v, _i64, _i64, _v, _v, _v, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+                              _i64, _v],
+    "lm_paged_read": [_v, _v, _v, _i64, _i64, _i64, _i64, _v, _v, _i64, _i64, _i64, _v, _v, _v],
+    "lm_kv_evict": [_v, _v, _v, _v, _i64, _i64, _i64, _i64, _v, _v, _i64, _i64, _i64, _i64, _i64, _i64, _v, _v, _v, _v],
+    "lm_flash_decode_paged_workspace_size": [_i64, _i64, _i64, _i64, _i64, _i32, C.POINTER(C.c_int64)],
+    "lm_flash_decode_paged": [_v, _i64, _i64, _v, _v, _v, _i64, _i64, _i64, _v, _i64, _i64, _i64, _i64, _f32, _i64, _i64,
+                              _v, _v, _v, _v, _i64, _v],
+    "lm_flash_decode_paged_qkv": [_v, _i64, _v, _i64, _i64, _i32, _i32, _v, _v, _v, _v, _v, _i64, _i64, _i64, _v, _v,
+                                  _i64, _i64, _i64, _i64, _f32, _i64, _i64, _v, _v, _i32, _v, _v, _i64, _v],
     "lm_flash_decode_workspace_size": [_i64, _i64, _i64, _i64, C.POINTER(C.c_int64)],
     "lm_flash_decode": [_v, _i64, _i64, _v, _v, _v, _i64, _i64, _i64, _i64, _i64, _f32, _i64,
                         _i64, _v, _v, _i64, _v],

@@ -2,8 +2,9 @@
 
 The public surface is the reference's (litemoe/engine.py:15-221): ``Request``,
 ``Engine(model, requests, world, rank, mode, ignore_eos, poll, capacity,
-host_process, kv_bits)`` (``kv_bits`` 8 or 4 holds the KV cache quantised, which
-the reference does not have), ``decode_step()``, ``prefill()``, ``prepare_graph()``,
+host_process, kv_bits, kv_page)`` (``kv_bits`` 8 or 4 holds the KV cache quantised,
+``kv_page`` in pages of so many positions, each request with pages for its own length;
+the reference has neither), ``decode_step()``, ``prefill()``, ``prepare_graph()``,
 ``stopped()`` and ``generate()`` with the same metrics keys, the same
 ``emit [B, 3] = (token, index, valid)`` snapshot and its ordering check.
 The engine runs one GPU (world 1). What differs is how a step runs:
@@ -30,8 +31,9 @@ from dataclasses import dataclass
 
 import torch
 
-from .cache import KVCache, QuantKVCache
+from .cache import KVCache, PagedKVCache, QuantKVCache
 from .execution import OutputRing, capture_decode
+from .kv_paged import PAGES
 from .step import greedy_epilogue
 
 CONTEXT_LIMIT = 4096
@@ -86,9 +88,11 @@ class Engine:
     ring_depth = 4
 
     def __init__(self, model, requests, world=1, rank=0, mode="eager", ignore_eos=False, poll=1,
-                 capacity=None, host_process=None, kv_bits=16):
+                 capacity=None, host_process=None, kv_bits=16, kv_page=None):
         if kv_bits not in (4, 8, 16):
             raise ValueError("The KV cache holds 16 bits per element, or 8 or 4 quantised")
+        if kv_page is not None and (kv_page not in PAGES or kv_bits != 16):
+            raise ValueError("The KV cache's pages hold a power of two from 16 to 65536 positions, of 16 bits per element")
         if world != 1 or rank != 0:
             raise ValueError("This build runs one engine per GPU (world == 1)")
         if poll < 1 or mode not in ("eager", "graph", "graph-async"):
@@ -114,7 +118,12 @@ class Engine:
             raise ValueError("Full Decode Graph requires a graph-safe expert backend")
         cfg = model.cfg
         sizes = cfg, self.batch, self.capacity, self.device, self.dtype
-        self.cache = self.cache_type(*sizes) if kv_bits == 16 else QuantKVCache(*sizes, bits=kv_bits)
+        if kv_page is not None:
+            need = [len(r.prompt) + r.budget - 1 for r in self.requests]
+            self.cache = PagedKVCache(*sizes, page=kv_page, pages=sum(-(-n // kv_page) for n in need))
+            self.cache.reserve(list(range(self.batch)), need)
+        else:
+            self.cache = self.cache_type(*sizes) if kv_bits == 16 else QuantKVCache(*sizes, bits=kv_bits)
         self.state = {name: torch.zeros(self.batch, dtype=dtype, device=self.device)
                       for name, dtype in STATE_FIELDS}
         self.emit = torch.zeros(self.batch, 3, dtype=torch.int64, device=self.device)

@@ -15,8 +15,9 @@ import math
 
 import torch
 
-from . import _lib, kv_quant
+from . import _lib, kv_paged, kv_quant
 from .linear import FragRows
+from .rope import check_table
 
 
 def default_splits(batch, kv_heads, maximum, target_workgroups=512, min_keys=256, max_splits=16):
@@ -266,4 +267,138 @@ class QuantFlashDecode:
                      used.data_ptr(), _lib.ptr(row_order), b, q_heads, self.kv_heads, self.capacity, 64, self.bits,
                      float(scale), self.maximum, self.splits, int(frag_out), out_ptr, self.workspace.data_ptr(),
                      self.workspace.numel())
+        return out
+
+
+def paged_splits(batch, kv_heads, maximum):
+    """Key-range splits over a paged cache."""
+    pairs = max(1, batch * kv_heads)
+    longest = -(-maximum // 256) if maximum >= 3 * 256 else 1
+    return max(1, min(max(16, maximum // 4096), 512 // pairs, longest))
+
+
+class PagedFlashDecode:
+    """:class:`FlashDecode` over a :class:`~litemoe_amd.cache.PagedKVCache`
+    (``lm_flash_decode_paged``, ``lm_flash_decode_paged_qkv``): the same plan and calls,
+    the cache layer given as ``k, v, table`` (``cache.layer(i)``), up to 16 query heads
+    per KV head, heads of 64 or 128 channels. ``capacity`` is the cache's. Calls that
+    overlap (on two streams, or recorded into graphs that replay at once) need an object
+    each: partial results lie in its workspace."""
+
+    def __init__(self, batch, kv_heads, groups, capacity, device, maximum=None, num_splits=None, ordered=False,
+                 head_dim=64):
+        if maximum is not None and not 0 < maximum <= capacity:
+            raise ValueError("Decode attention requires a valid length bound")
+        if head_dim not in kv_paged.HEAD_DIMS:
+            raise ValueError("Decode attention over a paged cache takes head_dim 64 or 128")
+        if not 1 <= groups <= 16:
+            raise ValueError("Decode attention over a paged cache takes 1 to 16 query heads per KV head")
+        self.batch, self.kv_heads, self.groups, self.capacity = batch, kv_heads, groups, capacity
+        self.head_dim = head_dim
+        self.maximum = capacity if maximum is None else maximum
+        self.splits = num_splits or paged_splits(batch, kv_heads, self.maximum)
+        self.device = torch.device(device)
+        self.workspace = self._space(False)
+        self.weigh_space = None  # the larger workspace of a call with weights, made by the first
+        self.row_order = (torch.empty(batch, dtype=torch.int32, device=self.device)
+                          if ordered and self.device.type == "cuda" else None)
+
+    def _space(self, weighed):
+        size = _lib.size_query("lm_flash_decode_paged_workspace_size", self.batch, self.kv_heads * self.groups,
+                               self.head_dim, self.maximum, self.splits, int(weighed)) \
+            if self.device.type == "cuda" else 0
+        return torch.empty(max(size, 1), dtype=torch.uint8, device=self.device)
+
+    def _check(self, k, v, table, q_heads, rows):
+        """The layer's device index, once it is what this object was built for."""
+        index = kv_paged.check_layer(k, v, table)
+        _, heads, page, dim = k.shape
+        if rows > self.batch or table.shape[0] < rows or table.shape[1] * page != self.capacity:
+            raise ValueError("Decode attention built for another batch/capacity")
+        if heads != self.kv_heads or dim != self.head_dim:
+            raise ValueError("Decode attention built for other cache heads")
+        if q_heads != heads * self.groups:
+            raise ValueError("Query heads do not match the cache heads")
+        if self.workspace.get_device() != index:
+            raise ValueError("Decode attention built for another device")
+        return index
+
+    def _weights(self, weights, weights_out, rows, index):
+        """The pointers of a call's weights and the workspace it takes."""
+        if weights is None:
+            if weights_out is not None:
+                raise ValueError("weights_out goes with weights")
+            return None, None, self.workspace
+        weights_out = weights if weights_out is None else weights_out
+        for w in (weights, weights_out):
+            if (w.dtype != torch.float32 or w.dim() != 3 or w.shape[0] < rows
+                    or w.shape[1:] != (self.kv_heads, self.capacity) or not w.is_contiguous()
+                    or w.get_device() != index or w.data_ptr() % 16):
+                raise ValueError("Weights must be contiguous fp32 [B, H, capacity] on the cache's device")
+        if self.weigh_space is None:
+            self.weigh_space = self._space(True)
+        return weights.data_ptr(), weights_out.data_ptr(), self.weigh_space
+
+    def __call__(self, q, k, v, table, lengths, active, scale, used=None, weights=None, weights_out=None):
+        """Attention of ``q [B, Hq, 1, D]`` over the first ``used[b]`` positions of each
+        row (``where(active, lengths + 1, 1)`` unless given) that have a page; a row with
+        none gives zeros. ``weights [B, Hkv, capacity]`` (fp32): each position's
+        probability, summed over the query heads of its KV head, is added to it, in place
+        or into ``weights_out``; entries from ``used[b]`` on are not written."""
+        b, hq, s, d = q.shape
+        if s != 1 or d != self.head_dim:
+            raise ValueError("Decode attention takes one query position with the cache's head_dim")
+        index = self._check(k, v, table, hq, b)
+        if q.dtype != torch.bfloat16:
+            raise ValueError("Decode attention supports BF16")
+        if q.get_device() != index:
+            raise ValueError("Queries and cache must be on one device")
+        rows, heads, _, channels = q.stride()
+        rows, heads = rows if b > 1 else 0, heads if hq > 1 else 0  # of a single one the stride says nothing
+        if channels != 1 or rows % 8 or heads % 8 or q.data_ptr() % 16:
+            raise ValueError("Decode attention needs contiguous channels and 16-byte aligned query heads")
+        if used is None:
+            used = torch.where(active, lengths + 1, 1)
+        used = kv_quant.per_row(used, b, torch.int32, index, "used")
+        before, after, space = self._weights(weights, weights_out, b, index)
+        out = torch.empty_like(q) if q.is_contiguous() else torch.empty(q.shape, device=q.device, dtype=q.dtype)
+        _lib.call_on(index, "lm_flash_decode_paged", q.data_ptr(), rows, heads, k.data_ptr(), v.data_ptr(),
+                     table.data_ptr(), table.shape[1], k.shape[0], k.shape[2], used.data_ptr(), b, hq, self.kv_heads, d,
+                     float(scale), self.maximum, self.splits, before, after, out.data_ptr(), space.data_ptr(),
+                     space.numel())
+        return out
+
+    def fused_qkv(self, partials, cos_sin, positions, active, k, v, table, scale, used, q_heads, row_order=None,
+                  frag_out=False, is_neox=True, weights=None, weights_out=None):
+        """:meth:`FlashDecode.fused_qkv`: the new token's key and value go to position
+        ``used[b] - 1`` of the row, which has a page of its own there; ``positions[b]``
+        is what they and the query are rotated by (the same, or past it where the row was
+        evicted from). Rows with ``active`` false, when given, with ``used`` past the
+        plan's bound, or without that page store nothing and attend what they hold.
+        Rotation as :func:`rope.rotate_kv_write` has it, weights as :meth:`__call__`."""
+        splits, b, ncols = partials.shape
+        index = self._check(k, v, table, q_heads, b)
+        if ncols != (q_heads + 2 * self.kv_heads) * self.head_dim:
+            raise ValueError("QKV partials do not match the cache heads")
+        if partials.dtype != torch.float32 or not partials.is_contiguous() or partials.get_device() != index:
+            raise ValueError("QKV partials must be contiguous fp32 on the cache's device")
+        check_table(cos_sin, index, self.head_dim)
+        positions = kv_quant.per_row(positions, b, torch.int64, index, "positions")
+        used = kv_quant.per_row(used, b, torch.int32, index, "used")
+        active = None if active is None else kv_quant.per_row(active, b, torch.bool, index, "active")
+        if row_order is not None and (row_order.dtype != torch.int32 or row_order.shape != (b,)
+                                      or row_order.get_device() != index or not row_order.is_contiguous()):
+            raise ValueError("row_order must be an int32 [B] permutation")
+        before, after, space = self._weights(weights, weights_out, b, index)
+        if frag_out:
+            out = FragRows(b, q_heads * self.head_dim, k.device)
+            out_ptr = out.data.data_ptr()
+        else:
+            out = torch.empty((b, q_heads, 1, self.head_dim), device=k.device, dtype=torch.bfloat16)
+            out_ptr = out.data_ptr()
+        _lib.call_on(index, "lm_flash_decode_paged_qkv", partials.data_ptr(), splits, cos_sin.data_ptr(), *cos_sin.shape,
+                     int(cos_sin.dtype == torch.float32), int(bool(is_neox)), positions.data_ptr(), _lib.ptr(active),
+                     k.data_ptr(), v.data_ptr(), table.data_ptr(), table.shape[1], k.shape[0], k.shape[2],
+                     used.data_ptr(), _lib.ptr(row_order), b, q_heads, self.kv_heads, self.head_dim, float(scale),
+                     self.maximum, self.splits, before, after, int(frag_out), out_ptr, space.data_ptr(), space.numel())
         return out

@@ -1,0 +1,133 @@
+"""The paged cache's store, read-back and eviction (``lm_paged_rotate_write``,
+``lm_paged_read``, ``lm_kv_evict``) for :class:`~litemoe_amd.cache.PagedKVCache`.
+
+Keys and values lie in pages of a pool, and a table names each row's pages, so
+that a row takes memory by its own length, rows may share the pages of a common
+beginning, and an eviction gives pages back. The reference's cache is one page of
+the whole capacity per row (litemoe/cache.py:7-20, flash_decode.py:10-12).
+"""
+import torch
+
+from . import _lib
+from .kv_quant import per_row
+
+PAGES = tuple(1 << s for s in range(4, 17))  # positions of a page
+HEAD_DIMS = (64, 128)
+
+
+def check_layer(k, v, table):
+    """The device index of one layer's buffers ``k, v [P, H, page, D]``, ``table [B, W]``."""
+    index, shape = k.get_device(), k.shape
+    if index < 0 or v.get_device() != index or table.get_device() != index:
+        _lib.require_cuda(k, v, table, what="paged KV cache")
+        raise ValueError("Paged KV cache layers must share one device")
+    if len(shape) != 4 or v.shape != shape or shape[2] not in PAGES or shape[3] not in HEAD_DIMS:
+        raise ValueError("Paged KV cache layers are k, v [P, H, page, D], page a power of two from 16 to 65536, "
+                         "D 64 or 128")
+    if not (k.dtype == v.dtype == torch.bfloat16 and k.is_contiguous() and v.is_contiguous()):
+        raise ValueError("Paged KV cache layers must be contiguous BF16")
+    check_table(table)
+    return index
+
+
+def check_table(table, rows=None):
+    if table.dtype != torch.int32 or table.dim() != 2 or not table.is_contiguous() or not table.shape[1]:
+        raise ValueError("A page table is contiguous int32 [rows, pages of a row]")
+    if rows is not None and table.shape[0] != rows:
+        raise ValueError("The page table needs one line per row")
+
+
+def aligned(x):
+    """``x [rows, heads, D]`` as the kernels take it: contiguous channels, rows and
+    heads that start at 16 bytes (a copy where it is not so)."""
+    s = x.stride()
+    ok = (s[2] == 1 and (s[0] % 8 == 0 or x.shape[0] == 1) and (s[1] % 8 == 0 or x.shape[1] == 1)
+          and x.data_ptr() % 16 == 0)
+    return x if ok else x.clone(memory_format=torch.contiguous_format)
+
+
+def strides(x):
+    """Row and head stride of ``x [rows, heads, D]``; of a single one the stride says nothing."""
+    s = x.stride()
+    return s[0] if x.shape[0] > 1 else 0, s[1] if x.shape[1] > 1 else 0
+
+
+def write(cache, layer, k, v, positions, active, slots):
+    """Store ``k[row, h, 0, :]`` at position ``positions[row]`` of ``slots[row]`` for
+    active rows (same for v), as :func:`kv_write.write`. ``k, v [rows, H, 1, D]``
+    bf16 with any strides; ``active`` may be None (every row). Rows out of range or
+    without a page there are skipped. One row per target."""
+    kc, vc, table = cache.layer(layer)
+    index = check_layer(kc, vc, table)
+    pages, heads, page, dim = kc.shape
+    if k.dim() != 4 or k.shape[1:] != (heads, 1, dim) or v.shape != k.shape:
+        raise ValueError("KV write takes k, v [rows, H, 1, D] of the cache's heads")
+    if k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
+        raise ValueError("The paged KV write supports BF16")
+    if k.get_device() != index or v.get_device() != index:
+        raise ValueError("KV write tensors must be on the cache's device")
+    rows = k.shape[0]
+    positions = per_row(positions, rows, torch.int64, index, "positions")
+    slots = per_row(slots, rows, torch.int64, index, "slots")
+    active = None if active is None else per_row(active, rows, torch.bool, index, "active")
+    k, v = aligned(k[:, :, 0]), aligned(v[:, :, 0])
+    _lib.call_on(index, "lm_paged_rotate_write", None, 0, 0, k.data_ptr(), *strides(k), v.data_ptr(), *strides(v), None, 0,
+                 0, 0, 0, positions.data_ptr(), None, _lib.ptr(active), slots.data_ptr(), None, 0, 0, None, 0, 0,
+                 kc.data_ptr(), vc.data_ptr(), table.data_ptr(), table.shape[0], table.shape[1], pages, page, rows, 0,
+                 heads, dim)
+
+
+def read(cache, layer, positions, slots):
+    """What the cache holds at ``(slots[row], h, positions[row])``: ``k, v [rows, H,
+    1, D]``, the layout :func:`write` takes. Rows out of range or without a page
+    there give zeros."""
+    kc, vc, table = cache.layer(layer)
+    index = check_layer(kc, vc, table)
+    pages, heads, page, dim = kc.shape
+    rows = positions.numel()
+    positions = per_row(positions, rows, torch.int64, index, "positions")
+    slots = per_row(slots, rows, torch.int64, index, "slots")
+    k = torch.empty((rows, heads, 1, dim), dtype=torch.bfloat16, device=kc.device)
+    v = torch.empty_like(k)
+    _lib.call_on(index, "lm_paged_read", kc.data_ptr(), vc.data_ptr(), table.data_ptr(), table.shape[0], table.shape[1],
+                 pages, page, positions.data_ptr(), slots.data_ptr(), rows, heads, dim, k.data_ptr(), v.data_ptr())
+    return k, v
+
+
+def evict(cache, weights, used, keep, recent, target, table=None, weights_out=None):
+    """Of each row's ``used[b]`` positions, per layer and KV head, the ``recent`` last
+    and the heaviest of the others by ``weights [L, B, H, W * page]`` (fp32; see
+    :meth:`flash_decode.PagedFlashDecode.__call__`) are copied, ``keep`` in all and in
+    their order, to the pages that ``target [B, W']`` names. Returns the weights of
+    what stays (then zeros; in ``weights_out``, which may be ``weights``, if given), the
+    positions kept ``[L, B, H, keep]`` (int32, then -1) and the rows' new ``used``.
+
+    Of equal weights the first stays; a NaN counts as the heaviest. ``table`` is the
+    rows' present table (the cache's own unless given). Pages of ``target`` must not be
+    in it: the rows' present pages are read and not written, so another row may share
+    them. :meth:`PagedKVCache.evict` takes care of both and moves the cache's table."""
+    k, v, own = cache.k, cache.v, cache.table
+    table = own if table is None else table
+    index = check_layer(k[0], v[0], table)
+    layers, pages, heads, page, dim = k.shape
+    if not (k.is_contiguous() and v.is_contiguous()):
+        raise ValueError("Eviction takes a cache of contiguous layers")
+    rows, width = table.shape
+    check_table(target, rows)
+    if target.get_device() != index or weights.get_device() != index:
+        raise ValueError("Eviction's tables and weights must be on the cache's device")
+    shape = (layers, rows, heads, width * page)
+    for w in (weights,) if weights_out is None else (weights, weights_out):
+        if w.dtype != torch.float32 or w.shape != shape or not w.is_contiguous() or w.get_device() != index:
+            raise ValueError("Weights must be contiguous fp32 [L, B, H, positions of a row] on the cache's device")
+    keep, recent = int(keep), int(recent)
+    if not 1 <= keep <= width * page or not 0 <= recent <= keep:
+        raise ValueError("Eviction keeps 1 to all positions of a row, and at most that many recent ones")
+    used = per_row(used, rows, torch.int32, index, "used")
+    out = torch.empty_like(weights) if weights_out is None else weights_out
+    kept = torch.empty((layers, rows, heads, keep), dtype=torch.int32, device=k.device)
+    left = torch.empty(rows, dtype=torch.int32, device=k.device)
+    _lib.call_on(index, "lm_kv_evict", k.data_ptr(), v.data_ptr(), table.data_ptr(), target.data_ptr(), width,
+                 target.shape[1], pages, page, used.data_ptr(), weights.data_ptr(), layers, rows, heads, dim, keep,
+                 recent, out.data_ptr(), kept.data_ptr(), left.data_ptr())
+    return out, kept, left

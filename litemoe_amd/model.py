@@ -31,19 +31,28 @@ import torch
 import torch.nn.functional as F
 
 from . import _lib
-from .cache import QuantKVCache
+from .cache import PagedKVCache, QuantKVCache
 from .config import validate_config
-from .flash_decode import FlashDecode, QuantFlashDecode
+from .flash_decode import FlashDecode, PagedFlashDecode, QuantFlashDecode
 from .experts import combine_supported, finish_add_rmsnorm, pack_expert_weights, scan_path
 from .linear import (linear_dense, linear_rope_kv, linear_splitk, linear_splitk_frag, linear_splitk_rmsnorm,
                      pick_splits)
 from .norm import add_rmsnorm, rmsnorm
 from .packed import PackedPrefill, build_packed, varlen_attention
-from .rope import rope_kv_write, rotary_embedding
+from .rope import rope_kv_write, rotary_embedding, rotate_kv_write
 from .router import add_rmsnorm_route as route_add_rmsnorm
 from .router import add_rmsnorm_route_splitk as route_add_rmsnorm_splitk
 from .router import route
 from .step import PackedHead, decode_prologue, greedy_epilogue, greedy_head, head_supported
+
+
+def decode_kind(cache):
+    """The decode attention over ``cache``, and what its construction takes besides sizes."""
+    if isinstance(cache, PagedKVCache):
+        return PagedFlashDecode, {}
+    if isinstance(cache, QuantKVCache):
+        return QuantFlashDecode, dict(bits=cache.bits)
+    return FlashDecode, {}
 
 
 class Granite:
@@ -114,15 +123,16 @@ class Granite:
                 w["input_linear_packed"], w["output_linear_packed"] = pack_expert_weights(w1, w2)
 
     def _decode_attention(self, batch, cache):
-        bits = getattr(cache, "bits", 16)
-        if self.decode_flash is not None:
-            if getattr(self.decode_flash, "bits", 16) != bits:
+        kind, more = decode_kind(cache)
+        flash = self.decode_flash
+        if flash is not None:
+            if getattr(flash, "bits", 16) != getattr(cache, "bits", 16) or \
+                    isinstance(flash, PagedFlashDecode) != isinstance(cache, PagedKVCache):
                 raise ValueError("The decode attention was built for another KV cache type")
-            return self.decode_flash
-        key = (batch, cache.capacity, bits)
+            return flash
+        key = (batch, cache.capacity, kind, *more.values())
         if key not in self._flash:
             cfg = self.cfg
-            kind, more = (FlashDecode, {}) if bits == 16 else (QuantFlashDecode, dict(bits=bits))
             self._flash[key] = kind(batch, cfg.num_key_value_heads, cfg.num_attention_heads // cfg.num_key_value_heads,
                                     cache.capacity, cache.k.device, **more)
         return self._flash[key]
@@ -130,7 +140,8 @@ class Granite:
     @staticmethod
     def _layer_cache(cache, layer):
         """The buffers of one cache layer as the decode attention takes them."""
-        return cache.layer(layer) if isinstance(cache, QuantKVCache) else (cache.k[layer], cache.v[layer])
+        own = isinstance(cache, (PagedKVCache, QuantKVCache))
+        return cache.layer(layer) if own else (cache.k[layer], cache.v[layer])
 
     def attention(self, z, w, cache, layer, rope_positions, active, positions, slot):
         """Packed QKV projection, RoPE + KV store, attention, output projection
@@ -141,23 +152,27 @@ class Granite:
         hq, hkv = cfg.num_attention_heads, cfg.num_key_value_heads
         packed = isinstance(slot, PackedPrefill)
         slots = slot.slots if packed else None
-        # a quantised cache is written from the rotated rows, in a pass of its own
-        quant = isinstance(cache, QuantKVCache)
+        # a quantised or paged cache is written from the rotated rows, in a pass of its own
+        apart = isinstance(cache, (PagedKVCache, QuantKVCache))
         if self.qkv_epilogue:
             qkv = linear_rope_kv(z, w["self_attn.qkv_proj"], hq, hkv, rope_positions, active, self.cos_sin,
-                                 None if quant else cache, layer, slots)
+                                 None if apart else cache, layer, slots)
         else:
             qkv = linear_dense(z, w["self_attn.qkv_proj"])
         q = qkv[:, :hq * d].view(rows, hq, d)
         k = qkv[:, hq * d:(hq + hkv) * d].view(rows, hkv, d)
         v = qkv[:, (hq + hkv) * d:].view(rows, hkv, d)
+        stored = False
         if not self.qkv_epilogue:
-            if quant:
+            stored = not isinstance(cache, QuantKVCache)
+            if not stored:
                 rotary_embedding(rope_positions, q, k, d, self.cos_sin)
+            elif apart:
+                q, k = rotate_kv_write(q, k, v, rope_positions, active, self.cos_sin, cache, layer, slots, keep_k=packed)
             else:
                 rope_kv_write(q, k, v, rope_positions, active, self.cos_sin, cache, layer, slots=slots,
                               write_k=packed)
-        if quant:
+        if apart and not stored:
             cache.write(layer, k.unsqueeze(2), v.unsqueeze(2), rope_positions, active, slots)
         if packed:
             a = varlen_attention(q, k, v, slot.cu, slot.maximum, cfg.attention_multiplier)
@@ -408,10 +423,10 @@ class Granite:
         _lib.require_cuda(tokens, positions, valid, cache.k, what="model inputs")
         b, s = tokens.shape
         if isinstance(slot, slice):
-            rows = list(range(*slot.indices(cache.k.shape[1])))
+            rows = list(range(*slot.indices(cache.slots.numel())))
         else:
             rows = [int(slot)]
-        if len(rows) != b or not all(0 <= row < cache.k.shape[1] for row in rows):
+        if len(rows) != b or not all(0 <= row < cache.slots.numel() for row in rows):
             raise ValueError("Prefill slots must name one cache row per batch row")
         if tuple(positions.shape) != (b, s) or tuple(valid.shape) != (b, s):
             raise ValueError("tokens, positions and valid must all be [rows, width]")
@@ -430,7 +445,7 @@ class Granite:
             raise ValueError("Prompt width exceeds the KV capacity")
         for row, n in zip(rows, counts):  # cache.py:28-29 stores k * valid: zeros past the prompt
             if n < s:
-                if isinstance(cache, QuantKVCache):
+                if isinstance(cache, (PagedKVCache, QuantKVCache)):
                     cache.clear(row, n, s)
                     continue
                 cache.k[:, row, :, n:s].zero_()

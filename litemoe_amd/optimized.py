@@ -24,7 +24,7 @@ from contextlib import contextmanager
 from dataclasses import dataclass
 
 from .batch import BatchPrefillEngine
-from .flash_decode import FlashDecode, QuantFlashDecode
+from .model import decode_kind
 from .packed import optimized_prefill_logits
 
 _MODEL_FLAGS = ("decode_flash", "decode_lean", "prefill_lean")
@@ -102,11 +102,10 @@ class OptimizedEngine(BatchPrefillEngine):
         # A ragged batch (longest prompt above 1.25x the shortest) dispatches
         # its attention rows longest first.
         ragged = max(prompts) > 1.25 * min(prompts)
-        bits = getattr(self.cache, "bits", 16)
-        kind, more = (FlashDecode, {}) if bits == 16 else (QuantFlashDecode, dict(bits=bits))
+        kind, more = decode_kind(self.cache)
         self.flash_attention = kind(self.batch, cfg.num_key_value_heads,
                                     cfg.num_attention_heads // cfg.num_key_value_heads,
-                                    self.capacity, self.device, longest, num_splits, ordered=ragged, **more)
+                                    self.cache.capacity, self.device, longest, num_splits, ordered=ragged, **more)
 
     def prepare_graph(self):
         with optimized_policy(self):

@@ -1,14 +1,77 @@
-"""Neox rotary embedding, alone or fused with the KV-cache store.
+"""Rotary embedding, alone or fused with the KV-cache store.
 
 ``rotary_embedding`` keeps the signature of vLLM's
 ``_custom_ops.rotary_embedding(positions, query, key, head_size, cos_sin_cache,
 is_neox)`` as the reference calls it (litemoe/model.py:58,63-64): in place on
 strided ``[T, heads, D]`` views. Arithmetic matches the torch path
 ``q * cos + rotate_half(q) * sin`` in bf16 (model.py:66-67) bit for bit.
+
+The reference turns whole heads in halves by a bf16 table. :func:`rotary_embedding`
+and :func:`rotate_kv_write` also turn interleaved pairs, the first channels of a head
+alone, and by an fp32 table (:func:`rotary_table`), whose products and sums stay fp32
+and are rounded once: a bf16 cosine is off by 2^-9, whatever the position.
 """
+import math
+
 import torch
 
-from . import _lib
+from . import _lib, kv_paged
+from .cache import PagedKVCache
+from .kv_quant import per_row
+
+
+def rotary_table(length, rotary, theta, scaling=None, device="cpu", dtype=torch.float32):
+    """cos | sin ``[length, rotary]`` of positions ``0 .. length-1``, angles formed in
+    64 bits. ``scaling``, for contexts ``factor`` times longer than the ``original``
+    positions that the frequencies were made for:
+
+    * ``dict(type="linear", factor=)``: every frequency divided by it;
+    * ``dict(type="ntk", factor=)``: ``theta`` times ``factor ** (rotary / (rotary - 2))``,
+      which divides the lowest frequency by it and leaves the highest;
+    * ``dict(type="yarn", factor=, original=)`` (Peng et al., 2023): pairs that turn more
+      than ``beta_fast`` (32) times within ``original`` positions keep their frequency,
+      those that turn less than ``beta_slow`` (1) times have it divided, with a ramp
+      between, and the values are times ``attention_factor`` (``0.1 ln(factor) + 1``)."""
+    if length < 1 or rotary < 2 or rotary % 2 or theta <= 0:
+        raise ValueError("A rotary table needs positions and an even number of channels")
+    scaling = dict(scaling or {})
+    kind, factor = scaling.pop("type", None), float(scaling.pop("factor", 1.0))
+    allowed = {None: set(), "linear": set(), "ntk": set(),
+               "yarn": {"original", "beta_fast", "beta_slow", "attention_factor"}}
+    if kind not in allowed or factor < 1 or set(scaling) - allowed[kind] or (kind is None and factor != 1):
+        raise ValueError("Rotary scaling is linear, ntk or yarn, with a factor of at least 1")
+    if kind == "ntk":
+        if rotary < 4:
+            raise ValueError("Rotary scaling by the base needs two pairs")
+        theta = theta * factor ** (rotary / (rotary - 2))
+    i = torch.arange(rotary // 2, dtype=torch.float64, device=device)
+    frequency, size = theta ** (-2 * i / rotary), 1.0
+    if kind == "linear":
+        frequency = frequency / factor
+    elif kind == "yarn":
+        if "original" not in scaling:
+            raise ValueError("YaRN scaling needs the original positions")
+
+        def pair(turns):  # the index of the pair that turns so often within the original positions
+            return rotary * math.log(scaling["original"] / (turns * 2 * math.pi)) / (2 * math.log(theta))
+        low = max(math.floor(pair(scaling.get("beta_fast", 32.0))), 0)
+        high = min(math.ceil(pair(scaling.get("beta_slow", 1.0))), rotary - 1)
+        ramp = ((i - low) / max(high - low, 0.001)).clamp(0, 1)
+        frequency = frequency * (1 - ramp) + frequency / factor * ramp
+        size = scaling.get("attention_factor")
+        size = 0.1 * math.log(factor) + 1 if size is None else size
+    angle = torch.arange(length, dtype=torch.float64, device=device)[:, None] * frequency
+    return (torch.cat((angle.cos(), angle.sin()), -1) * size).to(dtype)
+
+
+def check_table(cos_sin, index, dim):
+    """``cos_sin [table_len, rotary]`` as the kernels with any rotation take it."""
+    if (cos_sin.dtype not in (torch.float32, torch.bfloat16) or cos_sin.dim() != 2 or not cos_sin.is_contiguous()
+            or cos_sin.get_device() != index or not cos_sin.shape[0] or cos_sin.data_ptr() % 16):
+        raise ValueError("Rotation needs a contiguous FP32 or BF16 [table_len, rotary] cos/sin table on one device "
+                         "with its tensors")
+    if cos_sin.shape[1] % 16 or not 16 <= cos_sin.shape[1] <= dim:
+        raise ValueError("Rotated channels are a multiple of 16, at most the head's")
 
 
 def _check(q, k, cos_sin, positions):
@@ -25,18 +88,83 @@ def _check(q, k, cos_sin, positions):
 
 
 def rotary_embedding(positions, query, key, head_size, cos_sin_cache, is_neox=True):
-    """In-place neox rotation of ``query [T, Hq, D]`` and ``key [T, Hkv, D]``."""
-    if not is_neox:
-        raise ValueError('Only neox-style rotation is implemented (Granite)')
+    """In-place rotation of ``query [T, Hq, D]`` and ``key [T, Hkv, D]`` by the table
+    ``cos_sin_cache [table_len, R]``: its width says how many of a head's channels
+    turn, and its type the arithmetic (see :func:`rotate_kv_write`). ``is_neox``: pairs
+    in halves, else interleaved."""
     if head_size != query.shape[-1]:
         raise ValueError('head_size must equal the last query dimension')
-    _check(query, key, cos_sin_cache, positions)
-    positions = positions.to(torch.int64).contiguous()
-    rows = query.shape[0]
-    _lib.call("lm_rope_kv_write", query.data_ptr(), query.stride(0), query.stride(1),
-              key.data_ptr(), key.stride(0), key.stride(1), None, 0, 0,
-              cos_sin_cache.data_ptr(), cos_sin_cache.shape[0], positions.data_ptr(), None, None,
-              None, None, rows, query.shape[1], key.shape[1], 64, 1, 1, 1, _lib.stream(query.device))
+    if is_neox and head_size == 64 and cos_sin_cache.shape[-1] == 64 and cos_sin_cache.dtype == torch.bfloat16:
+        _check(query, key, cos_sin_cache, positions)
+        positions = positions.to(torch.int64).contiguous()
+        rows = query.shape[0]
+        _lib.call("lm_rope_kv_write", query.data_ptr(), query.stride(0), query.stride(1),
+                  key.data_ptr(), key.stride(0), key.stride(1), None, 0, 0,
+                  cos_sin_cache.data_ptr(), cos_sin_cache.shape[0], positions.data_ptr(), None, None,
+                  None, None, rows, query.shape[1], key.shape[1], 64, 1, 1, 1, _lib.stream(query.device))
+        return
+    for t in (query, key):
+        if t.dim() != 3 or t.dtype != torch.bfloat16 or kv_paged.aligned(t) is not t:
+            raise ValueError('Rotation in place needs BF16 [T, heads, D] of contiguous channels, 16-byte aligned rows '
+                             'and heads (strides multiple of 8)')
+    _rotate(query, key, positions, cos_sin_cache, is_neox, query, key)
+
+
+def _rotate(q, k, positions, cos_sin, is_neox, q_out, k_out, v=None, cache=None, layer=0, at=None, active=None,
+            slots=None):
+    """The call of ``lm_paged_rotate_write``; its tensors but per-row ones are checked."""
+    rows, dim = q.shape[0], q.shape[2]
+    index = q.get_device()
+    if index < 0:
+        _lib.require_cuda(q, k, cos_sin, what="RoPE tensors")
+    if k.shape[0] != rows or k.shape[2] != dim or k.get_device() != index:
+        raise ValueError("Queries and keys need the same rows and channels, on one device")
+    if dim % 16 or dim > 256:
+        raise ValueError("Rotation takes heads of a multiple of 16 channels, at most 256")
+    check_table(cos_sin, index, dim)
+    positions = per_row(positions, rows, torch.int64, index, "positions")
+    where = [None, None, None, 0, 0, 0, 0]
+    if cache is not None:
+        kc, vc, table = cache.layer(layer)
+        if kv_paged.check_layer(kc, vc, table) != index:
+            raise ValueError("The cache must be on its tensors' device")
+        pages, heads, page, channels = kc.shape
+        if heads != k.shape[1] or channels != dim or v.shape != k.shape or v.get_device() != index:
+            raise ValueError("Keys and values do not match the cache's heads")
+        at = None if at is None else per_row(at, rows, torch.int64, index, "at")
+        slots = None if slots is None else per_row(slots, rows, torch.int64, index, "slots")
+        active = None if active is None else per_row(active, rows, torch.bool, index, "active")
+        where = [kc.data_ptr(), vc.data_ptr(), table.data_ptr(), table.shape[0], table.shape[1], pages, page]
+    none = (None, 0, 0)
+
+    def view(x):
+        return none if x is None else (x.data_ptr(), *kv_paged.strides(x))
+    _lib.call_on(index, "lm_paged_rotate_write", *view(q), *view(k), *view(v), cos_sin.data_ptr(), *cos_sin.shape,
+                 int(cos_sin.dtype == torch.float32), int(bool(is_neox)), positions.data_ptr(), _lib.ptr(at),
+                 _lib.ptr(active), _lib.ptr(slots), *view(q_out), *view(k_out), *where, rows, q.shape[1], k.shape[1], dim)
+
+
+def rotate_kv_write(q, k, v, positions, active, cos_sin, cache, layer, slots=None, at=None, is_neox=True, keep_k=False):
+    """Rotate ``q [T, Hq, D]`` and ``k [T, Hkv, D]`` by ``positions``, and store rotated k
+    and ``v`` into a :class:`~litemoe_amd.cache.PagedKVCache` at ``(slots[t], h, at[t])``
+    for active rows (``slots`` None: row t; ``at`` None: ``positions``, which a row that
+    was evicted from has moved past; ``active`` None: all). Rows out of range or without
+    a page there are not stored. Returns the rotated ``q``, and with ``keep_k`` the
+    rotated ``k`` (else None), as new tensors.
+
+    The first ``R`` channels turn, for a table ``cos_sin [table_len, R]``, in halves
+    (``is_neox``) or interleaved pairs; positions past the table are not turned. An
+    fp32 table: fp32 arithmetic, rounded once. A bf16 table: each product and each sum
+    is rounded, as :func:`rope_kv_write` and litemoe/model.py:66-67 have it."""
+    if not isinstance(cache, PagedKVCache):
+        raise ValueError("rotate_kv_write stores into a paged KV cache")
+    if any(t.dim() != 3 or t.dtype != torch.bfloat16 for t in (q, k, v)):
+        raise ValueError("RoPE supports BF16 [T, heads, D] queries, keys and values")
+    q, k, v = (kv_paged.aligned(t) for t in (q, k, v))
+    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device) if keep_k else None
+    _rotate(q, k, positions, cos_sin, is_neox, q_out, k_out, v, cache, layer, at, active, slots)
+    return q_out, k_out
 
 
 def rope_kv_write(q, k, v, positions, active, cos_sin, cache, layer, slots=None, write_k=False):

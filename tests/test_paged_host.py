@@ -1,0 +1,339 @@
+"""The paged KV cache without a GPU: pages handed out and given back, tables, rotary
+tables, and the calls that are refused before anything is launched."""
+import copy
+import ctypes as C
+import math
+import pickle
+
+import pytest
+import torch
+
+from litemoe_amd import _lib, kv_paged, rope
+from litemoe_amd.cache import KVCache, PagedKVCache
+from litemoe_amd.config import preset
+from litemoe_amd.engine import Engine
+from litemoe_amd.flash_decode import PagedFlashDecode, paged_splits
+from oracle import paged
+
+_P = 1 << 20
+
+
+def cache_of(rows=3, capacity=64, page=16, pages=None):
+    return PagedKVCache.empty(2, rows, 4, 64, capacity, "cpu", page=page, pages=pages)
+
+
+def lines(cache):
+    return [[p for p in line if p >= 0] for line in cache.table.tolist()]
+
+
+def test_sizes():
+    cfg = preset("granite-3b", num_hidden_layers=2)
+    cache = PagedKVCache(cfg, 3, 100, "cpu", torch.bfloat16, page=32, pages=7)
+    assert cache.k.shape == cache.v.shape == (2, 7, 8, 32, 64)
+    assert cache.table.shape == (3, 4) and cache.capacity == 128 and cache.page == 32
+    assert cache.slots.tolist() == [0, 1, 2] and cache.keys.numel() == 128
+    assert bool((cache.table == -1).all()) and cache.free_pages == 7
+    layer = cache.layer(1)
+    assert layer.k.data_ptr() == cache.k[1].data_ptr() and layer.table is cache.table
+    assert PagedKVCache(cfg, 3, 100, "cpu", torch.bfloat16).k.shape[1] == 6
+
+
+def test_pages_are_handed_out_and_given_back():
+    cache = cache_of(pages=8)
+    cache.reserve([0, 1], [17, 16])
+    assert [len(x) for x in lines(cache)] == [2, 1, 0] and cache.free_pages == 5
+    assert cache.held(0) == 32 and cache.held(2) == 0
+    first = lines(cache)
+    cache.reserve([0, 1], [17, 20])  # what a row has stays in its place
+    assert lines(cache)[0] == first[0] and lines(cache)[1][:1] == first[1] and len(lines(cache)[1]) == 2
+    used = [p for line in lines(cache) for p in line]
+    assert len(set(used)) == len(used)
+    before = cache.table.clone()
+    with pytest.raises(ValueError, match="4 free pages, 6 are wanted"):
+        cache.reserve([0, 2], [64, 64])
+    assert torch.equal(cache.table, before) and cache.free_pages == 4
+    cache.release(0)
+    assert lines(cache)[0] == [] and cache.free_pages == 6 and cache.held(0) == 0
+    cache.reserve(2, 64)
+    assert len(lines(cache)[2]) == 4
+    cache.release([1, 2])
+    assert cache.free_pages == 8 and bool((cache.table == -1).all())
+
+
+def test_shared_pages_go_back_when_the_last_row_gives_them_back():
+    cache = cache_of(pages=6)
+    cache.reserve(0, 40)
+    cache.share(1, 0, 32)
+    assert lines(cache)[1] == lines(cache)[0][:2] and cache.free_pages == 3
+    cache.reserve(1, 48)
+    assert len(set(lines(cache)[0] + lines(cache)[1])) == 4
+    cache.release(0)
+    assert cache.free_pages == 3
+    cache.release(1)
+    assert cache.free_pages == 6
+    for args, text in [((0, 0, 0), "without pages"), ((0, 1, 16), "whole pages"), ((0, 5, 0), "No such")]:
+        with pytest.raises(ValueError, match=text):
+            cache.share(*args)
+    cache.reserve([0, 1], 16)
+    with pytest.raises(ValueError, match="without pages"):
+        cache.share(0, 1, 16)
+    with pytest.raises(ValueError, match="whole pages"):
+        cache.share(2, 1, 8)
+
+
+@pytest.mark.parametrize("call,text", [
+    (lambda c: c.reserve(3, 16), "No such"), (lambda c: c.reserve(-1, 16), "No such"),
+    (lambda c: c.reserve(0, 65), "capacity"), (lambda c: c.reserve(0, -1), "capacity"),
+    (lambda c: c.reserve([0, 0], 16), "once"), (lambda c: c.reserve([0, 1], [16]), "capacity"),
+    (lambda c: c.release([1, 1]), "once"), (lambda c: c.release(9), "No such"),
+    (lambda c: c.evict(None, None, 60, room=10), "capacity"), (lambda c: c.evict(None, None, 4, room=-1), "capacity"),
+])
+def test_page_calls_refused(call, text):
+    cache = cache_of()
+    cache.reserve([0, 1], 20)
+    before = cache.table.clone()
+    with pytest.raises(ValueError, match=text):
+        call(cache)
+    assert torch.equal(cache.table, before) and cache.free_pages == 8
+
+
+def test_a_refused_eviction_gives_its_pages_back():
+    cache = cache_of()
+    cache.reserve([0, 1], 40)
+    before, free = cache.table.clone(), cache.free_pages
+    weights = torch.zeros(2, 3, 4, 64)
+    with pytest.raises(ValueError, match="ROCm device"):
+        cache.evict(weights, torch.tensor([40, 40, 0]), 16)
+    assert torch.equal(cache.table, before) and cache.free_pages == free
+    tight = cache_of(pages=6)
+    tight.reserve([0, 1], 40)
+    with pytest.raises(ValueError, match="0 free pages, 2 are wanted"):
+        tight.evict(weights, torch.tensor([40, 40, 0]), 16)
+
+
+def test_a_cache_over_buffers():
+    k = torch.zeros(2, 5, 4, 16, 64, dtype=torch.bfloat16)
+    table = torch.zeros(3, 2, dtype=torch.int32)
+    cache = PagedKVCache.over(k, k.clone(), table)
+    assert cache.k is k and cache.table is table and cache.capacity == 32
+    for call in (lambda: cache.reserve(0, 1), lambda: cache.release(0), lambda: cache.share(0, 1, 0),
+                 lambda: cache.free_pages, lambda: cache.held(0), lambda: cache.evict(None, None, 1)):
+        with pytest.raises(ValueError, match="caller's"):
+            call()
+    for args, text in [((k[0], k[0], table), "buffers are"), ((k, k[:, :, :2], table), "buffers are"),
+                       ((k[..., :32].contiguous(), k[..., :32].contiguous(), table), "buffers are"),
+                       ((k[:, :, :, :8].contiguous(), k[:, :, :, :8].contiguous(), table), "buffers are"),
+                       ((k.float(), k.float(), table), "BF16"), ((k[:, 1:], k[:, 1:], table), "contiguous"),
+                       ((k, k, table.long()), "int32"), ((k, k, table[:, :1]), "int32"), ((k, k, table[0]), "int32")]:
+        with pytest.raises(ValueError, match=text):
+            PagedKVCache.over(*args)
+
+
+@pytest.mark.parametrize("twin", [copy.deepcopy, lambda c: pickle.loads(pickle.dumps(c))])
+def test_a_copy_has_buffers_and_pages_of_its_own(twin):
+    cache = cache_of()
+    cache.reserve(0, 20)
+    other = twin(cache)
+    other.reserve(1, 16)
+    other.layer(1).k.fill_(3)
+    assert bool((other.k[1] == 3).all()) and not cache.k.any()
+    assert other.layer(0).table.data_ptr() == other.table.data_ptr() and lines(cache)[1] == []
+    assert cache.free_pages == other.free_pages + 1
+
+
+@pytest.mark.parametrize("kwargs,text", [
+    (dict(page=24), "power of two"), (dict(page=8), "power of two"), (dict(page=1 << 17), "power of two"),
+    (dict(pages=0), "needs"), (dict(dtype=torch.float32), "BF16"), (dict(batch=0), "needs"),
+])
+def test_caches_refused(kwargs, text):
+    cfg = preset("granite-1b", num_hidden_layers=1)
+    args = dict(cfg=cfg, batch=2, capacity=64, device="cpu", dtype=torch.bfloat16, **{})
+    with pytest.raises(ValueError, match=text):
+        PagedKVCache(**{**args, **kwargs})
+    if "page" in kwargs:
+        with pytest.raises(ValueError, match="power of two"):
+            Engine(None, [], kv_page=kwargs["page"])
+    with pytest.raises(ValueError, match="16 bits"):
+        Engine(None, [], kv_page=16, kv_bits=8)
+
+
+def test_host_tensors_are_refused():
+    cache = cache_of()
+    x, at = torch.zeros(3, 4, 1, 64, dtype=torch.bfloat16), torch.zeros(3, dtype=torch.int64)
+    flash = PagedFlashDecode(3, 4, 2, cache.capacity, "cpu")
+    cos_sin = rope.rotary_table(16, 64, 1e4)
+    q = torch.zeros(3, 8, 1, 64, dtype=torch.bfloat16)
+    for call in (lambda: cache.write(0, x, x, at, None), lambda: cache.read(0),
+                 lambda: flash(q, *cache.layer(0), None, None, 1.0, used=at),
+                 lambda: flash.fused_qkv(torch.zeros(1, 3, 16 * 64), cos_sin, at, None, *cache.layer(0), 1.0, at, 8),
+                 lambda: rope.rotate_kv_write(q[:, :, 0], x[:, :, 0], x[:, :, 0], at, None, cos_sin, cache, 0),
+                 lambda: rope.rotary_embedding(at, q[:, :, 0], x[:, :, 0], 64, cos_sin, is_neox=False),
+                 lambda: kv_paged.evict(cache, torch.zeros(2, 3, 4, 64), at, 2, 0, cache.table)):
+        with pytest.raises(ValueError, match="ROCm device"):
+            call()
+    plain = KVCache(preset("granite-1b", num_hidden_layers=1), 1, 16, "cpu", torch.bfloat16)
+    with pytest.raises(ValueError, match="paged KV cache"):
+        rope.rotate_kv_write(q[:, :, 0], x[:, :, 0], x[:, :, 0], at, None, cos_sin, plain, 0)
+
+
+@pytest.mark.parametrize("kwargs,text", [(dict(maximum=0), "length bound"), (dict(maximum=65), "length bound"),
+                                         (dict(head_dim=32), "head_dim"), (dict(groups=17), "16 query heads"),
+                                         (dict(groups=0), "16 query heads")])
+def test_plans_refused(kwargs, text):
+    with pytest.raises(ValueError, match=text):
+        PagedFlashDecode(**{**dict(batch=2, kv_heads=4, groups=2, capacity=64, device="cpu"), **kwargs})
+
+
+def test_splits_are_within_bounds():
+    for batch in (1, 2, 3, 8, 17, 32, 33, 64, 128, 1000):
+        for heads in (1, 2, 8, 32):
+            for maximum in (1, 16, 255, 767, 768, 1279, 4095, 32768, 1 << 20):
+                splits = paged_splits(batch, heads, maximum)
+                assert 1 <= splits <= 1024
+                assert splits == 1 or maximum >= 32 * splits
+
+
+# ------------------------------------------------------------ rotary tables --
+
+@pytest.mark.parametrize("rotary,theta", [(64, 10000.0), (128, 1e6), (2, 100.0)])
+def test_rotary_table_is_the_definition(rotary, theta):
+    """Angles in 64 bits: at position 10^6 an fp32 angle is off by up to 0.03."""
+    table = rope.rotary_table(1_000_001, rotary, theta)
+    at = torch.tensor([0, 1, 999, 1_000_000])
+    cos, sin = paged.angles(at, rotary, theta)
+    exp = torch.cat((cos, sin), -1)
+    # one rounding to fp32, and an angle in 64 bits: 10^6 2^-53 and theta's power's few of its own
+    assert bool(((table[at].double() - exp).abs() <= 2.0 ** -24 + 1e-8).all())
+    assert table.dtype == torch.float32 and table.shape == (1_000_001, rotary)
+
+
+def test_rotary_scaling():
+    linear = rope.rotary_table(64, 32, 1e4, dict(type="linear", factor=4.0), dtype=torch.float64)
+    plain = rope.rotary_table(16, 32, 1e4, dtype=torch.float64)
+    assert torch.allclose(linear[::4], plain, atol=1e-13)
+    ntk = rope.rotary_table(2, 32, 1e4, dict(type="ntk", factor=8.0), dtype=torch.float64)
+    angle = torch.atan2(ntk[1, 16:], ntk[1, :16])
+    base = 1e4 ** (-torch.arange(16).double() / 16)
+    assert math.isclose(float(angle[0]), 1.0, rel_tol=1e-12)
+    assert math.isclose(float(angle[-1]), float(base[-1]) / 8, rel_tol=1e-9)
+    # YaRN: the fastest pairs as they were, the slowest divided, monotone between; the size of the values
+    yarn = rope.rotary_table(2, 64, 1e4, dict(type="yarn", factor=8.0, original=4096), dtype=torch.float64)
+    angle = torch.atan2(yarn[1, 32:], yarn[1, :32])
+    base = 1e4 ** (-torch.arange(32).double() / 32)
+    share = base / angle
+    turns = 4096 * base / (2 * math.pi)
+    assert torch.allclose(share[turns > 64], torch.ones((), dtype=torch.float64), atol=1e-9)
+    assert torch.allclose(share[turns < 0.5], torch.full((), 8.0, dtype=torch.float64), atol=1e-9)
+    assert bool((share[1:] >= share[:-1] - 1e-9).all())
+    assert math.isclose(float(yarn[0, 0]), 0.1 * math.log(8.0) + 1, rel_tol=1e-12)
+    own = dict(type="yarn", factor=8.0, original=4096, beta_fast=16, beta_slow=2, attention_factor=1.0)
+    assert float(rope.rotary_table(2, 64, 1e4, own)[0, 0]) == 1.0
+
+
+@pytest.mark.parametrize("args,scaling", [
+    ((0, 64, 1e4), None), ((4, 63, 1e4), None), ((4, 64, 0.0), None), ((4, 64, 1e4), dict(type="other", factor=2.0)),
+    ((4, 64, 1e4), dict(type="linear", factor=0.5)), ((4, 64, 1e4), dict(type="yarn", factor=2.0)),
+    ((4, 64, 1e4), dict(type="linear", factor=2.0, original=4)), ((4, 64, 1e4), dict(factor=2.0)),
+    ((4, 2, 1e4), dict(type="ntk", factor=2.0))])
+def test_rotary_tables_refused(args, scaling):
+    with pytest.raises(ValueError):
+        rope.rotary_table(*args, scaling)
+
+
+# ------------------------------------------------------------------- C ABI --
+
+def rotate(h, q=_P, v=_P, cos=_P, table_len=16, rotary=64, pos=_P, k_pages=_P, v_pages=_P, table=_P, batch=2, width=4,
+           pages=8, page=16, rows=3, hq=4, hkv=2, dim=64, qs=64, q_out=_P, k_out=None):
+    return h.lm_paged_rotate_write(q, qs, 64, _P, 64, 64, v, 64, 64, cos, table_len, rotary, 1, 1, pos, None, None, None,
+                                   q_out, 64, 64, k_out, 64, 64, k_pages, v_pages, table, batch, width, pages, page, rows,
+                                   hq, hkv, dim, None)
+
+
+def read(h, k=_P, page=16, dim=64, rows=3, table=_P, out=_P):
+    return h.lm_paged_read(k, _P, table, 2, 4, 8, page, _P, None, rows, 2, dim, out, _P, None)
+
+
+def decode(h, q=_P, page=16, width=4, pages=8, batch=2, hq=4, hkv=2, dim=64, max_len=64, splits=1, w=None, w_out=None,
+           ws=_P, size=1 << 30, table=_P, qs=64):
+    return h.lm_flash_decode_paged(q, qs, 64, _P, _P, table, width, pages, page, _P, batch, hq, hkv, dim, C.c_float(1.0),
+                                   max_len, splits, w, w_out, _P, ws, size, None)
+
+
+def fused(h, part=_P, slices=3, cos=_P, rotary=64, page=16, batch=2, frag=0, pos=_P, ws=_P, size=1 << 30, splits=1):
+    return h.lm_flash_decode_paged_qkv(part, slices, cos, 16, rotary, 1, 1, pos, None, _P, _P, _P, 4, 8, page, _P, None,
+                                       batch, 4, 2, 64, C.c_float(1.0), 64, splits, None, None, frag, _P, ws, size, None)
+
+
+def evict(h, page=16, keep=5, recent=2, layers=2, batch=2, width=4, w=_P, dim=64, target=_P):
+    return h.lm_kv_evict(_P, _P, _P, target, width, 2, 8, page, _P, w, layers, batch, 2, dim, keep, recent, _P, _P, _P,
+                         None)
+
+
+@pytest.mark.parametrize("call,expected", [
+    (lambda h: rotate(h, rows=0), 0), (lambda h: rotate(h, rows=-1), 1), (lambda h: rotate(h, page=24), 2),
+    (lambda h: rotate(h, page=8), 2), (lambda h: rotate(h, dim=96), 2), (lambda h: rotate(h, dim=72), 2),
+    (lambda h: rotate(h, v_pages=None), 1), (lambda h: rotate(h, table=None), 1), (lambda h: rotate(h, v=None), 1),
+    (lambda h: rotate(h, rotary=24), 1), (lambda h: rotate(h, rotary=80), 1), (lambda h: rotate(h, rotary=0), 1),
+    (lambda h: rotate(h, cos=None), 1), (lambda h: rotate(h, pos=None), 1), (lambda h: rotate(h, q=_P + 2), 1),
+    (lambda h: rotate(h, qs=60), 1), (lambda h: rotate(h, q_out=None), 1), (lambda h: rotate(h, table_len=0), 1),
+    (lambda h: rotate(h, width=0), 1), (lambda h: rotate(h, pages=0), 1), (lambda h: rotate(h, pages=1 << 31), 1),
+    (lambda h: rotate(h, width=1 << 27), 1), (lambda h: rotate(h, batch=0), 1), (lambda h: rotate(h, rows=1 << 40), 1),
+    (lambda h: rotate(h, k_pages=None, v_pages=None), 1),  # neither k_out nor a cache
+    (lambda h: read(h, rows=0), 0), (lambda h: read(h, page=48), 2), (lambda h: read(h, dim=32), 2),
+    (lambda h: read(h, table=None), 1), (lambda h: read(h, out=_P + 8), 1), (lambda h: read(h, rows=1 << 40), 1),
+    (lambda h: decode(h, batch=0), 0), (lambda h: decode(h, hq=5), 1), (lambda h: decode(h, hq=34), 2),
+    (lambda h: decode(h, dim=96), 2), (lambda h: decode(h, page=17), 2), (lambda h: decode(h, q=None), 1),
+    (lambda h: decode(h, q=_P + 4), 1), (lambda h: decode(h, qs=65), 1), (lambda h: decode(h, table=None), 1),
+    (lambda h: decode(h, max_len=0), 1), (lambda h: decode(h, splits=0), 1), (lambda h: decode(h, splits=1025), 1),
+    (lambda h: decode(h, w=_P), 1), (lambda h: decode(h, w_out=_P), 1), (lambda h: decode(h, w=_P + 4, w_out=_P), 1),
+    (lambda h: decode(h, splits=2, size=100), 4), (lambda h: decode(h, w=_P, w_out=_P, ws=None), 4),
+    (lambda h: decode(h, splits=2, ws=_P + 4), 1), (lambda h: decode(h, batch=65536), 1),
+    (lambda h: fused(h, batch=0), 0), (lambda h: fused(h, slices=9), 2), (lambda h: fused(h, slices=0), 1),
+    (lambda h: fused(h, rotary=72), 1), (lambda h: fused(h, cos=None), 1), (lambda h: fused(h, part=_P + 4), 1),
+    (lambda h: fused(h, batch=129, frag=1), 2), (lambda h: fused(h, pos=None), 1), (lambda h: fused(h, page=20), 2),
+    (lambda h: fused(h, splits=2, size=8), 4),
+    (lambda h: evict(h, batch=0), 0), (lambda h: evict(h, keep=0), 1), (lambda h: evict(h, recent=6), 1),
+    (lambda h: evict(h, recent=-1), 1), (lambda h: evict(h, keep=65), 1), (lambda h: evict(h, page=15), 2),
+    (lambda h: evict(h, w=None), 1), (lambda h: evict(h, layers=0), 1), (lambda h: evict(h, layers=300, batch=300), 1),
+    (lambda h: evict(h, dim=80), 2), (lambda h: evict(h, target=None), 1),
+])
+def test_invalid_arguments_rejected_on_host(call, expected):
+    assert call(_lib.load()) == expected
+
+
+def test_workspace_sizes():
+    def size(splits, weighed, max_len=100):
+        return _lib.size_query("lm_flash_decode_paged_workspace_size", 3, 8, 128, max_len, splits, weighed)
+    assert size(1, 0) == 0
+    assert size(4, 0) == 3 * 8 * 4 * 128 * 4 + 2 * 512
+    assert size(1, 1) == 3 * 256 + 3 * 8 * 128 * 4
+    assert size(4, 1) == 3 * 8 * 4 * 128 * 4 + 3 * 512 + 3 * 8 * 128 * 4
+
+
+# ------------------------------------------------------------------ oracle --
+
+def test_oracle_against_dense_torch():
+    """The oracle's rows, attention, rotation and choice against torch on a dense cache."""
+    g = torch.Generator().manual_seed(1)
+    k, v = (torch.randn(6, 2, 16, 64, generator=g).to(torch.bfloat16) for _ in range(2))
+    table = torch.tensor([[3, 0, 5], [1, -1, 2]], dtype=torch.int32)
+    q = torch.randn(2, 4, 64, generator=g).to(torch.bfloat16)
+    out, p = paged.attention(q, k, v, table, [40, 48], 0.125)
+    dense_k, dense_v = (torch.cat([x[i] for i in (3, 0, 5)], 1)[:, :40].double() for x in (k, v))
+    s = q[0].double().view(2, 2, 64) @ dense_k.transpose(1, 2) * 0.125
+    assert torch.allclose(out[0].view(2, 2, 64), torch.softmax(s, -1) @ dense_v, atol=1e-12)
+    assert p[1].shape == (2, 2, 48) and bool((p[1][:, :, 16:32] == 0).all())
+    assert torch.allclose(p[1].sum(-1), torch.ones(2, 2, dtype=torch.float64))
+    pos = torch.tensor([0, 5, 77])
+    cos, sin = paged.angles(pos, 64, 1e4)
+    x = torch.randn(3, 2, 64, generator=g).double()
+    half = torch.cat((-x[..., 32:], x[..., :32]), -1)
+    c2, s2 = (torch.cat((a, a), -1)[:, None] for a in (cos, sin))
+    assert torch.allclose(paged.rotate(x, cos, sin, True), x * c2 + half * s2, atol=1e-12)
+    inter = paged.rotate(x, cos, sin, False)
+    z = torch.view_as_complex(x.view(3, 2, 32, 2).contiguous()) * torch.polar(torch.ones_like(cos), torch.atan2(
+        sin, cos))[:, None]
+    assert torch.allclose(inter, torch.view_as_real(z).flatten(-2), atol=1e-12)
+    w = torch.tensor([1.0, 3.0, 2.0, 3.0, 0.5, 9.0])
+    assert paged.keep(w, 6, 3, 1) == [1, 3, 5] and paged.keep(w, 6, 2, 2) == [4, 5] and paged.keep(w, 2, 3, 0) == [0, 1]
+    assert paged.keep(torch.tensor([1.0, math.nan, 1.0]), 3, 2, 0) == [0, 1]
