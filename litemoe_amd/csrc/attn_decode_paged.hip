@@ -40,6 +40,8 @@ namespace lm {
 namespace {
 
 constexpr int kTile = 32;
+constexpr int kWaves = 4;
+constexpr int kThreads = kWaves * kWave;
 constexpr int kMaxQkvSplits = 8;
 constexpr int kMaxGroups = 16;
 
@@ -69,19 +71,19 @@ struct QkvIn {
 };
 
 struct Shape {
-  int q_heads, G, max_len, splits, least;  // least: the fewest tiles of a split
+  int q_heads, G, max_len, splits;
   float scale;
   int64_t batch;
 };
 
 // Positions of row b that are looked at.
-__device__ __forceinline__ int row_length(const int32_t *used, int64_t b, const Shape &sh, const PagedKV &kv) {
-  return max(0, min(min(used[b], sh.max_len), kv.width << kv.shift));
+__device__ __forceinline__ int row_length(int used, const Shape &sh, const PagedKV &kv) {
+  return max(0, min(min(used, sh.max_len), kv.width << kv.shift));
 }
-// Tiles per split of a row of n positions: its own length cut evenly.
-__device__ __forceinline__ int row_chunk(int n, const Shape &sh) {
-  const uint32_t tiles = (uint32_t)(n + kTile - 1) / kTile;
-  return max((int)((tiles + sh.splits - 1) / (uint32_t)sh.splits), sh.least);
+// Splits that hold a tile of a row of n positions: tiles go to the waves of all
+// splits in turn, kWaves a split.
+__device__ __forceinline__ int row_splits(int n, const Shape &sh) {
+  return min(sh.splits, (n + kTile * kWaves - 1) / (kTile * kWaves));
 }
 
 template <int D>
@@ -101,12 +103,11 @@ __device__ __forceinline__ T constant(const T *p) {
   return *(const __attribute__((address_space(4))) T *)p;
 }
 
-template <int D, bool kFused, bool kWeigh, int kWaves>
+template <int D, bool kFused, bool kWeigh>
 __global__ void __launch_bounds__(kWaves *kWave, D == 64 ? 4 : 2)
 decode_paged_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, PagedKV kv,
                     const int32_t *__restrict__ table, const int32_t *__restrict__ used, Shape sh, Partial part,
                     QkvIn in, bf16 *__restrict__ out, int out_mb) {
-  constexpr int kThreads = kWaves * kWave;
   constexpr int kSteps = D / 32, kCh = D / 16;  // k steps of a score; channels a lane takes of a V row
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int h = blockIdx.x, split = blockIdx.y;
@@ -156,11 +157,24 @@ decode_paged_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, PagedK
                     : u32x4{0, 0, 0, 0};
   }
 
-  const int n = scalar(row_length(used, b, sh, kv));
+  const int first = split * kWaves + wave, stride = sh.splits * kWaves;  // this wave's tiles
+  const int32_t *row_table = table + b * kv.width;
+  const uint32_t k_off = (uint32_t)(r * D + g * 8) * 2, v_off = (uint32_t)(4 * g * D + r * kCh) * 2;
+  const int page_mask = (1 << kv.shift) - 1;
+  struct Ids {
+    int id[2];
+  };
+  auto ids_of = [&](int tile) {
+    Ids x;
+    const int j = tile * kTile;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) x.id[t] = constant(row_table + min((j + 16 * t) >> kv.shift, kv.width - 1));
+    return x;
+  };
+  const Ids ia = ids_of(first), ib = ids_of(first + stride);
+  const int held = constant(used + b), n = row_length(held, sh, kv);
   const int tiles = (n + kTile - 1) / kTile;
-  const int chunk = scalar(row_chunk(n, sh));
-  const int t0 = split * chunk, t1 = min(tiles, t0 + chunk);
-  if (t0 >= t1) {
+  if (split * kWaves >= tiles) {
     // nothing of this row here: with one split its zeros are written
     if (sh.splits == 1) {
       for (int t = threadIdx.x; t < G * D; t += kThreads) {
@@ -170,34 +184,18 @@ decode_paged_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, PagedK
     }
     return;
   }
-  const int niter = (t1 - t0 - wave + kWaves - 1) / kWaves;
 
-  const int32_t *row_table = table + b * kv.width;
-  const uint32_t k_off = (uint32_t)(r * D + g * 8) * 2, v_off = (uint32_t)(4 * g * D + r * kCh) * 2;
-  const int page_mask = (1 << kv.shift) - 1;
-  struct Ids {
-    int id[2];
-  };
-  auto tile_of = [&](int it) { return min(t0 + wave + it * kWaves, t1 - 1); };
-  auto ids_of = [&](int it) {
-    Ids x;
-    const int j = tile_of(it) * kTile;
-#pragma unroll
-    for (int t = 0; t < 2; ++t) x.id[t] = constant(row_table + min((j + 16 * t) >> kv.shift, kv.width - 1));
-    return x;
-  };
-  // Every load is unconditional and in bounds (a tile past the end is the last one
-  // again, a page that does not exist is page 0): a load under a branch would make
-  // the wait counts fall back to waiting for all of them.
-  auto load = [&](Kv<D> &x, const Ids &ids, int it) {
-    const int j = tile_of(it) * kTile;
+  // In bounds whatever the table holds: a page that does not exist, and a tile past the
+  // row's end, are read from page 0. So the table's words need not wait for the length.
+  auto load = [&](Kv<D> &x, const Ids &ids, int tile) {
+    const int j = tile * kTile;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const int id = scalar(ids.id[t]);
+      const int id = ids.id[t];
       x.ok[t] = (uint32_t)id < (uint32_t)kv.pages;
-      const int64_t first =
-          ((((int64_t)(x.ok[t] ? id : 0) * kv.heads + h) << kv.shift) + ((j + 16 * t) & page_mask)) * D;
-      const char *kb = reinterpret_cast<const char *>(kv.k + first), *vb = reinterpret_cast<const char *>(kv.v + first);
+      const int64_t from =
+          ((((int64_t)(x.ok[t] && tile < tiles ? id : 0) * kv.heads + h) << kv.shift) + ((j + 16 * t) & page_mask)) * D;
+      const char *kb = reinterpret_cast<const char *>(kv.k + from), *vb = reinterpret_cast<const char *>(kv.v + from);
 #pragma unroll
       for (int s = 0; s < kSteps; ++s)
         x.k[t][s] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(kb + k_off + 64 * s));
@@ -206,13 +204,12 @@ decode_paged_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, PagedK
         x.v[t][i] = __builtin_nontemporal_load(reinterpret_cast<const typename Kv<D>::V *>(vb + v_off + 2 * D * i));
     }
   };
+  // The first two tiles are on their way before anything else is waited for, without a
+  // branch: loads under one would make the wait counts fall back to waiting for all.
   Kv<D> xa, xb;
-  {
-    const Ids ia = ids_of(0), ib = ids_of(1);
-    load(xa, ia, 0);
-    load(xb, ib, 1);
-  }
-  Ids na = ids_of(2), nb = ids_of(3);
+  load(xa, ia, first);
+  load(xb, ib, first + stride);
+  Ids na = ids_of(first + 2 * stride), nb = ids_of(first + 3 * stride);
 
   // The query heads as B operands; fused, also the new key and value (rows G and
   // G + 1 of sm_rot), rotated and rounded.
@@ -257,7 +254,7 @@ decode_paged_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, PagedK
       qw[s] = r < G ? *reinterpret_cast<const u32x4 *>(&sm_rot[r][32 * s + 8 * g]) : u32x4{0, 0, 0, 0};
     // The new token's place is the row's last, if the row was not cut short.
     const int last = n - 1;
-    if (writes && used[b] == n && t1 == tiles) {
+    if (writes && held == n && (tiles - 1) / kWaves % sh.splits == split) {
       const int id = constant(row_table + (last >> kv.shift));
       own = (uint32_t)id < (uint32_t)kv.pages;
       new_cell = ((((int64_t)(own ? id : 0) * kv.heads + h) << kv.shift) + (last & page_mask)) * D;
@@ -271,8 +268,7 @@ decode_paged_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, PagedK
   for (int c = 0; c < kCh; ++c) acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
   const u32x4 ones{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
 
-  auto compute = [&](Kv<D> &x, int it) {
-    const int tile = t0 + wave + it * kWaves;
+  auto compute = [&](Kv<D> &x, int tile) {
     const int left = n - tile * kTile;  // positions of the row from this tile on
     const bool edge = left < kTile || (kFused && own && tile == tiles - 1) || !x.ok[0] || !x.ok[1];
     if (kFused && own && tile == tiles - 1) {
@@ -364,14 +360,19 @@ decode_paged_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, PagedK
     }
   };
 
-  for (int it = 0; it < niter; it += 2) {
-    compute(xa, it);
-    load(xa, na, it + 2);
-    na = ids_of(it + 4);
-    if (it + 1 < niter) compute(xb, it + 1);
-    load(xb, nb, it + 3);
-    nb = ids_of(it + 5);
+  // Tiles in pairs while there is one to load for the first of the two; the second may
+  // be past the row's end, once.
+  int tile = first;
+  for (; tile + 2 * stride < tiles; tile += 2 * stride) {
+    compute(xa, tile);
+    load(xa, na, tile + 2 * stride);
+    compute(xb, tile + stride);
+    load(xb, nb, tile + 3 * stride);
+    na = ids_of(tile + 4 * stride);
+    nb = ids_of(tile + 5 * stride);
   }
+  if (tile < tiles) compute(xa, tile);
+  if (tile + stride < tiles) compute(xb, tile + stride);
 
   if constexpr (kFused) {
     // Stored behind the stream, which does not wait for it.
@@ -455,8 +456,7 @@ decode_paged_combine_kernel(const int32_t *__restrict__ used, Shape sh, PagedKV 
     }
   };
   load(0);
-  const int n = row_length(used, b, sh, kv), chunk = row_chunk(n, sh);
-  const int valid = ((n + kTile - 1) / kTile + chunk - 1) / chunk;
+  const int valid = row_splits(row_length(used[b], sh, kv), sh);
   float mx = kEmpty;
 #pragma unroll
   for (int i = 0; i < kBatch; ++i) mx = fmaxf(mx, i < valid ? ms[i] : kEmpty);
@@ -478,43 +478,82 @@ decode_paged_combine_kernel(const int32_t *__restrict__ used, Shape sh, PagedKV 
 }
 
 // after[b, h, j] = before[b, h, j] + sum over the KV head's query heads of their
-// probability of position j, j < the row's length. A thread four positions.
-constexpr int kWeighThreads = 256, kWeighSpan = 4 * kWeighThreads;
+// probability of position j, j < the row's length. A thread four positions. With
+// splits the first workgroup of a (row, KV head) also joins their results, in place of
+// the launch above.
+constexpr int kWeighThreads = 256, kWeighSpan = 4 * kWeighThreads, kAhead = 4;
+template <int D>
 __global__ void __launch_bounds__(kWeighThreads)
-weigh_kernel(const int32_t *__restrict__ used, Shape sh, PagedKV kv, Partial part, const float *before, float *after) {
+weigh_kernel(const int32_t *__restrict__ used, Shape sh, PagedKV kv, Partial part, const float *before, float *after,
+             bf16 *__restrict__ out, int out_mb) {
   __shared__ float sm_m[kMaxGroups], sm_f[kMaxGroups];
-  const int h = blockIdx.y;
+  const int h = blockIdx.y, G = sh.G;
   const int64_t b = blockIdx.z;
-  const int n = row_length(used, b, sh, kv), j = (blockIdx.x * kWeighThreads + threadIdx.x) * 4;
-  if ((int)blockIdx.x * kWeighSpan >= n) return;
-  if ((int)threadIdx.x < sh.G) {
-    const int64_t base = (b * sh.q_heads + h * sh.G + threadIdx.x) * sh.splits;
-    const int chunk = row_chunk(n, sh), valid = ((n + kTile - 1) / kTile + chunk - 1) / chunk;
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int n = row_length(used[b], sh, kv), valid = row_splits(n, sh);
+  const int j = (blockIdx.x * kWeighThreads + threadIdx.x) * 4;
+  const bool joins = blockIdx.x == 0 && sh.splits > 1;
+  if ((int)blockIdx.x * kWeighSpan >= n && !joins) return;
+  // The scores and weights of this thread's positions are on their way while the
+  // heads' sums are joined. The buffers hold a multiple of 16 positions a row.
+  const float *sc = part.s + (b * sh.q_heads + h * G) * part.padded + j;
+  const int64_t at = (b * kv.heads + h) * ((int64_t)kv.width << kv.shift) + j;
+  f32x4 s[kAhead], old{0.f, 0.f, 0.f, 0.f};
+  if (j < n) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) s[i] = *reinterpret_cast<const f32x4 *>(sc + min(i, G - 1) * part.padded);
+    old = *reinterpret_cast<const f32x4 *>(before + at);
+  }
+  for (int gh = wave; gh < G; gh += kWeighThreads / kWave) {
+    const int64_t base = (b * sh.q_heads + h * G + gh) * sh.splits;
     float mx = kEmpty, l = 0.f;
-    for (int s = 0; s < valid; ++s) mx = fmaxf(mx, part.m[base + s]);
-    for (int s = 0; s < valid; ++s) l += part.lw[base + s] * __builtin_amdgcn_exp2f(part.m[base + s] - mx);
-    sm_m[threadIdx.x] = mx;
-    sm_f[threadIdx.x] = l == 0.f ? 0.f : 1.f / l;
+    for (int s0 = lane; s0 < valid; s0 += kWave) mx = fmaxf(mx, part.m[base + s0]);
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) mx = fmaxf(mx, shfl_xor(mx, d));
+    for (int s0 = lane; s0 < valid; s0 += kWave) l += part.lw[base + s0] * __builtin_amdgcn_exp2f(part.m[base + s0] - mx);
+    l = wave_sum(l);
+    if (lane == 0) {
+      sm_m[gh] = mx;
+      sm_f[gh] = l == 0.f ? 0.f : 1.f / l;
+    }
   }
   __syncthreads();
-  if (j >= n) return;
-  const float *sc = part.s + (b * sh.q_heads + h * sh.G) * part.padded + j;
-  const int64_t at = (b * kv.heads + h) * ((int64_t)kv.width << kv.shift) + j;
-  float w[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int gh = 0; gh < sh.G; ++gh) {
-    const f32x4 s = *reinterpret_cast<const f32x4 *>(sc + gh * part.padded);
-    const float m = sm_m[gh], f = sm_f[gh];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] += __builtin_amdgcn_exp2f(s[i] - m) * f;
+  if (joins) {
+    for (int t = threadIdx.x; t < G * D; t += kWeighThreads) {
+      const int gh = t / D, c = t % D, hq = h * G + gh;
+      const int64_t base = (b * sh.q_heads + hq) * sh.splits;
+      float lsum = 0.f, o = 0.f;
+#pragma unroll 4
+      for (int i = 0; i < valid; ++i) {
+        const float f = __builtin_amdgcn_exp2f(part.m[base + i] - sm_m[gh]);
+        lsum += part.l[base + i] * f;
+        o += part.o[(base + i) * D + c] * f;
+      }
+      out[out_mb ? frag_offset_rows(b, (int64_t)hq * D + c, out_mb) : (b * sh.q_heads + hq) * D + c] =
+          (bf16)f32_to_bf16(lsum == 0.f ? 0.f : o / lsum);
+    }
   }
-  // a row's positions in the weights are a multiple of 16, so four of them lie in it
-  const f32x4 old = *reinterpret_cast<const f32x4 *>(before + at);
+  if (j >= n) return;
+  float w[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int g0 = 0; g0 < G; g0 += kAhead) {
+    if (g0) {
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) s[i] = *reinterpret_cast<const f32x4 *>(sc + min(g0 + i, G - 1) * part.padded);
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (g0 + i >= G) break;
+      const float m = sm_m[g0 + i], f = sm_f[g0 + i];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) w[x] += __builtin_amdgcn_exp2f(s[i][x] - m) * f;
+    }
+  }
   if (j + 4 <= n) {
     *reinterpret_cast<f32x4 *>(after + at) = f32x4{old[0] + w[0], old[1] + w[1], old[2] + w[2], old[3] + w[3]};
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (j + i < n) after[at + i] = old[i] + w[i];
+    for (int x = 0; x < 4; ++x)
+      if (j + x < n) after[at + x] = old[x] + w[x];
   }
 }
 
@@ -549,16 +588,15 @@ template <int D, bool kFused, bool kWeigh>
 int launch_sized(const Call &c, const bf16 *q, int64_t qs0, int64_t qs1, const PagedKV &kv, const int32_t *table,
                  const int32_t *used, const Shape &sh, const Partial &part, const QkvIn &in, bf16 *out, int out_mb,
                  const float *before, float *after, hipStream_t s) {
-  constexpr int kWaves = 4;
   // KV heads fastest: workgroups go to the XCDs in turn, so that each XCD has a share
   // of every split.
   const dim3 grid((unsigned)c.kv_heads, (unsigned)sh.splits, (unsigned)c.batch);
   const size_t merge = (size_t)kWaves * sh.G * (D + 3) * 4;
   const size_t rot = kFused ? (size_t)(sh.G + 2) * D * (2 + 4) : 0;
-  decode_paged_kernel<D, kFused, kWeigh, kWaves><<<grid, kWaves * kWave, merge > rot ? merge : rot, s>>>(
+  decode_paged_kernel<D, kFused, kWeigh><<<grid, kWaves * kWave, merge > rot ? merge : rot, s>>>(
       q, qs0, qs1, kv, table, used, sh, part, in, out, out_mb);
   LM_CHECK_LAUNCH();
-  if (sh.splits > 1) {
+  if (!kWeigh && sh.splits > 1) {
     auto combine = sh.splits <= 4   ? decode_paged_combine_kernel<D, 4>
                    : sh.splits <= 8 ? decode_paged_combine_kernel<D, 8>
                                     : decode_paged_combine_kernel<D, 16>;
@@ -567,8 +605,8 @@ int launch_sized(const Call &c, const bf16 *q, int64_t qs0, int64_t qs1, const P
     LM_CHECK_LAUNCH();
   }
   if (kWeigh) {
-    weigh_kernel<<<dim3((unsigned)cdiv(sh.max_len, kWeighSpan), (unsigned)c.kv_heads, (unsigned)c.batch),
-                   kWeighThreads, 0, s>>>(used, sh, kv, part, before, after);
+    weigh_kernel<D><<<dim3((unsigned)cdiv(sh.max_len, kWeighSpan), (unsigned)c.kv_heads, (unsigned)c.batch),
+                      kWeighThreads, 0, s>>>(used, sh, kv, part, before, after, out, out_mb);
     LM_CHECK_LAUNCH();
   }
   return LM_OK;
@@ -604,7 +642,7 @@ int launch_decode_paged(const Call &c, const void *q, int64_t qs0, int64_t qs1, 
   }
   const PagedKV kv{(bf16 *)k_pages, (bf16 *)v_pages, c.pages, (int)c.width, page_shift(c.page), (int)c.kv_heads};
   const int G = (int)(c.q_heads / c.kv_heads);
-  const Shape sh{(int)c.q_heads, G, (int)longest, (int)splits, 1, scale, c.batch};
+  const Shape sh{(int)c.q_heads, G, (int)longest, (int)splits, scale, c.batch};
   auto go = [&](auto dim, auto fused, auto weigh) {
     return launch_sized<decltype(dim)::value, decltype(fused)::value, decltype(weigh)::value>(
         c, (const bf16 *)q, qs0, qs1, kv, table, used, sh, part, in, (bf16 *)out, out_mb, before, after,

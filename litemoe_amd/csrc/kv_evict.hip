@@ -19,9 +19,7 @@
 namespace lm {
 namespace {
 
-constexpr int kThreads = 1024;
-constexpr int kWaves = kThreads / kWave;
-constexpr int kBins = 2048;
+constexpr int kBits = 11, kBins = 1 << kBits;
 
 // Larger floats, larger keys: -0 as 0, a NaN above every number.
 __device__ __forceinline__ uint32_t key_of(float w) {
@@ -30,93 +28,166 @@ __device__ __forceinline__ uint32_t key_of(float w) {
   return u ^ ((int32_t)u < 0 ? 0xffffffffu : 0x80000000u);
 }
 
-// Exclusive prefix over the workgroup of each thread's count, and the total.
-__device__ __forceinline__ int block_prefix(int v, int *sm, int &total) {
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+// Sum of the lanes below this one, by shuffles over the wave.
+__device__ __forceinline__ int wave_prefix(int v, int lane, int &total) {
   int x = v;
 #pragma unroll
   for (int d = 1; d < kWave; d *= 2) {
     const int y = __shfl_up(x, d, kWave);
     if (lane >= d) x += y;
   }
-  __syncthreads();
-  if (lane == kWave - 1) sm[wave] = x;
-  __syncthreads();
-  int before = 0;
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    const int c = sm[w];
-    before += w < wave ? c : 0;
-    total += c;
-  }
-  return before + x - v;
+  total = __shfl(x, kWave - 1, kWave);
+  return x - v;
 }
 
+// kThreads threads take kPer weights each at a time, thread t those at t, t + kThreads,
+// ... of the chunk. A row of one chunk is read once and stays in registers.
+template <int kThreads, int kPer>
 __global__ void __launch_bounds__(kThreads)
 evict_select_kernel(const int32_t *__restrict__ used, const float *weights, int64_t capacity, int keep, int recent,
                     float *weights_out, int32_t *__restrict__ kept, int32_t *__restrict__ used_out) {
-  __shared__ int bins[kBins];
-  __shared__ int sm[kWaves];
+  constexpr int kWaves = kThreads / kWave, kChunk = kThreads * kPer, kOwn = kBins / kThreads;
+  static_assert(kWaves * kPer <= 4 * kWave, "a wave scans the chunk's counts, four a lane");
+  __shared__ __attribute__((aligned(16))) int bins[kBins];
+  __shared__ int sm_wave[kWaves];
   __shared__ int sm_found[2];
+  __shared__ int sm_count[2][kPer * kWaves];  // by (round, wave): equal ones, then kept ones
+  __shared__ int sm_total[2];
   const int h = blockIdx.x, heads = gridDim.x;
   const int64_t b = blockIdx.y, batch = gridDim.y, layer = blockIdx.z;
   const int64_t row = (layer * batch + b) * heads + h;
   const float *w = weights + row * capacity;
   float *w_out = weights_out + row * capacity;
   int32_t *to = kept + row * keep;
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
   const int n = max(0, (int)min((int64_t)used[b], capacity));
   const int left = min(n, keep);
   if (h == 0 && layer == 0 && threadIdx.x == 0) used_out[b] = left;
   // The first `free` positions are chosen from, `want` of them.
   const int free = n > keep ? n - min(recent, keep) : 0, want = left - (n - free);
+  const bool choose = free > 0 && want > 0;
+  float x[kPer];
+  auto load = [&](int j0) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int j = j0 + i * kThreads + threadIdx.x;
+      x[i] = j < n ? w[j] : 0.f;
+    }
+  };
+  load(0);
+  // The threshold: bits of the want-th largest key from the top, and how many of
+  // its equals are wanted.
   uint32_t prefix = 0, mask = 0;
-  int need = want;  // of the keys that share the prefix found so far
-  if (free > 0 && want > 0) {
+  int need = want;
+  if (choose) {
     for (int pass = 0; pass < 3; ++pass) {
-      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, count = pass == 2 ? 1 << 10 : 1 << 11;
-      for (int i = threadIdx.x; i < count; i += kThreads) bins[i] = 0;
+      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+#pragma unroll
+      for (int i = 0; i < kBins; i += kThreads) bins[i + threadIdx.x] = 0;
       __syncthreads();
-      for (int j = threadIdx.x; j < free; j += kThreads) {
-        const uint32_t key = key_of(w[j]);
-        if ((key & mask) == prefix) atomicAdd(&bins[(key >> shift) & (count - 1)], 1);
+      for (int j0 = 0; j0 < free; j0 += kChunk) {
+        if (n > kChunk) load(j0);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+          const int j = j0 + i * kThreads + threadIdx.x;
+          const uint32_t key = key_of(x[i]);
+          if (j < free && (key & mask) == prefix) atomicAdd(&bins[(key >> shift) & ((1 << bits) - 1)], 1);
+        }
       }
       __syncthreads();
-      // From the top: the bin in which the need-th key lies. A thread two bins.
-      const int hi = count - 1 - 2 * (int)threadIdx.x;
-      const int c1 = hi >= 0 ? bins[hi] : 0, c2 = hi >= 1 ? bins[hi - 1] : 0;
+      // From the top: the bin in which the need-th key lies. A thread kOwn bins in a
+      // row, the last thread the lowest (with 10 bits the upper half is empty).
+      const int top = kBins - 1 - kOwn * (int)threadIdx.x;
+      int own[kOwn], sum = 0;
+#pragma unroll
+      for (int i = 0; i < kOwn; ++i) sum += own[i] = bins[top - i];
       int total;
-      const int above = block_prefix(c1 + c2, sm, total);
-      if (above < need && need <= above + c1 + c2) {
-        const bool first = need <= above + c1;
-        sm_found[0] = first ? hi : hi - 1;
-        sm_found[1] = need - above - (first ? 0 : c1);
+      int above = wave_prefix(sum, lane, total);
+      if (lane == 0) sm_wave[wave] = total;
+      __syncthreads();
+#pragma unroll
+      for (int v = 0; v < kWaves; ++v) above += v < wave ? sm_wave[v] : 0;
+      if (above < need && need <= above + sum) {
+        int at = 0;
+#pragma unroll
+        for (int i = 0; i < kOwn - 1; ++i) {
+          const bool past = need > above + own[i] && at == i;
+          above += past ? own[i] : 0;
+          at += past;
+        }
+        sm_found[0] = top - at;
+        sm_found[1] = need - above;
       }
       __syncthreads();
       prefix |= (uint32_t)sm_found[0] << shift;
-      mask |= (uint32_t)(count - 1) << shift;
+      mask |= (uint32_t)((1 << bits) - 1) << shift;
       need = sm_found[1];
-      __syncthreads();
     }
   }
   // In order: the kept indices and their weights. A chunk is read before it is
   // written, and what is kept never moves up, so the weights may be their own output.
-  int done = 0, ties = 0;  // kept and taken from the equal ones so far
-  for (int j0 = 0; j0 < n; j0 += kThreads) {
-    const int j = j0 + threadIdx.x;
-    const float x = j < n ? w[j] : 0.f;
-    const uint32_t key = key_of(x);
-    const bool equal = j < free && want > 0 && key == prefix;
-    int equals = 0, total = 0;
-    const int rank = ties + block_prefix(equal ? 1 : 0, sm, equals);
-    const bool stays = j < n && (j >= free || (want > 0 && key > prefix) || (equal && rank < need));
-    const int at = done + block_prefix(stays ? 1 : 0, sm, total);
-    ties += equals;
-    done += total;
-    if (stays) {
-      to[at] = j;
-      w_out[at] = x;
+  const uint64_t below = ((uint64_t)1 << lane) - 1;
+  // Exclusive sums of a chunk's counts in the order of the positions, by the first wave.
+  auto scan = [&](int *count, int *chunk_total) {
+    __syncthreads();
+    if (wave == 0) {
+      int c[4], sum = 0, total;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int at = 4 * lane + i;
+        c[i] = at < kPer * kWaves ? count[at] : 0;
+        sum += c[i];
+      }
+      int before = wave_prefix(sum, lane, total);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int at = 4 * lane + i;
+        if (at < kPer * kWaves) count[at] = before;
+        before += c[i];
+      }
+      if (lane == 0) *chunk_total = total;
     }
+    __syncthreads();
+  };
+  int done = 0, ties = 0;  // kept, and equal ones seen, in the chunks before
+  for (int j0 = 0; j0 < n; j0 += kChunk) {
+    if (n > kChunk) load(j0);
+    uint64_t equal[kPer], stay[kPer];
+    if (choose) {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const int j = j0 + i * kThreads + threadIdx.x;
+        equal[i] = __ballot(j < free && key_of(x[i]) == prefix);
+        if (lane == 0) sm_count[0][i * kWaves + wave] = __popcll(equal[i]);
+      }
+      scan(sm_count[0], &sm_total[0]);
+    }
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int j = j0 + i * kThreads + threadIdx.x;
+      bool stays = j < n;
+      if (choose && j < free) {
+        const bool same = (equal[i] >> lane) & 1;
+        const int rank = ties + sm_count[0][i * kWaves + wave] + __popcll(equal[i] & below);
+        stays = same ? rank < need : key_of(x[i]) > prefix;
+      } else if (j < free) {
+        stays = false;
+      }
+      stay[i] = __ballot(stays);
+      if (lane == 0) sm_count[1][i * kWaves + wave] = __popcll(stay[i]);
+    }
+    scan(sm_count[1], &sm_total[1]);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      if ((stay[i] >> lane) & 1) {
+        const int at = done + sm_count[1][i * kWaves + wave] + __popcll(stay[i] & below);
+        to[at] = j0 + i * kThreads + threadIdx.x;
+        w_out[at] = x[i];
+      }
+    }
+    if (choose) ties += sm_total[0];
+    done += sm_total[1];
+    __syncthreads();
   }
   for (int j = left + threadIdx.x; j < keep; j += kThreads) to[j] = -1;
   __syncthreads();
@@ -168,8 +239,12 @@ extern "C" int lm_kv_evict(void *k_pages, void *v_pages, const int32_t *source, 
   LM_REQUIRE(k_pages && v_pages && source && target && used && weights && weights_out && kept && used_out);
   LM_REQUIRE(aligned16(k_pages) && aligned16(v_pages));
   hipStream_t s = (hipStream_t)stream;
-  evict_select_kernel<<<dim3((unsigned)heads, (unsigned)batch, (unsigned)layers), kThreads, 0, s>>>(
-      used, weights, width * page, (int)keep, (int)recent, weights_out, kept, used_out);
+  const int64_t capacity = width * page;
+  auto select = capacity <= 1024 ? evict_select_kernel<256, 4>
+                : capacity <= 4096 ? evict_select_kernel<256, 16>
+                                   : evict_select_kernel<1024, 8>;
+  select<<<dim3((unsigned)heads, (unsigned)batch, (unsigned)layers), capacity <= 4096 ? 256 : 1024, 0, s>>>(
+      used, weights, capacity, (int)keep, (int)recent, weights_out, kept, used_out);
   LM_CHECK_LAUNCH();
   const PagedKV kv{(bf16 *)k_pages, (bf16 *)v_pages, pages, (int)width, page_shift(page), (int)heads};
   const int64_t per_block = kMoveThreads / (head_dim / 8);
