@@ -154,6 +154,10 @@ int lm_kv_quant_read(const void *k_codes, const void *v_codes,
 
 /* -------------------------------------------------------- paged kv cache -- */
 
+/* The entry points over a paged cache take their arguments in a struct of 8-byte
+ * fields (pointers, int64_t, double), read before the call returns: filled by one
+ * call from a scripting host, where 36 arguments cost more than the launch. */
+
 /* The paged cache of one layer: k_pages, v_pages [pages, heads, page, head_dim]
  * bf16, contiguous, 16-byte aligned, head_dim 64 or 128, page (positions of a
  * page) a power of two from 16 to 65536. block_table [batch, width] int32
@@ -175,36 +179,53 @@ int lm_kv_quant_read(const void *k_codes, const void *v_codes,
  * nonzero; products and sums in fp32, rounded once) or bf16 (each product and
  * each sum rounded to bf16, lm_rope_kv_write's arithmetic). Positions outside
  * the table are not turned. With cos_sin NULL and rotary 0 nothing is.
- * at NULL: at = positions (one of the two is needed for a store); slots NULL:
- * slot = row; active NULL: every row is written. k_pages and v_pages NULL:
+ * at (int64, or int32 with at_i32 nonzero) NULL: at = positions (one of the two is
+ * needed for a store); slots NULL: slot = row; active NULL: every row is written. k_pages and v_pages NULL:
  * nothing is stored (v, block_table, at, active and slots are not looked at; any
  * head_dim that is a multiple of 16, to 256). q_heads 0: no queries. k_out may
  * be NULL with a store. q_out and k_out may be q and k (in place). Strides in
  * elements, multiples of 8, pointers 16-byte aligned, channels contiguous.
  * One row per target, as lm_kv_write. Replaces vLLM `_custom_ops.rotary_embedding`
  * at litemoe/model.py:58,63-64 with `cache.write` (model.py:59,70). */
-int lm_paged_rotate_write(const void *q, int64_t qs0, int64_t qs1,
-                          const void *k, int64_t ks0, int64_t ks1,
-                          const void *v, int64_t vs0, int64_t vs1,
-                          const void *cos_sin, int64_t table_len,
-                          int64_t rotary, int table_f32, int neox,
-                          const int64_t *positions, const int64_t *at,
-                          const uint8_t *active, const int64_t *slots,
-                          void *q_out, int64_t qo0, int64_t qo1, void *k_out,
-                          int64_t ko0, int64_t ko1, void *k_pages,
-                          void *v_pages, const int32_t *block_table,
-                          int64_t batch, int64_t width, int64_t pages,
-                          int64_t page, int64_t rows, int64_t q_heads,
-                          int64_t kv_heads, int64_t head_dim, void *stream);
+typedef struct lm_paged_rotate_args {
+  const void *q;
+  int64_t qs0, qs1;
+  const void *k;
+  int64_t ks0, ks1;
+  const void *v;
+  int64_t vs0, vs1;
+  const void *cos_sin;
+  int64_t table_len, rotary, table_f32, neox;
+  const int64_t *positions;
+  const void *at;
+  int64_t at_i32;
+  const uint8_t *active;
+  const int64_t *slots;
+  void *q_out;
+  int64_t qo0, qo1;
+  void *k_out;
+  int64_t ko0, ko1;
+  void *k_pages, *v_pages;
+  const int32_t *block_table;
+  int64_t batch, width, pages, page, rows, q_heads, kv_heads, head_dim;
+} lm_paged_rotate_args;
+int lm_paged_rotate_write(const lm_paged_rotate_args *args, void *stream);
 
 /* What the paged cache holds at (slots[r], h, positions[r]): k and v [rows,
- * heads, head_dim] contiguous, 16-byte aligned. Rows whose position or slot is
- * out of range or in no page get zeros; slots may be NULL (slot = row). */
-int lm_paged_read(const void *k_pages, const void *v_pages,
-                  const int32_t *block_table, int64_t batch, int64_t width,
-                  int64_t pages, int64_t page, const int64_t *positions,
-                  const int64_t *slots, int64_t rows, int64_t heads,
-                  int64_t head_dim, void *k, void *v, void *stream);
+ * heads, head_dim] contiguous, 16-byte aligned. positions int64, or int32 with
+ * positions_i32 nonzero. Rows whose position or slot is out of range or in no page
+ * get zeros; slots may be NULL (slot = row). */
+typedef struct lm_paged_read_args {
+  const void *k_pages, *v_pages;
+  const int32_t *block_table;
+  int64_t batch, width, pages, page;
+  const void *positions;
+  int64_t positions_i32;
+  const int64_t *slots;
+  int64_t rows, heads, head_dim;
+  void *k, *v;
+} lm_paged_read_args;
+int lm_paged_read(const lm_paged_read_args *args, void *stream);
 
 /* Eviction by weight, all layers at once: k_pages, v_pages [layers, pages,
  * heads, page, head_dim], weights fp32 [layers, batch, heads, width * page].
@@ -222,13 +243,17 @@ int lm_paged_read(const void *k_pages, const void *v_pages,
  * call; `source`'s pages are not written, so another row may share them.
  * 0 <= recent <= keep, 1 <= keep <= width * page, layers * batch <= 65535. The
  * reference holds every position to the end (litemoe/cache.py:7-20). */
-int lm_kv_evict(void *k_pages, void *v_pages, const int32_t *source,
-                const int32_t *target, int64_t width, int64_t target_width,
-                int64_t pages, int64_t page, const int32_t *used,
-                const float *weights, int64_t layers, int64_t batch,
-                int64_t heads, int64_t head_dim, int64_t keep, int64_t recent,
-                float *weights_out, int32_t *kept, int32_t *used_out,
-                void *stream);
+typedef struct lm_kv_evict_args {
+  void *k_pages, *v_pages;
+  const int32_t *source, *target;
+  int64_t width, target_width, pages, page;
+  const int32_t *used;
+  const float *weights;
+  int64_t layers, batch, heads, head_dim, keep, recent;
+  float *weights_out;
+  int32_t *kept, *used_out;
+} lm_kv_evict_args;
+int lm_kv_evict(const lm_kv_evict_args *args, void *stream);
 
 /* ------------------------------------------------------------ attention -- */
 
@@ -365,15 +390,22 @@ int lm_flash_decode_paged_workspace_size(int64_t batch, int64_t q_heads,
  * (0 for a position without a page); other entries are not written. Two calls
  * in flight at once need workspaces of their own (16-byte aligned). Replaces
  * litemoe/flash_decode.py:16-22 with a block table of more than one page a row. */
-int lm_flash_decode_paged(const void *q, int64_t qs0, int64_t qs1,
-                          const void *k_pages, const void *v_pages,
-                          const int32_t *block_table, int64_t width,
-                          int64_t pages, int64_t page, const int32_t *used,
-                          int64_t batch, int64_t q_heads, int64_t kv_heads,
-                          int64_t head_dim, float scale, int64_t max_len,
-                          int64_t num_splits, const float *weights,
-                          float *weights_out, void *out, void *workspace,
-                          int64_t workspace_bytes, void *stream);
+typedef struct lm_flash_decode_paged_args {
+  const void *q;
+  int64_t qs0, qs1;
+  const void *k_pages, *v_pages;
+  const int32_t *block_table;
+  int64_t width, pages, page;
+  const int32_t *used;
+  int64_t batch, q_heads, kv_heads, head_dim;
+  double scale;
+  int64_t max_len, num_splits;
+  const float *weights;
+  float *weights_out;
+  void *out, *workspace;
+  int64_t workspace_bytes;
+} lm_flash_decode_paged_args;
+int lm_flash_decode_paged(const lm_flash_decode_paged_args *args, void *stream);
 
 /* lm_flash_decode_qkv over a paged cache, head_dim 64 or 128: the partials'
  * sum (rounded to bf16 first where the table is bf16), the rotation of
@@ -385,19 +417,27 @@ int lm_flash_decode_paged(const void *q, int64_t qs0, int64_t qs1,
  * the same heads followed by lm_flash_decode_paged. Two rows of one call may not
  * store to the same page. row_order and frag_out (nonzero: batch <= 128) as
  * lm_flash_decode_quant_qkv; qkv_partials 16-byte aligned. */
-int lm_flash_decode_paged_qkv(const float *qkv_partials, int64_t qkv_splits,
-                              const void *cos_sin, int64_t table_len,
-                              int64_t rotary, int table_f32, int neox,
-                              const int64_t *positions, const uint8_t *active,
-                              void *k_pages, void *v_pages,
-                              const int32_t *block_table, int64_t width,
-                              int64_t pages, int64_t page, const int32_t *used,
-                              const int32_t *row_order, int64_t batch,
-                              int64_t q_heads, int64_t kv_heads,
-                              int64_t head_dim, float scale, int64_t max_len,
-                              int64_t num_splits, const float *weights,
-                              float *weights_out, int frag_out, void *out,
-                              void *workspace, int64_t workspace_bytes,
+typedef struct lm_flash_decode_paged_qkv_args {
+  const float *qkv_partials;
+  int64_t qkv_splits;
+  const void *cos_sin;
+  int64_t table_len, rotary, table_f32, neox;
+  const int64_t *positions;
+  const uint8_t *active;
+  void *k_pages, *v_pages;
+  const int32_t *block_table;
+  int64_t width, pages, page;
+  const int32_t *used, *row_order;
+  int64_t batch, q_heads, kv_heads, head_dim;
+  double scale;
+  int64_t max_len, num_splits;
+  const float *weights;
+  float *weights_out;
+  int64_t frag_out;
+  void *out, *workspace;
+  int64_t workspace_bytes;
+} lm_flash_decode_paged_qkv_args;
+int lm_flash_decode_paged_qkv(const lm_flash_decode_paged_qkv_args *args,
                               void *stream);
 
 /* Variable-length attention over a packed batch (one row per token):

@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 from pathlib import Path
 
 import torch
@@ -35,16 +36,12 @@ _SIGNATURES = {
                               _v, _v, _i64, _v],
     "lm_flash_decode_quant_qkv": [_v, _i64, _v, _i64, _v, _v, _v, _v, _v, _v, _v, _i64, _i64, _i64, _i64, _i64, _i64,
                                   _f32, _i64, _i64, _i32, _v, _v, _i64, _v],
-    "lm_paged_rotate_write": [_v, _i64, _i64, _v, _i64, _i64, _v, _i64, _i64, _v, _i64, _i64, _i32, _i32, _v, _v, _v, _v,
-                              _v, _i64, _i64, _v, _i64, _i64, _v, _v, _v, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
-                              _i64, _v],
-    "lm_paged_read": [_v, _v, _v, _i64, _i64, _i64, _i64, _v, _v, _i64, _i64, _i64, _v, _v, _v],
-    "lm_kv_evict": [_v, _v, _v, _v, _i64, _i64, _i64, _i64, _v, _v, _i64, _i64, _i64, _i64, _i64, _i64, _v, _v, _v, _v],
+    "lm_paged_rotate_write": [C.c_char_p, _v],
+    "lm_paged_read": [C.c_char_p, _v],
+    "lm_kv_evict": [C.c_char_p, _v],
     "lm_flash_decode_paged_workspace_size": [_i64, _i64, _i64, _i64, _i64, _i32, C.POINTER(C.c_int64)],
-    "lm_flash_decode_paged": [_v, _i64, _i64, _v, _v, _v, _i64, _i64, _i64, _v, _i64, _i64, _i64, _i64, _f32, _i64, _i64,
-                              _v, _v, _v, _v, _i64, _v],
-    "lm_flash_decode_paged_qkv": [_v, _i64, _v, _i64, _i64, _i32, _i32, _v, _v, _v, _v, _v, _i64, _i64, _i64, _v, _v,
-                                  _i64, _i64, _i64, _i64, _f32, _i64, _i64, _v, _v, _i32, _v, _v, _i64, _v],
+    "lm_flash_decode_paged": [C.c_char_p, _v],
+    "lm_flash_decode_paged_qkv": [C.c_char_p, _v],
     "lm_flash_decode_workspace_size": [_i64, _i64, _i64, _i64, C.POINTER(C.c_int64)],
     "lm_flash_decode": [_v, _i64, _i64, _v, _v, _v, _i64, _i64, _i64, _i64, _i64, _f32, _i64,
                         _i64, _v, _v, _i64, _v],
@@ -101,6 +98,11 @@ _SIGNATURES = {
                        _i64, _i32, _v, _i64, _v, _v, _i64, _v],
 }
 _RESTYPE = {"lm_version": C.c_char_p, "lm_status_string": C.c_char_p}
+
+# Arguments that go in a struct of 8-byte fields: pointers and integers q, doubles d.
+_STRUCTS = {name: struct.Struct(fields) for name, fields in {
+    "lm_paged_rotate_write": "36q", "lm_paged_read": "15q", "lm_kv_evict": "19q", "lm_flash_decode_paged": "14qd7q",
+    "lm_flash_decode_paged_qkv": "21qd8q"}.items()}
 
 EXPORTED = tuple(_SIGNATURES)
 
@@ -188,6 +190,17 @@ def call_on(index: int, name: str, *args) -> None:
         with torch.cuda.device(index):
             return call(name, *args, torch._C._cuda_getCurrentRawStream(index))
     status = getattr(lib(), name)(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        raise _error(name, status)
+
+
+def call_struct(index: int, name: str, *args) -> None:
+    """:func:`call_on` for an entry point that takes its arguments in a struct; a null
+    pointer is 0. Packing 36 of them costs 0.9 us, passing them one by one 3.6."""
+    if index != torch._C._cuda_getDevice():
+        with torch.cuda.device(index):
+            return call(name, _STRUCTS[name].pack(*args), torch._C._cuda_getCurrentRawStream(index))
+    status = getattr(_LIB or lib(), name)(_STRUCTS[name].pack(*args), torch._C._cuda_getCurrentRawStream(index))
     if status:
         raise _error(name, status)
 

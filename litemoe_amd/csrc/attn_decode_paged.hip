@@ -669,44 +669,36 @@ extern "C" int lm_flash_decode_paged_workspace_size(int64_t batch, int64_t q_hea
   return LM_OK;
 }
 
-extern "C" int lm_flash_decode_paged(const void *q, int64_t qs0, int64_t qs1, const void *k_pages,
-                                     const void *v_pages, const int32_t *block_table, int64_t width, int64_t pages,
-                                     int64_t page, const int32_t *used, int64_t batch, int64_t q_heads,
-                                     int64_t kv_heads, int64_t head_dim, float scale, int64_t max_len,
-                                     int64_t num_splits, const float *weights, float *weights_out, void *out,
-                                     void *workspace, int64_t workspace_bytes_, void *stream) {
-  const Call c{batch, q_heads, kv_heads, head_dim, width, pages, page, max_len, num_splits};
+extern "C" int lm_flash_decode_paged(const lm_flash_decode_paged_args *args, void *stream) {
+  LM_REQUIRE(args);
+  const auto &a = *args;
+  const Call c{a.batch, a.q_heads, a.kv_heads, a.head_dim, a.width, a.pages, a.page, a.max_len, a.num_splits};
   bool run;
   const int status = check_call(c, &run);
   if (status != LM_OK || !run) return status;
-  LM_REQUIRE(q && k_pages && v_pages && block_table && used && out);
-  LM_REQUIRE(aligned16(q) && qs0 % 8 == 0 && qs1 % 8 == 0);
+  LM_REQUIRE(a.q && a.k_pages && a.v_pages && a.block_table && a.used && a.out);
+  LM_REQUIRE(aligned16(a.q) && a.qs0 % 8 == 0 && a.qs1 % 8 == 0);
   const QkvIn in{nullptr, 0, {nullptr, 0, 0, false, false}, nullptr, nullptr, nullptr};
-  return launch_decode_paged(c, q, qs0, qs1, const_cast<void *>(k_pages), const_cast<void *>(v_pages), block_table,
-                             used, scale, in, out, 0, weights, weights_out, workspace, workspace_bytes_, stream);
+  return launch_decode_paged(c, a.q, a.qs0, a.qs1, const_cast<void *>(a.k_pages), const_cast<void *>(a.v_pages),
+                             a.block_table, a.used, (float)a.scale, in, a.out, 0, a.weights, a.weights_out, a.workspace,
+                             a.workspace_bytes, stream);
 }
 
-extern "C" int lm_flash_decode_paged_qkv(const float *qkv_partials, int64_t qkv_splits, const void *cos_sin,
-                                         int64_t table_len, int64_t rotary, int table_f32, int neox,
-                                         const int64_t *positions, const uint8_t *active, void *k_pages,
-                                         void *v_pages, const int32_t *block_table, int64_t width, int64_t pages,
-                                         int64_t page, const int32_t *used, const int32_t *row_order, int64_t batch,
-                                         int64_t q_heads, int64_t kv_heads, int64_t head_dim, float scale,
-                                         int64_t max_len, int64_t num_splits, const float *weights,
-                                         float *weights_out, int frag_out, void *out, void *workspace,
-                                         int64_t workspace_bytes_, void *stream) {
-  const Call c{batch, q_heads, kv_heads, head_dim, width, pages, page, max_len, num_splits};
+extern "C" int lm_flash_decode_paged_qkv(const lm_flash_decode_paged_qkv_args *args, void *stream) {
+  LM_REQUIRE(args);
+  const auto &a = *args;
+  const Call c{a.batch, a.q_heads, a.kv_heads, a.head_dim, a.width, a.pages, a.page, a.max_len, a.num_splits};
   bool run;
   const int status = check_call(c, &run);
   if (status != LM_OK) return status;
-  LM_REQUIRE(qkv_splits >= 1);
-  if (qkv_splits > kMaxQkvSplits || (frag_out && batch > 128)) return LM_EUNSUPPORTED;
+  LM_REQUIRE(a.qkv_splits >= 1);
+  if (a.qkv_splits > kMaxQkvSplits || (a.frag_out && a.batch > 128)) return LM_EUNSUPPORTED;
   if (!run) return LM_OK;
-  LM_REQUIRE(qkv_partials && positions && k_pages && v_pages && block_table && used && out);
-  LM_REQUIRE(aligned16(qkv_partials) && rotation_ok(cos_sin, table_len, rotary, head_dim));
-  const QkvIn in{qkv_partials, (int)qkv_splits, {cos_sin, table_len, (int)rotary, table_f32 != 0, neox != 0},
-                 positions, active, row_order};
-  return launch_decode_paged(c, nullptr, 0, 0, k_pages, v_pages, block_table, used, scale, in, out,
-                             frag_out ? frag_row_blocks(batch) : 0, weights, weights_out, workspace, workspace_bytes_,
-                             stream);
+  LM_REQUIRE(a.qkv_partials && a.positions && a.k_pages && a.v_pages && a.block_table && a.used && a.out);
+  LM_REQUIRE(aligned16(a.qkv_partials) && rotation_ok(a.cos_sin, a.table_len, a.rotary, a.head_dim));
+  const Rotation rot{a.cos_sin, a.table_len, (int)a.rotary, a.table_f32 != 0, a.neox != 0};
+  const QkvIn in{a.qkv_partials, (int)a.qkv_splits, rot, a.positions, a.active, a.row_order};
+  return launch_decode_paged(c, nullptr, 0, 0, a.k_pages, a.v_pages, a.block_table, a.used, (float)a.scale, in, a.out,
+                             a.frag_out ? frag_row_blocks(a.batch) : 0, a.weights, a.weights_out, a.workspace,
+                             a.workspace_bytes, stream);
 }

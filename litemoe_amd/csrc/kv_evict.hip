@@ -225,11 +225,10 @@ evict_move_kernel(PagedKV kv, int64_t layer_elems, const int32_t *__restrict__ s
 
 using namespace lm;
 
-extern "C" int lm_kv_evict(void *k_pages, void *v_pages, const int32_t *source, const int32_t *target, int64_t width,
-                           int64_t target_width, int64_t pages, int64_t page, const int32_t *used,
-                           const float *weights, int64_t layers, int64_t batch, int64_t heads, int64_t head_dim,
-                           int64_t keep, int64_t recent, float *weights_out, int32_t *kept, int32_t *used_out,
-                           void *stream) {
+extern "C" int lm_kv_evict(const lm_kv_evict_args *args, void *stream) {
+  LM_REQUIRE(args);
+  const auto &[k_pages, v_pages, source, target, width, target_width, pages, page, used, weights, layers, batch, heads,
+               head_dim, keep, recent, weights_out, kept, used_out] = *args;
   LM_REQUIRE(layers > 0 && batch >= 0 && heads > 0 && heads <= 65535 && batch <= 65535 && layers <= 65535 &&
              layers * batch <= 65535 && keep > 0 && recent >= 0 && recent <= keep && target_width > 0);
   const int status = paged_args_ok(width, pages, page, head_dim);

@@ -31,7 +31,13 @@ struct RotateArgs {
   int rot_items, head_items, v_items;  // of a head: turned items, all items; of a v head
   uint32_t items;                      // of a token
   int64_t total;                       // items of the call
+  bool at_i32;
 };
+
+// Places in the cache come as int64, or as int32 (a row's `used`).
+__device__ __forceinline__ int64_t index_at(const void *p, bool i32, int64_t i) {
+  return i32 ? static_cast<const int32_t *>(p)[i] : static_cast<const int64_t *>(p)[i];
+}
 
 template <bool kF32>
 __device__ __forceinline__ void load_angles(const void *row, int at, float *f) {
@@ -50,7 +56,7 @@ __device__ __forceinline__ void load_angles(const void *row, int at, float *f) {
 
 template <bool kNeox, bool kF32>
 __global__ void __launch_bounds__(kThreads)
-rotate_write_kernel(RotateArgs a, const int64_t *__restrict__ pos, const int64_t *__restrict__ at,
+rotate_write_kernel(RotateArgs a, const int64_t *__restrict__ pos, const void *__restrict__ at,
                     const uint8_t *__restrict__ active, const int64_t *__restrict__ slots,
                     const int32_t *__restrict__ table) {
   const int64_t id = (int64_t)blockIdx.x * kThreads + threadIdx.x;
@@ -75,7 +81,7 @@ rotate_write_kernel(RotateArgs a, const int64_t *__restrict__ pos, const int64_t
   bf16 *cell = nullptr;
   const int64_t p = pos ? pos[token] : 0;
   if (!is_q && a.kv.k && (!active || active[token])) {
-    const int64_t row = slots ? slots[token] : token, j = at ? at[token] : p;
+    const int64_t row = slots ? slots[token] : token, j = at ? index_at(at, a.at_i32, token) : p;
     if (row >= 0 && row < a.batch && j >= 0 && (j >> a.kv.shift) < a.kv.width) {
       const int64_t page = table[row * a.kv.width + (j >> a.kv.shift)];
       if (page >= 0 && page < a.kv.pages)
@@ -146,7 +152,7 @@ rotate_write_kernel(RotateArgs a, const int64_t *__restrict__ pos, const int64_t
 
 // A thread a 16-byte unit of k and of v.
 __global__ void __launch_bounds__(kThreads)
-read_kernel(PagedKV kv, const int32_t *__restrict__ table, int64_t batch, const int64_t *__restrict__ pos,
+read_kernel(PagedKV kv, const int32_t *__restrict__ table, int64_t batch, const void *__restrict__ pos, bool pos_i32,
             const int64_t *__restrict__ slots, int dim, int64_t total, bf16 *__restrict__ k, bf16 *__restrict__ v) {
   const int64_t id = (int64_t)blockIdx.x * kThreads + threadIdx.x;
   if (id >= total) return;
@@ -154,7 +160,7 @@ read_kernel(PagedKV kv, const int32_t *__restrict__ table, int64_t batch, const 
   const int64_t token = (uint64_t)id / each;
   const uint32_t item = (uint32_t)(id - token * each);
   const int head = item / units, unit = item % units;
-  const int64_t row = slots ? slots[token] : token, j = pos[token];
+  const int64_t row = slots ? slots[token] : token, j = index_at(pos, pos_i32, token);
   u32x4 wk{0, 0, 0, 0}, wv{0, 0, 0, 0};
   if (row >= 0 && row < batch && j >= 0 && (j >> kv.shift) < kv.width) {
     const int64_t page = table[row * kv.width + (j >> kv.shift)];
@@ -175,14 +181,11 @@ bool view_ok(const void *p, int64_t s0, int64_t s1) { return aligned16(p) && s0 
 
 using namespace lm;
 
-extern "C" int lm_paged_rotate_write(const void *q, int64_t qs0, int64_t qs1, const void *k, int64_t ks0, int64_t ks1,
-                                     const void *v, int64_t vs0, int64_t vs1, const void *cos_sin, int64_t table_len,
-                                     int64_t rotary, int table_f32, int neox, const int64_t *positions,
-                                     const int64_t *at, const uint8_t *active, const int64_t *slots, void *q_out,
-                                     int64_t qo0, int64_t qo1, void *k_out, int64_t ko0, int64_t ko1, void *k_pages,
-                                     void *v_pages, const int32_t *block_table, int64_t batch, int64_t width,
-                                     int64_t pages, int64_t page, int64_t rows, int64_t q_heads, int64_t kv_heads,
-                                     int64_t head_dim, void *stream) {
+extern "C" int lm_paged_rotate_write(const lm_paged_rotate_args *args, void *stream) {
+  LM_REQUIRE(args);
+  const auto &[q, qs0, qs1, k, ks0, ks1, v, vs0, vs1, cos_sin, table_len, rotary, table_f32, neox, positions, at, at_i32,
+               active, slots, q_out, qo0, qo1, k_out, ko0, ko1, k_pages, v_pages, block_table, batch, width, pages, page,
+               rows, q_heads, kv_heads, head_dim] = *args;
   LM_REQUIRE(rows >= 0 && q_heads >= 0 && kv_heads >= 0 && q_heads + kv_heads > 0 && q_heads <= 65535 &&
              kv_heads <= 65535 && head_dim > 0);
   if (head_dim % 16 || head_dim > 256) return LM_EUNSUPPORTED;
@@ -200,6 +203,7 @@ extern "C" int lm_paged_rotate_write(const void *q, int64_t qs0, int64_t qs1, co
   LM_REQUIRE(!store || (v && view_ok(v, vs0, vs1)));
   LM_REQUIRE(cos_sin ? positions && rotation_ok(cos_sin, table_len, rotary, head_dim) : rotary == 0);
   RotateArgs a;
+  a.at_i32 = at_i32 != 0;
   a.q = {(const bf16 *)q, qs0, qs1};
   a.k = {(const bf16 *)k, ks0, ks1};
   a.v = {(const bf16 *)v, vs0, vs1};
@@ -225,10 +229,10 @@ extern "C" int lm_paged_rotate_write(const void *q, int64_t qs0, int64_t qs1, co
   return LM_OK;
 }
 
-extern "C" int lm_paged_read(const void *k_pages, const void *v_pages, const int32_t *block_table, int64_t batch,
-                             int64_t width, int64_t pages, int64_t page, const int64_t *positions,
-                             const int64_t *slots, int64_t rows, int64_t heads, int64_t head_dim, void *k, void *v,
-                             void *stream) {
+extern "C" int lm_paged_read(const lm_paged_read_args *args, void *stream) {
+  LM_REQUIRE(args);
+  const auto &[k_pages, v_pages, block_table, batch, width, pages, page, positions, positions_i32, slots, rows, heads,
+               head_dim, k, v] = *args;
   LM_REQUIRE(rows >= 0 && batch > 0 && heads > 0 && heads <= 65535);
   const int status = paged_args_ok(width, pages, page, head_dim);
   if (status != LM_OK) return status;
@@ -240,7 +244,7 @@ extern "C" int lm_paged_read(const void *k_pages, const void *v_pages, const int
                    page_shift(page), (int)heads};
   const int64_t total = rows * heads * (head_dim / 8);
   read_kernel<<<dim3((unsigned)cdiv(total, kThreads)), kThreads, 0, (hipStream_t)stream>>>(
-      kv, block_table, batch, positions, slots, (int)head_dim, total, (bf16 *)k, (bf16 *)v);
+      kv, block_table, batch, positions, positions_i32 != 0, slots, (int)head_dim, total, (bf16 *)k, (bf16 *)v);
   LM_CHECK_LAUNCH();
   return LM_OK;
 }

@@ -328,7 +328,7 @@ class PagedFlashDecode:
         if weights is None:
             if weights_out is not None:
                 raise ValueError("weights_out goes with weights")
-            return None, None, self.workspace
+            return 0, 0, self.workspace
         weights_out = weights if weights_out is None else weights_out
         for w in (weights, weights_out):
             if (w.dtype != torch.float32 or w.dim() != 3 or w.shape[0] < rows
@@ -362,10 +362,10 @@ class PagedFlashDecode:
         used = kv_quant.per_row(used, b, torch.int32, index, "used")
         before, after, space = self._weights(weights, weights_out, b, index)
         out = torch.empty_like(q) if q.is_contiguous() else torch.empty(q.shape, device=q.device, dtype=q.dtype)
-        _lib.call_on(index, "lm_flash_decode_paged", q.data_ptr(), rows, heads, k.data_ptr(), v.data_ptr(),
-                     table.data_ptr(), table.shape[1], k.shape[0], k.shape[2], used.data_ptr(), b, hq, self.kv_heads, d,
-                     float(scale), self.maximum, self.splits, before, after, out.data_ptr(), space.data_ptr(),
-                     space.numel())
+        _lib.call_struct(index, "lm_flash_decode_paged", q.data_ptr(), rows, heads, k.data_ptr(), v.data_ptr(),
+                         table.data_ptr(), table.shape[1], k.shape[0], k.shape[2], used.data_ptr(), b, hq, self.kv_heads,
+                         d, scale, self.maximum, self.splits, before, after, out.data_ptr(), space.data_ptr(),
+                         space.numel())
         return out
 
     def fused_qkv(self, partials, cos_sin, positions, active, k, v, table, scale, used, q_heads, row_order=None,
@@ -396,9 +396,11 @@ class PagedFlashDecode:
         else:
             out = torch.empty((b, q_heads, 1, self.head_dim), device=k.device, dtype=torch.bfloat16)
             out_ptr = out.data_ptr()
-        _lib.call_on(index, "lm_flash_decode_paged_qkv", partials.data_ptr(), splits, cos_sin.data_ptr(), *cos_sin.shape,
-                     int(cos_sin.dtype == torch.float32), int(bool(is_neox)), positions.data_ptr(), _lib.ptr(active),
-                     k.data_ptr(), v.data_ptr(), table.data_ptr(), table.shape[1], k.shape[0], k.shape[2],
-                     used.data_ptr(), _lib.ptr(row_order), b, q_heads, self.kv_heads, self.head_dim, float(scale),
-                     self.maximum, self.splits, before, after, int(frag_out), out_ptr, space.data_ptr(), space.numel())
+        _lib.call_struct(index, "lm_flash_decode_paged_qkv", partials.data_ptr(), splits, cos_sin.data_ptr(),
+                         *cos_sin.shape, cos_sin.dtype == torch.float32, bool(is_neox), positions.data_ptr(),
+                         0 if active is None else active.data_ptr(), k.data_ptr(), v.data_ptr(), table.data_ptr(),
+                         table.shape[1], k.shape[0], k.shape[2], used.data_ptr(),
+                         0 if row_order is None else row_order.data_ptr(), b, q_heads, self.kv_heads, self.head_dim, scale,
+                         self.maximum, self.splits, before, after, bool(frag_out), out_ptr, space.data_ptr(),
+                         space.numel())
         return out

@@ -11,7 +11,7 @@ import torch
 from . import _lib
 from .kv_quant import per_row
 
-PAGES = tuple(1 << s for s in range(4, 17))  # positions of a page
+PAGES = frozenset(1 << s for s in range(4, 17))  # positions of a page
 HEAD_DIMS = (64, 128)
 
 
@@ -24,9 +24,10 @@ def check_layer(k, v, table):
     if len(shape) != 4 or v.shape != shape or shape[2] not in PAGES or shape[3] not in HEAD_DIMS:
         raise ValueError("Paged KV cache layers are k, v [P, H, page, D], page a power of two from 16 to 65536, "
                          "D 64 or 128")
-    if not (k.dtype == v.dtype == torch.bfloat16 and k.is_contiguous() and v.is_contiguous()):
+    if k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16 or not k.is_contiguous() or not v.is_contiguous():
         raise ValueError("Paged KV cache layers must be contiguous BF16")
-    check_table(table)
+    if table.dtype != torch.int32 or table.dim() != 2 or not table.is_contiguous():
+        check_table(table)
     return index
 
 
@@ -35,6 +36,11 @@ def check_table(table, rows=None):
         raise ValueError("A page table is contiguous int32 [rows, pages of a row]")
     if rows is not None and table.shape[0] != rows:
         raise ValueError("The page table needs one line per row")
+
+
+def places(t, rows, index, what):
+    """``t``, a place in the cache per row, as the kernels take it: int64 or int32."""
+    return per_row(t, rows, torch.int32 if t.dtype == torch.int32 else torch.int64, index, what)
 
 
 def aligned(x):
@@ -67,14 +73,14 @@ def write(cache, layer, k, v, positions, active, slots):
     if k.get_device() != index or v.get_device() != index:
         raise ValueError("KV write tensors must be on the cache's device")
     rows = k.shape[0]
-    positions = per_row(positions, rows, torch.int64, index, "positions")
+    at = places(positions, rows, index, "positions")
     slots = per_row(slots, rows, torch.int64, index, "slots")
-    active = None if active is None else per_row(active, rows, torch.bool, index, "active")
+    active = 0 if active is None else per_row(active, rows, torch.bool, index, "active").data_ptr()
     k, v = aligned(k[:, :, 0]), aligned(v[:, :, 0])
-    _lib.call_on(index, "lm_paged_rotate_write", None, 0, 0, k.data_ptr(), *strides(k), v.data_ptr(), *strides(v), None, 0,
-                 0, 0, 0, positions.data_ptr(), None, _lib.ptr(active), slots.data_ptr(), None, 0, 0, None, 0, 0,
-                 kc.data_ptr(), vc.data_ptr(), table.data_ptr(), table.shape[0], table.shape[1], pages, page, rows, 0,
-                 heads, dim)
+    _lib.call_struct(index, "lm_paged_rotate_write", 0, 0, 0, k.data_ptr(), *strides(k), v.data_ptr(), *strides(v), 0, 0,
+                     0, 0, 0, 0, at.data_ptr(), at.dtype == torch.int32, active, slots.data_ptr(), 0, 0, 0, 0, 0, 0,
+                     kc.data_ptr(), vc.data_ptr(), table.data_ptr(), table.shape[0], table.shape[1], pages, page, rows, 0,
+                     heads, dim)
 
 
 def read(cache, layer, positions, slots):
@@ -85,12 +91,13 @@ def read(cache, layer, positions, slots):
     index = check_layer(kc, vc, table)
     pages, heads, page, dim = kc.shape
     rows = positions.numel()
-    positions = per_row(positions, rows, torch.int64, index, "positions")
+    positions = places(positions, rows, index, "positions")
     slots = per_row(slots, rows, torch.int64, index, "slots")
     k = torch.empty((rows, heads, 1, dim), dtype=torch.bfloat16, device=kc.device)
     v = torch.empty_like(k)
-    _lib.call_on(index, "lm_paged_read", kc.data_ptr(), vc.data_ptr(), table.data_ptr(), table.shape[0], table.shape[1],
-                 pages, page, positions.data_ptr(), slots.data_ptr(), rows, heads, dim, k.data_ptr(), v.data_ptr())
+    _lib.call_struct(index, "lm_paged_read", kc.data_ptr(), vc.data_ptr(), table.data_ptr(), table.shape[0],
+                     table.shape[1], pages, page, positions.data_ptr(), positions.dtype == torch.int32, slots.data_ptr(),
+                     rows, heads, dim, k.data_ptr(), v.data_ptr())
     return k, v
 
 
@@ -106,12 +113,14 @@ def evict(cache, weights, used, keep, recent, target, table=None, weights_out=No
     rows' present table (the cache's own unless given). Pages of ``target`` must not be
     in it: the rows' present pages are read and not written, so another row may share
     them. :meth:`PagedKVCache.evict` takes care of both and moves the cache's table."""
-    k, v, own = cache.k, cache.v, cache.table
-    table = own if table is None else table
-    index = check_layer(k[0], v[0], table)
+    k, v = cache.k, cache.v
+    table = cache.table if table is None else table
     layers, pages, heads, page, dim = k.shape
-    if not (k.is_contiguous() and v.is_contiguous()):
-        raise ValueError("Eviction takes a cache of contiguous layers")
+    index = k.get_device()
+    if index < 0 or table.get_device() != index:
+        _lib.require_cuda(k, table, what="paged KV cache")
+        raise ValueError("Eviction's tables and weights must be on the cache's device")
+    check_table(table)
     rows, width = table.shape
     check_table(target, rows)
     if target.get_device() != index or weights.get_device() != index:
@@ -127,7 +136,7 @@ def evict(cache, weights, used, keep, recent, target, table=None, weights_out=No
     out = torch.empty_like(weights) if weights_out is None else weights_out
     kept = torch.empty((layers, rows, heads, keep), dtype=torch.int32, device=k.device)
     left = torch.empty(rows, dtype=torch.int32, device=k.device)
-    _lib.call_on(index, "lm_kv_evict", k.data_ptr(), v.data_ptr(), table.data_ptr(), target.data_ptr(), width,
-                 target.shape[1], pages, page, used.data_ptr(), weights.data_ptr(), layers, rows, heads, dim, keep,
-                 recent, out.data_ptr(), kept.data_ptr(), left.data_ptr())
+    _lib.call_struct(index, "lm_kv_evict", k.data_ptr(), v.data_ptr(), table.data_ptr(), target.data_ptr(), width,
+                     target.shape[1], pages, page, used.data_ptr(), weights.data_ptr(), layers, rows, heads, dim, keep,
+                     recent, out.data_ptr(), kept.data_ptr(), left.data_ptr())
     return out, kept, left

@@ -123,7 +123,7 @@ def _rotate(q, k, positions, cos_sin, is_neox, q_out, k_out, v=None, cache=None,
         raise ValueError("Rotation takes heads of a multiple of 16 channels, at most 256")
     check_table(cos_sin, index, dim)
     positions = per_row(positions, rows, torch.int64, index, "positions")
-    where = [None, None, None, 0, 0, 0, 0]
+    where, values, place, slot, mask = (0,) * 7, (0, 0, 0), (0, 0), 0, 0
     if cache is not None:
         kc, vc, table = cache.layer(layer)
         if kv_paged.check_layer(kc, vc, table) != index:
@@ -131,17 +131,24 @@ def _rotate(q, k, positions, cos_sin, is_neox, q_out, k_out, v=None, cache=None,
         pages, heads, page, channels = kc.shape
         if heads != k.shape[1] or channels != dim or v.shape != k.shape or v.get_device() != index:
             raise ValueError("Keys and values do not match the cache's heads")
-        at = None if at is None else per_row(at, rows, torch.int64, index, "at")
-        slots = None if slots is None else per_row(slots, rows, torch.int64, index, "slots")
-        active = None if active is None else per_row(active, rows, torch.bool, index, "active")
-        where = [kc.data_ptr(), vc.data_ptr(), table.data_ptr(), table.shape[0], table.shape[1], pages, page]
-    none = (None, 0, 0)
-
-    def view(x):
-        return none if x is None else (x.data_ptr(), *kv_paged.strides(x))
-    _lib.call_on(index, "lm_paged_rotate_write", *view(q), *view(k), *view(v), cos_sin.data_ptr(), *cos_sin.shape,
-                 int(cos_sin.dtype == torch.float32), int(bool(is_neox)), positions.data_ptr(), _lib.ptr(at),
-                 _lib.ptr(active), _lib.ptr(slots), *view(q_out), *view(k_out), *where, rows, q.shape[1], k.shape[1], dim)
+        if at is not None:
+            at = kv_paged.places(at, rows, index, "at")
+            place = at.data_ptr(), at.dtype == torch.int32
+        if slots is not None:
+            slots = per_row(slots, rows, torch.int64, index, "slots")
+            slot = slots.data_ptr()
+        if active is not None:
+            active = per_row(active, rows, torch.bool, index, "active")
+            mask = active.data_ptr()
+        where = kc.data_ptr(), vc.data_ptr(), table.data_ptr(), *table.shape, pages, page
+        values = v.data_ptr(), *kv_paged.strides(v)
+    q_view, k_view = (q.data_ptr(), *kv_paged.strides(q)), (k.data_ptr(), *kv_paged.strides(k))
+    # results are new and contiguous, or the operands themselves
+    q_to = q_view if q_out is q else (q_out.data_ptr(), q.shape[1] * dim, dim)
+    k_to = k_view if k_out is k else (0, 0, 0) if k_out is None else (k_out.data_ptr(), k.shape[1] * dim, dim)
+    _lib.call_struct(index, "lm_paged_rotate_write", *q_view, *k_view, *values, cos_sin.data_ptr(), *cos_sin.shape,
+                     cos_sin.dtype == torch.float32, bool(is_neox), positions.data_ptr(), *place, mask, slot, *q_to, *k_to,
+                     *where, rows, q.shape[1], k.shape[1], dim)
 
 
 def rotate_kv_write(q, k, v, positions, active, cos_sin, cache, layer, slots=None, at=None, is_neox=True, keep_k=False):
@@ -161,8 +168,8 @@ def rotate_kv_write(q, k, v, positions, active, cos_sin, cache, layer, slots=Non
     if any(t.dim() != 3 or t.dtype != torch.bfloat16 for t in (q, k, v)):
         raise ValueError("RoPE supports BF16 [T, heads, D] queries, keys and values")
     q, k, v = (kv_paged.aligned(t) for t in (q, k, v))
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device) if keep_k else None
+    q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    k_out = torch.empty_like(k, memory_format=torch.contiguous_format) if keep_k else None
     _rotate(q, k, positions, cos_sin, is_neox, q_out, k_out, v, cache, layer, at, active, slots)
     return q_out, k_out
 

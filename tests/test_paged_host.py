@@ -1,9 +1,10 @@
 """The paged KV cache without a GPU: pages handed out and given back, tables, rotary
 tables, and the calls that are refused before anything is launched."""
 import copy
-import ctypes as C
 import math
 import pickle
+import re
+from pathlib import Path
 
 import pytest
 import torch
@@ -242,31 +243,56 @@ def test_rotary_tables_refused(args, scaling):
 
 # ------------------------------------------------------------------- C ABI --
 
+def packed(name, values):
+    """The arguments' struct: every field takes 8 bytes, in the header's order."""
+    return _lib._STRUCTS[name].pack(*[0 if x is None else x for x in values])
+
+
 def rotate(h, q=_P, v=_P, cos=_P, table_len=16, rotary=64, pos=_P, k_pages=_P, v_pages=_P, table=_P, batch=2, width=4,
            pages=8, page=16, rows=3, hq=4, hkv=2, dim=64, qs=64, q_out=_P, k_out=None):
-    return h.lm_paged_rotate_write(q, qs, 64, _P, 64, 64, v, 64, 64, cos, table_len, rotary, 1, 1, pos, None, None, None,
-                                   q_out, 64, 64, k_out, 64, 64, k_pages, v_pages, table, batch, width, pages, page, rows,
-                                   hq, hkv, dim, None)
+    return h.lm_paged_rotate_write(packed("lm_paged_rotate_write", [
+        q, qs, 64, _P, 64, 64, v, 64, 64, cos, table_len, rotary, 1, 1, pos, None, 0, None, None, q_out, 64, 64, k_out, 64,
+        64, k_pages, v_pages, table, batch, width, pages, page, rows, hq, hkv, dim]), None)
 
 
 def read(h, k=_P, page=16, dim=64, rows=3, table=_P, out=_P):
-    return h.lm_paged_read(k, _P, table, 2, 4, 8, page, _P, None, rows, 2, dim, out, _P, None)
+    return h.lm_paged_read(packed("lm_paged_read", [k, _P, table, 2, 4, 8, page, _P, 0, None, rows, 2, dim, out, _P]), None)
 
 
 def decode(h, q=_P, page=16, width=4, pages=8, batch=2, hq=4, hkv=2, dim=64, max_len=64, splits=1, w=None, w_out=None,
            ws=_P, size=1 << 30, table=_P, qs=64):
-    return h.lm_flash_decode_paged(q, qs, 64, _P, _P, table, width, pages, page, _P, batch, hq, hkv, dim, C.c_float(1.0),
-                                   max_len, splits, w, w_out, _P, ws, size, None)
+    return h.lm_flash_decode_paged(packed("lm_flash_decode_paged", [
+        q, qs, 64, _P, _P, table, width, pages, page, _P, batch, hq, hkv, dim, 1.0, max_len, splits, w, w_out, _P, ws,
+        size]), None)
 
 
 def fused(h, part=_P, slices=3, cos=_P, rotary=64, page=16, batch=2, frag=0, pos=_P, ws=_P, size=1 << 30, splits=1):
-    return h.lm_flash_decode_paged_qkv(part, slices, cos, 16, rotary, 1, 1, pos, None, _P, _P, _P, 4, 8, page, _P, None,
-                                       batch, 4, 2, 64, C.c_float(1.0), 64, splits, None, None, frag, _P, ws, size, None)
+    return h.lm_flash_decode_paged_qkv(packed("lm_flash_decode_paged_qkv", [
+        part, slices, cos, 16, rotary, 1, 1, pos, None, _P, _P, _P, 4, 8, page, _P, None, batch, 4, 2, 64, 1.0, 64, splits,
+        None, None, frag, _P, ws, size]), None)
 
 
 def evict(h, page=16, keep=5, recent=2, layers=2, batch=2, width=4, w=_P, dim=64, target=_P):
-    return h.lm_kv_evict(_P, _P, _P, target, width, 2, 8, page, _P, w, layers, batch, 2, dim, keep, recent, _P, _P, _P,
-                         None)
+    return h.lm_kv_evict(packed("lm_kv_evict", [
+        _P, _P, _P, target, width, 2, 8, page, _P, w, layers, batch, 2, dim, keep, recent, _P, _P, _P]), None)
+
+
+@pytest.mark.parametrize("name", ["lm_paged_rotate_write", "lm_paged_read", "lm_kv_evict", "lm_flash_decode_paged",
+                                  "lm_flash_decode_paged_qkv"])
+def test_structs_are_the_headers(name):
+    """Fields and their kinds, in order; no struct at all is refused."""
+    text = (Path(__file__).resolve().parents[1] / "include" / "litemoe_amd.h").read_text()
+    tag = name.replace("_write", "") + "_args"
+    body = re.search(r"typedef struct %s \{(.*?)\} %s;" % (tag, tag), text, re.S).group(1)
+    kinds = ""
+    for line in body.split(";")[:-1]:
+        count = line.count(",") + 1
+        assert "*" in line or re.match(r"\s*(int64_t|double) ", line), line
+        kinds += ("d" if line.split()[0] == "double" else "q") * count
+    fields = _lib._STRUCTS[name].format
+    assert kinds == "".join(kind * int(n or 1) for n, kind in re.findall(r"(\d*)([qd])", fields))
+    assert _lib._STRUCTS[name].size == 8 * len(kinds)
+    assert getattr(_lib.load(), name)(None, None) == 1
 
 
 @pytest.mark.parametrize("call,expected", [
