@@ -369,8 +369,9 @@ int lm_flash_decode_quant_qkv(const float *qkv_partials, int64_t qkv_splits,
 
 /* Workspace for lm_flash_decode_paged and _qkv; weighed nonzero: with weights. */
 int lm_flash_decode_paged_workspace_size(int64_t batch, int64_t q_heads,
-                                         int64_t head_dim, int64_t max_len,
-                                         int64_t num_splits, int weighed,
+                                         int64_t kv_heads, int64_t head_dim,
+                                         int64_t max_len, int64_t num_splits,
+                                         int64_t num_shares, int weighed,
                                          int64_t *bytes);
 
 /* lm_flash_decode over a paged cache (see lm_paged_rotate_write): out[b,h] =
@@ -381,8 +382,9 @@ int lm_flash_decode_paged_workspace_size(int64_t batch, int64_t q_heads,
  * and positions without a page may hold anything. q_heads / kv_heads at most
  * 16; q 16-byte aligned, its strides multiples of 8; out [batch, q_heads,
  * head_dim] contiguous.
- * Each row is cut by its own length into at most num_splits pieces of whole
- * tiles of 32 positions. weights and weights_out (both or neither; fp32
+ * num_splits (1 to 1024) workgroups take a row's tiles of 32 positions in turn; or,
+ * with num_splits 1, num_shares (0: not; to 65535) workgroups per KV head take equal
+ * shares of the tiles of all rows. weights and weights_out (both or neither; fp32
  * [batch, kv_heads, width * page], 16-byte aligned, may be one buffer): for
  * every j below the row's length
  *   weights_out[b,g,j] = weights[b,g,j] + sum of the probabilities of j over
@@ -399,7 +401,7 @@ typedef struct lm_flash_decode_paged_args {
   const int32_t *used;
   int64_t batch, q_heads, kv_heads, head_dim;
   double scale;
-  int64_t max_len, num_splits;
+  int64_t max_len, num_splits, num_shares;
   const float *weights;
   float *weights_out;
   void *out, *workspace;

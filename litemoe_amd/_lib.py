@@ -39,7 +39,7 @@ _SIGNATURES = {
     "lm_paged_rotate_write": [C.c_char_p, _v],
     "lm_paged_read": [C.c_char_p, _v],
     "lm_kv_evict": [C.c_char_p, _v],
-    "lm_flash_decode_paged_workspace_size": [_i64, _i64, _i64, _i64, _i64, _i32, C.POINTER(C.c_int64)],
+    "lm_flash_decode_paged_workspace_size": [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _i32, C.POINTER(C.c_int64)],
     "lm_flash_decode_paged": [C.c_char_p, _v],
     "lm_flash_decode_paged_qkv": [C.c_char_p, _v],
     "lm_flash_decode_workspace_size": [_i64, _i64, _i64, _i64, C.POINTER(C.c_int64)],
@@ -101,7 +101,7 @@ _RESTYPE = {"lm_version": C.c_char_p, "lm_status_string": C.c_char_p}
 
 # Arguments that go in a struct of 8-byte fields: pointers and integers q, doubles d.
 _STRUCTS = {name: struct.Struct(fields) for name, fields in {
-    "lm_paged_rotate_write": "36q", "lm_paged_read": "15q", "lm_kv_evict": "19q", "lm_flash_decode_paged": "14qd7q",
+    "lm_paged_rotate_write": "36q", "lm_paged_read": "15q", "lm_kv_evict": "19q", "lm_flash_decode_paged": "14qd8q",
     "lm_flash_decode_paged_qkv": "21qd8q"}.items()}
 
 EXPORTED = tuple(_SIGNATURES)

@@ -42,7 +42,7 @@ namespace {
 constexpr int kTile = 32;
 constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * kWave;
-constexpr int kMaxQkvSplits = 8;
+constexpr int kMaxQkvSplits = 8, kEarlySplits = 4;  // slices of the projection, those requested before the KV stream
 constexpr int kMaxGroups = 16;
 
 // Running maximum before any position: below every finite score, and finite, so
@@ -52,12 +52,16 @@ constexpr float kAbove = 8.f;
 
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
+// Results that other workgroups add to, in slots of G query heads of a KV head: one per
+// (row, split), or two per share, of a row that another share began and of one that it
+// began itself.
 struct Partial {
-  float *o;   // [batch, q_heads, splits, D]
-  float *m;   // [batch, q_heads, splits]
-  float *l;   // sums of the rounded probabilities, as m
-  float *lw;  // weighed: sums of the probabilities, as m
-  float *s;   // weighed: scores in log2 units, [batch, q_heads, padded]
+  int32_t *off;    // shares: [batch + 1] tiles before each row
+  float *o;        // [slot][G][D]
+  float *m, *l;    // [slot][G]; l: sums of the rounded probabilities
+  float *lw;       // weighed: sums of the probabilities, as m
+  float *rm, *rw;  // weighed: m and lw of rows that one workgroup held, [batch, q_heads]
+  float *s;        // weighed: scores in log2 units, [batch, q_heads, padded]
   int64_t padded;
 };
 
@@ -71,19 +75,21 @@ struct QkvIn {
 };
 
 struct Shape {
-  int q_heads, G, max_len, splits;
+  int q_heads, G, max_len;
+  int splits;  // workgroups that take a row's tiles in turn
+  int shares;  // or equal pieces that all rows' tiles are cut into (0: not)
   float scale;
-  int64_t batch;
+  int batch;
 };
 
-// Positions of row b that are looked at.
+// Positions of a row that are looked at, and their tiles.
 __device__ __forceinline__ int row_length(int used, const Shape &sh, const PagedKV &kv) {
   return max(0, min(min(used, sh.max_len), kv.width << kv.shift));
 }
-// Splits that hold a tile of a row of n positions: tiles go to the waves of all
-// splits in turn, kWaves a split.
-__device__ __forceinline__ int row_splits(int n, const Shape &sh) {
-  return min(sh.splits, (n + kTile * kWaves - 1) / (kTile * kWaves));
+__device__ __forceinline__ int row_tiles(int n) { return (n + kTile - 1) / kTile; }
+// Tiles of a share: all rows' tiles cut evenly, one for each wave at least.
+__device__ __forceinline__ uint32_t share_tiles(uint32_t total, const Shape &sh) {
+  return max((total + sh.shares - 1) / (uint32_t)sh.shares, (uint32_t)kWaves);
 }
 
 template <int D>
@@ -103,40 +109,77 @@ __device__ __forceinline__ T constant(const T *p) {
   return *(const __attribute__((address_space(4))) T *)p;
 }
 
-template <int D, bool kFused, bool kWeigh>
-__global__ void __launch_bounds__(kWaves *kWave, D == 64 ? 4 : 2)
-decode_paged_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, PagedKV kv,
-                    const int32_t *__restrict__ table, const int32_t *__restrict__ used, Shape sh, Partial part,
-                    QkvIn in, bf16 *__restrict__ out, int out_mb) {
+// Bytes of LDS before the scores: the merge of the waves and the fused prologue use the
+// same ones in turn; the heads' factors behind them.
+constexpr int kRingFloats = 32 * kTile;  // of a wave: 32 tiles times heads
+__host__ __device__ constexpr int lds_bytes(int D, int G, bool fused) {
+  const int merge = kWaves * G * (D + 3) * 4, rot = fused ? (G + 2) * D * (2 + 4) : 0;
+  return ((merge > rot ? merge : rot) + 2 * G * 4 + 15) / 16 * 16;
+}
+
+// What a launch reads and writes.
+struct Args {
+  const bf16 *q;
+  int64_t qs0, qs1;
+  PagedKV kv;
+  const int32_t *table, *used;
+  Shape sh;
+  Partial part;
+  QkvIn in;
+  const float *before;
+  float *after;
+  bf16 *out;
+  int out_mb;
+};
+
+// Weights: none; scores to the workspace, for a launch of their own; or scores in LDS
+// and the weights added here, where a workgroup holds the row.
+enum Weigh { kNone, kScores, kHeld };
+
+__device__ __forceinline__ int64_t out_index(const Args &a, int64_t b, int hq, int c, int dim) {
+  return a.out_mb ? frag_offset_rows(b, (int64_t)hq * dim + c, a.out_mb) : (b * a.sh.q_heads + hq) * dim + c;
+}
+
+// Row b, which holds `held` positions, n of them looked at, for KV head h: tiles lo to
+// hi - 1, of each `stride` the first kWaves. The row's result where that is all of it
+// (whole), else a partial one in `slot`. Every thread of the workgroup calls it.
+template <int D, bool kFused, int kWeigh>
+__device__ __forceinline__ void attend(const Args &a, const bf16 *__restrict__ q, const int32_t *__restrict__ table,
+                                       int64_t b, int h, int held, int n, int lo, int hi, int stride, bool whole,
+                                       int64_t slot, char *smem) {
   constexpr int kSteps = D / 32, kCh = D / 16;  // k steps of a score; channels a lane takes of a V row
-  extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int h = blockIdx.x, split = blockIdx.y;
-  const int64_t b = kFused && in.order ? constant(in.order + blockIdx.z) : blockIdx.z;
-  const int lane = threadIdx.x % kWave, wave = scalar(threadIdx.x / kWave);
+  const PagedKV &kv = a.kv;
+  const Shape &sh = a.sh;
+  const QkvIn &in = a.in;
+  const Partial &part = a.part;
+  // Opaque, so that what follows from it is not kept in registers from row to row.
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));
+  const int lane = tid % kWave, wave = scalar(tid / kWave);
   const int r = lane & 15, g = lane >> 4;
   const int G = sh.G;
 
   // Fused: loads of the partials first, so that nothing of the KV stream stands before them.
   const int ncols = (sh.q_heads + 2 * kv.heads) * D;
   const int stages = (G + 2) * (D / 4);  // threads' work staging 4 channels each
-  f32x4 pv[kMaxQkvSplits];
+  f32x4 pv[kEarlySplits];
   auto source = [&](int t) {
     const int hs = t / (D / 4), c4 = t % (D / 4) * 4;
     const int head = hs < G ? h * G + hs : (hs == G ? sh.q_heads + h : sh.q_heads + kv.heads + h);
     return in.part + b * ncols + (int64_t)head * D + c4;
   };
-  // and the angles of pair threadIdx.x % (D / 2), the pair that the thread turns.
+  // and the angles of pair tid % (D / 2), the pair that the thread turns.
   constexpr int kPairs = D / 2;
   static_assert(kThreads % kPairs == 0, "a thread turns one pair of every head it takes");
-  const int pair = threadIdx.x % kPairs, half = in.rot.rotary / 2;
+  const int pair = tid % kPairs, half = in.rot.rotary / 2;
   bool in_table = false, writes = false;
   float turn_c = 1.f, turn_s = 0.f;
   u32x4 qw[kSteps];
   if constexpr (kFused) {
-    if ((int)threadIdx.x < stages) {
-      const float *src = source(threadIdx.x);
+    if (tid < stages) {
+      const float *src = source(tid);
 #pragma unroll
-      for (int s = 0; s < kMaxQkvSplits; ++s)
+      for (int s = 0; s < kEarlySplits; ++s)
         if (s < in.splits) pv[s] = *reinterpret_cast<const f32x4 *>(src + (int64_t)s * sh.batch * ncols);
     }
     const int64_t p = constant(in.pos + b);
@@ -153,11 +196,11 @@ decode_paged_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, PagedK
   } else {
 #pragma unroll
     for (int s = 0; s < kSteps; ++s)
-      qw[s] = r < G ? *reinterpret_cast<const u32x4 *>(q + b * qs0 + (int64_t)(h * G + r) * qs1 + 32 * s + 8 * g)
+      qw[s] = r < G ? *reinterpret_cast<const u32x4 *>(q + b * a.qs0 + (int64_t)(h * G + r) * a.qs1 + 32 * s + 8 * g)
                     : u32x4{0, 0, 0, 0};
   }
 
-  const int first = split * kWaves + wave, stride = sh.splits * kWaves;  // this wave's tiles
+  const int first = lo + wave, tiles = row_tiles(n);  // this wave's tiles: first, first + stride, ...
   const int32_t *row_table = table + b * kv.width;
   const uint32_t k_off = (uint32_t)(r * D + g * 8) * 2, v_off = (uint32_t)(4 * g * D + r * kCh) * 2;
   const int page_mask = (1 << kv.shift) - 1;
@@ -171,22 +214,8 @@ decode_paged_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, PagedK
     for (int t = 0; t < 2; ++t) x.id[t] = constant(row_table + min((j + 16 * t) >> kv.shift, kv.width - 1));
     return x;
   };
-  const Ids ia = ids_of(first), ib = ids_of(first + stride);
-  const int held = constant(used + b), n = row_length(held, sh, kv);
-  const int tiles = (n + kTile - 1) / kTile;
-  if (split * kWaves >= tiles) {
-    // nothing of this row here: with one split its zeros are written
-    if (sh.splits == 1) {
-      for (int t = threadIdx.x; t < G * D; t += kThreads) {
-        const int hq = h * G + t / D, c = t % D;
-        out[out_mb ? frag_offset_rows(b, (int64_t)hq * D + c, out_mb) : (b * sh.q_heads + hq) * D + c] = 0;
-      }
-    }
-    return;
-  }
-
   // In bounds whatever the table holds: a page that does not exist, and a tile past the
-  // row's end, are read from page 0. So the table's words need not wait for the length.
+  // end, are read from page 0. So the table's words need not wait for the row's length.
   auto load = [&](Kv<D> &x, const Ids &ids, int tile) {
     const int j = tile * kTile;
 #pragma unroll
@@ -194,7 +223,7 @@ decode_paged_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, PagedK
       const int id = ids.id[t];
       x.ok[t] = (uint32_t)id < (uint32_t)kv.pages;
       const int64_t from =
-          ((((int64_t)(x.ok[t] && tile < tiles ? id : 0) * kv.heads + h) << kv.shift) + ((j + 16 * t) & page_mask)) * D;
+          ((((int64_t)(x.ok[t] && tile < hi ? id : 0) * kv.heads + h) << kv.shift) + ((j + 16 * t) & page_mask)) * D;
       const char *kb = reinterpret_cast<const char *>(kv.k + from), *vb = reinterpret_cast<const char *>(kv.v + from);
 #pragma unroll
       for (int s = 0; s < kSteps; ++s)
@@ -207,6 +236,7 @@ decode_paged_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, PagedK
   // The first two tiles are on their way before anything else is waited for, without a
   // branch: loads under one would make the wait counts fall back to waiting for all.
   Kv<D> xa, xb;
+  const Ids ia = ids_of(first), ib = ids_of(first + stride);
   load(xa, ia, first);
   load(xb, ib, first + stride);
   Ids na = ids_of(first + 2 * stride), nb = ids_of(first + 3 * stride);
@@ -223,14 +253,16 @@ decode_paged_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, PagedK
 #pragma unroll
       for (int i = 0; i < 4; ++i) sm_x[hs][c4 + i] = in.rot.f32 ? sum[i] : round_bf16(sum[i]);
     };
-    if ((int)threadIdx.x < stages) {
+    if (tid < stages) {
       f32x4 sum = pv[0];
 #pragma unroll
-      for (int s = 1; s < kMaxQkvSplits; ++s)
+      for (int s = 1; s < kEarlySplits; ++s)
         if (s < in.splits) sum += pv[s];
-      stage(threadIdx.x, sum);
+      for (int s = kEarlySplits; s < in.splits; ++s)
+        sum += *reinterpret_cast<const f32x4 *>(source(tid) + (int64_t)s * sh.batch * ncols);
+      stage(tid, sum);
     }
-    for (int t = threadIdx.x + kThreads; t < stages; t += kThreads) {
+    for (int t = tid + kThreads; t < stages; t += kThreads) {
       const float *src = source(t);
       f32x4 sum = *reinterpret_cast<const f32x4 *>(src);
       for (int s = 1; s < in.splits; ++s)
@@ -241,7 +273,7 @@ decode_paged_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, PagedK
     // Pair i of a head: the rotation's pairs first, then the channels past them in twos.
     const bool spread = pair < half && in.rot.neox;
     const int c1 = spread ? pair : 2 * pair, c2 = spread ? pair + half : 2 * pair + 1;
-    for (int hs = threadIdx.x / kPairs; hs < G + 2; hs += kThreads / kPairs) {
+    for (int hs = tid / kPairs; hs < G + 2; hs += kThreads / kPairs) {
       const float x1 = sm_x[hs][c1], x2 = sm_x[hs][c2];
       float o1 = x1, o2 = x2;
       if (in_table && hs <= G && pair < half) turn_pair(in.rot.f32, x1, x2, turn_c, turn_s, o1, o2);
@@ -254,13 +286,34 @@ decode_paged_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, PagedK
       qw[s] = r < G ? *reinterpret_cast<const u32x4 *>(&sm_rot[r][32 * s + 8 * g]) : u32x4{0, 0, 0, 0};
     // The new token's place is the row's last, if the row was not cut short.
     const int last = n - 1;
-    if (writes && held == n && (tiles - 1) / kWaves % sh.splits == split) {
+    if (writes && held == n && (tiles - 1 - lo) % stride < kWaves && hi == tiles) {
       const int id = constant(row_table + (last >> kv.shift));
       own = (uint32_t)id < (uint32_t)kv.pages;
       new_cell = ((((int64_t)(own ? id : 0) * kv.heads + h) << kv.shift) + (last & page_mask)) * D;
     }
   }
 
+  // kHeld: factors of the query heads, and the row's scores
+  float *sm_f = reinterpret_cast<float *>(smem + lds_bytes(D, G, kFused)) - 2 * G;
+  float *sm_s = sm_f + 2 * G;
+  const int sm_padded = (sh.max_len + kTile - 1) / kTile * kTile;
+  // kScores: a wave's scores of its last tiles, stored together, whole lines of one head by
+  // eight lanes. Loads and stores return in the order they were issued, so a store behind
+  // every tile holds the stream up: 64 rows of 500 to 8000 positions, 3 query heads per KV
+  // head, 137 us with one behind every tile, 133 in this way.
+  const int ring = G <= 4 ? 8 : G <= 8 ? 4 : 2;
+  float *sm_ring = sm_f + 2 * G + wave * kRingFloats;
+  int ringed = 0;
+  auto store_scores = [&](int end) {  // of the tiles before `end`
+    // 8 lanes a tile and head, four positions each
+    const int at = lane / 8 % ring, c = lane % 8 * 4;
+    const int64_t to = (int64_t)(end - (ringed - at) * stride) * kTile + c;
+    for (int gh = lane / 8 / ring; gh < G; gh += 8 / ring)
+      if (at < ringed)
+        *reinterpret_cast<f32x4 *>(part.s + (b * sh.q_heads + h * G + gh) * part.padded + to) =
+            *reinterpret_cast<const f32x4 *>(sm_ring + (at * G + gh) * kTile + c);
+    ringed = 0;
+  };
   const float sl2 = sh.scale * 1.4426950408889634f;
   float m = kEmpty, lw = 0.f;
   f32x4 l{0.f, 0.f, 0.f, 0.f}, acc[kCh];
@@ -309,13 +362,14 @@ decode_paged_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, PagedK
           for (int w = 0; w < kCh / 2; ++w) x.v[t][i][w] = ok ? x.v[t][i][w] : 0u;
         }
     }
-    if constexpr (kWeigh) {
+    if constexpr (kWeigh != kNone) {
       if (r < G) {
-        float *to = part.s + (b * sh.q_heads + h * G + r) * part.padded + (int64_t)tile * kTile + 4 * g;
+        float *to = kWeigh == kHeld ? sm_s + r * sm_padded + tile * kTile : sm_ring + (ringed * G + r) * kTile;
 #pragma unroll
         for (int t = 0; t < 2; ++t)
-          *reinterpret_cast<f32x4 *>(to + 16 * t) = f32x4{sc[t][0], sc[t][1], sc[t][2], sc[t][3]};
+          *reinterpret_cast<f32x4 *>(to + 4 * g + 16 * t) = f32x4{sc[t][0], sc[t][1], sc[t][2], sc[t][3]};
       }
+      ++ringed;
     }
     float mx = sc[0][0];
 #pragma unroll
@@ -340,7 +394,7 @@ decode_paged_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, PagedK
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const float p0 = __builtin_amdgcn_exp2f(sc[t][2 * i] - m), p1 = __builtin_amdgcn_exp2f(sc[t][2 * i + 1] - m);
-        if constexpr (kWeigh) {
+        if constexpr (kWeigh != kNone) {
           lw += p0;
           lw += p1;
         }
@@ -361,29 +415,33 @@ decode_paged_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, PagedK
   };
 
   // Tiles in pairs while there is one to load for the first of the two; the second may
-  // be past the row's end, once.
+  // be past the end, once.
   int tile = first;
-  for (; tile + 2 * stride < tiles; tile += 2 * stride) {
+  for (; tile + 2 * stride < hi; tile += 2 * stride) {
     compute(xa, tile);
     load(xa, na, tile + 2 * stride);
     compute(xb, tile + stride);
     load(xb, nb, tile + 3 * stride);
     na = ids_of(tile + 4 * stride);
     nb = ids_of(tile + 5 * stride);
+    if constexpr (kWeigh == kScores) {
+      if (ringed == ring) store_scores(tile + 2 * stride);
+    }
   }
-  if (tile < tiles) compute(xa, tile);
-  if (tile + stride < tiles) compute(xb, tile + stride);
+  if (tile < hi) compute(xa, tile);
+  if (tile + stride < hi) compute(xb, tile + stride);
+  if constexpr (kWeigh == kScores) store_scores(tile + (tile < hi) * stride + (tile + stride < hi) * stride);
 
   if constexpr (kFused) {
     // Stored behind the stream, which does not wait for it.
-    if (own && (int)threadIdx.x < D / 4) {
-      const int side = threadIdx.x / (D / 8), c = threadIdx.x % (D / 8) * 8;
+    if (own && tid < D / 4) {
+      const int side = tid / (D / 8), c = tid % (D / 8) * 8;
       *reinterpret_cast<u32x4 *>((side ? kv.v : kv.k) + new_cell + c) =
           *reinterpret_cast<const u32x4 *>(&sm_rot[G + side][c]);
     }
     __syncthreads();  // sm_rot is done with
   }
-  if constexpr (kWeigh) {
+  if constexpr (kWeigh != kNone) {
     lw += xor_lanes<16>(lw);
     lw += xor_lanes<32>(lw);
   }
@@ -404,7 +462,7 @@ decode_paged_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, PagedK
     }
   }
   __syncthreads();
-  for (int t = threadIdx.x; t < G * D; t += kThreads) {
+  for (int t = tid; t < G * D; t += kThreads) {
     const int gh = t / D, c = t % D;
     float mx = sm_m[gh];
 #pragma unroll
@@ -418,119 +476,250 @@ decode_paged_kernel(const bf16 *__restrict__ q, int64_t qs0, int64_t qs1, PagedK
       o += sm_o[(w * G + gh) * D + c] * f;
     }
     const int hq = h * G + gh;
-    const int64_t at = (b * sh.q_heads + hq) * sh.splits + split;
-    if (sh.splits == 1) {
-      out[out_mb ? frag_offset_rows(b, (int64_t)hq * D + c, out_mb) : (b * sh.q_heads + hq) * D + c] =
-          (bf16)f32_to_bf16(lsum == 0.f ? 0.f : o / lsum);
+    if (whole) {
+      a.out[out_index(a, b, hq, c, D)] = (bf16)f32_to_bf16(lsum == 0.f ? 0.f : o / lsum);
+      if constexpr (kWeigh == kScores) {
+        if (c == 0) {
+          part.rm[b * sh.q_heads + hq] = mx;
+          part.rw[b * sh.q_heads + hq] = wsum;
+        }
+      }
+      if constexpr (kWeigh == kHeld) {
+        if (c == 0) {
+          sm_f[gh] = mx;
+          sm_f[G + gh] = wsum == 0.f ? 0.f : 1.f / wsum;
+        }
+      }
     } else {
+      const int64_t at = slot * G + gh;
       part.o[at * D + c] = o;
+      if (c == 0) {
+        part.m[at] = mx;
+        part.l[at] = lsum;
+        if constexpr (kWeigh != kNone) part.lw[at] = wsum;
+      }
     }
-    if (c == 0 && (kWeigh || sh.splits > 1)) {
-      part.m[at] = mx;
-      part.l[at] = lsum;
-      if constexpr (kWeigh) part.lw[at] = wsum;
+  }
+  if constexpr (kWeigh == kHeld) {
+    __syncthreads();
+    // Four positions a thread; a row's positions in the weights are a multiple of 16.
+    const int64_t row = (b * kv.heads + h) * ((int64_t)kv.width << kv.shift);
+    for (int j = 4 * tid; j < n; j += 4 * kThreads) {
+      const f32x4 old = *reinterpret_cast<const f32x4 *>(a.before + row + j);
+      float w[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int gh = 0; gh < G; ++gh) {
+        const f32x4 sc = *reinterpret_cast<const f32x4 *>(sm_s + gh * sm_padded + j);
+        const float mg = sm_f[gh], f = sm_f[G + gh];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] += __builtin_amdgcn_exp2f(sc[i] - mg) * f;
+      }
+      if (j + 4 <= n) {
+        *reinterpret_cast<f32x4 *>(a.after + row + j) = f32x4{old[0] + w[0], old[1] + w[1], old[2] + w[2], old[3] + w[3]};
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (j + i < n) a.after[row + j + i] = old[i] + w[i];
+      }
     }
   }
 }
 
-// grid (groups of query heads, batch), one thread per channel: the splits'
-// partials by log-sum-exp, those of kBatch splits requested together.
-constexpr int kCombineHeads = 2;
-template <int D, int kBatch>
+// grid (kv heads, splits, rows): a row's tiles go to the waves of all its splits in
+// turn, so that nothing but the end of the loop waits for its length. Or grid (kv
+// heads, shares): the tiles of all rows, one row after the other, are cut evenly, so
+// that every workgroup streams as many bytes whatever the rows' lengths. A CU alone
+// reads some 35 GB/s, so the rate of the whole falls with its emptiest CU; a workgroup
+// adds up the rows' tiles itself.
+// Registers: four waves per SIMD where splits give a CU four workgroups (D = 64). With
+// scores to store that would spill (145 us for the 133 above), and shares give a CU two.
+template <int D, bool kFused, int kWeigh, bool kShares>
+__global__ void __launch_bounds__(kThreads, D == 128 || kShares ? 2 : kWeigh == kScores ? 3 : 4)
+decode_paged_kernel(const bf16 *__restrict__ q, const int32_t *__restrict__ table, Args a) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int h = blockIdx.x;
+  if constexpr (!kShares) {
+    const int split = blockIdx.y, splits = a.sh.splits;
+    const int64_t b = kFused && a.in.order ? constant(a.in.order + blockIdx.z) : blockIdx.z;
+    const int held = constant(a.used + b), n = row_length(held, a.sh, a.kv), tiles = row_tiles(n);
+    if (splits > 1 && split * kWaves >= tiles) return;
+    attend<D, kFused, kWeigh>(a, q, table, b, h, held, n, split * kWaves, tiles, splits * kWaves,
+                              splits == 1 || tiles <= kWaves, (b * splits + split) * a.kv.heads + h, smem);
+  } else {
+    const int lane = threadIdx.x % kWave, batch = a.sh.batch;
+    uint32_t total = 0;
+    for (int b = lane; b < batch; b += kWave) total += row_tiles(row_length(a.used[b], a.sh, a.kv));
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) total += shfl_xor(total, d);
+    total = scalar(total);
+    const uint32_t share = share_tiles(total, a.sh);
+    const uint32_t start = min(blockIdx.y * share, total), end = min(start + share, total);
+    const bool writer = h == 0 && blockIdx.y == 0 && threadIdx.x < kWave;
+    uint32_t before = 0, row_off = 0;
+    int row = batch;  // the row that holds tile `start`, and the tiles before it
+    for (int b0 = 0; b0 < batch && (row == batch || writer); b0 += kWave) {
+      const int b = b0 + lane;
+      const uint32_t mine = b < batch ? row_tiles(row_length(a.used[b], a.sh, a.kv)) : 0;
+      uint32_t upto = mine;
+#pragma unroll
+      for (int d = 1; d < kWave; d *= 2) {
+        const uint32_t y = __shfl_up(upto, d, kWave);
+        upto += lane >= d ? y : 0;
+      }
+      if (writer && b < batch) a.part.off[b] = (int)(before + upto - mine);
+      const uint64_t there = __ballot(start < before + upto);
+      if (row == batch && there) {
+        const int at = __builtin_ctzll(there);
+        row = b0 + at;
+        row_off = before + __shfl(upto - mine, at, kWave);
+      }
+      before += __shfl(upto, kWave - 1, kWave);
+    }
+    if (writer && lane == 0) a.part.off[batch] = (int)total;
+    if (start >= end) return;  // more shares than the rows have tiles for
+    row = scalar(row);
+    row_off = scalar(row_off);
+    while (row_off < end) {  // uniform: every wave has the same numbers
+      const int held = constant(a.used + row), n = row_length(held, a.sh, a.kv), tiles = row_tiles(n);
+      if (tiles) {
+        const int lo = row_off < start ? (int)(start - row_off) : 0, hi = (int)min((uint32_t)tiles, end - row_off);
+        attend<D, kFused, kWeigh>(a, q, table, row, h, held, n, lo, hi, kWaves, lo == 0 && hi == tiles,
+                                  ((int64_t)blockIdx.y * a.kv.heads + h) * 2 + (lo ? 0 : 1), smem);
+        __syncthreads();  // the next row takes the same LDS
+      }
+      row_off += tiles;
+      ++row;
+    }
+  }
+}
+
+// The partial results of a row: `count` of them, 0 of an empty row, 1 where a workgroup
+// held it all and wrote its result.
+struct Pieces {
+  int n, count;
+  int64_t first;  // shares: the first one; splits: b * splits
+  bool shares;
+};
+__device__ __forceinline__ Pieces pieces_of(const Args &a, int64_t b) {
+  Pieces x;
+  x.n = row_length(a.used[b], a.sh, a.kv);
+  x.shares = a.sh.shares > 0;
+  if (x.shares) {
+    const uint32_t at = a.part.off[b], next = a.part.off[b + 1], share = share_tiles(a.part.off[a.sh.batch], a.sh);
+    x.first = at / share;
+    x.count = next > at ? (int)((next - 1) / share - at / share) + 1 : 0;
+  } else {
+    x.first = b * a.sh.splits;
+    x.count = min(a.sh.splits, (row_tiles(x.n) + kWaves - 1) / kWaves);
+  }
+  return x;
+}
+// Query head gh of KV head h in the row's i-th piece (its first share began the row).
+__device__ __forceinline__ int64_t slot_of(const Args &a, const Pieces &x, int i, int h, int gh) {
+  const int64_t at = (x.first + i) * a.kv.heads + h;
+  return (x.shares ? 2 * at + (i ? 0 : 1) : at) * a.sh.G + gh;
+}
+
+// Rows in several pieces: their results by log-sum-exp; rows that hold nothing: zeros.
+// grid (groups of query heads, batch), one thread per channel; the results of kBatch
+// pieces are requested together.
+constexpr int kCombineHeads = 2, kBatch = 8;
+template <int D>
 __global__ void __launch_bounds__(kCombineHeads *D)
-decode_paged_combine_kernel(const int32_t *__restrict__ used, Shape sh, PagedKV kv, Partial part,
-                            bf16 *__restrict__ out, int out_mb) {
+decode_paged_combine_kernel(Args a) {
   const int hq = blockIdx.x * kCombineHeads + threadIdx.x / D;
-  if (hq >= sh.q_heads) return;
   const int64_t b = blockIdx.y;
-  const int c = threadIdx.x % D;
-  const int64_t base = (b * sh.q_heads + hq) * sh.splits;
-  float ms[kBatch], ls[kBatch], os[kBatch];
-  auto load = [&](int s0) {
+  const Pieces x = pieces_of(a, b);
+  if (hq >= a.sh.q_heads || x.count == 1) return;
+  const int c = threadIdx.x % D, h = hq / a.sh.G, gh = hq % a.sh.G;
+  const Partial &part = a.part;
+  // The first results need not wait for the row's length: every split has a slot, and
+  // what a split past the row's end has there is not looked at.
+  const int slots = x.shares ? x.count : a.sh.splits;
+  float mx = kEmpty, lsum = 0.f, o = 0.f;
+  for (int s0 = 0; s0 < x.count; s0 += kBatch) {
+    float ms[kBatch], ls[kBatch], os[kBatch], to = mx;
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
-      const int64_t at = base + min(s0 + i, sh.splits - 1);
+      const int64_t at = slot_of(a, x, min(s0 + i, slots - 1), h, gh);
       ms[i] = part.m[at];
       ls[i] = part.l[at];
       os[i] = part.o[at * D + c];
     }
-  };
-  load(0);
-  const int valid = row_splits(row_length(used[b], sh, kv), sh);
-  float mx = kEmpty;
 #pragma unroll
-  for (int i = 0; i < kBatch; ++i) mx = fmaxf(mx, i < valid ? ms[i] : kEmpty);
-  for (int s = kBatch; s < valid; ++s) mx = fmaxf(mx, part.m[base + s]);
-  float lsum = 0.f, o = 0.f;
-  for (int s0 = 0; s0 < valid; s0 += kBatch) {
-    if (s0) load(s0);
+    for (int i = 0; i < kBatch; ++i) to = fmaxf(to, s0 + i < x.count ? ms[i] : kEmpty);
+    const float f0 = __builtin_amdgcn_exp2f(mx - to);
+    lsum *= f0;
+    o *= f0;
+    mx = to;
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
-      // a split past the row's end was never written: selected away, not scaled
-      const bool live = s0 + i < valid;
+      const bool live = s0 + i < x.count;
       const float f = live ? __builtin_amdgcn_exp2f(ms[i] - mx) : 0.f;
       lsum += live ? ls[i] * f : 0.f;
       o += live ? os[i] * f : 0.f;
     }
   }
-  const int64_t at = out_mb ? frag_offset_rows(b, (int64_t)hq * D + c, out_mb) : (b * sh.q_heads + hq) * D + c;
-  out[at] = (bf16)f32_to_bf16(lsum == 0.f ? 0.f : o / lsum);
+  a.out[out_index(a, b, hq, c, D)] = (bf16)f32_to_bf16(lsum == 0.f ? 0.f : o / lsum);
 }
 
 // after[b, h, j] = before[b, h, j] + sum over the KV head's query heads of their
-// probability of position j, j < the row's length. A thread four positions. With
-// splits the first workgroup of a (row, KV head) also joins their results, in place of
-// the launch above.
+// probability of position j, j < the row's length. A thread four positions. The first
+// workgroup of a (row, KV head) also joins the pieces' results, as the launch above.
 constexpr int kWeighThreads = 256, kWeighSpan = 4 * kWeighThreads, kAhead = 4;
 template <int D>
 __global__ void __launch_bounds__(kWeighThreads)
-weigh_kernel(const int32_t *__restrict__ used, Shape sh, PagedKV kv, Partial part, const float *before, float *after,
-             bf16 *__restrict__ out, int out_mb) {
+weigh_kernel(Args a) {
   __shared__ float sm_m[kMaxGroups], sm_f[kMaxGroups];
-  const int h = blockIdx.y, G = sh.G;
+  const int h = blockIdx.y, G = a.sh.G;
   const int64_t b = blockIdx.z;
+  const Partial &part = a.part;
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  const int n = row_length(used[b], sh, kv), valid = row_splits(n, sh);
-  const int j = (blockIdx.x * kWeighThreads + threadIdx.x) * 4;
-  const bool joins = blockIdx.x == 0 && sh.splits > 1;
-  if ((int)blockIdx.x * kWeighSpan >= n && !joins) return;
+  const int n = row_length(a.used[b], a.sh, a.kv), j = (blockIdx.x * kWeighThreads + threadIdx.x) * 4;
+  if (blockIdx.x && (int)blockIdx.x * kWeighSpan >= n) return;
   // The scores and weights of this thread's positions are on their way while the
   // heads' sums are joined. The buffers hold a multiple of 16 positions a row.
-  const float *sc = part.s + (b * sh.q_heads + h * G) * part.padded + j;
-  const int64_t at = (b * kv.heads + h) * ((int64_t)kv.width << kv.shift) + j;
+  const float *sc = part.s + (b * a.sh.q_heads + h * G) * part.padded + j;
+  const int64_t at = (b * a.kv.heads + h) * ((int64_t)a.kv.width << a.kv.shift) + j;
   f32x4 s[kAhead], old{0.f, 0.f, 0.f, 0.f};
   if (j < n) {
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) s[i] = *reinterpret_cast<const f32x4 *>(sc + min(i, G - 1) * part.padded);
-    old = *reinterpret_cast<const f32x4 *>(before + at);
+    old = *reinterpret_cast<const f32x4 *>(a.before + at);
   }
+  const Pieces x = pieces_of(a, b);
   for (int gh = wave; gh < G; gh += kWeighThreads / kWave) {
-    const int64_t base = (b * sh.q_heads + h * G + gh) * sh.splits;
     float mx = kEmpty, l = 0.f;
-    for (int s0 = lane; s0 < valid; s0 += kWave) mx = fmaxf(mx, part.m[base + s0]);
+    if (x.count == 1) {
+      mx = part.rm[b * a.sh.q_heads + h * G + gh];
+      l = part.rw[b * a.sh.q_heads + h * G + gh];
+    } else {
+      for (int i = lane; i < x.count; i += kWave) mx = fmaxf(mx, part.m[slot_of(a, x, i, h, gh)]);
 #pragma unroll
-    for (int d = 1; d < kWave; d *= 2) mx = fmaxf(mx, shfl_xor(mx, d));
-    for (int s0 = lane; s0 < valid; s0 += kWave) l += part.lw[base + s0] * __builtin_amdgcn_exp2f(part.m[base + s0] - mx);
-    l = wave_sum(l);
+      for (int d = 1; d < kWave; d *= 2) mx = fmaxf(mx, shfl_xor(mx, d));
+      for (int i = lane; i < x.count; i += kWave) {
+        const int64_t slot = slot_of(a, x, i, h, gh);
+        l += part.lw[slot] * __builtin_amdgcn_exp2f(part.m[slot] - mx);
+      }
+      l = wave_sum(l);
+    }
     if (lane == 0) {
       sm_m[gh] = mx;
       sm_f[gh] = l == 0.f ? 0.f : 1.f / l;
     }
   }
   __syncthreads();
-  if (joins) {
+  if (blockIdx.x == 0 && x.count != 1) {
     for (int t = threadIdx.x; t < G * D; t += kWeighThreads) {
-      const int gh = t / D, c = t % D, hq = h * G + gh;
-      const int64_t base = (b * sh.q_heads + hq) * sh.splits;
+      const int gh = t / D, c = t % D;
       float lsum = 0.f, o = 0.f;
 #pragma unroll 4
-      for (int i = 0; i < valid; ++i) {
-        const float f = __builtin_amdgcn_exp2f(part.m[base + i] - sm_m[gh]);
-        lsum += part.l[base + i] * f;
-        o += part.o[(base + i) * D + c] * f;
+      for (int i = 0; i < x.count; ++i) {
+        const int64_t slot = slot_of(a, x, i, h, gh);
+        const float f = __builtin_amdgcn_exp2f(part.m[slot] - sm_m[gh]);
+        lsum += part.l[slot] * f;
+        o += part.o[slot * D + c] * f;
       }
-      out[out_mb ? frag_offset_rows(b, (int64_t)hq * D + c, out_mb) : (b * sh.q_heads + hq) * D + c] =
-          (bf16)f32_to_bf16(lsum == 0.f ? 0.f : o / lsum);
+      a.out[out_index(a, b, h * G + gh, c, D)] = (bf16)f32_to_bf16(lsum == 0.f ? 0.f : o / lsum);
     }
   }
   if (j >= n) return;
@@ -545,115 +734,144 @@ weigh_kernel(const int32_t *__restrict__ used, Shape sh, PagedKV kv, Partial par
       if (g0 + i >= G) break;
       const float m = sm_m[g0 + i], f = sm_f[g0 + i];
 #pragma unroll
-      for (int x = 0; x < 4; ++x) w[x] += __builtin_amdgcn_exp2f(s[i][x] - m) * f;
+      for (int y = 0; y < 4; ++y) w[y] += __builtin_amdgcn_exp2f(s[i][y] - m) * f;
     }
   }
   if (j + 4 <= n) {
-    *reinterpret_cast<f32x4 *>(after + at) = f32x4{old[0] + w[0], old[1] + w[1], old[2] + w[2], old[3] + w[3]};
+    *reinterpret_cast<f32x4 *>(a.after + at) = f32x4{old[0] + w[0], old[1] + w[1], old[2] + w[2], old[3] + w[3]};
   } else {
 #pragma unroll
-    for (int x = 0; x < 4; ++x)
-      if (j + x < n) after[at + x] = old[x] + w[x];
+    for (int y = 0; y < 4; ++y)
+      if (j + y < n) a.after[at + y] = old[y] + w[y];
   }
 }
 
 struct Call {
-  int64_t batch, q_heads, kv_heads, head_dim, width, pages, page, max_len, num_splits;
+  int64_t batch, q_heads, kv_heads, head_dim, width, pages, page, max_len, num_splits, num_shares;
 };
 
 int64_t padded_scores(int64_t max_len) { return align_up(max_len, kTile); }
 
-int64_t workspace_bytes(int64_t batch, int64_t q_heads, int64_t head_dim, int64_t max_len, int64_t splits,
-                        bool weighed) {
-  if (splits <= 1 && !weighed) return 0;
-  const int64_t n = batch * q_heads * splits;
-  return (splits > 1 ? n * head_dim * 4 : 0) + (weighed ? 3 : 2) * align_up(n * 4, 256) +
-         (weighed ? batch * q_heads * padded_scores(max_len) * 4 : 0);
+// Scores that a workgroup keeps: three of them and the merge fit a CU's 160 KB of LDS.
+constexpr int64_t kHeldBytes = 32 << 10;
+bool scores_held(int64_t groups, int64_t max_len) { return groups * padded_scores(max_len) * 4 <= kHeldBytes; }
+
+// Weights added by the workgroup that holds the row.
+bool weighs_held(int64_t groups, int64_t max_len, int64_t splits, int64_t shares) {
+  return splits == 1 && !shares && scores_held(groups, max_len);
+}
+
+int64_t slot_count(int64_t batch, int64_t kv_heads, int64_t splits, int64_t shares) {
+  return shares ? shares * kv_heads * 2 : splits > 1 ? batch * splits * kv_heads : 0;
+}
+
+int64_t workspace_bytes(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t max_len,
+                        int64_t splits, int64_t shares, bool weighed) {
+  const int64_t n = slot_count(batch, kv_heads, splits, shares) * (q_heads / kv_heads);
+  const bool scores = weighed && !weighs_held(q_heads / kv_heads, max_len, splits, shares);
+  return (shares ? align_up((batch + 1) * 4, 256) : 0) + align_up(n * head_dim * 4, 256) + 2 * align_up(n * 4, 256) +
+         (scores ? align_up(n * 4, 256) + 2 * align_up(batch * q_heads * 4, 256) +
+                       batch * q_heads * padded_scores(max_len) * 4
+                 : 0);
+}
+
+bool pieces_ok(int64_t splits, int64_t shares) {
+  return splits >= 1 && splits <= 1024 && shares >= 0 && shares <= 65535 && (splits == 1 || shares == 0);
 }
 
 // Argument checks of both entry points; *run false where nothing is to launch.
 int check_call(const Call &c, bool *run) {
   *run = false;
   LM_REQUIRE(c.batch >= 0 && c.q_heads > 0 && c.kv_heads > 0 && c.q_heads % c.kv_heads == 0 && c.max_len > 0 &&
-             c.num_splits > 0 && c.num_splits <= 1024 && c.max_len < ((int64_t)1 << 30) && c.batch <= 65535 &&
+             pieces_ok(c.num_splits, c.num_shares) && c.max_len < ((int64_t)1 << 30) && c.batch <= 65535 &&
              c.kv_heads <= 65535);
   const int status = paged_args_ok(c.width, c.pages, c.page, c.head_dim);
   if (status != LM_OK) return status;
   if (c.q_heads / c.kv_heads > kMaxGroups) return LM_EUNSUPPORTED;
+  // tiles of all rows are counted in 32 bits
+  LM_REQUIRE(c.batch <= ((int64_t)1 << 31) / cdiv(c.max_len, kTile));
   *run = c.batch > 0;
   return LM_OK;
 }
 
-template <int D, bool kFused, bool kWeigh>
-int launch_sized(const Call &c, const bf16 *q, int64_t qs0, int64_t qs1, const PagedKV &kv, const int32_t *table,
-                 const int32_t *used, const Shape &sh, const Partial &part, const QkvIn &in, bf16 *out, int out_mb,
-                 const float *before, float *after, hipStream_t s) {
-  // KV heads fastest: workgroups go to the XCDs in turn, so that each XCD has a share
-  // of every split.
-  const dim3 grid((unsigned)c.kv_heads, (unsigned)sh.splits, (unsigned)c.batch);
-  const size_t merge = (size_t)kWaves * sh.G * (D + 3) * 4;
-  const size_t rot = kFused ? (size_t)(sh.G + 2) * D * (2 + 4) : 0;
-  decode_paged_kernel<D, kFused, kWeigh><<<grid, kWaves * kWave, merge > rot ? merge : rot, s>>>(
-      q, qs0, qs1, kv, table, used, sh, part, in, out, out_mb);
+template <int D, bool kFused, int kWeigh, bool kShares>
+int launch_sized(const Call &c, const Args &a, hipStream_t s) {
+  // KV heads fastest: workgroups go to the XCDs in turn, so that each XCD has some of
+  // every row.
+  const dim3 grid = kShares ? dim3((unsigned)c.kv_heads, (unsigned)a.sh.shares)
+                            : dim3((unsigned)c.kv_heads, (unsigned)a.sh.splits, (unsigned)c.batch);
+  const int64_t lds = lds_bytes(D, a.sh.G, kFused) + (kWeigh == kHeld     ? a.sh.G * padded_scores(a.sh.max_len) * 4
+                                                      : kWeigh == kScores ? kWaves * kRingFloats * 4
+                                                                          : 0);
+  decode_paged_kernel<D, kFused, kWeigh, kShares><<<grid, kThreads, lds, s>>>(a.q, a.table, a);
   LM_CHECK_LAUNCH();
-  if (!kWeigh && sh.splits > 1) {
-    auto combine = sh.splits <= 4   ? decode_paged_combine_kernel<D, 4>
-                   : sh.splits <= 8 ? decode_paged_combine_kernel<D, 8>
-                                    : decode_paged_combine_kernel<D, 16>;
-    combine<<<dim3((unsigned)cdiv(c.q_heads, kCombineHeads), (unsigned)c.batch), kCombineHeads * D, 0, s>>>(
-        used, sh, kv, part, out, out_mb);
+  if (kWeigh == kNone && (kShares || a.sh.splits > 1)) {
+    decode_paged_combine_kernel<D><<<dim3((unsigned)cdiv(c.q_heads, kCombineHeads), (unsigned)c.batch),
+                                     kCombineHeads * D, 0, s>>>(a);
     LM_CHECK_LAUNCH();
   }
-  if (kWeigh) {
-    weigh_kernel<D><<<dim3((unsigned)cdiv(sh.max_len, kWeighSpan), (unsigned)c.kv_heads, (unsigned)c.batch),
-                      kWeighThreads, 0, s>>>(used, sh, kv, part, before, after, out, out_mb);
+  if (kWeigh == kScores) {
+    weigh_kernel<D><<<dim3((unsigned)cdiv(a.sh.max_len, kWeighSpan), (unsigned)c.kv_heads, (unsigned)c.batch),
+                      kWeighThreads, 0, s>>>(a);
     LM_CHECK_LAUNCH();
   }
   return LM_OK;
 }
 
-int launch_decode_paged(const Call &c, const void *q, int64_t qs0, int64_t qs1, void *k_pages, void *v_pages,
-                        const int32_t *table, const int32_t *used, float scale, const QkvIn &in, void *out,
-                        int out_mb, const float *before, float *after, void *workspace, int64_t workspace_bytes_,
-                        void *stream) {
-  LM_REQUIRE(aligned16(k_pages) && aligned16(v_pages) && (before == nullptr) == (after == nullptr) &&
-             aligned16(before) && aligned16(after));
-  const bool weighed = after != nullptr;
-  // No row is longer than the table; what the plan allows beyond it needs no split.
-  const int64_t room = c.width * c.page, longest = c.max_len < room ? c.max_len : room;
-  const int64_t need = workspace_bytes(c.batch, c.q_heads, c.head_dim, c.max_len, c.num_splits, weighed);
+int launch_decode_paged(const Call &c, Args a, void *workspace, int64_t workspace_bytes_, void *stream) {
+  LM_REQUIRE(aligned16(a.kv.k) && aligned16(a.kv.v) && (a.before == nullptr) == (a.after == nullptr) &&
+             aligned16(a.before) && aligned16(a.after));
+  const bool weighed = a.after != nullptr;
+  const int64_t G = c.q_heads / c.kv_heads;
+  const bool held = weighed && weighs_held(G, c.max_len, c.num_splits, c.num_shares);
+  const int64_t need = workspace_bytes(c.batch, c.q_heads, c.kv_heads, c.head_dim, c.max_len, c.num_splits,
+                                       c.num_shares, weighed);
   if (need > 0 && (!workspace || workspace_bytes_ < need)) return LM_EWORKSPACE;
   LM_REQUIRE(need == 0 || aligned16(workspace));
-  const int64_t splits = c.num_splits < cdiv(longest, kTile) ? c.num_splits : cdiv(longest, kTile);
-  Partial part{nullptr, nullptr, nullptr, nullptr, nullptr, padded_scores(c.max_len)};
-  const int64_t n = c.batch * c.q_heads * splits;
+  // No row is longer than the table.
+  const int64_t room = c.width * c.page, longest = c.max_len < room ? c.max_len : room;
+  a.sh.q_heads = (int)c.q_heads;
+  a.sh.G = (int)G;
+  a.sh.max_len = (int)longest;
+  a.sh.splits = (int)c.num_splits;
+  a.sh.shares = (int)c.num_shares;
+  a.sh.batch = (int)c.batch;
+  a.kv.pages = c.pages;
+  a.kv.width = (int)c.width;
+  a.kv.shift = page_shift(c.page);
+  a.kv.heads = (int)c.kv_heads;
+  a.part = Partial{};
+  a.part.padded = padded_scores(c.max_len);
   char *w = static_cast<char *>(workspace);
-  auto take = [&](int64_t bytes) {
-    float *at = reinterpret_cast<float *>(w);
-    w += bytes;
-    return at;
+  auto take = [&](int64_t count) {
+    char *at = w;
+    w += align_up(count * 4, 256);
+    return reinterpret_cast<float *>(at);
   };
-  if (weighed) part.s = take(c.batch * c.q_heads * part.padded * 4);
-  if (splits > 1) part.o = take(n * c.head_dim * 4);
-  if (splits > 1 || weighed) {
-    part.m = take(align_up(n * 4, 256));
-    part.l = take(align_up(n * 4, 256));
-    if (weighed) part.lw = take(align_up(n * 4, 256));
+  const int64_t n = slot_count(c.batch, c.kv_heads, c.num_splits, c.num_shares) * G;
+  if (c.num_shares) a.part.off = reinterpret_cast<int32_t *>(take(c.batch + 1));
+  a.part.o = take(n * c.head_dim);
+  a.part.m = take(n);
+  a.part.l = take(n);
+  if (weighed && !held) {
+    a.part.lw = take(n);
+    a.part.rm = take(c.batch * c.q_heads);
+    a.part.rw = take(c.batch * c.q_heads);
+    a.part.s = take(c.batch * c.q_heads * a.part.padded);
   }
-  const PagedKV kv{(bf16 *)k_pages, (bf16 *)v_pages, c.pages, (int)c.width, page_shift(c.page), (int)c.kv_heads};
-  const int G = (int)(c.q_heads / c.kv_heads);
-  const Shape sh{(int)c.q_heads, G, (int)longest, (int)splits, scale, c.batch};
-  auto go = [&](auto dim, auto fused, auto weigh) {
-    return launch_sized<decltype(dim)::value, decltype(fused)::value, decltype(weigh)::value>(
-        c, (const bf16 *)q, qs0, qs1, kv, table, used, sh, part, in, (bf16 *)out, out_mb, before, after,
-        (hipStream_t)stream);
+  hipStream_t s = (hipStream_t)stream;
+  auto run = [&](auto dim, auto fused) {
+    constexpr int D = decltype(dim)::value;
+    constexpr bool kFused = decltype(fused)::value;
+    if (held) return launch_sized<D, kFused, kHeld, false>(c, a, s);
+    if constexpr (!kFused) {
+      if (c.num_shares)
+        return weighed ? launch_sized<D, false, kScores, true>(c, a, s) : launch_sized<D, false, kNone, true>(c, a, s);
+    }
+    return weighed ? launch_sized<D, kFused, kScores, false>(c, a, s) : launch_sized<D, kFused, kNone, false>(c, a, s);
   };
-  auto sized = [&](auto fused, auto weigh) {
-    return c.head_dim == 64 ? go(std::integral_constant<int, 64>{}, fused, weigh)
-                            : go(std::integral_constant<int, 128>{}, fused, weigh);
-  };
-  if (in.part) return weighed ? sized(std::true_type{}, std::true_type{}) : sized(std::true_type{}, std::false_type{});
-  return weighed ? sized(std::false_type{}, std::true_type{}) : sized(std::false_type{}, std::false_type{});
+  auto sized = [&](auto dim) { return a.in.part ? run(dim, std::true_type{}) : run(dim, std::false_type{}); };
+  return c.head_dim == 64 ? sized(std::integral_constant<int, 64>{}) : sized(std::integral_constant<int, 128>{});
 }
 
 }  // namespace
@@ -661,44 +879,63 @@ int launch_decode_paged(const Call &c, const void *q, int64_t qs0, int64_t qs1, 
 
 using namespace lm;
 
-extern "C" int lm_flash_decode_paged_workspace_size(int64_t batch, int64_t q_heads, int64_t head_dim, int64_t max_len,
-                                                    int64_t num_splits, int weighed, int64_t *bytes) {
-  LM_REQUIRE(bytes && batch >= 0 && q_heads > 0 && max_len > 0 && num_splits > 0);
+extern "C" int lm_flash_decode_paged_workspace_size(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                                                    int64_t max_len, int64_t num_splits, int64_t num_shares,
+                                                    int weighed, int64_t *bytes) {
+  LM_REQUIRE(bytes && batch >= 0 && q_heads > 0 && kv_heads > 0 && q_heads % kv_heads == 0 && max_len > 0 &&
+             pieces_ok(num_splits, num_shares));
   if (head_dim != 64 && head_dim != 128) return LM_EUNSUPPORTED;
-  *bytes = workspace_bytes(batch, q_heads, head_dim, max_len, num_splits, weighed != 0);
+  *bytes = workspace_bytes(batch, q_heads, kv_heads, head_dim, max_len, num_splits, num_shares, weighed != 0);
   return LM_OK;
 }
 
 extern "C" int lm_flash_decode_paged(const lm_flash_decode_paged_args *args, void *stream) {
   LM_REQUIRE(args);
-  const auto &a = *args;
-  const Call c{a.batch, a.q_heads, a.kv_heads, a.head_dim, a.width, a.pages, a.page, a.max_len, a.num_splits};
+  const auto &x = *args;
+  const Call c{x.batch, x.q_heads, x.kv_heads, x.head_dim, x.width, x.pages, x.page, x.max_len, x.num_splits, x.num_shares};
   bool run;
   const int status = check_call(c, &run);
   if (status != LM_OK || !run) return status;
-  LM_REQUIRE(a.q && a.k_pages && a.v_pages && a.block_table && a.used && a.out);
-  LM_REQUIRE(aligned16(a.q) && a.qs0 % 8 == 0 && a.qs1 % 8 == 0);
-  const QkvIn in{nullptr, 0, {nullptr, 0, 0, false, false}, nullptr, nullptr, nullptr};
-  return launch_decode_paged(c, a.q, a.qs0, a.qs1, const_cast<void *>(a.k_pages), const_cast<void *>(a.v_pages),
-                             a.block_table, a.used, (float)a.scale, in, a.out, 0, a.weights, a.weights_out, a.workspace,
-                             a.workspace_bytes, stream);
+  LM_REQUIRE(x.q && x.k_pages && x.v_pages && x.block_table && x.used && x.out);
+  LM_REQUIRE(aligned16(x.q) && x.qs0 % 8 == 0 && x.qs1 % 8 == 0);
+  Args a{};
+  a.q = (const bf16 *)x.q;
+  a.qs0 = x.qs0;
+  a.qs1 = x.qs1;
+  a.kv.k = (bf16 *)const_cast<void *>(x.k_pages);
+  a.kv.v = (bf16 *)const_cast<void *>(x.v_pages);
+  a.table = x.block_table;
+  a.used = x.used;
+  a.sh.scale = (float)x.scale;
+  a.before = x.weights;
+  a.after = x.weights_out;
+  a.out = (bf16 *)x.out;
+  return launch_decode_paged(c, a, x.workspace, x.workspace_bytes, stream);
 }
 
 extern "C" int lm_flash_decode_paged_qkv(const lm_flash_decode_paged_qkv_args *args, void *stream) {
   LM_REQUIRE(args);
-  const auto &a = *args;
-  const Call c{a.batch, a.q_heads, a.kv_heads, a.head_dim, a.width, a.pages, a.page, a.max_len, a.num_splits};
+  const auto &x = *args;
+  const Call c{x.batch, x.q_heads, x.kv_heads, x.head_dim, x.width, x.pages, x.page, x.max_len, x.num_splits, 0};
   bool run;
   const int status = check_call(c, &run);
   if (status != LM_OK) return status;
-  LM_REQUIRE(a.qkv_splits >= 1);
-  if (a.qkv_splits > kMaxQkvSplits || (a.frag_out && a.batch > 128)) return LM_EUNSUPPORTED;
+  LM_REQUIRE(x.qkv_splits >= 1);
+  if (x.qkv_splits > kMaxQkvSplits || (x.frag_out && x.batch > 128)) return LM_EUNSUPPORTED;
   if (!run) return LM_OK;
-  LM_REQUIRE(a.qkv_partials && a.positions && a.k_pages && a.v_pages && a.block_table && a.used && a.out);
-  LM_REQUIRE(aligned16(a.qkv_partials) && rotation_ok(a.cos_sin, a.table_len, a.rotary, a.head_dim));
-  const Rotation rot{a.cos_sin, a.table_len, (int)a.rotary, a.table_f32 != 0, a.neox != 0};
-  const QkvIn in{a.qkv_partials, (int)a.qkv_splits, rot, a.positions, a.active, a.row_order};
-  return launch_decode_paged(c, nullptr, 0, 0, a.k_pages, a.v_pages, a.block_table, a.used, (float)a.scale, in, a.out,
-                             a.frag_out ? frag_row_blocks(a.batch) : 0, a.weights, a.weights_out, a.workspace,
-                             a.workspace_bytes, stream);
+  LM_REQUIRE(x.qkv_partials && x.positions && x.k_pages && x.v_pages && x.block_table && x.used && x.out);
+  LM_REQUIRE(aligned16(x.qkv_partials) && rotation_ok(x.cos_sin, x.table_len, x.rotary, x.head_dim));
+  Args a{};
+  a.kv.k = (bf16 *)x.k_pages;
+  a.kv.v = (bf16 *)x.v_pages;
+  a.table = x.block_table;
+  a.used = x.used;
+  a.sh.scale = (float)x.scale;
+  a.in = {x.qkv_partials, (int)x.qkv_splits,
+          {x.cos_sin, x.table_len, (int)x.rotary, x.table_f32 != 0, x.neox != 0}, x.positions, x.active, x.row_order};
+  a.before = x.weights;
+  a.after = x.weights_out;
+  a.out = (bf16 *)x.out;
+  a.out_mb = x.frag_out ? frag_row_blocks(x.batch) : 0;
+  return launch_decode_paged(c, a, x.workspace, x.workspace_bytes, stream);
 }

@@ -272,9 +272,15 @@ class QuantFlashDecode:
 
 def paged_splits(batch, kv_heads, maximum):
     """Key-range splits over a paged cache."""
-    pairs = max(1, batch * kv_heads)
-    longest = -(-maximum // 256) if maximum >= 3 * 256 else 1
-    return max(1, min(max(16, maximum // 4096), 512 // pairs, longest))
+    tiles, pairs = -(-maximum // 32), max(1, batch * kv_heads)
+    return max(1, min(256 // pairs, -(-tiles // 8))) if tiles >= 24 else 1
+
+
+def paged_shares(batch, kv_heads, maximum, head_dim):
+    """Equal shares per KV head that the rows of a paged cache are cut into, or 0."""
+    if batch * maximum * kv_heads * head_dim * 4 < 256e6 or batch > 1024:
+        return 0
+    return max(1, (512 if head_dim == 64 else 256) // kv_heads)
 
 
 class PagedFlashDecode:
@@ -297,6 +303,8 @@ class PagedFlashDecode:
         self.head_dim = head_dim
         self.maximum = capacity if maximum is None else maximum
         self.splits = num_splits or paged_splits(batch, kv_heads, self.maximum)
+        # calls without a new token of their own, and unless the caller asks for splits
+        self.shares = 0 if num_splits else paged_shares(batch, kv_heads, self.maximum, head_dim)
         self.device = torch.device(device)
         self.workspace = self._space(False)
         self.weigh_space = None  # the larger workspace of a call with weights, made by the first
@@ -304,9 +312,11 @@ class PagedFlashDecode:
                           if ordered and self.device.type == "cuda" else None)
 
     def _space(self, weighed):
-        size = _lib.size_query("lm_flash_decode_paged_workspace_size", self.batch, self.kv_heads * self.groups,
-                               self.head_dim, self.maximum, self.splits, int(weighed)) \
-            if self.device.type == "cuda" else 0
+        size = 0
+        if self.device.type == "cuda":  # one for calls in splits and calls in shares
+            sizes = self.batch, self.kv_heads * self.groups, self.kv_heads, self.head_dim, self.maximum
+            size = max(_lib.size_query("lm_flash_decode_paged_workspace_size", *sizes, *cut, int(weighed))
+                       for cut in ((self.splits, 0), (1, self.shares)))
         return torch.empty(max(size, 1), dtype=torch.uint8, device=self.device)
 
     def _check(self, k, v, table, q_heads, rows):
@@ -364,7 +374,7 @@ class PagedFlashDecode:
         out = torch.empty_like(q) if q.is_contiguous() else torch.empty(q.shape, device=q.device, dtype=q.dtype)
         _lib.call_struct(index, "lm_flash_decode_paged", q.data_ptr(), rows, heads, k.data_ptr(), v.data_ptr(),
                          table.data_ptr(), table.shape[1], k.shape[0], k.shape[2], used.data_ptr(), b, hq, self.kv_heads,
-                         d, scale, self.maximum, self.splits, before, after, out.data_ptr(), space.data_ptr(),
+                         d, scale, self.maximum, 1 if self.shares else self.splits, self.shares, before, after, out.data_ptr(), space.data_ptr(),
                          space.numel())
         return out
 

@@ -13,7 +13,7 @@ from litemoe_amd import _lib, kv_paged, rope
 from litemoe_amd.cache import KVCache, PagedKVCache
 from litemoe_amd.config import preset
 from litemoe_amd.engine import Engine
-from litemoe_amd.flash_decode import PagedFlashDecode, paged_splits
+from litemoe_amd.flash_decode import PagedFlashDecode, paged_shares, paged_splits
 from oracle import paged
 
 _P = 1 << 20
@@ -185,13 +185,14 @@ def test_plans_refused(kwargs, text):
         PagedFlashDecode(**{**dict(batch=2, kv_heads=4, groups=2, capacity=64, device="cpu"), **kwargs})
 
 
-def test_splits_are_within_bounds():
-    for batch in (1, 2, 3, 8, 17, 32, 33, 64, 128, 1000):
+def test_pieces_are_within_bounds():
+    for batch in (1, 2, 3, 8, 17, 32, 33, 64, 128, 1000, 3000):
         for heads in (1, 2, 8, 32):
             for maximum in (1, 16, 255, 767, 768, 1279, 4095, 32768, 1 << 20):
                 splits = paged_splits(batch, heads, maximum)
-                assert 1 <= splits <= 1024
-                assert splits == 1 or maximum >= 32 * splits
+                assert 1 <= splits <= 256 and (splits == 1 or maximum >= 128 * splits)
+                for dim in (64, 128):
+                    assert 0 <= paged_shares(batch, heads, maximum, dim) <= 512
 
 
 # ------------------------------------------------------------ rotary tables --
@@ -259,10 +260,10 @@ def read(h, k=_P, page=16, dim=64, rows=3, table=_P, out=_P):
     return h.lm_paged_read(packed("lm_paged_read", [k, _P, table, 2, 4, 8, page, _P, 0, None, rows, 2, dim, out, _P]), None)
 
 
-def decode(h, q=_P, page=16, width=4, pages=8, batch=2, hq=4, hkv=2, dim=64, max_len=64, splits=1, w=None, w_out=None,
+def decode(h, q=_P, page=16, width=4, pages=8, batch=2, hq=4, hkv=2, dim=64, max_len=64, splits=1, shares=0, w=None, w_out=None,
            ws=_P, size=1 << 30, table=_P, qs=64):
     return h.lm_flash_decode_paged(packed("lm_flash_decode_paged", [
-        q, qs, 64, _P, _P, table, width, pages, page, _P, batch, hq, hkv, dim, 1.0, max_len, splits, w, w_out, _P, ws,
+        q, qs, 64, _P, _P, table, width, pages, page, _P, batch, hq, hkv, dim, 1.0, max_len, splits, shares, w, w_out, _P, ws,
         size]), None)
 
 
@@ -311,9 +312,11 @@ def test_structs_are_the_headers(name):
     (lambda h: decode(h, dim=96), 2), (lambda h: decode(h, page=17), 2), (lambda h: decode(h, q=None), 1),
     (lambda h: decode(h, q=_P + 4), 1), (lambda h: decode(h, qs=65), 1), (lambda h: decode(h, table=None), 1),
     (lambda h: decode(h, max_len=0), 1), (lambda h: decode(h, splits=0), 1), (lambda h: decode(h, splits=1025), 1),
+    (lambda h: decode(h, shares=-1), 1), (lambda h: decode(h, shares=65536), 1), (lambda h: decode(h, splits=2, shares=2), 1),
     (lambda h: decode(h, w=_P), 1), (lambda h: decode(h, w_out=_P), 1), (lambda h: decode(h, w=_P + 4, w_out=_P), 1),
-    (lambda h: decode(h, splits=2, size=100), 4), (lambda h: decode(h, w=_P, w_out=_P, ws=None), 4),
-    (lambda h: decode(h, splits=2, ws=_P + 4), 1), (lambda h: decode(h, batch=65536), 1),
+    (lambda h: decode(h, shares=2, size=100), 4), (lambda h: decode(h, shares=2, w=_P, w_out=_P, ws=None), 4),
+    (lambda h: decode(h, shares=2, ws=_P + 4), 1), (lambda h: decode(h, splits=2, size=100), 4),
+    (lambda h: decode(h, w=_P, w_out=_P, max_len=4097, width=300, size=100), 4), (lambda h: decode(h, batch=65536), 1),
     (lambda h: fused(h, batch=0), 0), (lambda h: fused(h, slices=9), 2), (lambda h: fused(h, slices=0), 1),
     (lambda h: fused(h, rotary=72), 1), (lambda h: fused(h, cos=None), 1), (lambda h: fused(h, part=_P + 4), 1),
     (lambda h: fused(h, batch=129, frag=1), 2), (lambda h: fused(h, pos=None), 1), (lambda h: fused(h, page=20), 2),
@@ -328,12 +331,15 @@ def test_invalid_arguments_rejected_on_host(call, expected):
 
 
 def test_workspace_sizes():
-    def size(splits, weighed, max_len=100):
-        return _lib.size_query("lm_flash_decode_paged_workspace_size", 3, 8, 128, max_len, splits, weighed)
-    assert size(1, 0) == 0
-    assert size(4, 0) == 3 * 8 * 4 * 128 * 4 + 2 * 512
-    assert size(1, 1) == 3 * 256 + 3 * 8 * 128 * 4
-    assert size(4, 1) == 3 * 8 * 4 * 128 * 4 + 3 * 512 + 3 * 8 * 128 * 4
+    def size(splits, shares, weighed, max_len=100):
+        return _lib.size_query("lm_flash_decode_paged_workspace_size", 3, 8, 2, 128, max_len, splits, shares, weighed)
+    assert size(1, 0, 0) == size(1, 0, 1) == 0
+    assert size(4, 0, 0) == 3 * 4 * 8 * 128 * 4 + 2 * 512
+    assert size(1, 5, 0) == 256 + 5 * 8 * 2 * 128 * 4 + 2 * 512
+    scores = 2 * 256 + 3 * 8 * 128 * 4
+    assert size(4, 0, 1) == size(4, 0, 0) + 512 + scores and size(1, 5, 1) == size(1, 5, 0) + 512 + scores
+    # four query heads' scores of 2080 positions are more than a workgroup keeps
+    assert size(1, 0, 1, 2048) == 0 and size(1, 0, 1, 2049) == 2 * 256 + 3 * 8 * 2080 * 4
 
 
 # ------------------------------------------------------------------ oracle --
