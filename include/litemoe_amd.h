@@ -377,8 +377,8 @@ int lm_flash_decode_paged_workspace_size(int64_t batch, int64_t q_heads,
 /* lm_flash_decode over a paged cache (see lm_paged_rotate_write): out[b,h] =
  * softmax(scale * q[b,h] . K_j, j < used[b]) V over the positions that have a
  * page; a row that has none gives zeros. used[b] is held to [0, max_len] and
- * to width * page. Scores, maxima and sums in fp32, the probabilities rounded
- * to bf16 for the matrix cores and summed as rounded. Positions from used[b] on
+ * to width * page. Scores, maxima and sums in fp32, the probabilities in two bf16
+ * parts for the matrix cores. Positions from used[b] on
  * and positions without a page may hold anything. q_heads / kv_heads at most
  * 16; q 16-byte aligned, its strides multiples of 8; out [batch, q_heads,
  * head_dim] contiguous.

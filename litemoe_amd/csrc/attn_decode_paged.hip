@@ -20,8 +20,7 @@
 // (8 or 16 bytes each, rows of one position contiguous over 16 lanes) and pairs
 // them per channel with v_perm, 2 instructions a position and 64 bytes. A row of
 // the result is then a channel of the same 16-fold stride, and the lane's
-// accumulators are D/4 consecutive channels. The row sums of P come from one more
-// MFMA with ones, so they sum the probabilities as they were rounded.
+// accumulators are D/4 consecutive channels.
 //
 // The running maximum is a column's own reference, kept kAbove over the score that
 // set it and moved only when a score passes it, so nothing crosses lanes in the
@@ -58,9 +57,8 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 struct Partial {
   int32_t *off;    // shares: [batch + 1] tiles before each row
   float *o;        // [slot][G][D]
-  float *m, *l;    // [slot][G]; l: sums of the rounded probabilities
-  float *lw;       // weighed: sums of the probabilities, as m
-  float *rm, *rw;  // weighed: m and lw of rows that one workgroup held, [batch, q_heads]
+  float *m, *l;    // [slot][G] maxima (log2 units) and sums of the probabilities
+  float *rm, *rl;  // weighed: those of rows that one workgroup held, [batch, q_heads]
   float *s;        // weighed: scores in log2 units, [batch, q_heads, padded]
   int64_t padded;
 };
@@ -113,7 +111,7 @@ __device__ __forceinline__ T constant(const T *p) {
 // same ones in turn; the heads' factors behind them.
 constexpr int kRingFloats = 32 * kTile;  // of a wave: 32 tiles times heads
 __host__ __device__ constexpr int lds_bytes(int D, int G, bool fused) {
-  const int merge = kWaves * G * (D + 3) * 4, rot = fused ? (G + 2) * D * (2 + 4) : 0;
+  const int merge = kWaves * G * (D + 2) * 4, rot = fused ? (G + 2) * D * (2 + 4) : 0;
   return ((merge > rot ? merge : rot) + 2 * G * 4 + 15) / 16 * 16;
 }
 
@@ -315,11 +313,10 @@ __device__ __forceinline__ void attend(const Args &a, const bf16 *__restrict__ q
     ringed = 0;
   };
   const float sl2 = sh.scale * 1.4426950408889634f;
-  float m = kEmpty, lw = 0.f;
-  f32x4 l{0.f, 0.f, 0.f, 0.f}, acc[kCh];
+  float m = kEmpty, l = 0.f;  // l: of the lane's own positions
+  f32x4 acc[kCh];
 #pragma unroll
   for (int c = 0; c < kCh; ++c) acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const u32x4 ones{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
 
   auto compute = [&](Kv<D> &x, int tile) {
     const int left = n - tile * kTile;  // positions of the row from this tile on
@@ -383,24 +380,27 @@ __device__ __forceinline__ void attend(const Args &a, const bf16 *__restrict__ q
       const float to = mx + kAbove;
       const float f = up ? __builtin_amdgcn_exp2f(m - to) : 1.f;
       m = up ? to : m;
-      lw *= f;
       l *= f;
 #pragma unroll
       for (int cb = 0; cb < kCh; ++cb) acc[cb] *= f;
     }
-    u32x4 p;
+    // Probabilities for the matrix cores in two bf16 parts, cut and rest: with one, rounded
+    // (2^-9 of each off), results were off by 2.2e-3 (relative, RMS), with two by 1.7e-3, the
+    // output's own rounding, in the same time. The rest is taken 2^-18 of the whole larger,
+    // so that it is above 0 where the probability is: 0 times an infinity in V is no number.
+    u32x4 p, rest;
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const float p0 = __builtin_amdgcn_exp2f(sc[t][2 * i] - m), p1 = __builtin_amdgcn_exp2f(sc[t][2 * i + 1] - m);
-        if constexpr (kWeigh != kNone) {
-          lw += p0;
-          lw += p1;
-        }
-        p[2 * t + i] = pack_bf16_nc(p0, p1);
+        l += p0;
+        l += p1;
+        const uint32_t b0 = __float_as_uint(p0), b1 = __float_as_uint(p1);
+        p[2 * t + i] = __builtin_amdgcn_perm(b1, b0, 0x07060302u);
+        rest[2 * t + i] = pack_bf16_nc(__builtin_fmaf(p0, 1.f + 0x1p-18f, -hi_f32(b0)),
+                                       __builtin_fmaf(p1, 1.f + 0x1p-18f, -hi_f32(b1)));
       }
-    l = mfma16x16x32(ones, p, l);
 #pragma unroll
     for (int cb = 0; cb < kCh; ++cb) {
       const uint32_t sel = cb % 2 ? 0x07060302u : 0x05040100u;
@@ -411,6 +411,7 @@ __device__ __forceinline__ void attend(const Args &a, const bf16 *__restrict__ q
         for (int i = 0; i < 2; ++i)
           vt[2 * t + i] = __builtin_amdgcn_perm(x.v[t][2 * i + 1][cb / 2], x.v[t][2 * i][cb / 2], sel);
       acc[cb] = mfma16x16x32(vt, p, acc[cb]);
+      acc[cb] = mfma16x16x32(vt, rest, acc[cb]);
     }
   };
 
@@ -441,13 +442,11 @@ __device__ __forceinline__ void attend(const Args &a, const bf16 *__restrict__ q
     }
     __syncthreads();  // sm_rot is done with
   }
-  if constexpr (kWeigh != kNone) {
-    lw += xor_lanes<16>(lw);
-    lw += xor_lanes<32>(lw);
-  }
-  // Waves merge: [wave][G][D] accumulators, then [wave][G] of m, l and lw.
+  l += xor_lanes<16>(l);
+  l += xor_lanes<32>(l);
+  // Waves merge: [wave][G][D] accumulators, then [wave][G] of m and l.
   float *sm_o = reinterpret_cast<float *>(smem);
-  float *sm_m = sm_o + kWaves * G * D, *sm_l = sm_m + kWaves * G, *sm_w = sm_l + kWaves * G;
+  float *sm_m = sm_o + kWaves * G * D, *sm_l = sm_m + kWaves * G;
   if (r < G) {
 #pragma unroll
     for (int x = 0; x < 4; ++x)
@@ -457,8 +456,7 @@ __device__ __forceinline__ void attend(const Args &a, const bf16 *__restrict__ q
             f32x4{acc[cb][x], acc[cb + 1][x], acc[cb + 2][x], acc[cb + 3][x]};
     if (g == 0) {
       sm_m[wave * G + r] = m;
-      sm_l[wave * G + r] = l[0];
-      if constexpr (kWeigh) sm_w[wave * G + r] = lw;
+      sm_l[wave * G + r] = l;
     }
   }
   __syncthreads();
@@ -467,12 +465,11 @@ __device__ __forceinline__ void attend(const Args &a, const bf16 *__restrict__ q
     float mx = sm_m[gh];
 #pragma unroll
     for (int w = 1; w < kWaves; ++w) mx = fmaxf(mx, sm_m[w * G + gh]);
-    float lsum = 0.f, wsum = 0.f, o = 0.f;
+    float lsum = 0.f, o = 0.f;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
       const float f = __builtin_amdgcn_exp2f(sm_m[w * G + gh] - mx);
       lsum += sm_l[w * G + gh] * f;
-      if constexpr (kWeigh) wsum += sm_w[w * G + gh] * f;
       o += sm_o[(w * G + gh) * D + c] * f;
     }
     const int hq = h * G + gh;
@@ -481,13 +478,13 @@ __device__ __forceinline__ void attend(const Args &a, const bf16 *__restrict__ q
       if constexpr (kWeigh == kScores) {
         if (c == 0) {
           part.rm[b * sh.q_heads + hq] = mx;
-          part.rw[b * sh.q_heads + hq] = wsum;
+          part.rl[b * sh.q_heads + hq] = lsum;
         }
       }
       if constexpr (kWeigh == kHeld) {
         if (c == 0) {
           sm_f[gh] = mx;
-          sm_f[G + gh] = wsum == 0.f ? 0.f : 1.f / wsum;
+          sm_f[G + gh] = lsum == 0.f ? 0.f : 1.f / lsum;
         }
       }
     } else {
@@ -496,7 +493,6 @@ __device__ __forceinline__ void attend(const Args &a, const bf16 *__restrict__ q
       if (c == 0) {
         part.m[at] = mx;
         part.l[at] = lsum;
-        if constexpr (kWeigh != kNone) part.lw[at] = wsum;
       }
     }
   }
@@ -691,14 +687,14 @@ weigh_kernel(Args a) {
     float mx = kEmpty, l = 0.f;
     if (x.count == 1) {
       mx = part.rm[b * a.sh.q_heads + h * G + gh];
-      l = part.rw[b * a.sh.q_heads + h * G + gh];
+      l = part.rl[b * a.sh.q_heads + h * G + gh];
     } else {
       for (int i = lane; i < x.count; i += kWave) mx = fmaxf(mx, part.m[slot_of(a, x, i, h, gh)]);
 #pragma unroll
       for (int d = 1; d < kWave; d *= 2) mx = fmaxf(mx, shfl_xor(mx, d));
       for (int i = lane; i < x.count; i += kWave) {
         const int64_t slot = slot_of(a, x, i, h, gh);
-        l += part.lw[slot] * __builtin_amdgcn_exp2f(part.m[slot] - mx);
+        l += part.l[slot] * __builtin_amdgcn_exp2f(part.m[slot] - mx);
       }
       l = wave_sum(l);
     }
@@ -770,9 +766,7 @@ int64_t workspace_bytes(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_
   const int64_t n = slot_count(batch, kv_heads, splits, shares) * (q_heads / kv_heads);
   const bool scores = weighed && !weighs_held(q_heads / kv_heads, max_len, splits, shares);
   return (shares ? align_up((batch + 1) * 4, 256) : 0) + align_up(n * head_dim * 4, 256) + 2 * align_up(n * 4, 256) +
-         (scores ? align_up(n * 4, 256) + 2 * align_up(batch * q_heads * 4, 256) +
-                       batch * q_heads * padded_scores(max_len) * 4
-                 : 0);
+         (scores ? 2 * align_up(batch * q_heads * 4, 256) + batch * q_heads * padded_scores(max_len) * 4 : 0);
 }
 
 bool pieces_ok(int64_t splits, int64_t shares) {
@@ -854,9 +848,8 @@ int launch_decode_paged(const Call &c, Args a, void *workspace, int64_t workspac
   a.part.m = take(n);
   a.part.l = take(n);
   if (weighed && !held) {
-    a.part.lw = take(n);
     a.part.rm = take(c.batch * c.q_heads);
-    a.part.rw = take(c.batch * c.q_heads);
+    a.part.rl = take(c.batch * c.q_heads);
     a.part.s = take(c.batch * c.q_heads * a.part.padded);
   }
   hipStream_t s = (hipStream_t)stream;

@@ -69,9 +69,9 @@ def rotated_bound(x, exact, size=1.0):
 
 def attention_bound(q, pk, pv, table, used, scale, out, limit=None):
     """How far outputs may be off, per element, with A = sum p|v| / sum p, n the row's positions:
-    * probabilities are rounded to bf16, p(1 + d), |d| <= 2^-8, and summed as rounded: sum p(1 + d) v / sum p(1 +
-      d) - out = sum p d (v - out) / sum p(1 + d), at most 2^-8 (A + |out|) / (1 - 2^-8); the result's own rounding
-      adds 2^-8 of it: together less than 2^-8 (1 + 2^-6) (A + 2|out|);
+    * a probability enters the product as two bf16 parts, its first 8 bits (less than 2^-7 of it lost) and the rest,
+      rounded (2^-8 of that) and 2^-18 of the whole larger: 2^-15 A + 2^-18 A; the result's own rounding adds 2^-8 of
+      it (2^-8 (1 + 2^-6) |out| with what the others move it by);
     * a score's D products are summed in fp32 (D roundings of at most 2^-24 of S = scale sum|q k|), scaled (one of
       the score, one of the scale), and its distance to the reference, at most 2 S + 6, is rounded: (D + 8) S + 8 in
       units of 2^-24; that moves p by the same share, in numerator and denominator;
@@ -91,7 +91,7 @@ def attention_bound(q, pk, pv, table, used, scale, out, limit=None):
         a = (p @ v.abs()).reshape(hq, d)
         size = (qi.abs() @ k.abs().transpose(1, 2)).amax(-1).reshape(hq, 1) * scale
         o = out[i].abs()
-        tol[i] = 2.0 ** -8 * (1 + 2.0 ** -6) * (a + 2 * o) + 2.0 ** -24 * (2 * ((d + 8) * size + 8) + n + 64) * (a + o)
+        tol[i] = 2.0 ** -8 * (1 + 2.0 ** -6) * o + 1.125 * 2.0 ** -15 * a + 2.0 ** -24 * (2 * ((d + 8) * size + 8) + n + 64) * (a + o)
     return tol + 1e-30
 
 

@@ -337,7 +337,7 @@ def test_workspace_sizes():
     assert size(4, 0, 0) == 3 * 4 * 8 * 128 * 4 + 2 * 512
     assert size(1, 5, 0) == 256 + 5 * 8 * 2 * 128 * 4 + 2 * 512
     scores = 2 * 256 + 3 * 8 * 128 * 4
-    assert size(4, 0, 1) == size(4, 0, 0) + 512 + scores and size(1, 5, 1) == size(1, 5, 0) + 512 + scores
+    assert size(4, 0, 1) == size(4, 0, 0) + scores and size(1, 5, 1) == size(1, 5, 0) + scores
     # four query heads' scores of 2080 positions are more than a workgroup keeps
     assert size(1, 0, 1, 2048) == 0 and size(1, 0, 1, 2049) == 2 * 256 + 3 * 8 * 2080 * 4
 
