@@ -234,7 +234,8 @@ int lm_paged_read(const lm_paged_read_args *args, void *stream);
  * min(n, keep) in all (of equal weights the first; a NaN counts as the heaviest,
  * -0 as 0), in their order:
  *   kept        int32 [layers, batch, heads, keep]: their positions, then -1
- *   weights_out like weights: theirs, then zeros; may be weights itself
+ *   weights_out like weights: theirs, then zeros; may be weights itself where a row
+ *               has at most 12288 positions (both 16-byte aligned)
  *   used_out    int32 [batch]: min(n, keep)
  * and their K and V are copied to positions 0 .. of the row in `target` [batch,
  * target_width], a table over the same pages. Positions that `source` (the

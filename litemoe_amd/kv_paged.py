@@ -13,6 +13,7 @@ from .kv_quant import per_row
 
 PAGES = frozenset(1 << s for s in range(4, 17))  # positions of a page
 HEAD_DIMS = (64, 128)
+IN_PLACE = 12288  # positions of a row whose weights an eviction may write where it reads them
 
 
 def check_layer(k, v, table):
@@ -134,6 +135,8 @@ def evict(cache, weights, used, keep, recent, target, table=None, weights_out=No
         raise ValueError("Eviction keeps 1 to all positions of a row, and at most that many recent ones")
     used = per_row(used, rows, torch.int32, index, "used")
     out = torch.empty_like(weights) if weights_out is None else weights_out
+    if out.data_ptr() == weights.data_ptr() and width * page > IN_PLACE:
+        weights = weights.clone()
     kept = torch.empty((layers, rows, heads, keep), dtype=torch.int32, device=k.device)
     left = torch.empty(rows, dtype=torch.int32, device=k.device)
     _lib.call_struct(index, "lm_kv_evict", k.data_ptr(), v.data_ptr(), table.data_ptr(), target.data_ptr(), width,

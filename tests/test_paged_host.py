@@ -324,7 +324,8 @@ def test_structs_are_the_headers(name):
     (lambda h: evict(h, batch=0), 0), (lambda h: evict(h, keep=0), 1), (lambda h: evict(h, recent=6), 1),
     (lambda h: evict(h, recent=-1), 1), (lambda h: evict(h, keep=65), 1), (lambda h: evict(h, page=15), 2),
     (lambda h: evict(h, w=None), 1), (lambda h: evict(h, layers=0), 1), (lambda h: evict(h, layers=300, batch=300), 1),
-    (lambda h: evict(h, dim=80), 2), (lambda h: evict(h, target=None), 1),
+    (lambda h: evict(h, dim=80), 2), (lambda h: evict(h, target=None), 1), (lambda h: evict(h, w=_P + 8), 1),
+    (lambda h: evict(h, width=769), 1),  # in place, rows of more than 12288 positions
 ])
 def test_invalid_arguments_rejected_on_host(call, expected):
     assert call(_lib.load()) == expected
