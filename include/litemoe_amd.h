@@ -180,9 +180,9 @@ int lm_kv_quant_read(const void *k_codes, const void *v_codes,
  * each sum rounded to bf16, lm_rope_kv_write's arithmetic). Positions outside
  * the table are not turned. With cos_sin NULL and rotary 0 nothing is.
  * at (int64, or int32 with at_i32 nonzero) NULL: at = positions (one of the two is
- * needed for a store); slots NULL: slot = row; active NULL: every row is written. k_pages and v_pages NULL:
- * nothing is stored (v, block_table, at, active and slots are not looked at; any
- * head_dim that is a multiple of 16, to 256). q_heads 0: no queries. k_out may
+ * needed for a store); slots NULL: slot = row; active NULL: every row is written.
+ * k_pages and v_pages NULL: nothing is stored (v, block_table, at, active and slots
+ * are not looked at; any head_dim that is a multiple of 16, to 256). q_heads 0: no queries. k_out may
  * be NULL with a store. q_out and k_out may be q and k (in place). Strides in
  * elements, multiples of 8, pointers 16-byte aligned, channels contiguous.
  * One row per target, as lm_kv_write. Replaces vLLM `_custom_ops.rotary_embedding`
@@ -235,12 +235,12 @@ int lm_paged_read(const lm_paged_read_args *args, void *stream);
  * -0 as 0), in their order:
  *   kept        int32 [layers, batch, heads, keep]: their positions, then -1
  *   weights_out like weights: theirs, then zeros; may be weights itself where a row
- *               has at most 12288 positions (both 16-byte aligned)
+ *               has at most 12288 positions, else apart from it (both 16-byte aligned)
  *   used_out    int32 [batch]: min(n, keep)
  * and their K and V are copied to positions 0 .. of the row in `target` [batch,
- * target_width], a table over the same pages. Positions that `source` (the
- * row's present table, [batch, width]) or `target` has no page for are not
- * copied. No page of `target` may be one that a row of `source` reads in this
+ * target_width], a table over the same pages. Positions that `target` has no
+ * page for are not copied, those that `source` (the row's present table, [batch,
+ * width]) has none for are zeros there. No page of `target` may be one that a row of `source` reads in this
  * call; `source`'s pages are not written, so another row may share them.
  * 0 <= recent <= keep, 1 <= keep <= width * page, layers * batch <= 65535. The
  * reference holds every position to the end (litemoe/cache.py:7-20). */
@@ -386,8 +386,8 @@ int lm_flash_decode_paged_workspace_size(int64_t batch, int64_t q_heads,
  * num_splits (1 to 1024) workgroups take a row's tiles of 32 positions in turn; or,
  * with num_splits 1, num_shares (0: not; to 65535) workgroups per KV head take equal
  * shares of the tiles of all rows. weights and weights_out (both or neither; fp32
- * [batch, kv_heads, width * page], 16-byte aligned, may be one buffer): for
- * every j below the row's length
+ * [batch, kv_heads, width * page], 16-byte aligned, one buffer or two that share
+ * nothing): for every j below the row's length
  *   weights_out[b,g,j] = weights[b,g,j] + sum of the probabilities of j over
  *                        the query heads of KV head g
  * (0 for a position without a page); other entries are not written. Two calls
@@ -415,10 +415,10 @@ int lm_flash_decode_paged(const lm_flash_decode_paged_args *args, void *stream);
  * lm_paged_rotate_write by positions[b], the store of the new token's key and
  * value at position used[b] - 1 of its row, and attention over the first used[b]
  * positions with them. Nothing is stored, and the cache is attended as it is,
- * where active[b] is 0, used[b] is above max_len or width * page, or the
+ * where active[b] is 0, used[b] is below 1 or above max_len or width * page, or the
  * position has no page. Results are bitwise those of lm_paged_rotate_write on
- * the same heads followed by lm_flash_decode_paged. Two rows of one call may not
- * store to the same page. row_order and frag_out (nonzero: batch <= 128) as
+ * the same heads followed by lm_flash_decode_paged with the same num_splits. A page
+ * that a row stores to may be no other row's. row_order and frag_out (nonzero: batch <= 128) as
  * lm_flash_decode_quant_qkv; qkv_partials 16-byte aligned. */
 typedef struct lm_flash_decode_paged_qkv_args {
   const float *qkv_partials;

@@ -385,8 +385,8 @@ class PagedKVCache:
 
     def evict(self, weights, used, keep, recent=0, room=0):
         """Hold every row to ``keep`` positions (:func:`kv_paged.evict`): per layer and
-        KV head the ``recent`` last and the heaviest others of the row's ``used[b]`` stay,
-        in their order, in fresh pages; the old ones go back to the pool. ``weights [L,
+        KV head the ``recent`` last and the heaviest others of the row's ``used[b]`` (no
+        more than it has pages for) stay, in their order, in fresh pages; the old ones go back to the pool. ``weights [L,
         B, H, capacity]`` (fp32) is compacted in place. ``room``: positions that each row
         gets pages for beyond ``keep``, if it had more than ``keep``. Returns the positions
         kept ``[L, B, H, keep]`` and the rows' new ``used``; a row goes on at that
@@ -402,9 +402,13 @@ class PagedKVCache:
             raise ValueError(f"The KV pool has {len(self._free)} free pages, {sum(grow)} are wanted")
         fresh = [self._take(n) for n in grow]
         width = max([1, *grow])
-        target = torch.tensor([p + [-1] * (width - len(p)) for p in fresh], dtype=torch.int32).to(self._table.device)
+        # each row's pages to come, and the positions that it has pages for
+        lines = [p + [-1] * (width - len(p)) + [len(old) * self.page] for p, old in zip(fresh, self._held)]
         try:
-            _, kept, left = kv_paged.evict(self, weights, used, keep, recent, target, weights_out=weights)
+            lines = torch.tensor(lines, dtype=torch.int32).to(self._table.device)
+            used = kv_quant.per_row(used, len(fresh), torch.int32, lines.get_device(), "used").minimum(lines[:, width])
+            _, kept, left = kv_paged.evict(self, weights, used, keep, recent, lines[:, :width].contiguous(),
+                                           weights_out=weights)
         except Exception:
             for pages in fresh:
                 self._drop(pages)

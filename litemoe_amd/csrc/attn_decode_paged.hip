@@ -284,7 +284,7 @@ __device__ __forceinline__ void attend(const Args &a, const bf16 *__restrict__ q
       qw[s] = r < G ? *reinterpret_cast<const u32x4 *>(&sm_rot[r][32 * s + 8 * g]) : u32x4{0, 0, 0, 0};
     // The new token's place is the row's last, if the row was not cut short.
     const int last = n - 1;
-    if (writes && held == n && (tiles - 1 - lo) % stride < kWaves && hi == tiles) {
+    if (writes && n > 0 && held == n && (tiles - 1 - lo) % stride < kWaves && hi == tiles) {
       const int id = constant(row_table + (last >> kv.shift));
       own = (uint32_t)id < (uint32_t)kv.pages;
       new_cell = ((((int64_t)(own ? id : 0) * kv.heads + h) << kv.shift) + (last & page_mask)) * D;
@@ -303,6 +303,7 @@ __device__ __forceinline__ void attend(const Args &a, const bf16 *__restrict__ q
   float *sm_ring = sm_f + 2 * G + wave * kRingFloats;
   int ringed = 0;
   auto store_scores = [&](int end) {  // of the tiles before `end`
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // other lanes wrote what this one reads
     // 8 lanes a tile and head, four positions each
     const int at = lane / 8 % ring, c = lane % 8 * 4;
     const int64_t to = (int64_t)(end - (ringed - at) * stride) * kTile + c;
@@ -310,6 +311,7 @@ __device__ __forceinline__ void attend(const Args &a, const bf16 *__restrict__ q
       if (at < ringed)
         *reinterpret_cast<f32x4 *>(part.s + (b * sh.q_heads + h * G + gh) * part.padded + to) =
             *reinterpret_cast<const f32x4 *>(sm_ring + (at * G + gh) * kTile + c);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     ringed = 0;
   };
   const float sl2 = sh.scale * 1.4426950408889634f;
@@ -615,22 +617,12 @@ __device__ __forceinline__ int64_t slot_of(const Args &a, const Pieces &x, int i
   return (x.shares ? 2 * at + (i ? 0 : 1) : at) * a.sh.G + gh;
 }
 
-// Rows in several pieces: their results by log-sum-exp; rows that hold nothing: zeros.
-// grid (groups of query heads, batch), one thread per channel; the results of kBatch
-// pieces are requested together.
-constexpr int kCombineHeads = 2, kBatch = 8;
+// Channel c of a row's result from its pieces, by log-sum-exp; the results of kBatch
+// pieces are requested together, of the first `slots` ones.
+constexpr int kBatch = 8;
 template <int D>
-__global__ void __launch_bounds__(kCombineHeads *D)
-decode_paged_combine_kernel(Args a) {
-  const int hq = blockIdx.x * kCombineHeads + threadIdx.x / D;
-  const int64_t b = blockIdx.y;
-  const Pieces x = pieces_of(a, b);
-  if (hq >= a.sh.q_heads || x.count == 1) return;
-  const int c = threadIdx.x % D, h = hq / a.sh.G, gh = hq % a.sh.G;
+__device__ __forceinline__ float joined(const Args &a, const Pieces &x, int slots, int h, int gh, int c) {
   const Partial &part = a.part;
-  // The first results need not wait for the row's length: every split has a slot, and
-  // what a split past the row's end has there is not looked at.
-  const int slots = x.shares ? x.count : a.sh.splits;
   float mx = kEmpty, lsum = 0.f, o = 0.f;
   for (int s0 = 0; s0 < x.count; s0 += kBatch) {
     float ms[kBatch], ls[kBatch], os[kBatch], to = mx;
@@ -655,7 +647,24 @@ decode_paged_combine_kernel(Args a) {
       o += live ? os[i] * f : 0.f;
     }
   }
-  a.out[out_index(a, b, hq, c, D)] = (bf16)f32_to_bf16(lsum == 0.f ? 0.f : o / lsum);
+  return lsum == 0.f ? 0.f : o / lsum;
+}
+
+// Rows in several pieces: their results; rows that hold nothing: zeros. grid (groups of
+// query heads, batch), one thread per channel.
+constexpr int kCombineHeads = 2;
+template <int D>
+__global__ void __launch_bounds__(kCombineHeads *D)
+decode_paged_combine_kernel(Args a) {
+  const int hq = blockIdx.x * kCombineHeads + threadIdx.x / D;
+  const int64_t b = blockIdx.y;
+  const Pieces x = pieces_of(a, b);
+  if (hq >= a.sh.q_heads || x.count == 1) return;
+  const int c = threadIdx.x % D;
+  // The first results need not wait for the row's length: every split has a slot, and
+  // what a split past the row's end has there is not looked at.
+  const float o = joined<D>(a, x, x.shares ? x.count : a.sh.splits, hq / a.sh.G, hq % a.sh.G, c);
+  a.out[out_index(a, b, hq, c, D)] = (bf16)f32_to_bf16(o);
 }
 
 // after[b, h, j] = before[b, h, j] + sum over the KV head's query heads of their
@@ -707,15 +716,7 @@ weigh_kernel(Args a) {
   if (blockIdx.x == 0 && x.count != 1) {
     for (int t = threadIdx.x; t < G * D; t += kWeighThreads) {
       const int gh = t / D, c = t % D;
-      float lsum = 0.f, o = 0.f;
-#pragma unroll 4
-      for (int i = 0; i < x.count; ++i) {
-        const int64_t slot = slot_of(a, x, i, h, gh);
-        const float f = __builtin_amdgcn_exp2f(part.m[slot] - sm_m[gh]);
-        lsum += part.l[slot] * f;
-        o += part.o[slot * D + c] * f;
-      }
-      a.out[out_index(a, b, h * G + gh, c, D)] = (bf16)f32_to_bf16(lsum == 0.f ? 0.f : o / lsum);
+      a.out[out_index(a, b, h * G + gh, c, D)] = (bf16)f32_to_bf16(joined<D>(a, x, x.count, h, gh, c));
     }
   }
   if (j >= n) return;
@@ -815,6 +816,7 @@ int launch_sized(const Call &c, const Args &a, hipStream_t s) {
 int launch_decode_paged(const Call &c, Args a, void *workspace, int64_t workspace_bytes_, void *stream) {
   LM_REQUIRE(aligned16(a.kv.k) && aligned16(a.kv.v) && (a.before == nullptr) == (a.after == nullptr) &&
              aligned16(a.before) && aligned16(a.after));
+  LM_REQUIRE(in_place_or_apart(a.before, a.after, c.batch * c.kv_heads * c.width * c.page * 4));
   const bool weighed = a.after != nullptr;
   const int64_t G = c.q_heads / c.kv_heads;
   const bool held = weighed && weighs_held(G, c.max_len, c.num_splits, c.num_shares);

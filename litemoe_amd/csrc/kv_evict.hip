@@ -256,13 +256,17 @@ evict_move_kernel(PagedKV kv, int64_t layer_elems, const int32_t *__restrict__ s
   if (from < 0 || (from >> kv.shift) >= kv.width || (to >> kv.shift) >= target_width) return;
   const int64_t old_page = source[(int64_t)b * kv.width + (from >> kv.shift)];
   const int64_t new_page = target[(int64_t)b * target_width + (to >> kv.shift)];
-  if (old_page < 0 || old_page >= kv.pages || new_page < 0 || new_page >= kv.pages) return;
+  if (new_page < 0 || new_page >= kv.pages) return;
   const int in_page = (1 << kv.shift) - 1;
   const int64_t at = layer * layer_elems + c;
   const int64_t src = at + (((old_page * kv.heads + h) << kv.shift) + (from & in_page)) * dim;
   const int64_t dst = at + (((new_page * kv.heads + h) << kv.shift) + (to & in_page)) * dim;
-  const u32x4 wk = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(kv.k + src));
-  const u32x4 wv = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(kv.v + src));
+  // A position that had no page gives zeros, as it reads: its new page was another's before.
+  u32x4 wk{0, 0, 0, 0}, wv{0, 0, 0, 0};
+  if (old_page >= 0 && old_page < kv.pages) {
+    wk = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(kv.k + src));
+    wv = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(kv.v + src));
+  }
   *reinterpret_cast<u32x4 *>(kv.k + dst) = wk;
   *reinterpret_cast<u32x4 *>(kv.v + dst) = wv;
 }
@@ -288,6 +292,7 @@ extern "C" int lm_kv_evict(const lm_kv_evict_args *args, void *stream) {
   const int64_t capacity = width * page;
   const bool held = capacity <= kHeldWeights;
   LM_REQUIRE(held || weights != weights_out);
+  LM_REQUIRE(in_place_or_apart(weights, weights_out, layers * batch * heads * capacity * 4));
   // One step of four weights a thread, or two: a wave alone on its SIMD waits for every
   // instruction. One row of 4096 weights 12.4 us with 256 threads, 9.2 with 512; 1024 such
   // rows 20.5 and 22.0 (bytes in and out 7, the rest latency).

@@ -27,6 +27,11 @@ inline int page_shift(int64_t page) {
 }
 
 inline bool aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+// Two buffers of `bytes` that are one, or share none.
+inline bool in_place_or_apart(const void *x, const void *y, int64_t bytes) {
+  const intptr_t a = reinterpret_cast<intptr_t>(x), b = reinterpret_cast<intptr_t>(y);
+  return a == b || a + bytes <= b || b + bytes <= a;
+}
 
 // cos | sin [table_len, rotary]: the first `rotary` channels of a head are turned
 // in pairs (i, i + rotary / 2) (neox) or (2 i, 2 i + 1).

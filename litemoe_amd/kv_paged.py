@@ -110,8 +110,8 @@ def evict(cache, weights, used, keep, recent, target, table=None, weights_out=No
     what stays (then zeros; in ``weights_out``, which may be ``weights``, if given), the
     positions kept ``[L, B, H, keep]`` (int32, then -1) and the rows' new ``used``.
 
-    Of equal weights the first stays; a NaN counts as the heaviest. ``table`` is the
-    rows' present table (the cache's own unless given). Pages of ``target`` must not be
+    Of equal weights the first stays; a NaN counts as the heaviest. A position that has
+    no page stays as zeros, as it is read. ``table`` is the rows' present table (the cache's own unless given). Pages of ``target`` must not be
     in it: the rows' present pages are read and not written, so another row may share
     them. :meth:`PagedKVCache.evict` takes care of both and moves the cache's table."""
     k, v = cache.k, cache.v

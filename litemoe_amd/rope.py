@@ -104,9 +104,10 @@ def rotary_embedding(positions, query, key, head_size, cos_sin_cache, is_neox=Tr
                   None, None, rows, query.shape[1], key.shape[1], 64, 1, 1, 1, _lib.stream(query.device))
         return
     for t in (query, key):
-        if t.dim() != 3 or t.dtype != torch.bfloat16 or kv_paged.aligned(t) is not t:
+        if (t.dim() != 3 or t.dtype != torch.bfloat16 or kv_paged.aligned(t) is not t
+                or any(size > 1 and not stride for size, stride in zip(t.shape, t.stride()))):
             raise ValueError('Rotation in place needs BF16 [T, heads, D] of contiguous channels, 16-byte aligned rows '
-                             'and heads (strides multiple of 8)')
+                             'and heads of their own (strides multiple of 8)')
     _rotate(query, key, positions, cos_sin_cache, is_neox, query, key)
 
 

@@ -10,6 +10,7 @@ import pytest
 import torch
 
 from litemoe_amd import kv_paged, rope, synth
+from litemoe_amd._lib import NativeError
 from litemoe_amd.batch import BatchPrefillEngine
 from litemoe_amd.cache import KVCache, PagedKVCache, QuantKVCache
 from litemoe_amd.config import preset
@@ -233,6 +234,10 @@ ATTENTIONS = [
     ([300, 5], 1, 16, 64, 32, None), ([300, 5], 1, 16, 64, 32, 3), ([95, 96, 97, 64], 3, 8, 64, 128, 2),
     ([1, 0, 33], 1, 1, 128, 16, None), ([700, 40, 0], 2, 4, 128, 256, None), ([513, 16, 31], 2, 5, 128, 32, 4),
     ([260], 1, 16, 128, 64, 1), ([2049, 4001], 2, 2, 64, 32, 16), ([2049, 1500], 1, 6, 64, 64, 40),
+    # one split, scores past what a workgroup keeps (8, 4 and 2 tiles stored together), and the most it keeps
+    ([4500, 100], 1, 2, 64, 16, 1), ([2900, 31, 257], 1, 3, 128, 64, 1), ([2000, 1], 1, 5, 64, 64, 1),
+    ([1100, 40, 0], 2, 8, 64, 32, 1), ([1000, 95], 1, 9, 128, 32, 1), ([600, 129], 1, 16, 64, 64, 1),
+    ([512, 480], 1, 16, 128, 64, 1),
 ]
 
 
@@ -267,6 +272,61 @@ def test_attention(lengths, hkv, groups, dim, page, splits, hole):
     flash(wide[..., :dim], *cache.layer(0), *args, used=used.to(DEV), weights=w_in)
     for i, n in enumerate(lengths):
         assert torch.equal(w_in[i, :, :n], w_out[i, :, :n]) and torch.equal(w_in[i, :, n:].cpu(), before[i, :, n:])
+
+
+SHARES = [
+    # lengths, kv heads, groups, dim, page, shares: more than there are tiles, one, ends inside rows, rows over many
+    ([700, 40, 0], 2, 4, 128, 256, 18), ([0, 0], 2, 3, 64, 16, 7), ([1], 1, 1, 64, 16, 5), ([33, 0, 1, 64], 2, 3, 64, 16, 1),
+    ([2000, 5, 1, 0, 900], 2, 2, 64, 64, 9), ([509] * 3, 8, 2, 64, 16, 4), ([128, 128, 256, 128], 1, 16, 64, 32, 5),
+    ([1500], 2, 9, 128, 32, 40), ([3000, 1], 1, 5, 64, 64, 23), ([*range(0, 130, 2)], 1, 2, 64, 16, 10),
+    ([(37 * i) % 211 for i in range(150)], 2, 3, 64, 16, 64), ([0] * 70 + [300] + [0] * 70, 1, 4, 64, 32, 3),
+]
+
+
+@pytest.mark.parametrize("lengths,hkv,groups,dim,page,shares", SHARES)
+@torch.inference_mode()
+def test_attention_in_shares(lengths, hkv, groups, dim, page, shares):
+    """The rows' tiles cut evenly, whatever the rows: outputs, and weights of calls in shares. Twice, bit for bit."""
+    seed = sum(lengths) + dim + shares
+    cache, k, v, table = random_cache(lengths, hkv, dim, page, seed, hole=len(lengths) == 5)
+    b, hq, scale = len(lengths), hkv * groups, dim ** -0.5
+    q = vectors((b, hq, dim), seed + 1)
+    flash = PagedFlashDecode(b, hkv, groups, cache.capacity, DEV, head_dim=dim)
+    flash.splits, flash.shares = 1, shares
+    flash.workspace = flash._space(False)
+    used = torch.tensor(lengths, dtype=torch.int32)
+    args = (q.to(DEV)[:, :, None], *cache.layer(0), None, None, scale, used.to(DEV))
+    flash.workspace.fill_(255)
+    got = flash(*args)
+    p = check_attention(got, q, k[0], v[0], table, used, scale)
+    before = torch.rand(b, hkv, cache.capacity, generator=gen(seed))
+    w = before.to(DEV)
+    assert torch.equal(flash(*args, weights=w), got)
+    for i, n in enumerate(lengths):
+        assert torch.equal(w[i, :, n:].cpu(), before[i, :, n:])
+        if n:
+            tol = weight_bound(q, k[0], table, i, n, scale, p[i], before[i, :, :n])
+            assert bool(((w[i, :, :n].double().cpu() - before[i, :, :n].double() - p[i].sum(1)).abs() <= tol).all())
+    again = flash(*args)
+    assert torch.equal(again, got)
+
+
+@torch.inference_mode()
+def test_shares_are_the_plan_of_large_batches():
+    """The plan takes shares where the caller asks for no splits, and their calls agree with the splits'."""
+    b, hkv, page, longest = 20, 8, 64, 4000
+    assert PagedFlashDecode(b, hkv, 2, 4032, DEV).shares == 0
+    b = 40
+    lengths = [1 + (1237 * i) % longest for i in range(b)]
+    cache, k, v, table = random_cache(lengths, hkv, 64, page, 3, capacity=4032)
+    flash = PagedFlashDecode(b, hkv, 2, cache.capacity, DEV)
+    split = PagedFlashDecode(b, hkv, 2, cache.capacity, DEV, num_splits=2)
+    assert flash.shares == 64 and split.shares == 0 and split.splits == 2
+    q = vectors((b, 16, 64), 4)
+    used = torch.tensor(lengths, dtype=torch.int32)
+    for f in (flash, split):
+        got = f(q.to(DEV)[:, :, None], *cache.layer(0), None, None, 0.125, used=used.to(DEV))
+        check_attention(got, q, k[0], v[0], table, used, 0.125)
 
 
 @torch.inference_mode()
@@ -354,7 +414,8 @@ def test_pages_past_32_bits():
 @pytest.mark.parametrize("neox,f32,rotary", [(True, False, 64), (True, True, 64), (False, True, 32), (False, False, 48)])
 @pytest.mark.parametrize("lengths,hkv,groups,dim,page,splits", [
     ([1], 1, 1, 64, 16, None), ([17, 32, 33, 1, 64], 2, 3, 64, 16, None), ([1000, 500, 31], 8, 2, 64, 64, 4),
-    ([130, 129, 128], 1, 16, 64, 128, 2), ([40, 257], 2, 4, 128, 32, None), ([600, 20], 1, 16, 128, 256, 3)])
+    ([130, 129, 128], 1, 16, 64, 128, 2), ([40, 257], 2, 4, 128, 32, None), ([600, 20], 1, 16, 128, 256, 3),
+    ([1100, 40, 97], 2, 8, 64, 32, 1), ([1000, 95], 1, 9, 128, 32, 1), ([512, 480], 1, 16, 128, 64, 1)])
 @torch.inference_mode()
 def test_fused_is_the_three_calls(lengths, hkv, groups, dim, page, splits, neox, f32, rotary, weighed):
     """The decode layer's form against rotate_kv_write and the attention, bit for bit: outputs, cache and weights;
@@ -395,6 +456,30 @@ def test_fused_is_the_three_calls(lengths, hkv, groups, dim, page, splits, neox,
     assert torch.equal(frag.to_rows(), exp.view(b, -1))
 
 
+@pytest.mark.parametrize("splits", [None, 3])
+@torch.inference_mode()
+def test_fused_row_without_a_place(splits):
+    """Rows of no positions, of fewer than none and of more than the plan's or the table's: nothing is stored."""
+    lengths, hkv, groups, dim = [48, 48, 96, 20, 70], 2, 3, 64
+    cache, k, v, table = random_cache(lengths, hkv, dim, 16, 2)
+    b, hq = len(lengths), hkv * groups
+    flash = PagedFlashDecode(b, hkv, groups, cache.capacity, DEV, maximum=90, num_splits=splits)
+    part = vectors((b, (hq + 2 * hkv) * dim), 1).float()[None].to(DEV)
+    cos_sin = rope.rotary_table(128, 64, 10000.0, device=DEV, dtype=BF16)
+    used = torch.tensor([0, -1, 91, 2 ** 31 - 1, 0], dtype=torch.int32)
+    pos = used.long() - 1
+    w = torch.ones(b, hkv, cache.capacity, device=DEV)
+    used_dev = used.to(DEV)
+    got = flash.fused_qkv(part, cos_sin, pos.to(DEV), None, *cache.layer(0), 0.125, used_dev, hq, weights=w)
+    assert torch.equal(cache.k.cpu().view(torch.int16), k.view(torch.int16))
+    assert torch.equal(cache.v.cpu().view(torch.int16), v.view(torch.int16))
+    for i in (0, 1, 4):
+        assert not got[i].any() and bool((w[i] == 1).all())
+    q = part.view(b, -1, dim)[:, :hq].to(BF16)
+    rope.rotary_embedding(pos.to(DEV), q, torch.zeros(b, 1, dim, dtype=BF16, device=DEV), dim, cos_sin)
+    check_attention(got[2:3], q[2:3].cpu(), k[0], v[0], table[2:3], [90], 0.125)
+
+
 @pytest.mark.parametrize("slices", [2, 3, 8])
 @torch.inference_mode()
 def test_fused_sums_slices(slices):
@@ -423,7 +508,8 @@ def test_fused_sums_slices(slices):
 @pytest.mark.parametrize("case", ["spread", "equal", "special", "negative"])
 @pytest.mark.parametrize("lengths,heads,dim,page,keep,recent", [
     ([5], 1, 64, 16, 1, 0), ([40, 16, 1, 0], 2, 64, 16, 16, 4), ([33, 100], 2, 128, 32, 33, 33),
-    ([1500, 1024, 1025, 700], 2, 64, 64, 1024, 100), ([4000, 2050], 1, 64, 256, 1500, 0), ([129], 3, 128, 16, 128, 1)])
+    ([1500, 1024, 1025, 700], 2, 64, 64, 1024, 100), ([4000, 2050], 1, 64, 256, 1500, 0), ([129], 3, 128, 16, 128, 1),
+    ([5000, 4097, 90], 1, 64, 64, 300, 7), ([12288, 8000], 1, 64, 64, 200, 0), ([13000, 12289, 5], 2, 64, 256, 100, 1)])
 @torch.inference_mode()
 def test_evict(lengths, heads, dim, page, keep, recent, case):
     layers, b = 2, len(lengths)
@@ -474,6 +560,79 @@ def test_evict(lengths, heads, dim, page, keep, recent, case):
     assert same is w_dev and torch.equal(kept2, kept)
     assert torch.equal(w_dev.cpu().view(torch.int32), exp_w.view(torch.int32))
     assert torch.equal(pk.cpu(), exp_k) and torch.equal(pv.cpu(), exp_v)
+
+
+@torch.inference_mode()
+def test_evict_positions_without_a_page():
+    """What stays of positions without a page is zeros in the target's pages, whose former contents were others'."""
+    cache, k, v, table = random_cache([80, 64], 2, 64, 16, 3, junk=3.0)
+    more = torch.full((1, 12, 2, 16, 64), 9.0, dtype=BF16, device=DEV)
+    pages = k.shape[1]
+    line = table.clone()
+    line[0, 1], line[1, 3] = -1, pages + 12
+    grown = PagedKVCache.over(torch.cat((cache.k, more), 1), torch.cat((cache.v, more), 1), line.to(DEV))
+    target = (pages + torch.arange(6, dtype=torch.int32)).view(2, 3)
+    w = torch.rand(1, 2, 2, cache.capacity, generator=gen(4))
+    before = grown.read(0)
+    _, kept, left = kv_paged.evict(grown, w.to(DEV), torch.tensor([80, 64], dtype=torch.int32, device=DEV), 45, 5,
+                                   target.to(DEV))
+    assert left.tolist() == [45, 45]
+    after = PagedKVCache.over(grown.k, grown.v, target.to(DEV)).read(0)
+    for b in range(2):
+        for h in range(2):
+            stay = paged.keep(w[0, b, h], [80, 64][b], 45, 5)
+            assert kept[0, b, h].tolist() == stay
+            lost = [j for j in stay if (16 <= j < 32 if b == 0 else j >= 48)]
+            assert lost
+            for x, y in zip(before, after):
+                assert torch.equal(x[b, h, stay], y[b, h, :45]) and not x[b, h, lost].any()
+                assert bool((y[b, h, 45:48] == 9).all())
+
+
+@torch.inference_mode()
+def test_cache_evicts_what_has_pages():
+    """``used`` past a row's pages is held to them, and a row of none stays so."""
+    cache = PagedKVCache.empty(1, 3, 2, 64, 128, DEV, page=16, pages=20)
+    cache.reserve([0, 1], [48, 20])
+    w = torch.rand(1, 3, 2, 128, device=DEV)
+    kept, left = cache.evict(w, torch.tensor([100, 100, 100], device=DEV), 40, 3)
+    assert left.tolist() == [40, 32, 0] and cache.free_pages == 20 - 3 - 2 and cache.held(2) == 0
+    assert kept[0, 1].tolist() == [[*range(32), *[-1] * 8]] * 2 and bool((kept[0, 2] == -1).all())
+
+
+@torch.inference_mode()
+def test_graph_replays_of_evictions():
+    """Weights and eviction recorded, with the weights read and written in place by the graph's own tensors."""
+    lengths = [100, 61]
+    cache, k, v, table = random_cache(lengths, 2, 64, 16, 3, capacity=112, junk=0.5)
+    grown = PagedKVCache.over(*(torch.cat((x, torch.zeros_like(x)), 1) for x in (cache.k, cache.v)), cache.table)
+    target = (k.shape[1] + torch.arange(4, dtype=torch.int32).view(2, 2)).to(DEV)
+    used = torch.tensor(lengths, dtype=torch.int32, device=DEV)
+    w = torch.rand(1, 2, 2, 112, generator=gen(1)).to(DEV)
+    kv_paged.evict(grown, w, used, 30, 4, target)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        with torch.cuda.graph(graph, stream=side):
+            out, kept, left = kv_paged.evict(grown, w, used, 30, 4, target)
+    torch.cuda.current_stream().wait_stream(side)
+    for turn in range(4):
+        w.copy_(torch.rand(1, 2, 2, 112, generator=gen(turn)))
+        used.sub_(7)
+        for x in (grown.k, grown.v):
+            x[:, k.shape[1]:] = 5
+        graph.replay()
+        got = [x.clone() for x in (out, kept, left, grown.k, grown.v)]
+        torch.cuda.synchronize()
+        for x in (grown.k, grown.v):
+            x[:, k.shape[1]:] = 5
+        exp = kv_paged.evict(grown, w, used, 30, 4, target)
+        assert all(torch.equal(x, y) for x, y in zip(got, (*exp, grown.k, grown.v)))
+        for b, n in enumerate(used.tolist()):
+            for h in range(2):
+                stay = paged.keep(w[0, b, h].cpu(), n, 30, 4)
+                assert kept[0, b, h].tolist() == stay + [-1] * (30 - len(stay))
 
 
 # ---------------------------------------------------------------- together --
@@ -567,7 +726,7 @@ def test_prefill_decode_evict_decode():
 
 @torch.inference_mode()
 def test_graph_replays_follow_the_table():
-    """Attention, weights, store and eviction recorded once and replayed as rows grow and their pages change, with
+    """Attention, weights and store recorded once and replayed as rows grow and their pages change, with
     eager work between the replays."""
     lengths = [30, 61]
     cache, k, v, table = random_cache(lengths, 2, 64, 16, 3, capacity=128, junk=0.5)
@@ -844,5 +1003,16 @@ def test_refusals():
         kv_paged.evict(cache, torch.zeros(1, 2, 2, 5, device=DEV), used, 4, 2, layer.table)
     with pytest.raises(ValueError, match="line per row"):
         kv_paged.evict(cache, torch.zeros(1, 2, 2, cache.capacity, device=DEV), used, 4, 2, layer.table[:1])
+    both = torch.zeros(9, 2, 2, cache.capacity, device=DEV)
+    with pytest.raises(NativeError):
+        flash(q, *layer, None, None, 0.125, used=used, weights=both[0], weights_out=both.view(-1, 2, cache.capacity)[1:3])
+    two = PagedKVCache.empty(2, 2, 2, 64, cache.capacity, DEV, page=16)
+    with pytest.raises(NativeError):
+        kv_paged.evict(two, both[:2], used, 4, 2, layer.table, weights_out=both[1:3])
+    turned = x[:, :, 0]
+    for t in (turned[:1].expand(2, -1, -1), turned[..., 1:33], turned[:, :, ::2]):
+        with pytest.raises(ValueError, match="in place"):
+            rope.rotary_embedding(pos, t, turned.clone(), t.shape[-1], rope.rotary_table(64, 32, 10000.0, device=DEV))
     # the buffers of the refused calls are as they were
+    assert not both.any() and not turned.any()
     assert bool((w == 0).all())
