@@ -371,11 +371,11 @@ class PagedFlashDecode:
             used = torch.where(active, lengths + 1, 1)
         used = kv_quant.per_row(used, b, torch.int32, index, "used")
         before, after, space = self._weights(weights, weights_out, b, index)
-        out = torch.empty_like(q) if q.is_contiguous() else torch.empty(q.shape, device=q.device, dtype=q.dtype)
+        out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(q.shape)
         _lib.call_struct(index, "lm_flash_decode_paged", q.data_ptr(), rows, heads, k.data_ptr(), v.data_ptr(),
                          table.data_ptr(), table.shape[1], k.shape[0], k.shape[2], used.data_ptr(), b, hq, self.kv_heads,
-                         d, scale, self.maximum, 1 if self.shares else self.splits, self.shares, before, after, out.data_ptr(), space.data_ptr(),
-                         space.numel())
+                         d, scale, self.maximum, 1 if self.shares else self.splits, self.shares, before, after,
+                         out.data_ptr(), space.data_ptr(), space.numel())
         return out
 
     def fused_qkv(self, partials, cos_sin, positions, active, k, v, table, scale, used, q_heads, row_order=None,
@@ -404,7 +404,7 @@ class PagedFlashDecode:
             out = FragRows(b, q_heads * self.head_dim, k.device)
             out_ptr = out.data.data_ptr()
         else:
-            out = torch.empty((b, q_heads, 1, self.head_dim), device=k.device, dtype=torch.bfloat16)
+            out = k.new_empty((b, q_heads, 1, self.head_dim))
             out_ptr = out.data_ptr()
         _lib.call_struct(index, "lm_flash_decode_paged_qkv", partials.data_ptr(), splits, cos_sin.data_ptr(),
                          *cos_sin.shape, cos_sin.dtype == torch.float32, bool(is_neox), positions.data_ptr(),

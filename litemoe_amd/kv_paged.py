@@ -44,19 +44,16 @@ def places(t, rows, index, what):
     return per_row(t, rows, torch.int32 if t.dtype == torch.int32 else torch.int64, index, what)
 
 
-def aligned(x):
-    """``x [rows, heads, D]`` as the kernels take it: contiguous channels, rows and
-    heads that start at 16 bytes (a copy where it is not so)."""
-    s = x.stride()
-    ok = (s[2] == 1 and (s[0] % 8 == 0 or x.shape[0] == 1) and (s[1] % 8 == 0 or x.shape[1] == 1)
-          and x.data_ptr() % 16 == 0)
-    return x if ok else x.clone(memory_format=torch.contiguous_format)
-
-
-def strides(x):
-    """Row and head stride of ``x [rows, heads, D]``; of a single one the stride says nothing."""
-    s = x.stride()
-    return s[0] if x.shape[0] > 1 else 0, s[1] if x.shape[1] > 1 else 0
+def view(x, rows, heads):
+    """``x [rows, heads, D]`` as the kernels take it, contiguous channels, rows and heads
+    that start at 16 bytes (a copy where it is not so), and its pointer and strides."""
+    at, (s0, s1, s2) = x.data_ptr(), x.stride()
+    # of a single row or head the stride says nothing
+    s0, s1 = s0 if rows > 1 else 0, s1 if heads > 1 else 0
+    if s2 != 1 or s0 % 8 or s1 % 8 or at % 16:
+        x = x.clone(memory_format=torch.contiguous_format)
+        return x, (x.data_ptr(), heads * x.shape[2], x.shape[2])
+    return x, (at, s0, s1)
 
 
 def write(cache, layer, k, v, positions, active, slots):
@@ -77,9 +74,8 @@ def write(cache, layer, k, v, positions, active, slots):
     at = places(positions, rows, index, "positions")
     slots = per_row(slots, rows, torch.int64, index, "slots")
     active = 0 if active is None else per_row(active, rows, torch.bool, index, "active").data_ptr()
-    k, v = aligned(k[:, :, 0]), aligned(v[:, :, 0])
-    _lib.call_struct(index, "lm_paged_rotate_write", 0, 0, 0, k.data_ptr(), *strides(k), v.data_ptr(), *strides(v), 0, 0,
-                     0, 0, 0, 0, at.data_ptr(), at.dtype == torch.int32, active, slots.data_ptr(), 0, 0, 0, 0, 0, 0,
+    (k, k_view), (v, v_view) = view(k[:, :, 0], rows, heads), view(v[:, :, 0], rows, heads)
+    _lib.call_struct(index, "lm_paged_rotate_write", 0, 0, 0, *k_view, *v_view, 0, 0, 0, 0, 0, 0, at.data_ptr(), at.dtype == torch.int32, active, slots.data_ptr(), 0, 0, 0, 0, 0, 0,
                      kc.data_ptr(), vc.data_ptr(), table.data_ptr(), table.shape[0], table.shape[1], pages, page, rows, 0,
                      heads, dim)
 
@@ -94,7 +90,7 @@ def read(cache, layer, positions, slots):
     rows = positions.numel()
     positions = places(positions, rows, index, "positions")
     slots = per_row(slots, rows, torch.int64, index, "slots")
-    k = torch.empty((rows, heads, 1, dim), dtype=torch.bfloat16, device=kc.device)
+    k = kc.new_empty((rows, heads, 1, dim))
     v = torch.empty_like(k)
     _lib.call_struct(index, "lm_paged_read", kc.data_ptr(), vc.data_ptr(), table.data_ptr(), table.shape[0],
                      table.shape[1], pages, page, positions.data_ptr(), positions.dtype == torch.int32, slots.data_ptr(),
@@ -127,8 +123,8 @@ def evict(cache, weights, used, keep, recent, target, table=None, weights_out=No
     if target.get_device() != index or weights.get_device() != index:
         raise ValueError("Eviction's tables and weights must be on the cache's device")
     shape = (layers, rows, heads, width * page)
-    for w in (weights,) if weights_out is None else (weights, weights_out):
-        if w.dtype != torch.float32 or w.shape != shape or not w.is_contiguous() or w.get_device() != index:
+    for w in (weights,) if weights_out is None or weights_out is weights else (weights, weights_out):
+        if w.dtype is not torch.float32 or w.shape != shape or not w.is_contiguous() or w.get_device() != index:
             raise ValueError("Weights must be contiguous fp32 [L, B, H, positions of a row] on the cache's device")
     keep, recent = int(keep), int(recent)
     if not 1 <= keep <= width * page or not 0 <= recent <= keep:
@@ -137,8 +133,7 @@ def evict(cache, weights, used, keep, recent, target, table=None, weights_out=No
     out = torch.empty_like(weights) if weights_out is None else weights_out
     if out.data_ptr() == weights.data_ptr() and width * page > IN_PLACE:
         weights = weights.clone()
-    kept = torch.empty((layers, rows, heads, keep), dtype=torch.int32, device=k.device)
-    left = torch.empty(rows, dtype=torch.int32, device=k.device)
+    kept, left = table.new_empty((layers, rows, heads, keep)), table.new_empty(rows)
     _lib.call_struct(index, "lm_kv_evict", k.data_ptr(), v.data_ptr(), table.data_ptr(), target.data_ptr(), width,
                      target.shape[1], pages, page, used.data_ptr(), weights.data_ptr(), layers, rows, heads, dim, keep,
                      recent, out.data_ptr(), kept.data_ptr(), left.data_ptr())

@@ -66,11 +66,12 @@ def rotary_table(length, rotary, theta, scaling=None, device="cpu", dtype=torch.
 
 def check_table(cos_sin, index, dim):
     """``cos_sin [table_len, rotary]`` as the kernels with any rotation take it."""
-    if (cos_sin.dtype not in (torch.float32, torch.bfloat16) or cos_sin.dim() != 2 or not cos_sin.is_contiguous()
-            or cos_sin.get_device() != index or not cos_sin.shape[0] or cos_sin.data_ptr() % 16):
+    shape = cos_sin.shape
+    if (cos_sin.dtype not in (torch.float32, torch.bfloat16) or len(shape) != 2 or not cos_sin.is_contiguous()
+            or cos_sin.get_device() != index or not shape[0] or cos_sin.data_ptr() % 16):
         raise ValueError("Rotation needs a contiguous FP32 or BF16 [table_len, rotary] cos/sin table on one device "
                          "with its tensors")
-    if cos_sin.shape[1] % 16 or not 16 <= cos_sin.shape[1] <= dim:
+    if shape[1] % 16 or not 16 <= shape[1] <= dim:
         raise ValueError("Rotated channels are a multiple of 16, at most the head's")
 
 
@@ -104,7 +105,7 @@ def rotary_embedding(positions, query, key, head_size, cos_sin_cache, is_neox=Tr
                   None, None, rows, query.shape[1], key.shape[1], 64, 1, 1, 1, _lib.stream(query.device))
         return
     for t in (query, key):
-        if (t.dim() != 3 or t.dtype != torch.bfloat16 or kv_paged.aligned(t) is not t
+        if (t.dim() != 3 or t.dtype != torch.bfloat16 or kv_paged.view(t, *t.shape[:2])[0] is not t
                 or any(size > 1 and not stride for size, stride in zip(t.shape, t.stride()))):
             raise ValueError('Rotation in place needs BF16 [T, heads, D] of contiguous channels, 16-byte aligned rows '
                              'and heads of their own (strides multiple of 8)')
@@ -113,28 +114,33 @@ def rotary_embedding(positions, query, key, head_size, cos_sin_cache, is_neox=Tr
 
 def _rotate(q, k, positions, cos_sin, is_neox, q_out, k_out, v=None, cache=None, layer=0, at=None, active=None,
             slots=None):
-    """The call of ``lm_paged_rotate_write``; its tensors but per-row ones are checked."""
-    rows, dim = q.shape[0], q.shape[2]
+    """The call of ``lm_paged_rotate_write`` on BF16 ``[T, heads, D]``; the rest is checked.
+    Results go to ``q_out`` and ``k_out``, new and contiguous or the operands themselves."""
+    rows, q_heads, dim = q.shape
+    k_rows, k_heads, k_dim = k.shape
     index = q.get_device()
     if index < 0:
         _lib.require_cuda(q, k, cos_sin, what="RoPE tensors")
-    if k.shape[0] != rows or k.shape[2] != dim or k.get_device() != index:
+    if k_rows != rows or k_dim != dim or k.get_device() != index:
         raise ValueError("Queries and keys need the same rows and channels, on one device")
     if dim % 16 or dim > 256:
         raise ValueError("Rotation takes heads of a multiple of 16 channels, at most 256")
     check_table(cos_sin, index, dim)
     positions = per_row(positions, rows, torch.int64, index, "positions")
-    where, values, place, slot, mask = (0,) * 7, (0, 0, 0), (0, 0), 0, 0
+    q_in, q_view = kv_paged.view(q, rows, q_heads)
+    k_in, k_view = kv_paged.view(k, rows, k_heads)
+    where, v_view, place, i32, slot, mask = (0,) * 7, (0, 0, 0), 0, False, 0, 0
     if cache is not None:
         kc, vc, table = cache.layer(layer)
         if kv_paged.check_layer(kc, vc, table) != index:
             raise ValueError("The cache must be on its tensors' device")
         pages, heads, page, channels = kc.shape
-        if heads != k.shape[1] or channels != dim or v.shape != k.shape or v.get_device() != index:
+        if heads != k_heads or channels != dim or v.shape != k.shape or v.get_device() != index:
             raise ValueError("Keys and values do not match the cache's heads")
+        v_in, v_view = kv_paged.view(v, rows, heads)
         if at is not None:
             at = kv_paged.places(at, rows, index, "at")
-            place = at.data_ptr(), at.dtype == torch.int32
+            place, i32 = at.data_ptr(), at.dtype is torch.int32
         if slots is not None:
             slots = per_row(slots, rows, torch.int64, index, "slots")
             slot = slots.data_ptr()
@@ -142,14 +148,11 @@ def _rotate(q, k, positions, cos_sin, is_neox, q_out, k_out, v=None, cache=None,
             active = per_row(active, rows, torch.bool, index, "active")
             mask = active.data_ptr()
         where = kc.data_ptr(), vc.data_ptr(), table.data_ptr(), *table.shape, pages, page
-        values = v.data_ptr(), *kv_paged.strides(v)
-    q_view, k_view = (q.data_ptr(), *kv_paged.strides(q)), (k.data_ptr(), *kv_paged.strides(k))
-    # results are new and contiguous, or the operands themselves
-    q_to = q_view if q_out is q else (q_out.data_ptr(), q.shape[1] * dim, dim)
-    k_to = k_view if k_out is k else (0, 0, 0) if k_out is None else (k_out.data_ptr(), k.shape[1] * dim, dim)
-    _lib.call_struct(index, "lm_paged_rotate_write", *q_view, *k_view, *values, cos_sin.data_ptr(), *cos_sin.shape,
-                     cos_sin.dtype == torch.float32, bool(is_neox), positions.data_ptr(), *place, mask, slot, *q_to, *k_to,
-                     *where, rows, q.shape[1], k.shape[1], dim)
+    q_to = q_view if q_out is q else (q_out.data_ptr(), q_heads * dim, dim)
+    k_to = k_view if k_out is k else (0, 0, 0) if k_out is None else (k_out.data_ptr(), k_heads * dim, dim)
+    _lib.call_struct(index, "lm_paged_rotate_write", *q_view, *k_view, *v_view, cos_sin.data_ptr(), *cos_sin.shape,
+                     cos_sin.dtype is torch.float32, bool(is_neox), positions.data_ptr(), place, i32, mask, slot, *q_to,
+                     *k_to, *where, rows, q_heads, k_heads, dim)
 
 
 def rotate_kv_write(q, k, v, positions, active, cos_sin, cache, layer, slots=None, at=None, is_neox=True, keep_k=False):
@@ -166,9 +169,9 @@ def rotate_kv_write(q, k, v, positions, active, cos_sin, cache, layer, slots=Non
     is rounded, as :func:`rope_kv_write` and litemoe/model.py:66-67 have it."""
     if not isinstance(cache, PagedKVCache):
         raise ValueError("rotate_kv_write stores into a paged KV cache")
-    if any(t.dim() != 3 or t.dtype != torch.bfloat16 for t in (q, k, v)):
-        raise ValueError("RoPE supports BF16 [T, heads, D] queries, keys and values")
-    q, k, v = (kv_paged.aligned(t) for t in (q, k, v))
+    for t in (q, k, v):
+        if t.dtype is not torch.bfloat16 or t.dim() != 3:
+            raise ValueError("RoPE supports BF16 [T, heads, D] queries, keys and values")
     q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
     k_out = torch.empty_like(k, memory_format=torch.contiguous_format) if keep_k else None
     _rotate(q, k, positions, cos_sin, is_neox, q_out, k_out, v, cache, layer, at, active, slots)
