@@ -107,6 +107,17 @@ __device__ __forceinline__ T constant(const T *p) {
   return *(const __attribute__((address_space(4))) T *)p;
 }
 
+// Lanes 8 .. 15 of each 16 have from `a` what lanes 0 .. 7 want to have from `b`: swapped.
+__device__ __forceinline__ void in_place(u32x4 &a, u32x4 &b) {
+  constexpr int kRowRor8 = 0x128;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int x = (int)a[i], y = (int)b[i];
+    a[i] = (uint32_t)__builtin_amdgcn_update_dpp(x, y, kRowRor8, 0xf, 0xc, false);
+    b[i] = (uint32_t)__builtin_amdgcn_update_dpp(y, x, kRowRor8, 0xf, 0x3, false);
+  }
+}
+
 // Bytes of LDS before the scores: the merge of the waves and the fused prologue use the
 // same ones in turn; the heads' factors behind them.
 constexpr int kRingFloats = 32 * kTile;  // of a wave: 32 tiles times heads
@@ -200,7 +211,9 @@ __device__ __forceinline__ void attend(const Args &a, const bf16 *__restrict__ q
 
   const int first = lo + wave, tiles = row_tiles(n);  // this wave's tiles: first, first + stride, ...
   const int32_t *row_table = table + b * kv.width;
-  const uint32_t k_off = (uint32_t)(r * D + g * 8) * 2, v_off = (uint32_t)(4 * g * D + r * kCh) * 2;
+  // K is loaded in whole lines, eight positions an instruction, and put in place by
+  // in_place(): lane (r, g) loads 16 bytes of positions r % 8 and r % 8 + 8.
+  const uint32_t k_off = (uint32_t)(r % 8 * D + (r / 8 * 4 + g) * 8) * 2, v_off = (uint32_t)(4 * g * D + r * kCh) * 2;
   const int page_mask = (1 << kv.shift) - 1;
   struct Ids {
     int id[2];
@@ -225,7 +238,7 @@ __device__ __forceinline__ void attend(const Args &a, const bf16 *__restrict__ q
       const char *kb = reinterpret_cast<const char *>(kv.k + from), *vb = reinterpret_cast<const char *>(kv.v + from);
 #pragma unroll
       for (int s = 0; s < kSteps; ++s)
-        x.k[t][s] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(kb + k_off + 64 * s));
+        x.k[t][s] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(kb + k_off + (s % 2 * 8 * D + s / 2 * 64) * 2));
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         x.v[t][i] = __builtin_nontemporal_load(reinterpret_cast<const typename Kv<D>::V *>(vb + v_off + 2 * D * i));
@@ -323,6 +336,10 @@ __device__ __forceinline__ void attend(const Args &a, const bf16 *__restrict__ q
   auto compute = [&](Kv<D> &x, int tile) {
     const int left = n - tile * kTile;  // positions of the row from this tile on
     const bool edge = left < kTile || (kFused && own && tile == tiles - 1) || !x.ok[0] || !x.ok[1];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int s = 0; s < kSteps; s += 2) in_place(x.k[t][s], x.k[t][s + 1]);
     if (kFused && own && tile == tiles - 1) {
       // The new key and value take the place of what was loaded.
       const int at = left - 1;
