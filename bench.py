@@ -83,9 +83,11 @@ def parse():
     ap.add_argument("--long-decode", action="store_true", help="cfg 5 decode step tok/s (own JSON line)")
     ap.add_argument("--kv-bits", type=int, default=16, choices=(4, 8, 16),
                     help="with --long-decode: bits per KV cache element (8 and 4 hold the cache quantised)")
+    ap.add_argument("--kv-page", type=int, default=None,
+                    help="with --long-decode: the KV cache in pages of so many positions (a power of two from 16)")
     args = ap.parse_args()
-    if args.kv_bits != 16 and not args.long_decode:
-        ap.error("--kv-bits goes with --long-decode")
+    if (args.kv_bits != 16 or args.kv_page is not None) and not args.long_decode:
+        ap.error("--kv-bits and --kv-page go with --long-decode")
     return args
 
 
@@ -496,7 +498,8 @@ def long_decode_bench(args):
     model = Granite(cfg, w, ep, cap)
     prompts = synth.prompts(batch, lengths, cfg.vocab_size, 1)
     requests = [Request(str(i), p, 48) for i, p in enumerate(prompts)]
-    engine = OptimizedEngine(model, requests, mode="graph", ignore_eos=True, capacity=cap, kv_bits=args.kv_bits)
+    engine = OptimizedEngine(model, requests, mode="graph", ignore_eos=True, capacity=cap, kv_bits=args.kv_bits,
+                             kv_page=args.kv_page)
     with torch.inference_mode():
         engine.prepare_graph()
         engine.reset()
@@ -531,6 +534,8 @@ def long_decode_bench(args):
     }
     if args.kv_bits != 16:
         line["config"]["kv_bits"] = args.kv_bits
+    if args.kv_page is not None:
+        line["config"]["kv_page"] = args.kv_page
     print(json.dumps(line), flush=True)
 
 
