@@ -78,6 +78,7 @@ struct Shape {
   int shares;  // or equal pieces that all rows' tiles are cut into (0: not)
   float scale;
   int batch;
+  int round;  // rows whose workgroups fill the CUs once
 };
 
 // Positions of a row that are looked at, and their tiles.
@@ -554,7 +555,14 @@ decode_paged_kernel(const bf16 *__restrict__ q, const int32_t *__restrict__ tabl
   const int h = blockIdx.x;
   if constexpr (!kShares) {
     const int split = blockIdx.y, splits = a.sh.splits;
-    const int64_t b = kFused && a.in.order ? constant(a.in.order + blockIdx.z) : blockIdx.z;
+    // An order's rows go to the CUs forth and back: one whose first row is a round's longest
+    // has the next round's shortest (128 rows of 1024 to 4095 positions, longest first:
+    // 105.0 us without, 101.1 so).
+    int64_t b = blockIdx.z;
+    if (kFused && a.in.order) {
+      const int z = blockIdx.z, from = z / a.sh.round * a.sh.round, to = min(from + a.sh.round, a.sh.batch);
+      b = constant(a.in.order + (z / a.sh.round % 2 ? from + to - 1 - z : z));
+    }
     const int held = constant(a.used + b), n = row_length(held, a.sh, a.kv), tiles = row_tiles(n);
     if (splits > 1 && split * kWaves >= tiles) return;
     attend<D, kFused, kWeigh>(a, q, table, b, h, held, n, split * kWaves, tiles, splits * kWaves,
@@ -849,6 +857,7 @@ int launch_decode_paged(const Call &c, Args a, void *workspace, int64_t workspac
   a.sh.splits = (int)c.num_splits;
   a.sh.shares = (int)c.num_shares;
   a.sh.batch = (int)c.batch;
+  a.sh.round = (int)(c.kv_heads < 256 ? 256 / c.kv_heads : 1);
   a.kv.pages = c.pages;
   a.kv.width = (int)c.width;
   a.kv.shift = page_shift(c.page);

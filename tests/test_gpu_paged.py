@@ -456,6 +456,24 @@ def test_fused_is_the_three_calls(lengths, hkv, groups, dim, page, splits, neox,
     assert torch.equal(frag.to_rows(), exp.view(b, -1))
 
 
+@pytest.mark.parametrize("rows,hkv", [(70, 8), (32, 8), (33, 8), (5, 130)])
+@torch.inference_mode()
+def test_fused_order_of_many_rows(rows, hkv):
+    """Every row once, whatever the order and however many rounds of workgroups the rows make."""
+    lengths = [1 + (11 * i) % 50 for i in range(rows)]
+    caches = [random_cache(lengths, hkv, 64, 16, 7)[0] for _ in range(2)]
+    part = torch.randn(2, rows, 3 * hkv * 64, generator=gen(3)).to(DEV)
+    cos_sin = rope.rotary_table(64, 64, 10000.0, device=DEV)
+    used = torch.tensor(lengths, dtype=torch.int32, device=DEV)
+    order = torch.argsort(used, descending=True, stable=True).int()
+    got = [PagedFlashDecode(rows, hkv, 1, c.capacity, DEV).fused_qkv(
+        part, cos_sin, used.long() - 1, None, *c.layer(0), 0.125, used, hkv, row_order=o)
+        for c, o in zip(caches, (None, order))]
+    assert bool(got[0].isfinite().all()) and torch.equal(*got)
+    for side in ("k", "v"):
+        assert torch.equal(*(getattr(c, side).view(torch.int16) for c in caches))
+
+
 @pytest.mark.parametrize("splits", [None, 3])
 @torch.inference_mode()
 def test_fused_row_without_a_place(splits):
