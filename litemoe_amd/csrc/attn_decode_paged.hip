@@ -1,17 +1,27 @@
-// Split-K decode attention over the paged KV cache on the matrix cores:
+// Decode attention over the paged KV cache on the matrix cores:
 //   out[b, h] = softmax_j(scale q_h . K_j) V,  j < used[b].
 //
-// Workgroup (kv head, split, row); its waves take the split's tiles of 32
-// positions in turn, each wave its own, without barriers, with two tiles of K and
-// V in registers on their way. A tile is two halves of 16 positions, and a page
-// holds a multiple of 16, so a half lies in one page: its number is a scalar load
-// two tiles ahead, and the lanes' offsets from the half's first position are
-// constants. Every KV byte is read once, straight into MFMA operands.
+// The KV stream bounds it (4 D bytes a position and KV head for 4 D operations of each
+// of its query heads), so everything serves that. A workgroup takes tiles of 32
+// positions of one row and KV head, each of its four waves its own, without barriers,
+// with two tiles of K and V in registers on their way. A tile is two halves of 16
+// positions, and a page holds a multiple of 16, so a half lies in one page: its number
+// is a scalar load two tiles ahead, and the lanes' offsets from the half's first
+// position are constants. Every KV byte is read once, straight into MFMA operands.
+//
+// us per launch in a graph, 24 query heads over 8 of D = 64, random pages of 64: 128 rows
+// of 1024 to 4095 positions 106.5 (6.3 TB/s of 6.9 that a bare read of such tiles
+// reaches), 101.3 fused and in an order (6.6 TB/s); 64 rows of 1025 to 1279 26.1 (5.8),
+// fused the same; 32 rows of 8191 to 32768 203 (6.6); 8 such rows of D = 128 106.5 (6.3);
+// one row of 509 5.6 (launch, three latencies, the merge). Pages of 16 cost 1%.
 //
 // Scores: S = K . q^T with v_mfma_f32_16x16x32_bf16, A the 16 positions of a half
 // (lane l: position l % 16, 16 bytes of channels), B the query heads of the KV head
 // (column l % 16; columns past the G heads are zero). Lane l then holds positions
-// 4 (l / 16) .. + 3 of both halves for query head l % 16.
+// 4 (l / 16) .. + 3 of both halves for query head l % 16. Loaded in that layout, an
+// instruction touches 16 lines and takes half of each. K is loaded in whole lines of
+// eight positions instead, and lanes 8 apart swap (24 vector instructions a tile of D
+// = 64): 128 ragged rows 112.4 -> 106.5 us, bare reads of such tiles 105.1 -> 96.9.
 //
 // P.V: O^T = V^T . P^T. The sum over positions may take them in any order that both
 // operands share, so a lane's eight probabilities are its B operand as they stand: k
@@ -24,7 +34,8 @@
 //
 // The running maximum is a column's own reference, kept kAbove over the score that
 // set it and moved only when a score passes it, so nothing crosses lanes in the
-// usual tile. Waves merge through LDS, splits by log-sum-exp in a second launch.
+// usual tile. Waves merge through LDS, a row's workgroups by log-sum-exp in a second
+// launch.
 //
 // Masked positions (past used[b], or in no page) may hold anything: their scores
 // become -inf and their V words 0. Only a row's last tile and tiles with a page
@@ -143,7 +154,8 @@ struct Args {
 };
 
 // Weights: none; scores to the workspace, for a launch of their own; or scores in LDS
-// and the weights added here, where a workgroup holds the row.
+// and the weights added here, where a workgroup holds the row (64 rows of 1025 to 1279
+// positions, 24 query heads over 8: 36.0 us by way of the workspace, 29.2 in LDS; now 27.1).
 enum Weigh { kNone, kScores, kHeld };
 
 __device__ __forceinline__ int64_t out_index(const Args &a, int64_t b, int hq, int c, int dim) {
@@ -312,7 +324,7 @@ __device__ __forceinline__ void attend(const Args &a, const bf16 *__restrict__ q
   // kScores: a wave's scores of its last tiles, stored together, whole lines of one head by
   // eight lanes. Loads and stores return in the order they were issued, so a store behind
   // every tile holds the stream up: 64 rows of 500 to 8000 positions, 3 query heads per KV
-  // head, 137 us with one behind every tile, 133 in this way.
+  // head, 137 us with one behind every tile, 133 in this way (K in half lines; now 124).
   const int ring = G <= 4 ? 8 : G <= 8 ? 4 : 2;
   float *sm_ring = sm_f + 2 * G + wave * kRingFloats;
   int ringed = 0;
@@ -547,7 +559,7 @@ __device__ __forceinline__ void attend(const Args &a, const bf16 *__restrict__ q
 // reads some 35 GB/s, so the rate of the whole falls with its emptiest CU; a workgroup
 // adds up the rows' tiles itself.
 // Registers: four waves per SIMD where splits give a CU four workgroups (D = 64). With
-// scores to store that would spill (145 us for the 133 above), and shares give a CU two.
+// scores to store that would spill (145 us for those 133), and shares give a CU two.
 template <int D, bool kFused, int kWeigh, bool kShares>
 __global__ void __launch_bounds__(kThreads, D == 128 || kShares ? 2 : kWeigh == kScores ? 3 : 4)
 decode_paged_kernel(const bf16 *__restrict__ q, const int32_t *__restrict__ table, Args a) {
@@ -695,6 +707,9 @@ decode_paged_combine_kernel(Args a) {
 // after[b, h, j] = before[b, h, j] + sum over the KV head's query heads of their
 // probability of position j, j < the row's length. A thread four positions. The first
 // workgroup of a (row, KV head) also joins the pieces' results, as the launch above.
+// Bound by the scores' way to memory and back (24 bytes a position and KV head of three
+// query heads, beside 256 of K and V) and, in small calls, by its launch: 64 rows of 500
+// to 8000 positions 124 us with weights and 89.5 without, 3 rows to 4001 12.5 and 10.6.
 constexpr int kWeighThreads = 256, kWeighSpan = 4 * kWeighThreads, kAhead = 4;
 template <int D>
 __global__ void __launch_bounds__(kWeighThreads)

@@ -12,7 +12,10 @@
 // Move: every kept position's K and V go from the row's pages to their place in the
 // target's pages, a second launch over (kept, KV head, layer and row). Out of place,
 // so that pages which another row shares are left as they are and no order of the
-// moves matters.
+// moves matters. Bound by the copy: 8 layers of 16 rows, 1024 positions of 8 heads of 64
+// channels each (537 MB in and out) 105 us, 5.1 TB/s (a copy of 2 GiB 4.9). The selection
+// of those 1024 rows of 2049 to 4095 weights, 33 MB in and out, takes 23 us: latency of
+// LDS and of the passes one after the other; 128 rows of 600 to 700 6.2 us.
 //
 // The reference holds every position to the end (litemoe/cache.py:7-20).
 #include "paged.h"

@@ -271,13 +271,44 @@ class QuantFlashDecode:
 
 
 def paged_splits(batch, kv_heads, maximum):
-    """Key-range splits over a paged cache."""
+    """Key-range splits over a paged cache: workgroups that take a row's tiles of 32
+    positions in turn, so that every row is cut by its own length.
+
+    Up to 256 (row, KV head) pairs the splits fill the CUs once, with eight tiles or
+    more for each (two for each of its waves); bounds under 768 positions are not split,
+    since the second launch costs 2 us. us per launch in a graph, 8 KV heads of 64
+    channels: one row of 509 positions 5.6 (1 split) and 6.4 to 6.8 (2 to 64); 767
+    7.3 (1), 7.2 (4) and 6.6 (8); 1000 8.5 (1), 7.3 (4) and 7.0 (8); 4000 24.8 (1),
+    11.6 (4), 8.8 (16) and 10.1 (32); 32768 174 (1), 19.4 (16), 18.5 (32) and 21.8
+    (64); 3 rows to 4001 25.0 (1), 9.6 (8), 10.3 (10) and 10.6 (16); 8 rows to 4095 25.6
+    (1), 13.3 (4) and 13.9 (8); 16 rows to 4095 26.4 (1), 20.4 (2) and 21.0 (8).
+
+    From 129 pairs on, one split: rows of one length lose by more (20 rows of 2000
+    positions 17.8 with 1 and 18.8 with 4, 28 rows 19.9 and 24.1, 28 rows of 800 10.4 and
+    14.0), ragged ones may gain (20 rows of 1024 to 4095 28.4 and 25.3, 24 rows 28.0 and
+    25.9, 28 rows 30.0 and 31.9, 64 rows 60.7 and 60.9)."""
     tiles, pairs = -(-maximum // 32), max(1, batch * kv_heads)
     return max(1, min(256 // pairs, -(-tiles // 8))) if tiles >= 24 else 1
 
 
 def paged_shares(batch, kv_heads, maximum, head_dim):
-    """Equal shares per KV head that the rows of a paged cache are cut into, or 0."""
+    """Equal shares per KV head that the tiles of all rows are cut into, one row after the
+    other, or 0 where rows are cut by :func:`paged_splits` instead.
+
+    Every workgroup then streams as many bytes, however ragged the rows, for a search of
+    the row that a share begins in, results of rows in several shares to be joined, and a
+    second launch. As many shares as run at once: two workgroups a CU, with heads of 128
+    channels one (more than fill the CUs evenly wait for a round of their own). Where the
+    bound's rows together are 256 MB or more (up to 1024 rows: every workgroup reads their
+    lengths). us per launch in a graph, splits (1 unless marked) and 64 shares, 8 KV heads
+    of 64 channels, rows of 1024 to 4095 positions: 24 rows 28.0 and 27.3, 32 32.3 and
+    33.1, 48 53.9 (47.1 with 4) and 45.6, 64 60.7 and 57.4, 128 116.3 (112.2 with 3) and
+    106.5; 64 rows of 500 to 8000 104.1 and 89.5; 256 rows of 300 to 4095 190.7 and 182.5;
+    rows of one length lose by it: 64 rows of 1025 to 1279 25.8 and 30.5, of 3500 to 4095
+    76.4 and 79.1, 128 rows of 2500 98.4 and 101.1. By the shares' number: 128 ragged rows
+    106.9 (32), 116.9 (48), 106.5 (64), 107.6 (96) and 108.4 (128); 8 rows of 8191 to 32768
+    with 128 channels 106.6 (24 and 32), 116.2 (48) and 108.5 (64), in splits 118.9 (4) and
+    112.0 (16)."""
     if batch * maximum * kv_heads * head_dim * 4 < 256e6 or batch > 1024:
         return 0
     return max(1, (512 if head_dim == 64 else 256) // kv_heads)
