@@ -132,7 +132,9 @@ __device__ __forceinline__ void in_place(u32x4 &a, u32x4 &b) {
 
 // Bytes of LDS before the scores: the merge of the waves and the fused prologue use the
 // same ones in turn; the heads' factors behind them.
-constexpr int kRingFloats = 32 * kTile;  // of a wave: 32 tiles times heads
+// Tiles whose scores a wave stores together; its ring takes 8 KB at most. (Eight tiles for
+// every G: 135 us against 136 at 8 heads a KV head, 159 and 158 at 16.)
+__host__ __device__ constexpr int ring_tiles(int G) { return G <= 4 ? 8 : 4; }
 __host__ __device__ constexpr int lds_bytes(int D, int G, bool fused) {
   const int merge = kWaves * G * (D + 2) * 4, rot = fused ? (G + 2) * D * (2 + 4) : 0;
   return ((merge > rot ? merge : rot) + 2 * G * 4 + 15) / 16 * 16;
@@ -325,8 +327,8 @@ __device__ __forceinline__ void attend(const Args &a, const bf16 *__restrict__ q
   // eight lanes. Loads and stores return in the order they were issued, so a store behind
   // every tile holds the stream up: 64 rows of 500 to 8000 positions, 3 query heads per KV
   // head, 137 us with one behind every tile, 133 in this way (K in half lines; now 124).
-  const int ring = G <= 4 ? 8 : G <= 8 ? 4 : 2;
-  float *sm_ring = sm_f + 2 * G + wave * kRingFloats;
+  const int ring = ring_tiles(G);
+  float *sm_ring = sm_f + 2 * G + wave * ring * G * kTile;
   int ringed = 0;
   auto store_scores = [&](int end) {  // of the tiles before `end`
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // other lanes wrote what this one reads
@@ -706,72 +708,78 @@ decode_paged_combine_kernel(Args a) {
 
 // after[b, h, j] = before[b, h, j] + sum over the KV head's query heads of their
 // probability of position j, j < the row's length. A thread four positions. The first
-// workgroup of a (row, KV head) also joins the pieces' results, as the launch above.
+// workgroups of a (row, KV head) join the pieces' results, as the launch above.
 // Bound by the scores' way to memory and back (24 bytes a position and KV head of three
 // query heads, beside 256 of K and V) and, in small calls, by its launch: 64 rows of 500
-// to 8000 positions 124 us with weights and 89.5 without, 3 rows to 4001 12.5 and 10.6.
-constexpr int kWeighThreads = 256, kWeighSpan = 4 * kWeighThreads, kAhead = 4;
+// to 8000 positions in shares 119 us with weights and 89.5 without, 3 rows to 4001 11.2 and
+// 10.6, 3 rows to 6157 with 16 query heads a KV head and D = 128 24.6 and 19.4. There the
+// first workgroup of a (row, KV head) joined all its pieces before: 43.4.
+constexpr int kWeighThreads = 256, kWeighSpan = 4 * kWeighThreads;
 template <int D>
 __global__ void __launch_bounds__(kWeighThreads)
 weigh_kernel(Args a) {
-  __shared__ float sm_m[kMaxGroups], sm_f[kMaxGroups];
-  const int h = blockIdx.y, G = a.sh.G;
+  const int h = blockIdx.y, G = a.sh.G, tid = threadIdx.x;
   const int64_t b = blockIdx.z;
   const Partial &part = a.part;
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  const int n = row_length(a.used[b], a.sh, a.kv), j = (blockIdx.x * kWeighThreads + threadIdx.x) * 4;
-  if (blockIdx.x && (int)blockIdx.x * kWeighSpan >= n) return;
+  const int joins = (G * D + kWeighThreads - 1) / kWeighThreads, span = (int)blockIdx.x - joins;
+  if (span < 0) {
+    const Pieces x = pieces_of(a, b);
+    const int t = blockIdx.x * kWeighThreads + tid, gh = t / D, c = t % D;
+    if (x.count == 1 || gh >= G) return;
+    a.out[out_index(a, b, h * G + gh, c, D)] = (bf16)f32_to_bf16(joined<D>(a, x, x.count, h, gh, c));
+    return;
+  }
+  const int n = row_length(a.used[b], a.sh, a.kv), j = span * kWeighSpan + tid * 4;
+  if (span * kWeighSpan >= n) return;
   // The scores and weights of this thread's positions are on their way while the
   // heads' sums are joined. The buffers hold a multiple of 16 positions a row.
   const float *sc = part.s + (b * a.sh.q_heads + h * G) * part.padded + j;
   const int64_t at = (b * a.kv.heads + h) * ((int64_t)a.kv.width << a.kv.shift) + j;
-  f32x4 s[kAhead], old{0.f, 0.f, 0.f, 0.f};
+  f32x4 s[kMaxGroups], old{0.f, 0.f, 0.f, 0.f};
   if (j < n) {
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) s[i] = *reinterpret_cast<const f32x4 *>(sc + min(i, G - 1) * part.padded);
+    for (int gh = 0; gh < kMaxGroups; ++gh)
+      if (gh < G) s[gh] = *reinterpret_cast<const f32x4 *>(sc + gh * part.padded);
     old = *reinterpret_cast<const f32x4 *>(a.before + at);
   }
+  // Every head by 16 lanes.
+  __shared__ float sm_m[kMaxGroups], sm_f[kMaxGroups];
   const Pieces x = pieces_of(a, b);
-  for (int gh = wave; gh < G; gh += kWeighThreads / kWave) {
-    float mx = kEmpty, l = 0.f;
+  constexpr int kLanes = kWeighThreads / kMaxGroups;
+  const int gh = tid / kLanes, lane = tid % kLanes;
+  float mx = kEmpty, l = 0.f;
+  if (gh < G) {
     if (x.count == 1) {
       mx = part.rm[b * a.sh.q_heads + h * G + gh];
-      l = part.rl[b * a.sh.q_heads + h * G + gh];
+      l = lane == 0 ? part.rl[b * a.sh.q_heads + h * G + gh] : 0.f;
     } else {
-      for (int i = lane; i < x.count; i += kWave) mx = fmaxf(mx, part.m[slot_of(a, x, i, h, gh)]);
-#pragma unroll
-      for (int d = 1; d < kWave; d *= 2) mx = fmaxf(mx, shfl_xor(mx, d));
-      for (int i = lane; i < x.count; i += kWave) {
+      for (int i = lane; i < x.count; i += kLanes) {
         const int64_t slot = slot_of(a, x, i, h, gh);
-        l += part.l[slot] * __builtin_amdgcn_exp2f(part.m[slot] - mx);
+        const float m = part.m[slot], more = part.l[slot], to = fmaxf(mx, m);
+        l = l * __builtin_amdgcn_exp2f(mx - to) + more * __builtin_amdgcn_exp2f(m - to);
+        mx = to;
       }
-      l = wave_sum(l);
     }
-    if (lane == 0) {
-      sm_m[gh] = mx;
-      sm_f[gh] = l == 0.f ? 0.f : 1.f / l;
-    }
+  }
+  float to = mx;
+#pragma unroll
+  for (int d = 1; d < kLanes; d *= 2) to = fmaxf(to, shfl_xor(to, d));
+  l *= __builtin_amdgcn_exp2f(mx - to);
+#pragma unroll
+  for (int d = 1; d < kLanes; d *= 2) l += shfl_xor(l, d);
+  if (lane == 0) {
+    sm_m[gh] = to;
+    sm_f[gh] = l == 0.f ? 0.f : 1.f / l;
   }
   __syncthreads();
-  if (blockIdx.x == 0 && x.count != 1) {
-    for (int t = threadIdx.x; t < G * D; t += kWeighThreads) {
-      const int gh = t / D, c = t % D;
-      a.out[out_index(a, b, h * G + gh, c, D)] = (bf16)f32_to_bf16(joined<D>(a, x, x.count, h, gh, c));
-    }
-  }
   if (j >= n) return;
   float w[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int g0 = 0; g0 < G; g0 += kAhead) {
-    if (g0) {
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) s[i] = *reinterpret_cast<const f32x4 *>(sc + min(g0 + i, G - 1) * part.padded);
-    }
+  for (int gh = 0; gh < kMaxGroups; ++gh) {
+    if (gh < G) {
+      const float m = sm_m[gh], f = sm_f[gh];
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      if (g0 + i >= G) break;
-      const float m = sm_m[g0 + i], f = sm_f[g0 + i];
-#pragma unroll
-      for (int y = 0; y < 4; ++y) w[y] += __builtin_amdgcn_exp2f(s[i][y] - m) * f;
+      for (int y = 0; y < 4; ++y) w[y] += __builtin_amdgcn_exp2f(s[gh][y] - m) * f;
     }
   }
   if (j + 4 <= n) {
@@ -789,8 +797,14 @@ struct Call {
 
 int64_t padded_scores(int64_t max_len) { return align_up(max_len, kTile); }
 
-// Scores that a workgroup keeps: three of them and the merge fit a CU's 160 KB of LDS.
-constexpr int64_t kHeldBytes = 32 << 10;
+// Scores that a workgroup keeps: with the merge they fit a CU's 160 KB of LDS, though one
+// workgroup then has it to itself. us with weights, in LDS and by way of memory (in shares,
+// where that is faster), 8 KV heads: 64 rows of 1025 to 1279 positions, 8 query heads each
+// (40 KB) 28.1 and 44.3, 16 (80 KB) 35.0 and 48.6; 64 rows of 1024 to 4000, 3 query heads
+// (47 KB) 62.0 and 72.9; 128 such rows, 6 query heads (94 KB) 119 and 154; 64 rows of 500 to
+// 8000, 3 (94 KB) 106 and 119; 32 rows of 500 to 9000, 3 (106 KB) 65.5 and 69.0.
+constexpr int64_t kHeldBytes = 120 << 10;
+static_assert(kHeldBytes + lds_bytes(128, kMaxGroups, true) <= 160 << 10, "the LDS of a CU");
 bool scores_held(int64_t groups, int64_t max_len) { return groups * padded_scores(max_len) * 4 <= kHeldBytes; }
 
 // Weights added by the workgroup that holds the row.
@@ -836,7 +850,7 @@ int launch_sized(const Call &c, const Args &a, hipStream_t s) {
   const dim3 grid = kShares ? dim3((unsigned)c.kv_heads, (unsigned)a.sh.shares)
                             : dim3((unsigned)c.kv_heads, (unsigned)a.sh.splits, (unsigned)c.batch);
   const int64_t lds = lds_bytes(D, a.sh.G, kFused) + (kWeigh == kHeld     ? a.sh.G * padded_scores(a.sh.max_len) * 4
-                                                      : kWeigh == kScores ? kWaves * kRingFloats * 4
+                                                      : kWeigh == kScores ? kWaves * ring_tiles(a.sh.G) * a.sh.G * kTile * 4
                                                                           : 0);
   decode_paged_kernel<D, kFused, kWeigh, kShares><<<grid, kThreads, lds, s>>>(a.q, a.table, a);
   LM_CHECK_LAUNCH();
@@ -846,7 +860,8 @@ int launch_sized(const Call &c, const Args &a, hipStream_t s) {
     LM_CHECK_LAUNCH();
   }
   if (kWeigh == kScores) {
-    weigh_kernel<D><<<dim3((unsigned)cdiv(a.sh.max_len, kWeighSpan), (unsigned)c.kv_heads, (unsigned)c.batch),
+    const int64_t joins = cdiv(a.sh.G * D, kWeighThreads);
+    weigh_kernel<D><<<dim3((unsigned)(joins + cdiv(a.sh.max_len, kWeighSpan)), (unsigned)c.kv_heads, (unsigned)c.batch),
                       kWeighThreads, 0, s>>>(a);
     LM_CHECK_LAUNCH();
   }

@@ -338,16 +338,20 @@ class PagedFlashDecode:
         self.shares = 0 if num_splits else paged_shares(batch, kv_heads, self.maximum, head_dim)
         self.device = torch.device(device)
         self.workspace = self._space(False)
-        self.weigh_space = None  # the larger workspace of a call with weights, made by the first
+        # calls with weights: their splits and shares, and a larger workspace, made by the first
+        self.weigh_cut = self.weigh_space = None
         self.row_order = (torch.empty(batch, dtype=torch.int32, device=self.device)
                           if ordered and self.device.type == "cuda" else None)
 
+    def _bytes(self, cut, weighed):
+        return _lib.size_query("lm_flash_decode_paged_workspace_size", self.batch, self.kv_heads * self.groups,
+                               self.kv_heads, self.head_dim, self.maximum, *cut, int(weighed))
+
     def _space(self, weighed):
+        """A workspace for calls in splits, which the fused ones are, and in shares."""
         size = 0
-        if self.device.type == "cuda":  # one for calls in splits and calls in shares
-            sizes = self.batch, self.kv_heads * self.groups, self.kv_heads, self.head_dim, self.maximum
-            size = max(_lib.size_query("lm_flash_decode_paged_workspace_size", *sizes, *cut, int(weighed))
-                       for cut in ((self.splits, 0), (1, self.shares)))
+        if self.device.type == "cuda":
+            size = max(self._bytes(cut, weighed) for cut in ((self.splits, 0), (1, self.shares)))
         return torch.empty(max(size, 1), dtype=torch.uint8, device=self.device)
 
     def _check(self, k, v, table, q_heads, rows):
@@ -365,11 +369,11 @@ class PagedFlashDecode:
         return index
 
     def _weights(self, weights, weights_out, rows, index):
-        """The pointers of a call's weights and the workspace it takes."""
+        """The pointers of a call's weights, the workspace it takes, and how it cuts the rows."""
         if weights is None:
             if weights_out is not None:
                 raise ValueError("weights_out goes with weights")
-            return 0, 0, self.workspace
+            return 0, 0, self.workspace, (1, self.shares) if self.shares else (self.splits, 0)
         weights_out = weights if weights_out is None else weights_out
         for w in (weights, weights_out):
             if (w.dtype != torch.float32 or w.dim() != 3 or w.shape[0] < rows
@@ -377,8 +381,12 @@ class PagedFlashDecode:
                     or w.get_device() != index or w.data_ptr() % 16):
                 raise ValueError("Weights must be contiguous fp32 [B, H, capacity] on the cache's device")
         if self.weigh_space is None:
+            # Rows that fill the CUs unsplit, their scores in LDS (no workspace is asked for then),
+            # are faster so than in shares: 128 rows of 1024 to 4000 positions 125 and 141 us.
+            held = self.splits == 1 and not self._bytes((1, 0), True)
+            self.weigh_cut = (self.splits, 0) if held or not self.shares else (1, self.shares)
             self.weigh_space = self._space(True)
-        return weights.data_ptr(), weights_out.data_ptr(), self.weigh_space
+        return weights.data_ptr(), weights_out.data_ptr(), self.weigh_space, self.weigh_cut
 
     def __call__(self, q, k, v, table, lengths, active, scale, used=None, weights=None, weights_out=None):
         """Attention of ``q [B, Hq, 1, D]`` over the first ``used[b]`` positions of each
@@ -401,12 +409,11 @@ class PagedFlashDecode:
         if used is None:
             used = torch.where(active, lengths + 1, 1)
         used = kv_quant.per_row(used, b, torch.int32, index, "used")
-        before, after, space = self._weights(weights, weights_out, b, index)
+        before, after, space, cut = self._weights(weights, weights_out, b, index)
         out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(q.shape)
         _lib.call_struct(index, "lm_flash_decode_paged", q.data_ptr(), rows, heads, k.data_ptr(), v.data_ptr(),
                          table.data_ptr(), table.shape[1], k.shape[0], k.shape[2], used.data_ptr(), b, hq, self.kv_heads,
-                         d, scale, self.maximum, 1 if self.shares else self.splits, self.shares, before, after,
-                         out.data_ptr(), space.data_ptr(), space.numel())
+                         d, scale, self.maximum, *cut, before, after, out.data_ptr(), space.data_ptr(), space.numel())
         return out
 
     def fused_qkv(self, partials, cos_sin, positions, active, k, v, table, scale, used, q_heads, row_order=None,
@@ -430,7 +437,7 @@ class PagedFlashDecode:
         if row_order is not None and (row_order.dtype != torch.int32 or row_order.shape != (b,)
                                       or row_order.get_device() != index or not row_order.is_contiguous()):
             raise ValueError("row_order must be an int32 [B] permutation")
-        before, after, space = self._weights(weights, weights_out, b, index)
+        before, after, space, _ = self._weights(weights, weights_out, b, index)
         if frag_out:
             out = FragRows(b, q_heads * self.head_dim, k.device)
             out_ptr = out.data.data_ptr()

@@ -234,8 +234,11 @@ ATTENTIONS = [
     ([300, 5], 1, 16, 64, 32, None), ([300, 5], 1, 16, 64, 32, 3), ([95, 96, 97, 64], 3, 8, 64, 128, 2),
     ([1, 0, 33], 1, 1, 128, 16, None), ([700, 40, 0], 2, 4, 128, 256, None), ([513, 16, 31], 2, 5, 128, 32, 4),
     ([260], 1, 16, 128, 64, 1), ([2049, 4001], 2, 2, 64, 32, 16), ([2049, 1500], 1, 6, 64, 64, 40),
-    # one split, scores past what a workgroup keeps (8, 4 and 2 tiles stored together), and the most it keeps
-    ([4500, 100], 1, 2, 64, 16, 1), ([2900, 31, 257], 1, 3, 128, 64, 1), ([2000, 1], 1, 5, 64, 64, 1),
+    # one split, scores past what a workgroup keeps (8 and 4 tiles stored together)
+    ([7800, 100], 1, 4, 64, 16, 1), ([10500, 1], 1, 3, 64, 64, 1), ([4000, 31, 257], 1, 8, 64, 64, 1),
+    ([2000, 129], 1, 16, 64, 64, 1), ([3500, 95, 0], 1, 9, 128, 32, 1),
+    # and the most it keeps
+    ([1920, 60], 1, 16, 128, 128, 1), ([3800, 10], 1, 8, 64, 64, 1), ([4500, 100], 1, 2, 64, 16, 1), ([2900, 31, 257], 1, 3, 128, 64, 1), ([2000, 1], 1, 5, 64, 64, 1),
     ([1100, 40, 0], 2, 8, 64, 32, 1), ([1000, 95], 1, 9, 128, 32, 1), ([600, 129], 1, 16, 64, 64, 1),
     ([512, 480], 1, 16, 128, 64, 1),
 ]
@@ -301,6 +304,7 @@ def test_attention_in_shares(lengths, hkv, groups, dim, page, shares):
     p = check_attention(got, q, k[0], v[0], table, used, scale)
     before = torch.rand(b, hkv, cache.capacity, generator=gen(seed))
     w = before.to(DEV)
+    flash.weigh_space, flash.weigh_cut = flash._space(True).fill_(255), (1, shares)
     assert torch.equal(flash(*args, weights=w), got)
     for i, n in enumerate(lengths):
         assert torch.equal(w[i, :, n:].cpu(), before[i, :, n:])
@@ -326,7 +330,17 @@ def test_shares_are_the_plan_of_large_batches():
     used = torch.tensor(lengths, dtype=torch.int32)
     for f in (flash, split):
         got = f(q.to(DEV)[:, :, None], *cache.layer(0), None, None, 0.125, used=used.to(DEV))
-        check_attention(got, q, k[0], v[0], table, used, 0.125)
+        p = check_attention(got, q, k[0], v[0], table, used, 0.125)
+        w = torch.zeros(b, hkv, cache.capacity, device=DEV)
+        f(q.to(DEV)[:, :, None], *cache.layer(0), None, None, 0.125, used=used.to(DEV), weights=w)
+        for i, n in enumerate(lengths):
+            tol = weight_bound(q, k[0], table, i, n, 0.125, p[i], torch.zeros(1))
+            assert bool(((w[i, :, :n].double().cpu() - p[i].sum(1)).abs() <= tol).all()) and not w[i, :, n:].any()
+    # with weights a workgroup keeps the rows' scores, where they fit; else the shares stand
+    assert flash.weigh_cut == (1, 0) and split.weigh_cut == (2, 0)
+    wide = PagedFlashDecode(b, hkv, 8, cache.capacity, DEV)
+    wide._weights(w, w, b, w.get_device())
+    assert wide.weigh_cut == (1, 64)
 
 
 @torch.inference_mode()
@@ -415,7 +429,8 @@ def test_pages_past_32_bits():
 @pytest.mark.parametrize("lengths,hkv,groups,dim,page,splits", [
     ([1], 1, 1, 64, 16, None), ([17, 32, 33, 1, 64], 2, 3, 64, 16, None), ([1000, 500, 31], 8, 2, 64, 64, 4),
     ([130, 129, 128], 1, 16, 64, 128, 2), ([40, 257], 2, 4, 128, 32, None), ([600, 20], 1, 16, 128, 256, 3),
-    ([1100, 40, 97], 2, 8, 64, 32, 1), ([1000, 95], 1, 9, 128, 32, 1), ([512, 480], 1, 16, 128, 64, 1)])
+    ([1100, 40, 97], 2, 8, 64, 32, 1), ([1000, 95], 1, 9, 128, 32, 1), ([512, 480], 1, 16, 128, 64, 1),
+    ([2000, 40], 1, 16, 128, 64, 1), ([1920, 60], 1, 16, 128, 128, 1)])
 @torch.inference_mode()
 def test_fused_is_the_three_calls(lengths, hkv, groups, dim, page, splits, neox, f32, rotary, weighed):
     """The decode layer's form against rotate_kv_write and the attention, bit for bit: outputs, cache and weights;

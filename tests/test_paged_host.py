@@ -316,7 +316,7 @@ def test_structs_are_the_headers(name):
     (lambda h: decode(h, w=_P), 1), (lambda h: decode(h, w_out=_P), 1), (lambda h: decode(h, w=_P + 4, w_out=_P), 1),
     (lambda h: decode(h, shares=2, size=100), 4), (lambda h: decode(h, shares=2, w=_P, w_out=_P, ws=None), 4),
     (lambda h: decode(h, shares=2, ws=_P + 4), 1), (lambda h: decode(h, splits=2, size=100), 4),
-    (lambda h: decode(h, w=_P, w_out=_P, max_len=4097, width=300, size=100), 4), (lambda h: decode(h, batch=65536), 1),
+    (lambda h: decode(h, w=_P, w_out=_P, max_len=15361, width=300, size=100), 4), (lambda h: decode(h, batch=65536), 1),
     (lambda h: fused(h, batch=0), 0), (lambda h: fused(h, slices=9), 2), (lambda h: fused(h, slices=0), 1),
     (lambda h: fused(h, rotary=72), 1), (lambda h: fused(h, cos=None), 1), (lambda h: fused(h, part=_P + 4), 1),
     (lambda h: fused(h, batch=129, frag=1), 2), (lambda h: fused(h, pos=None), 1), (lambda h: fused(h, page=20), 2),
@@ -339,8 +339,8 @@ def test_workspace_sizes():
     assert size(1, 5, 0) == 256 + 5 * 8 * 2 * 128 * 4 + 2 * 512
     scores = 2 * 256 + 3 * 8 * 128 * 4
     assert size(4, 0, 1) == size(4, 0, 0) + scores and size(1, 5, 1) == size(1, 5, 0) + scores
-    # four query heads' scores of 2080 positions are more than a workgroup keeps
-    assert size(1, 0, 1, 2048) == 0 and size(1, 0, 1, 2049) == 2 * 256 + 3 * 8 * 2080 * 4
+    # four query heads' scores of 7712 positions are more than a workgroup keeps
+    assert size(1, 0, 1, 7680) == 0 and size(1, 0, 1, 7681) == 2 * 256 + 3 * 8 * 7712 * 4
 
 
 # ------------------------------------------------------------------ oracle --
