@@ -355,10 +355,11 @@ class PagedFlashDecode:
         return torch.empty(max(size, 1), dtype=torch.uint8, device=self.device)
 
     def _check(self, k, v, table, q_heads, rows):
-        """The layer's device index, once it is what this object was built for."""
+        """The layer's device index and its ``width, pages, page``, once it is what this
+        object was built for."""
         index = kv_paged.check_layer(k, v, table)
-        _, heads, page, dim = k.shape
-        if rows > self.batch or table.shape[0] < rows or table.shape[1] * page != self.capacity:
+        (pages, heads, page, dim), (lines, width) = k.shape, table.shape
+        if rows > self.batch or lines < rows or width * page != self.capacity:
             raise ValueError("Decode attention built for another batch/capacity")
         if heads != self.kv_heads or dim != self.head_dim:
             raise ValueError("Decode attention built for other cache heads")
@@ -366,7 +367,7 @@ class PagedFlashDecode:
             raise ValueError("Query heads do not match the cache heads")
         if self.workspace.get_device() != index:
             raise ValueError("Decode attention built for another device")
-        return index
+        return index, (width, pages, page)
 
     def _weights(self, weights, weights_out, rows, index):
         """The pointers of a call's weights, the workspace it takes, and how it cuts the rows."""
@@ -375,10 +376,10 @@ class PagedFlashDecode:
                 raise ValueError("weights_out goes with weights")
             return 0, 0, self.workspace, (1, self.shares) if self.shares else (self.splits, 0)
         weights_out = weights if weights_out is None else weights_out
-        for w in (weights, weights_out):
-            if (w.dtype != torch.float32 or w.dim() != 3 or w.shape[0] < rows
-                    or w.shape[1:] != (self.kv_heads, self.capacity) or not w.is_contiguous()
-                    or w.get_device() != index or w.data_ptr() % 16):
+        for w in (weights,) if weights_out is weights else (weights, weights_out):
+            shape = w.shape
+            if (w.dtype is not torch.float32 or len(shape) != 3 or shape[0] < rows or shape[1] != self.kv_heads
+                    or shape[2] != self.capacity or not w.is_contiguous() or w.get_device() != index or w.data_ptr() % 16):
                 raise ValueError("Weights must be contiguous fp32 [B, H, capacity] on the cache's device")
         if self.weigh_space is None:
             # Rows that fill the CUs unsplit, their scores in LDS (no workspace is asked for then),
@@ -397,7 +398,7 @@ class PagedFlashDecode:
         b, hq, s, d = q.shape
         if s != 1 or d != self.head_dim:
             raise ValueError("Decode attention takes one query position with the cache's head_dim")
-        index = self._check(k, v, table, hq, b)
+        index, pages = self._check(k, v, table, hq, b)
         if q.dtype != torch.bfloat16:
             raise ValueError("Decode attention supports BF16")
         if q.get_device() != index:
@@ -412,8 +413,8 @@ class PagedFlashDecode:
         before, after, space, cut = self._weights(weights, weights_out, b, index)
         out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(q.shape)
         _lib.call_struct(index, "lm_flash_decode_paged", q.data_ptr(), rows, heads, k.data_ptr(), v.data_ptr(),
-                         table.data_ptr(), table.shape[1], k.shape[0], k.shape[2], used.data_ptr(), b, hq, self.kv_heads,
-                         d, scale, self.maximum, *cut, before, after, out.data_ptr(), space.data_ptr(), space.numel())
+                         table.data_ptr(), *pages, used.data_ptr(), b, hq, self.kv_heads, d, scale, self.maximum, *cut,
+                         before, after, out.data_ptr(), space.data_ptr(), space.numel())
         return out
 
     def fused_qkv(self, partials, cos_sin, positions, active, k, v, table, scale, used, q_heads, row_order=None,
@@ -425,7 +426,7 @@ class PagedFlashDecode:
         plan's bound, or without that page store nothing and attend what they hold.
         Rotation as :func:`rope.rotate_kv_write` has it, weights as :meth:`__call__`."""
         splits, b, ncols = partials.shape
-        index = self._check(k, v, table, q_heads, b)
+        index, pages = self._check(k, v, table, q_heads, b)
         if ncols != (q_heads + 2 * self.kv_heads) * self.head_dim:
             raise ValueError("QKV partials do not match the cache heads")
         if partials.dtype != torch.float32 or not partials.is_contiguous() or partials.get_device() != index:
@@ -447,8 +448,7 @@ class PagedFlashDecode:
         _lib.call_struct(index, "lm_flash_decode_paged_qkv", partials.data_ptr(), splits, cos_sin.data_ptr(),
                          *cos_sin.shape, cos_sin.dtype == torch.float32, bool(is_neox), positions.data_ptr(),
                          0 if active is None else active.data_ptr(), k.data_ptr(), v.data_ptr(), table.data_ptr(),
-                         table.shape[1], k.shape[0], k.shape[2], used.data_ptr(),
-                         0 if row_order is None else row_order.data_ptr(), b, q_heads, self.kv_heads, self.head_dim, scale,
-                         self.maximum, self.splits, before, after, bool(frag_out), out_ptr, space.data_ptr(),
-                         space.numel())
+                         *pages, used.data_ptr(), 0 if row_order is None else row_order.data_ptr(), b, q_heads,
+                         self.kv_heads, self.head_dim, scale, self.maximum, self.splits, before, after, bool(frag_out),
+                         out_ptr, space.data_ptr(), space.numel())
         return out

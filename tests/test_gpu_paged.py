@@ -758,6 +758,30 @@ def test_prefill_decode_evict_decode():
 
 
 @torch.inference_mode()
+def test_prompt_behind_a_shared_beginning():
+    """A prompt whose first pages another row holds: its other tokens are stored in pages of its own and attend the
+    whole as rows of one call, the cache row's table line repeated for each."""
+    hkv, groups, page, first, more = 2, 3, 16, 64, 21
+    cache = PagedKVCache.empty(1, 2, hkv, 64, 128, DEV, page=page)
+    cache.reserve(0, first + 5)
+    cos_sin = rope.rotary_table(128, 64, 10000.0, device=DEV)
+    qkv = vectors((first + 5 + more, groups * hkv + 2 * hkv, 64), 1).to(DEV)
+    q, k, v = qkv.split((groups * hkv, hkv, hkv), 1)
+    at = torch.arange(first + 5, device=DEV)
+    rope.rotate_kv_write(q[:first + 5], k[:first + 5], v[:first + 5], at, None, cos_sin, cache, 0, torch.zeros_like(at))
+    lent = [x.clone() for x in cache.read(0)]
+    cache.share(1, 0, first)
+    cache.reserve(1, first + more)
+    at = first + torch.arange(more, device=DEV)
+    turned, _ = rope.rotate_kv_write(q[-more:], k[-more:], v[-more:], at, None, cos_sin, cache, 0, torch.ones_like(at))
+    assert all(torch.equal(x[0], y[0]) for x, y in zip(cache.read(0), lent))
+    flash = PagedFlashDecode(more, hkv, groups, cache.capacity, DEV)
+    lines = cache.table[1:].repeat(more, 1)
+    got = flash(turned[:, :, None], cache.k[0], cache.v[0], lines, None, None, 0.125, used=(at + 1).int())
+    check_attention(got, turned.cpu(), cache.k[0].cpu(), cache.v[0].cpu(), lines.cpu(), (at + 1).cpu(), 0.125)
+
+
+@torch.inference_mode()
 def test_graph_replays_follow_the_table():
     """Attention, weights and store recorded once and replayed as rows grow and their pages change, with
     eager work between the replays."""
