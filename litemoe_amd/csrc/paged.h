@@ -43,13 +43,14 @@ struct Rotation {
   bool neox;
 };
 
-// One pair. With an fp32 table the sums are fp32, rounded where they are stored;
+// One pair. With an fp32 table the sums are fp32, rounded where they are stored, one
+// product of each in its sum (said here, so that every kernel rounds the same way);
 // with a bf16 table each product and each sum is rounded to bf16, the
 // arithmetic of lm_rope_kv_write.
 __device__ __forceinline__ void turn_pair(bool f32, float x1, float x2, float c, float s, float &o1, float &o2) {
   if (f32) {
-    o1 = x1 * c - x2 * s;
-    o2 = x2 * c + x1 * s;
+    o1 = __builtin_fmaf(x1, c, -(x2 * s));
+    o2 = __builtin_fmaf(x2, c, x1 * s);
   } else {
     o1 = round_bf16(x1 * c) - round_bf16(x2 * s);
     o2 = round_bf16(x2 * c) + round_bf16(x1 * s);

@@ -471,6 +471,29 @@ def test_fused_is_the_three_calls(lengths, hkv, groups, dim, page, splits, neox,
     assert torch.equal(frag.to_rows(), exp.view(b, -1))
 
 
+@pytest.mark.parametrize("neox", [True, False])
+@pytest.mark.parametrize("dim,rotary", [(64, 16), (64, 48), (64, 64), (128, 48), (128, 128)])
+@torch.inference_mode()
+def test_fused_rotation_is_the_stores(dim, rotary, neox):
+    """Many pairs by an fp32 table: one rounding more or less in either kernel would show, in the cache or in rows of
+    one position with V as they attend it."""
+    rows, hkv, groups = 96, 5, 3
+    lengths, hq = [3] * rows, 15
+    caches = [random_cache(lengths, hkv, dim, 16, 7)[0] for _ in range(2)]
+    heads = vectors((rows, hq + 2 * hkv, dim), 3).to(DEV)
+    cos_sin = rope.rotary_table(500, rotary, 10000.0, device=DEV)
+    used = torch.full((rows,), 3, dtype=torch.int32, device=DEV)
+    positions = torch.randint(0, 500, (rows,), generator=gen(4)).to(DEV)
+    flash = PagedFlashDecode(rows, hkv, groups, caches[0].capacity, DEV, head_dim=dim)
+    q, _ = rope.rotate_kv_write(*heads.split((hq, hkv, hkv), 1), positions, None, cos_sin, caches[0], 0, at=used - 1,
+                                is_neox=neox)
+    exp = flash(q[:, :, None], *caches[0].layer(0), None, None, 0.3, used=used)
+    got = flash.fused_qkv(heads.float().view(1, rows, -1), cos_sin, positions, None, *caches[1].layer(0), 0.3, used, hq,
+                          is_neox=neox)
+    assert torch.equal(caches[0].k.view(torch.int16), caches[1].k.view(torch.int16))
+    assert torch.equal(got, exp)
+
+
 @pytest.mark.parametrize("rows,hkv", [(70, 8), (32, 8), (33, 8), (5, 130)])
 @torch.inference_mode()
 def test_fused_order_of_many_rows(rows, hkv):
