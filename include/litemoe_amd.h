@@ -178,13 +178,14 @@ int lm_kv_quant_read(const void *k_codes, const void *v_codes,
  * cos_sin [table_len, rotary], cos of all pairs, then sin: fp32 (table_f32
  * nonzero; products and sums in fp32, x1 c and x2 c within their sums, which are
  * rounded once to bf16) or bf16 (each product and each sum rounded to bf16,
- * lm_rope_kv_write's arithmetic). Positions outside the table are not turned. With cos_sin NULL and rotary 0 nothing is.
- * at (int64, or int32 with at_i32 nonzero) NULL: at = positions (one of the two is
- * needed for a store); slots NULL: slot = row; active NULL: every row is written.
- * k_pages and v_pages NULL: nothing is stored (v, block_table, at, active and slots
- * are not looked at; any head_dim that is a multiple of 16, to 256). q_heads 0: no
- * queries. k_out may be NULL with a store. q_out and k_out may be q and k (in place). Strides in
- * elements, multiples of 8, pointers 16-byte aligned, channels contiguous.
+ * lm_rope_kv_write's arithmetic). Positions outside the table are not turned. With
+ * cos_sin NULL and rotary 0 nothing is. at (int64, or int32 with at_i32 nonzero)
+ * NULL: at = positions (one of the two is needed for a store); slots NULL: slot =
+ * row; active NULL: every row is written. k_pages and v_pages NULL: nothing is
+ * stored (v, block_table, at, active and slots are not looked at; any head_dim that
+ * is a multiple of 16, to 256). q_heads 0: no queries. k_out may be NULL with a
+ * store. q_out and k_out may be q and k (in place). Strides in elements, multiples
+ * of 8, pointers 16-byte aligned, channels contiguous.
  * One row per target, as lm_kv_write. Replaces vLLM `_custom_ops.rotary_embedding`
  * at litemoe/model.py:58,63-64 with `cache.write` (model.py:59,70). */
 typedef struct lm_paged_rotate_args {
