@@ -73,11 +73,13 @@ def write(cache, layer, k, v, positions, active, slots):
     rows = k.shape[0]
     at = places(positions, rows, index, "positions")
     slots = per_row(slots, rows, torch.int64, index, "slots")
-    active = 0 if active is None else per_row(active, rows, torch.bool, index, "active").data_ptr()
+    # held here until the launch: memory given back before it is the next copy's
+    active = None if active is None else per_row(active, rows, torch.bool, index, "active")
     (k, k_view), (v, v_view) = view(k[:, :, 0], rows, heads), view(v[:, :, 0], rows, heads)
-    _lib.call_struct(index, "lm_paged_rotate_write", 0, 0, 0, *k_view, *v_view, 0, 0, 0, 0, 0, 0, at.data_ptr(), at.dtype == torch.int32, active, slots.data_ptr(), 0, 0, 0, 0, 0, 0,
-                     kc.data_ptr(), vc.data_ptr(), table.data_ptr(), table.shape[0], table.shape[1], pages, page, rows, 0,
-                     heads, dim)
+    _lib.call_struct(index, "lm_paged_rotate_write", 0, 0, 0, *k_view, *v_view, 0, 0, 0, 0, 0, 0, at.data_ptr(),
+                     at.dtype == torch.int32, 0 if active is None else active.data_ptr(), slots.data_ptr(), 0, 0, 0, 0, 0,
+                     0, kc.data_ptr(), vc.data_ptr(), table.data_ptr(), table.shape[0], table.shape[1], pages, page, rows,
+                     0, heads, dim)
 
 
 def read(cache, layer, positions, slots):

@@ -187,6 +187,25 @@ def test_rotate_and_store(tokens, hq, hkv, dim, rotary, page, neox, f32):
     assert torch.equal(cache.k.cpu(), expected[0]) and torch.equal(cache.v.cpu(), expected[1])
 
 
+@pytest.mark.parametrize("layout", ["bytes", "strided", "int64"])
+@torch.inference_mode()
+def test_store_by_a_converted_mask(layout):
+    """A mask that is converted, with keys and values that have to be copied, in blocks of one size (512 bytes): the
+    rows that it names are stored, and no others."""
+    tokens, hkv, dim = 4, 1, 64
+    cache = PagedKVCache.empty(1, 1, hkv, dim, tokens, DEV, page=16)
+    cache.reserve(0, tokens)
+    odd = vectors((2, tokens, hkv, 1, dim + 1), 3).to(DEV)[..., 1:]
+    mask = torch.tensor([True, False, True, False])
+    active = {"bytes": mask.to(torch.uint8).to(DEV), "int64": mask.long().to(DEV),
+              "strided": torch.stack((mask, ~mask), 1).to(DEV)[:, 0]}[layout]
+    cache.write(0, odd[0], odd[1], torch.arange(tokens, device=DEV), active,
+                torch.zeros(tokens, dtype=torch.int64, device=DEV))
+    for got, x in zip(cache.read(0), odd.cpu()):
+        exp = torch.where(mask[:, None], x[:, 0, 0], torch.zeros((), dtype=BF16))
+        assert torch.equal(got[0, 0, :tokens].cpu(), exp) and not got[0, 0, tokens:].any()
+
+
 @torch.inference_mode()
 def test_bf16_table_is_the_contiguous_path():
     """With the reference's table the store is rope_kv_write bit for bit, in place too."""

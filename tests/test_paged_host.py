@@ -4,12 +4,13 @@ import copy
 import math
 import pickle
 import re
+import weakref
 from pathlib import Path
 
 import pytest
 import torch
 
-from litemoe_amd import _lib, kv_paged, rope
+from litemoe_amd import _lib, kv_paged, kv_quant, rope
 from litemoe_amd.cache import KVCache, PagedKVCache
 from litemoe_amd.config import preset
 from litemoe_amd.engine import Engine
@@ -175,6 +176,44 @@ def test_host_tensors_are_refused():
     plain = KVCache(preset("granite-1b", num_hidden_layers=1), 1, 16, "cpu", torch.bfloat16)
     with pytest.raises(ValueError, match="paged KV cache"):
         rope.rotate_kv_write(q[:, :, 0], x[:, :, 0], x[:, :, 0], at, None, cos_sin, plain, 0)
+
+
+@pytest.mark.parametrize("call", ["write", "read", "rotate", "attend", "fused"])
+def test_converted_arguments_live_through_the_call(call, monkeypatch):
+    """What a call converts or copies (a mask of bytes, places of another type, operands without alignment) is held
+    until its kernel is launched: memory given back before is the next copy's."""
+    made, missing = [], []
+
+    def recorded(function, result):
+        def wrapper(*args, **kwargs):
+            out = function(*args, **kwargs)
+            made.append(weakref.ref(result(out)))
+            return out
+        return wrapper
+    monkeypatch.setattr(kv_quant, "per_row", recorded(kv_quant.per_row, lambda t: t))
+    for module in (kv_paged, rope):
+        monkeypatch.setattr(module, "per_row", kv_quant.per_row)
+    monkeypatch.setattr(kv_paged, "view", recorded(kv_paged.view, lambda out: out[0]))
+    # the calls as far as their launch, on host tensors
+    monkeypatch.setattr(kv_paged, "check_layer", lambda k, v, table: -1)
+    monkeypatch.setattr(_lib, "require_cuda", lambda *tensors, what: None)
+    monkeypatch.setattr(_lib, "call_struct", lambda *args: missing.extend(r for r in made if r() is None))
+    cache = cache_of()
+    odd = torch.zeros(3, 4, 1, 65, dtype=torch.bfloat16)[..., 1:]
+    q, cos_sin = torch.zeros(3, 8, 1, 65, dtype=torch.bfloat16)[..., 1:], rope.rotary_table(16, 64, 1e4)
+    at, mask, short = torch.zeros(6, dtype=torch.int16)[::2], torch.ones(3, dtype=torch.uint8), torch.ones(3).short()
+    flash = PagedFlashDecode(3, 4, 2, cache.capacity, "cpu")
+    if call == "write":
+        cache.write(0, odd, odd, at, mask, short)
+    elif call == "read":
+        kv_paged.read(cache, 0, at, short)
+    elif call == "rotate":
+        rope.rotate_kv_write(q[:, :, 0], odd[:, :, 0], odd[:, :, 0], short, mask, cos_sin, cache, 0, short, at=at)
+    elif call == "attend":
+        flash(torch.zeros(3, 8, 1, 64, dtype=torch.bfloat16), *cache.layer(0), None, None, 1.0, used=short)
+    else:
+        flash.fused_qkv(torch.zeros(1, 3, 16 * 64), cos_sin, short, mask, *cache.layer(0), 1.0, short, 8)
+    assert made and not missing
 
 
 @pytest.mark.parametrize("kwargs,text", [(dict(maximum=0), "length bound"), (dict(maximum=65), "length bound"),
