@@ -184,8 +184,9 @@ int lm_kv_quant_read(const void *k_codes, const void *v_codes,
  * row; active NULL: every row is written. k_pages and v_pages NULL: nothing is
  * stored (v, block_table, at, active and slots are not looked at; any head_dim that
  * is a multiple of 16, to 256). q_heads 0: no queries. k_out may be NULL with a
- * store. q_out and k_out may be q and k (in place). Strides in elements, multiples
- * of 8, pointers 16-byte aligned, channels contiguous.
+ * store. q_out and k_out may be q and k (in place), else they share nothing with
+ * q, k and v; of the heads that are written none overlaps another. Strides in
+ * elements, multiples of 8, pointers 16-byte aligned, channels contiguous.
  * One row per target, as lm_kv_write. Replaces vLLM `_custom_ops.rotary_embedding`
  * at litemoe/model.py:58,63-64 with `cache.write` (model.py:59,70). */
 typedef struct lm_paged_rotate_args {

@@ -75,6 +75,9 @@ def check_table(cos_sin, index, dim):
         raise ValueError("Rotated channels are a multiple of 16, at most the head's")
 
 
+SHARED = "Rotation in place needs queries and keys whose rows and heads share no memory"
+
+
 def _check(q, k, cos_sin, positions):
     _lib.require_cuda(q, k, cos_sin, positions, what="RoPE tensors")
     if q.dtype != torch.bfloat16 or k.dtype != torch.bfloat16 or cos_sin.dtype != torch.bfloat16:
@@ -88,15 +91,59 @@ def _check(q, k, cos_sin, positions):
             raise ValueError('RoPE needs 16-byte aligned rows and heads (strides multiple of 8)')
 
 
+def _apart(q, k):
+    """Whether every head of ``q`` and of ``k`` (``[T, heads, D]``, contiguous channels) has memory of its own, as a
+    rotation in place needs it."""
+    (rows, heads, dim), (s0, s1, _) = q.shape, q.stride()
+    (k_rows, k_heads, k_dim), (k0, k1, _) = k.shape, k.stride()
+    width, k_width = (heads - 1) * s1 + dim, (k_heads - 1) * k1 + k_dim  # of a row
+    at = (k.data_ptr() - q.data_ptr()) // 2
+    rows_apart = (s0 >= width or rows == 1) and (k0 >= k_width or k_rows == 1)
+    if rows_apart and (s1 >= dim or heads == 1) and (k1 >= k_dim or k_heads == 1):
+        if at >= (rows - 1) * s0 + width or -at >= (k_rows - 1) * k0 + k_width:
+            return True  # one behind the other
+        if 0 < s0 == k0 and width <= at % s0 <= s0 - k_width:
+            return True  # columns of the same rows
+    if not q.numel():
+        rows, heads, width = 0, 0, 0
+    if not k.numel():
+        k_rows, k_heads, k_width = 0, 0, 0
+    if (heads <= 1 or s1 >= (rows - 1) * s0 + dim) and (k_heads <= 1 or k1 >= (k_rows - 1) * k0 + k_dim) \
+            and (rows <= 1 or s0 >= dim) and (k_rows <= 1 or k0 >= k_dim):
+        # of each head all rows, then the next head's
+        if at >= (heads - 1) * s1 + (rows - 1) * s0 + dim or -at >= (k_heads - 1) * k1 + (k_rows - 1) * k0 + k_dim:
+            return True
+
+    def free(starts, ends):
+        starts, order = starts.sort()
+        return not bool((starts[1:] < ends[order][:-1]).any())
+
+    def all_of(rows, heads, step, inner, dim, base):
+        starts = (base + step * torch.arange(rows, device="cpu")[:, None]
+                  + inner * torch.arange(heads, device="cpu")).flatten()
+        return starts, starts + dim
+    if rows_apart and s0 == k0 > 0 and min(rows, k_rows) > 1:
+        # rows repeat: the heads of one row, of what reaches into the next its place there too
+        (q_starts, q_ends), (k_starts, k_ends) = all_of(1, heads, 0, s1, dim, 0), all_of(1, k_heads, 0, k1, k_dim, at % s0)
+        starts, ends = torch.cat((q_starts, k_starts)), torch.cat((q_ends, k_ends))
+        if free(torch.cat((starts, starts + s0)), torch.cat((ends, ends + s0))):
+            return True
+    (q_starts, q_ends), (k_starts, k_ends) = all_of(rows, heads, s0, s1, dim, 0), all_of(k_rows, k_heads, k0, k1, k_dim, at)
+    return free(torch.cat((q_starts, k_starts)), torch.cat((q_ends, k_ends)))
+
+
 def rotary_embedding(positions, query, key, head_size, cos_sin_cache, is_neox=True):
     """In-place rotation of ``query [T, Hq, D]`` and ``key [T, Hkv, D]`` by the table
     ``cos_sin_cache [table_len, R]``: its width says how many of a head's channels
     turn, and its type the arithmetic (see :func:`rotate_kv_write`). ``is_neox``: pairs
-    in halves, else interleaved."""
+    in halves, else interleaved. Rows and heads have memory of their own, within each
+    tensor and between the two."""
     if head_size != query.shape[-1]:
         raise ValueError('head_size must equal the last query dimension')
     if is_neox and head_size == 64 and cos_sin_cache.shape[-1] == 64 and cos_sin_cache.dtype == torch.bfloat16:
         _check(query, key, cos_sin_cache, positions)
+        if not _apart(query, key):
+            raise ValueError(SHARED)
         positions = positions.to(torch.int64).contiguous()
         rows = query.shape[0]
         _lib.call("lm_rope_kv_write", query.data_ptr(), query.stride(0), query.stride(1),
@@ -105,10 +152,11 @@ def rotary_embedding(positions, query, key, head_size, cos_sin_cache, is_neox=Tr
                   None, None, rows, query.shape[1], key.shape[1], 64, 1, 1, 1, _lib.stream(query.device))
         return
     for t in (query, key):
-        if (t.dim() != 3 or t.dtype != torch.bfloat16 or kv_paged.view(t, *t.shape[:2])[0] is not t
-                or any(size > 1 and not stride for size, stride in zip(t.shape, t.stride()))):
+        if t.dim() != 3 or t.dtype != torch.bfloat16 or kv_paged.view(t, *t.shape[:2])[0] is not t:
             raise ValueError('Rotation in place needs BF16 [T, heads, D] of contiguous channels, 16-byte aligned rows '
-                             'and heads of their own (strides multiple of 8)')
+                             'and heads (strides multiple of 8)')
+    if not _apart(query, key):
+        raise ValueError(SHARED)
     _rotate(query, key, positions, cos_sin_cache, is_neox, query, key)
 
 

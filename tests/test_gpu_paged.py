@@ -244,6 +244,27 @@ def test_rotary_embedding_in_place(dim, rotary, neox, f32):
             assert torch.equal(got, exp.to(BF16))
 
 
+@pytest.mark.parametrize("f32", [True, False])
+@pytest.mark.parametrize("layout", ["columns", "in turn", "heads outside"])
+@torch.inference_mode()
+def test_rotary_embedding_in_place_of_packed_heads(layout, f32):
+    """Queries and keys that lie between each other are turned as those that stand alone, and what lies between them
+    stays."""
+    tokens, heads, dim = 37, 4, 64
+    x = vectors({"columns": (tokens, 3 * heads, dim), "in turn": (tokens, heads, 3, dim),
+                 "heads outside": (3 * heads, tokens, dim)}[layout], 1).to(DEV)
+    before = x.clone()
+    parts = {"columns": lambda t: t.split(heads, 1), "in turn": lambda t: t.unbind(2),
+             "heads outside": lambda t: t.transpose(0, 1).split(heads, 1)}[layout]
+    cos_sin = rope.rotary_table(90, 64, 500.0, device=DEV, dtype=torch.float32 if f32 else BF16)
+    positions = torch.randint(0, 90, (tokens,), generator=gen(9)).to(DEV)
+    (q, k, v), (q0, k0, v0) = parts(x), parts(before)
+    alone = q0.contiguous(), k0.contiguous()
+    rope.rotary_embedding(positions, *alone, dim, cos_sin)
+    rope.rotary_embedding(positions, q, k, dim, cos_sin)
+    assert torch.equal(q, alone[0]) and torch.equal(k, alone[1]) and torch.equal(v, v0)
+
+
 # --------------------------------------------------------------- attention --
 
 ATTENTIONS = [

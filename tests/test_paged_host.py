@@ -216,6 +216,74 @@ def test_converted_arguments_live_through_the_call(call, monkeypatch):
     assert made and not missing
 
 
+def heads_of(x, rows, heads, dim, s0, s1, offset=0):
+    """``[rows, heads, dim]`` within the buffer ``x``."""
+    return x.as_strided((rows, heads, dim), (s0, s1, 1), offset)
+
+
+# q's and k's rows, heads, strides and offset in one buffer
+APART = [
+    ((4, 4, 256, 64, 0), (4, 2, 128, 64, 1024)),            # one behind the other
+    ((4, 4, 512, 64, 0), (4, 2, 512, 64, 256)),             # columns of one projection
+    ((4, 2, 512, 64, 256), (4, 4, 512, 64, 384)),           # k's columns behind, q's first ones missing
+    ((4, 4, 512, 64, 128), (4, 2, 512, 64, 0)),             # k's columns before q's
+    ((4, 3, 576, 192, 0), (4, 3, 576, 192, 64)),            # heads in turn: q, k, v of each
+    ((1, 3, 0, 192, 0), (1, 3, 0, 192, 64)),                # of a single row
+    ((4, 4, 64, 256, 0), (4, 2, 64, 256, 1024)),            # heads outside, rows inside
+    ((2, 2, 128, 192, 0), (1, 1, 0, 0, 64)),                # neither nested in the other
+    ((3, 1, 128, 0, 0), (3, 1, 128, 0, 64)),                # rows in turn
+    ((0, 4, 256, 64, 0), (0, 4, 256, 64, 0)),               # no rows
+]
+OVERLAP = [
+    ((4, 4, 128, 32, 0), (4, 2, 128, 64, 2048)),            # heads half over the next
+    ((4, 4, 192, 64, 0), (4, 2, 128, 64, 2048)),            # rows over the next row's first head
+    ((4, 2, 256, 64, 2048), (4, 4, 32, 256, 0)),            # k's rows
+    ((4, 4, 256, 64, 0), (4, 4, 256, 64, 0)),               # one tensor as both
+    ((4, 4, 512, 64, 0), (4, 2, 512, 64, 192)),             # k begins in q's last head
+    ((4, 2, 512, 64, 448), (4, 2, 512, 64, 0)),             # q's last head is the next row's first of k
+    ((4, 3, 576, 192, 0), (4, 3, 576, 192, 32)),            # heads in turn, half over each other
+    ((1, 1, 0, 0, 32), (1, 3, 0, 64, 0)),
+    ((2, 2, 128, 192, 0), (1, 1, 0, 0, 96)),
+    ((4, 1, 0, 0, 0), (4, 1, 64, 0, 1024)),                 # one row for all
+]
+
+
+@pytest.mark.parametrize("whole", [False, True])
+@pytest.mark.parametrize("q,k,fine", [(*x, True) for x in APART] + [(*x, False) for x in OVERLAP])
+def test_rotation_in_place_needs_memory_of_its_own(q, k, fine, whole, monkeypatch):
+    """Heads that share memory, a tensor's own or those of queries and keys, would be turned by threads at once, some
+    of them twice: refused before the launch, by either kernel (``whole``: the reference's bf16 table)."""
+    def shares(*views):
+        seen = set()
+        for rows, heads, s0, s1, offset in views:
+            for start in (offset + r * s0 + h * s1 for r in range(rows) for h in range(heads)):
+                cells = set(range(start, start + 64))
+                if seen & cells:
+                    return True
+                seen |= cells
+        return False
+    assert shares(q, k) is not fine
+    launched = []
+    monkeypatch.setattr(_lib, "require_cuda", lambda *tensors, what: None)
+    monkeypatch.setattr(_lib, "stream", lambda device: None)
+    for name in ("call", "call_struct"):
+        monkeypatch.setattr(_lib, name, lambda *args: launched.append(args))
+    x = torch.zeros(4096, dtype=torch.bfloat16)
+    query, key = (heads_of(x, rows, heads, 64, s0, s1, offset) for rows, heads, s0, s1, offset in (q, k))
+    if query.shape[0] != key.shape[0]:  # the call needs the same rows: the check itself
+        assert rope._apart(query, key) is fine
+        return
+    cos_sin = rope.rotary_table(16, 64, 1e4, dtype=torch.bfloat16 if whole else torch.float32)
+    at = torch.zeros(query.shape[0], dtype=torch.int64)
+    if fine:
+        rope.rotary_embedding(at, query, key, 64, cos_sin)
+        assert launched
+    else:
+        with pytest.raises(ValueError, match="in place"):
+            rope.rotary_embedding(at, query, key, 64, cos_sin)
+        assert not launched
+
+
 @pytest.mark.parametrize("kwargs,text", [(dict(maximum=0), "length bound"), (dict(maximum=65), "length bound"),
                                          (dict(head_dim=32), "head_dim"), (dict(groups=17), "16 query heads"),
                                          (dict(groups=0), "16 query heads")])
