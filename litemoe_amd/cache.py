@@ -386,37 +386,42 @@ class PagedKVCache:
     def evict(self, weights, used, keep, recent=0, room=0):
         """Hold every row to ``keep`` positions (:func:`kv_paged.evict`): per layer and
         KV head the ``recent`` last and the heaviest others of the row's ``used[b]`` (no
-        more than it has pages for) stay, in their order, in fresh pages; the old ones go back to the pool. ``weights [L,
-        B, H, capacity]`` (fp32) is compacted in place. ``room``: positions that each row
-        gets pages for beyond ``keep``, if it had more than ``keep``. Returns the positions
-        kept ``[L, B, H, keep]`` and the rows' new ``used``; a row goes on at that
-        position, with rotary positions counted from where it was."""
+        more than it has pages for) stay, in their order, in fresh pages; the old ones go
+        back to the pool. A row that has pages for ``keep`` positions or fewer loses
+        nothing: its pages stay, shared ones too, and are not copied. ``weights [L, B, H,
+        capacity]`` (fp32) is compacted in place. ``room``: positions that each of the
+        others gets pages for beyond ``keep``. Returns the positions kept ``[L, B, H,
+        keep]`` and the rows' new ``used``; a row goes on at that position, with rotary
+        positions counted from where it was."""
         self._owned()
         keep, room = int(keep), int(room)
         if room < 0 or keep + room > self.capacity:
             raise ValueError("Positions of a row exceed the KV capacity")
-        want = [min(len(pages), -(-keep // self.page)) for pages in self._held]
-        grow = [max(n, -(-(keep + room) // self.page) if len(pages) * self.page > keep else n)
-                for n, pages in zip(want, self._held)]
-        if sum(grow) > len(self._free):
-            raise ValueError(f"The KV pool has {len(self._free)} free pages, {sum(grow)} are wanted")
-        fresh = [self._take(n) for n in grow]
-        width = max([1, *grow])
-        # each row's pages to come, and the positions that it has pages for
-        lines = [p + [-1] * (width - len(p)) + [len(old) * self.page] for p, old in zip(fresh, self._held)]
+        moved = [row for row, pages in enumerate(self._held) if len(pages) * self.page > keep]
+        each = max(0, -(-(keep + room) // self.page))
+        if len(moved) * each > len(self._free):
+            raise ValueError(f"The KV pool has {len(self._free)} free pages, {len(moved) * each} are wanted")
+        fresh = {row: self._take(each) for row in moved}
+        width = max(1, each)
+        # each row's pages to come (none where it keeps its own), and the positions that it has pages for
+        lines = []
+        for row, old in enumerate(self._held):
+            pages = fresh.get(row, [])
+            lines.append(pages + [-1] * (width - len(pages)) + [len(old) * self.page])
         try:
             lines = torch.tensor(lines, dtype=torch.int32).to(self._table.device)
-            used = kv_quant.per_row(used, len(fresh), torch.int32, lines.get_device(), "used").minimum(lines[:, width])
-            _, kept, left = kv_paged.evict(self, weights, used, keep, recent, lines[:, :width].contiguous(),
-                                           weights_out=weights)
+            used = kv_quant.per_row(used, len(self._held), torch.int32, lines.get_device(), "used")
+            _, kept, left = kv_paged.evict(self, weights, used.minimum(lines[:, width]), keep, recent,
+                                           lines[:, :width].contiguous(), weights_out=weights)
         except Exception:
-            for pages in fresh:
+            for pages in fresh.values():
                 self._drop(pages)
             raise
-        for row, pages in enumerate(fresh):
+        for row in moved:
             self._drop(self._held[row])
-            self._held[row] = pages
-        self._publish(list(range(len(fresh))))
+            self._held[row] = fresh[row]
+        if moved:
+            self._publish(moved)
         return kept, left
 
     # -- contents --------------------------------------------------------------

@@ -697,6 +697,39 @@ def test_cache_evicts_what_has_pages():
 
 
 @torch.inference_mode()
+def test_cache_evicts_from_long_rows_only():
+    """One row over its budget and two that are not, one beginning with the other's pages, in a pool that has free
+    pages for the first alone: it is held to its budget, and the others' pages, weights and contents are as they
+    were."""
+    cache = PagedKVCache.empty(2, 3, 2, 64, 128, DEV, page=16, pages=13)
+    cache.reserve([0, 1], [100, 32])
+    cache.share(2, 1, 32)
+    cache.reserve(2, 40)
+    assert cache.free_pages == 3
+    for side, seed in ((cache.k, 3), (cache.v, 4)):
+        side.copy_(vectors(side.shape, seed))
+    w = torch.rand(2, 3, 2, 128, generator=gen(5))
+    lengths = [97, 30, 35]
+    before, table, w_dev = [cache.read(layer) for layer in range(2)], cache.table.cpu(), w.to(DEV)
+    kept, left = cache.evict(w_dev, torch.tensor(lengths, dtype=torch.int32, device=DEV), 48, 4)
+    assert left.tolist() == [48, 30, 35] and cache.free_pages == 7
+    assert torch.equal(cache.table[1:].cpu(), table[1:])
+    for layer in range(2):
+        for x, y in zip(before[layer], cache.read(layer)):
+            assert torch.equal(x[1:], y[1:])
+            for h in range(2):
+                stay = paged.keep(w[layer, 0, h], 97, 48, 4)
+                assert kept[layer, 0, h].tolist() == stay and torch.equal(y[0, h, :48], x[0, h, stay])
+        for row, n in enumerate(lengths):
+            for h in range(2):
+                stay = paged.keep(w[layer, row, h], n, 48, 4)
+                exp = torch.zeros(128)
+                exp[:len(stay)] = w[layer, row, h, stay]
+                assert torch.equal(w_dev[layer, row, h].cpu(), exp)
+                assert kept[layer, row, h].tolist() == stay + [-1] * (48 - len(stay))
+
+
+@torch.inference_mode()
 def test_graph_replays_of_evictions():
     """Weights and eviction recorded, with the weights read and written in place by the graph's own tensors."""
     lengths = [100, 61]

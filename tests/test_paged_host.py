@@ -113,6 +113,36 @@ def test_a_refused_eviction_gives_its_pages_back():
         tight.evict(weights, torch.tensor([40, 40, 0]), 16)
 
 
+def test_an_eviction_leaves_rows_that_lose_nothing(monkeypatch):
+    """Rows with pages for no more than the budget keep them, in a pool that has free pages for the others only; a
+    shared beginning stays shared."""
+    cache = cache_of(rows=4, pages=10)
+    cache.reserve([0, 1], [64, 32])
+    cache.share(2, 1, 32)
+    cache.reserve(2, 48)
+    before, targets = lines(cache), []
+    assert cache.free_pages == 3
+
+    def moved(cache, weights, used, keep, recent, target, table=None, weights_out=None):
+        targets.append([[p for p in line if p >= 0] for line in target.tolist()])
+        return weights_out, None, used.clamp(max=keep)
+    monkeypatch.setattr(kv_paged, "evict", moved)
+    weights = torch.zeros(2, 4, 4, 64)
+    _, left = cache.evict(weights, torch.tensor([60, 40, 48, 5]), 48)
+    assert left.tolist() == [48, 32, 48, 0]
+    assert len(targets[0][0]) == 3 and targets[0][1:] == [[], [], []]
+    assert lines(cache) == [targets[0][0], *before[1:]] and lines(cache)[2][:2] == lines(cache)[1]
+    assert cache.free_pages == 10 - 3 - 3 and not set(lines(cache)[0]) & set(lines(cache)[2])
+    # nothing to evict: no free page is asked for
+    cache.reserve([1, 3], [64, 32])
+    assert cache.free_pages == 0
+    full = lines(cache)
+    cache.evict(weights, torch.tensor([48, 64, 48, 32]), 64)
+    assert lines(cache) == full and targets[1] == [[]] * 4
+    cache.release([0, 1, 2, 3])
+    assert cache.free_pages == 10
+
+
 def test_a_cache_over_buffers():
     k = torch.zeros(2, 5, 4, 16, 64, dtype=torch.bfloat16)
     table = torch.zeros(3, 2, dtype=torch.int32)
