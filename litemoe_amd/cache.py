@@ -177,6 +177,8 @@ class QuantKVCache:
             raise ValueError("Prompt width exceeds the KV capacity")
         if rows.numel() != b:
             raise ValueError("Prefill slots must name one cache row per batch row")
+        for row in range(*slot.indices(self.slots.numel())) if isinstance(slot, slice) else (slot,):
+            self.check_own(row, 0, s)
         zero, keep = torch.zeros((), dtype=k.dtype, device=k.device), valid[:, None, :, None]
         pos = self.keys[:s]
         flat = [torch.where(keep, x, zero).transpose(1, 2).reshape(b * s, h, 1, d) for x in (k, v)]
@@ -300,6 +302,15 @@ class PagedKVCache:
         if self._free is None:
             raise ValueError("The pages of this cache are its caller's to hand out")
 
+    def check_own(self, row, start, stop):
+        """Raise ValueError where positions ``start .. stop-1`` of row ``row`` lie in a
+        page that another row has too."""
+        if self._free is None:  # the caller's pages
+            return
+        pages = self._held[self._row(row)]
+        if start < stop and any(self._rows_of[page] > 1 for page in pages[start // self.page:-(-stop // self.page)]):
+            raise ValueError("Pages that another row shares are not stored to")
+
     def _publish(self, rows):
         """The table's lines of ``rows`` from the lists on the host."""
         width = self._table.shape[1]
@@ -357,8 +368,10 @@ class PagedKVCache:
 
     def share(self, row, other, positions):
         """Row ``row``, which has no pages, begins with those of the first ``positions``
-        positions of row ``other`` (a multiple of the page). Both read them; neither may
-        store there again."""
+        positions of row ``other`` (a multiple of the page), which ``other`` has stored
+        already. Both read them; neither may store there again: :meth:`clear`,
+        :meth:`prefill` by rows and the model's prefills refuse it (:meth:`check_own`),
+        a store by tensors of places is the caller's to keep out of them."""
         self._owned()
         row, other = self._row(row), self._row(other)
         if self._held[row] or row == other:
@@ -433,6 +446,8 @@ class PagedKVCache:
     def clear(self, row, start, stop):
         """Positions ``start .. stop-1`` of cache row ``row`` of every layer: zeros,
         where they have pages."""
+        start, stop, _ = slice(start, stop).indices(self.capacity)
+        self.check_own(row, start, stop)
         positions = self.keys[start:stop]
         n = positions.numel()
         zeros = self._k.new_zeros((n, self._k.shape[2], 1, self._k.shape[4]))
@@ -453,6 +468,8 @@ class PagedKVCache:
             raise ValueError("Prompt width exceeds the KV capacity")
         if rows.numel() != b:
             raise ValueError("Prefill slots must name one cache row per batch row")
+        for row in range(*slot.indices(self.slots.numel())) if isinstance(slot, slice) else (slot,):
+            self.check_own(row, 0, s)
         zero, keep = torch.zeros((), dtype=k.dtype, device=k.device), valid[:, None, :, None]
         pos = self.keys[:s]
         flat = [torch.where(keep, x, zero).transpose(1, 2).reshape(b * s, h, 1, d) for x in (k, v)]

@@ -443,6 +443,9 @@ class Granite:
                              "and positions equal to the column index")
         if s > cache.capacity:
             raise ValueError("Prompt width exceeds the KV capacity")
+        if isinstance(cache, PagedKVCache):
+            for row in rows:
+                cache.check_own(row, 0, s)
         for row, n in zip(rows, counts):  # cache.py:28-29 stores k * valid: zeros past the prompt
             if n < s:
                 if isinstance(cache, (PagedKVCache, QuantKVCache)):

@@ -9,6 +9,7 @@ from typing import NamedTuple
 import torch
 
 from . import _lib
+from .cache import PagedKVCache
 
 
 class PackedPrefill(NamedTuple):
@@ -62,6 +63,10 @@ def packed_prefill_logits(model, prompts, cache, slot_start=0):
     if not cache.k.is_cuda:
         raise ValueError("Packed Prefill requires the GPU path")
     lengths = [len(p) for p in prompts]
+    if isinstance(cache, PagedKVCache):
+        for row, n in enumerate(lengths, slot_start):
+            if 0 <= row < cache.slots.numel():  # others are not stored
+                cache.check_own(row, 0, n)
     packed, ends = build_packed(lengths, cache.k.device, slot_start)
     tokens = torch.tensor([t for p in prompts for t in p], device=cache.k.device)[None]
     return model.forward(tokens, packed.positions[None], torch.ones_like(tokens, dtype=torch.bool),

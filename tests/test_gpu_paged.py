@@ -11,7 +11,7 @@ import torch
 
 from litemoe_amd import kv_paged, rope, synth
 from litemoe_amd._lib import NativeError
-from litemoe_amd.batch import BatchPrefillEngine
+from litemoe_amd.batch import BatchPrefillEngine, prefill_logits
 from litemoe_amd.cache import KVCache, PagedKVCache, QuantKVCache
 from litemoe_amd.config import preset
 from litemoe_amd.engine import Engine, Request
@@ -21,7 +21,7 @@ from litemoe_amd.flash_decode import FlashDecode, PagedFlashDecode, QuantFlashDe
 from litemoe_amd.linear import linear_dense, linear_rope_kv, linear_splitk, linear_splitk_frag
 from litemoe_amd.model import Granite
 from litemoe_amd.optimized import OptimizedEngine
-from litemoe_amd.packed import build_packed
+from litemoe_amd.packed import build_packed, packed_prefill_logits
 from oracle import paged
 
 pytestmark = pytest.mark.gpu
@@ -983,6 +983,31 @@ def test_prefill_writes_what_the_contiguous_cache_holds(epilogue):
     for layer in range(2):
         for got, held in zip(caches[1].read(layer), (caches[0].k[layer], caches[0].v[layer])):
             assert torch.equal(got, held)
+
+
+@torch.inference_mode()
+def test_prefills_keep_out_of_shared_pages():
+    """A prompt into a row that begins with another's pages is refused by every prefill that goes by rows, with both
+    rows as they were; into a row that has its own it is taken."""
+    cfg, model = small_model()
+    cache = PagedKVCache(cfg, 3, 64, DEV, BF16, page=16)
+    cache.reserve([0, 2], 64)
+    prompts = synth.prompts(1, [40], cfg.vocab_size, 3)
+    packed_prefill_logits(model, prompts, cache)
+    cache.share(1, 0, 32)
+    cache.reserve(1, 64)
+    before = cache.k.clone(), cache.v.clone()
+    tokens = torch.tensor(prompts, device=DEV)
+    columns = torch.arange(40, device=DEV)[None]
+    for call in (lambda: packed_prefill_logits(model, prompts, cache, 1),
+                 lambda: packed_prefill_logits(model, prompts * 2, cache, 1),
+                 lambda: prefill_logits(model, prompts * 2, cache, 1),
+                 lambda: model.forward(tokens, columns, columns < 40, cache, slot=0)):
+        with pytest.raises(ValueError, match="shares"):
+            call()
+    assert torch.equal(cache.k, before[0]) and torch.equal(cache.v, before[1])
+    packed_prefill_logits(model, prompts, cache, 2)
+    assert all(torch.equal(x[2, :, :40], x[0, :, :40]) for layer in range(2) for x in cache.read(layer))
 
 
 @torch.inference_mode()

@@ -143,6 +143,39 @@ def test_an_eviction_leaves_rows_that_lose_nothing(monkeypatch):
     assert cache.free_pages == 10
 
 
+def test_stores_by_rows_keep_out_of_shared_pages(monkeypatch):
+    """After ``share`` neither row's first pages are cleared or prefilled; what lies behind them is, and all of it
+    when one of the rows has given them back."""
+    cache = cache_of(rows=3, pages=12)
+    cache.reserve([0, 2], 64)
+    cache.share(1, 0, 32)
+    cache.reserve(1, 64)
+    stored = []
+    monkeypatch.setattr(kv_paged, "write", lambda cache, layer, k, v, at, active, slots: stored.append(
+        sorted(set(zip(slots.tolist(), at.tolist())))))
+
+    def prefill(slot, width, rows=1):
+        x = torch.zeros(rows, 4, width, 64, dtype=torch.bfloat16)
+        return cache.prefill(0, slot, x, x, torch.ones(rows, width, dtype=torch.bool))
+    for call in (lambda: cache.clear(1, 0, 8), lambda: cache.clear(0, 31, 40), lambda: cache.clear(1, -64, 20),
+                 lambda: prefill(1, 1), lambda: prefill(0, 64), lambda: prefill(slice(1, 3), 20, 2),
+                 lambda: prefill(slice(0, 3), 3, 3)):
+        with pytest.raises(ValueError, match="shares"):
+            call()
+    assert not stored
+    cache.clear(1, 32, 40)
+    cache.clear(0, 20, 20)
+    cache.clear(2, 0, 3)
+    assert stored == 2 * [[(1, j) for j in range(32, 40)]] + 2 * [[(2, j) for j in range(3)]]
+    prefill(2, 5)
+    cache.release(0)
+    prefill(slice(0, 3), 2, 3)
+    assert stored[-2:] == [[(2, j) for j in range(5)], [(i, j) for i in range(3) for j in range(2)]]
+    # pages that are the caller's to hand out are not looked at
+    other = PagedKVCache.over(cache.k, cache.v, torch.zeros(3, 4, dtype=torch.int32))
+    other.clear(1, 0, 4)
+
+
 def test_a_cache_over_buffers():
     k = torch.zeros(2, 5, 4, 16, 64, dtype=torch.bfloat16)
     table = torch.zeros(3, 2, dtype=torch.int32)
