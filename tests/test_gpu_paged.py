@@ -599,6 +599,42 @@ def test_fused_sums_slices(slices):
     assert bool(((got - exp).abs() <= rotated_bound(heads[:, hkv * groups:-hkv], exp)).all())
 
 
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("slices", [1, 2, 5, 8])
+@pytest.mark.parametrize("hkv,groups,dim,splits", [(2, 3, 64, None), (1, 16, 128, None), (2, 16, 128, 2), (2, 15, 64, 1)])
+@torch.inference_mode()
+def test_fused_attends_by_the_sums(hkv, groups, dim, splits, slices, f32):
+    """Keys, values and results of heads summed from slices, with more channels than a workgroup's threads stage at
+    once too, against rotation, store and attention of the sums. bf16 table: sums in ascending order, in fp32, rounded.
+    fp32 table: multiples of 1/64 whose sums are bf16 values, so that they are what the rotation is given."""
+    lengths, hq = [40, 9, 300], hkv * groups
+    b = len(lengths)
+    cache, k, v, table = random_cache(lengths, hkv, dim, 16, 2)
+    part = torch.randn(slices, b, (hq + 2 * hkv) * dim, generator=gen(slices))
+    if f32:
+        part = (64 * part).round()
+        part[-1] += (64 * torch.randn(part[0].shape, generator=gen(9))).round().clamp(-128, 128) - part.sum(0)
+        part = part / 64
+    total = part[0]
+    for s in range(1, slices):
+        total = total + part[s]
+    heads = total.view(b, -1, dim).to(BF16)
+    assert not f32 or torch.equal(heads.float(), total.view(b, -1, dim))
+    cos_sin = rope.rotary_table(400, 64, 10000.0, device=DEV, dtype=torch.float32 if f32 else BF16)
+    used, pos = torch.tensor(lengths, dtype=torch.int32), torch.tensor([350, 8, 299])
+    flash = PagedFlashDecode(b, hkv, groups, cache.capacity, DEV, num_splits=splits, head_dim=dim)
+    got = flash.fused_qkv(part.to(DEV), cos_sin, pos.to(DEV), None, *cache.layer(0), dim ** -0.5, used.to(DEV), hq)
+    q, new_k, new_v = (x.clone() for x in heads.to(DEV).split((hq, hkv, hkv), 1))
+    rope.rotary_embedding(pos.to(DEV), q, new_k, dim, cos_sin)
+    for i, n in enumerate(lengths):
+        page, place = paged.cell(table, k.shape[1], 16, i, n - 1)
+        for pool, new in ((k, new_k), (v, new_v)):
+            pool[0, page, :, place] = new[i].cpu()
+    assert torch.equal(cache.k.cpu().view(torch.int16), k.view(torch.int16))
+    assert torch.equal(cache.v.cpu().view(torch.int16), v.view(torch.int16))
+    check_attention(got, q.cpu(), k[0], v[0], table, used, dim ** -0.5)
+
+
 # ---------------------------------------------------------------- eviction --
 
 @pytest.mark.parametrize("case", ["spread", "equal", "special", "negative"])
