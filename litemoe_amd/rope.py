@@ -94,8 +94,8 @@ def _check(q, k, cos_sin, positions):
 def _apart(q, k):
     """Whether every head of ``q`` and of ``k`` (``[T, heads, D]``, contiguous channels) has memory of its own, as a
     rotation in place needs it."""
-    (rows, heads, dim), (s0, s1, _) = q.shape, q.stride()
-    (k_rows, k_heads, k_dim), (k0, k1, _) = k.shape, k.stride()
+    (rows, heads, *_, dim), (s0, s1, *_) = q.shape, q.stride()
+    (k_rows, k_heads, *_, k_dim), (k0, k1, *_) = k.shape, k.stride()
     width, k_width = (heads - 1) * s1 + dim, (k_heads - 1) * k1 + k_dim  # of a row
     at = (k.data_ptr() - q.data_ptr()) // 2
     rows_apart = (s0 >= width or rows == 1) and (k0 >= k_width or k_rows == 1)
@@ -124,12 +124,11 @@ def _apart(q, k):
         return starts, starts + dim
     if rows_apart and s0 == k0 > 0 and min(rows, k_rows) > 1:
         # rows repeat: the heads of one row, of what reaches into the next its place there too
-        (q_starts, q_ends), (k_starts, k_ends) = all_of(1, heads, 0, s1, dim, 0), all_of(1, k_heads, 0, k1, k_dim, at % s0)
-        starts, ends = torch.cat((q_starts, k_starts)), torch.cat((q_ends, k_ends))
-        if free(torch.cat((starts, starts + s0)), torch.cat((ends, ends + s0))):
+        of_row = zip(all_of(1, heads, 0, s1, dim, 0), all_of(1, k_heads, 0, k1, k_dim, at % s0))
+        if free(*(torch.cat((x, y, x + s0, y + s0)) for x, y in of_row)):
             return True
-    (q_starts, q_ends), (k_starts, k_ends) = all_of(rows, heads, s0, s1, dim, 0), all_of(k_rows, k_heads, k0, k1, k_dim, at)
-    return free(torch.cat((q_starts, k_starts)), torch.cat((q_ends, k_ends)))
+    whole = zip(all_of(rows, heads, s0, s1, dim, 0), all_of(k_rows, k_heads, k0, k1, k_dim, at))
+    return free(*(torch.cat(x) for x in whole))
 
 
 def rotary_embedding(positions, query, key, head_size, cos_sin_cache, is_neox=True):

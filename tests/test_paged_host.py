@@ -347,6 +347,20 @@ def test_rotation_in_place_needs_memory_of_its_own(q, k, fine, whole, monkeypatc
         assert not launched
 
 
+def test_rotation_in_place_of_single_positions(monkeypatch):
+    """The reference's table takes ``[T, heads, 1, 64]`` too, as a decode step has its heads."""
+    launched = []
+    monkeypatch.setattr(_lib, "require_cuda", lambda *tensors, what: None)
+    monkeypatch.setattr(_lib, "stream", lambda device: None)
+    monkeypatch.setattr(_lib, "call", lambda *args: launched.append(args))
+    q, k, _ = torch.zeros(5, 12, 1, 64, dtype=torch.bfloat16).split((8, 2, 2), 1)
+    at, cos_sin = torch.zeros(5, dtype=torch.int64), rope.rotary_table(16, 64, 1e4, dtype=torch.bfloat16)
+    rope.rotary_embedding(at, q, k, 64, cos_sin)
+    assert launched[0][1:7] == (q.data_ptr(), 768, 64, k.data_ptr(), 768, 64)
+    with pytest.raises(ValueError, match="in place"):
+        rope.rotary_embedding(at, q, q[:, 1:], 64, cos_sin)
+
+
 @pytest.mark.parametrize("kwargs,text", [(dict(maximum=0), "length bound"), (dict(maximum=65), "length bound"),
                                          (dict(head_dim=32), "head_dim"), (dict(groups=17), "16 query heads"),
                                          (dict(groups=0), "16 query heads")])
