@@ -177,8 +177,6 @@ class QuantKVCache:
             raise ValueError("Prompt width exceeds the KV capacity")
         if rows.numel() != b:
             raise ValueError("Prefill slots must name one cache row per batch row")
-        for row in range(*slot.indices(self.slots.numel())) if isinstance(slot, slice) else (slot,):
-            self.check_own(row, 0, s)
         zero, keep = torch.zeros((), dtype=k.dtype, device=k.device), valid[:, None, :, None]
         pos = self.keys[:s]
         flat = [torch.where(keep, x, zero).transpose(1, 2).reshape(b * s, h, 1, d) for x in (k, v)]

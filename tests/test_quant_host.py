@@ -73,6 +73,19 @@ def test_cache_buffers_and_bytes():
         assert over.k is cache.k and over.bits == bits and over.capacity == 40
 
 
+@pytest.mark.parametrize("slot,rows", [(1, 1), (slice(0, 2), 2)])
+def test_prefill_by_rows_of_a_quantised_cache(slot, rows, monkeypatch):
+    """A quantised cache's rows share nothing: a prefill by rows stores every position of them."""
+    stored = []
+    monkeypatch.setattr(kv_quant, "write", lambda cache, layer, k, v, at, active, slots: stored.extend(
+        zip(slots.tolist(), at.tolist())))
+    cfg = preset("granite-1b", num_hidden_layers=1)
+    cache = QuantKVCache(cfg, 2, 16, "cpu", torch.bfloat16)
+    x = torch.zeros(rows, cfg.num_key_value_heads, 3, 64, dtype=torch.bfloat16)
+    cache.prefill(0, slot, x, x, torch.ones(rows, 3, dtype=torch.bool))
+    assert stored == [(row, j) for row in (range(2) if rows == 2 else [1]) for j in range(3)]
+
+
 def test_python_refusals():
     cfg = preset("granite-1b", num_hidden_layers=1)
     with pytest.raises(ValueError, match="4 or 8 bits"):
