@@ -418,8 +418,9 @@ int lm_flash_decode_paged(const lm_flash_decode_paged_args *args, void *stream);
  * value at position used[b] - 1 of its row, and attention over the first used[b]
  * positions with them. Nothing is stored, and the cache is attended as it is,
  * where active[b] is 0, used[b] is below 1 or above max_len or width * page, or the
- * position has no page. Results are bitwise those of lm_paged_rotate_write on
- * the same heads followed by lm_flash_decode_paged with the same num_splits. A page
+ * position has no page. Where the sums are bf16 values (a bf16 table rounds them
+ * to such) results are bitwise those of lm_paged_rotate_write on the same heads
+ * followed by lm_flash_decode_paged with the same num_splits. A page
  * that a row stores to may be no other row's. row_order and frag_out (nonzero: batch <= 128) as
  * lm_flash_decode_quant_qkv; qkv_partials 16-byte aligned. */
 typedef struct lm_flash_decode_paged_qkv_args {

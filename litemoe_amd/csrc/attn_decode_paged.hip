@@ -326,7 +326,7 @@ __device__ __forceinline__ void attend(const Args &a, const bf16 *__restrict__ q
   // kScores: a wave's scores of its last tiles, stored together, whole lines of one head by
   // eight lanes. Loads and stores return in the order they were issued, so a store behind
   // every tile holds the stream up: 64 rows of 500 to 8000 positions, 3 query heads per KV
-  // head, 137 us with one behind every tile, 133 in this way (K in half lines; now 124).
+  // head, 137 us with one behind every tile, 133 in this way (K in half lines; now 119).
   const int ring = ring_tiles(G);
   float *sm_ring = sm_f + 2 * G + wave * ring * G * kTile;
   int ringed = 0;
@@ -421,7 +421,9 @@ __device__ __forceinline__ void attend(const Args &a, const bf16 *__restrict__ q
     // Probabilities for the matrix cores in two bf16 parts, cut and rest: with one, rounded
     // (2^-9 of each off), results were off by 2.2e-3 (relative, RMS), with two by 1.7e-3, the
     // output's own rounding, in the same time. The rest is taken 2^-18 of the whole larger,
-    // so that it is above 0 where the probability is: 0 times an infinity in V is no number.
+    // so that for probabilities of 2^-108 and more (of the running maximum's) it is a normal
+    // number above 0: 0 times an infinity in V is no number, which an infinity attended by a
+    // smaller one may give.
     u32x4 p, rest;
 #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -561,7 +563,8 @@ __device__ __forceinline__ void attend(const Args &a, const bf16 *__restrict__ q
 // reads some 35 GB/s, so the rate of the whole falls with its emptiest CU; a workgroup
 // adds up the rows' tiles itself.
 // Registers: four waves per SIMD where splits give a CU four workgroups (D = 64). With
-// scores to store that would spill (145 us for those 133), and shares give a CU two.
+// scores to store that would spill (64 rows of 500 to 8000 positions, 3 query heads per KV
+// head, when three took 133 us: 145), and shares give a CU two.
 template <int D, bool kFused, int kWeigh, bool kShares>
 __global__ void __launch_bounds__(kThreads, D == 128 || kShares ? 2 : kWeigh == kScores ? 3 : 4)
 decode_paged_kernel(const bf16 *__restrict__ q, const int32_t *__restrict__ table, Args a) {

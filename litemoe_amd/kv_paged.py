@@ -77,9 +77,9 @@ def write(cache, layer, k, v, positions, active, slots):
     active = None if active is None else per_row(active, rows, torch.bool, index, "active")
     (k, k_view), (v, v_view) = view(k[:, :, 0], rows, heads), view(v[:, :, 0], rows, heads)
     _lib.call_struct(index, "lm_paged_rotate_write", 0, 0, 0, *k_view, *v_view, 0, 0, 0, 0, 0, 0, at.data_ptr(),
-                     at.dtype == torch.int32, 0 if active is None else active.data_ptr(), slots.data_ptr(), 0, 0, 0, 0, 0,
-                     0, kc.data_ptr(), vc.data_ptr(), table.data_ptr(), table.shape[0], table.shape[1], pages, page, rows,
-                     0, heads, dim)
+                     at.dtype == torch.int32, 0 if active is None else active.data_ptr(), slots.data_ptr(),
+                     0, 0, 0, 0, 0, 0, kc.data_ptr(), vc.data_ptr(), table.data_ptr(), table.shape[0], table.shape[1],
+                     pages, page, rows, 0, heads, dim)
 
 
 def read(cache, layer, positions, slots):
@@ -109,9 +109,10 @@ def evict(cache, weights, used, keep, recent, target, table=None, weights_out=No
     positions kept ``[L, B, H, keep]`` (int32, then -1) and the rows' new ``used``.
 
     Of equal weights the first stays; a NaN counts as the heaviest. A position that has
-    no page stays as zeros, as it is read. ``table`` is the rows' present table (the cache's own unless given). Pages of ``target`` must not be
-    in it: the rows' present pages are read and not written, so another row may share
-    them. :meth:`PagedKVCache.evict` takes care of both and moves the cache's table."""
+    no page stays as zeros, as it is read. ``table`` is the rows' present table (the
+    cache's own unless given). Pages of ``target`` must not be in it: the rows' present
+    pages are read and not written, so another row may share them.
+    :meth:`PagedKVCache.evict` takes care of both and moves the cache's table."""
     k, v = cache.k, cache.v
     table = cache.table if table is None else table
     layers, pages, heads, page, dim = k.shape
